@@ -29,6 +29,8 @@ VIEW_FRAME_RGB, VIEW_FRAME_PALETTE, VIEW_GRAY84 = 10, 11, 12
 VIEW_CENSUS = 13
 VIEW_PRESENT = 14   # presentation records [n][16 + video memory block]
 SHAPED_STATE_WORDS = 11   # NESLE_SMB_SHAPED_STATE_WORDS
+MEM_F32, MEM_BF16 = 0, 1
+QK_MAX_DIM, DELTA_MAX_DIM, DELTA_CHUNK = 256, 128, 32
 # Step-kernel census slots (nesle_amd/csrc/nes_layout.h, namespace census).
 CENSUS_FIELDS = ("waves", "iterations", "rare", "rare_io_write", "rare_side", "rare_idle", "rare_illegal",
                  "rare_timing", "rare_budget", "rare_outside", "rare_only_io_write", "dma", "present", "io_read",
@@ -80,6 +82,35 @@ class ShapedParams(ctypes.Structure):
               "bad_button_penalty")
     _fields_ = [(name, ctypes.c_float) for name in FLOATS] + [("stall_window", ctypes.c_int32),
                                                               ("repeated_jump_window", ctypes.c_int32)]
+
+
+class Heads(ctypes.Structure):
+    """nesle_heads (include/nesle_memory.h)."""
+    _fields_ = [("data", ctypes.c_void_p), ("stride_t", ctypes.c_int64), ("stride_n", ctypes.c_int64),
+                ("stride_h", ctypes.c_int64)]
+
+
+class QkArgs(ctypes.Structure):
+    """nesle_qk_args (include/nesle_memory.h)."""
+    _fields_ = ([(name, ctypes.c_uint32) for name in ("dtype", "steps", "batch", "q_heads", "k_heads", "dim", "rotated",
+                                                      "unit", "interleaved")]
+                + [("eps", ctypes.c_float), ("q", Heads), ("k", Heads)]
+                + [(name, ctypes.c_void_p) for name in ("q_weight", "k_weight", "positions", "table")]
+                + [("table_rows", ctypes.c_uint32)]
+                + [(name, ctypes.c_void_p) for name in ("q_out", "k_out")]
+                + [("dq_out", Heads), ("dk_out", Heads)]
+                + [(name, ctypes.c_void_p) for name in ("dq", "dk", "dq_weight", "dk_weight", "scratch")])
+
+
+class DeltaArgs(ctypes.Structure):
+    """nesle_delta_args (include/nesle_memory.h)."""
+    _fields_ = ([(name, ctypes.c_uint32) for name in ("dtype", "steps", "batch", "k_heads", "v_heads", "k_dim",
+                                                      "v_dim")]
+                + [("scale", ctypes.c_float), ("q", Heads), ("k", Heads), ("v", Heads)]
+                + [(name, ctypes.c_void_p) for name in ("g", "beta", "resets", "state", "out", "state_out", "saved")]
+                + [("dout", Heads)]
+                + [(name, ctypes.c_void_p) for name in ("dstate_out", "dq", "dk", "dv", "dg", "dbeta", "dstate",
+                                                        "scratch")])
 
 
 class RomInfo(ctypes.Structure):
@@ -171,6 +202,14 @@ def lib():
         "nesle_ppo_head_static": (ctypes.c_int, [vp, vp, vp, vp, vp, vp, ctypes.c_uint32, ctypes.c_uint32,
                                                  ctypes.c_double, ctypes.c_double, ctypes.c_double, vp, vp, vp, vp,
                                                  vp, vp]),
+        "nesle_qk_scratch_floats": (ctypes.c_uint64, [ctypes.POINTER(QkArgs)]),
+        "nesle_qk_norm_rotate": (ctypes.c_int, [ctypes.POINTER(QkArgs), vp]),
+        "nesle_qk_norm_rotate_grad": (ctypes.c_int, [ctypes.POINTER(QkArgs), vp]),
+        "nesle_delta_saved_floats": (ctypes.c_uint64, [ctypes.POINTER(DeltaArgs)]),
+        "nesle_delta_scratch_floats": (ctypes.c_uint64, [ctypes.POINTER(DeltaArgs)]),
+        "nesle_delta_step": (ctypes.c_int, [ctypes.POINTER(DeltaArgs), vp]),
+        "nesle_delta_forward": (ctypes.c_int, [ctypes.POINTER(DeltaArgs), vp]),
+        "nesle_delta_backward": (ctypes.c_int, [ctypes.POINTER(DeltaArgs), vp]),
         "nesle_smb_shaped_defaults": (None, [ctypes.POINTER(ShapedParams)]),
         "nesle_smb_shaped_reset": (ctypes.c_int, [vp, vp, ctypes.c_uint32, vp, vp]),
         "nesle_smb_shaped_reward": (ctypes.c_int, [vp, vp, vp, ctypes.c_uint32, ctypes.POINTER(ShapedParams), vp,

@@ -2,7 +2,7 @@
 
 Replaces the reference's nvcc build script (scripts/build_cuda_extension.py):
 
-* ``libnesle_hip.so``  -- kernels + C ABI (include/nesle_hip.h), built by hipcc
+* ``libnesle_hip.so``  -- kernels + C ABI (include/*.h), built by hipcc
   for ``--offload-arch=gfx950``;
 * ``_cuda_core_native*.so`` -- the pybind11 drop-in for nesle._cuda_core
   (re-exported by nesle_amd/_cuda_core.py), host-only C++ linked against
@@ -30,7 +30,9 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libnesle_hip.so"
 HIP_SOURCES = [CSRC / "nes_step.hip", CSRC / "nes_step_full.hip", CSRC / "nes_step_narrow.hip", CSRC / "nes_step_wave.hip", CSRC / "nes_step_solo.hip",
                CSRC / "nes_kernels.hip",
-               CSRC / "nes_render.hip", CSRC / "nes_host.hip", CSRC / "ppo_head.hip", CSRC / "smb_shaped.hip"]
+               CSRC / "nes_render.hip", CSRC / "nes_host.hip", CSRC / "ppo_head.hip", CSRC / "smb_shaped.hip",
+               CSRC / "mem_rotate.hip", CSRC / "mem_delta_step.hip", CSRC / "mem_delta_fwd.hip",
+               CSRC / "mem_delta_bwd.hip"]
 SHIM_SOURCE = CSRC / "cuda_core_module.cpp"
 
 HIP_FLAGS = [

@@ -1,0 +1,103 @@
+// mem_delta.h -- what the kernels of the gated delta rule share: their
+// arguments and the rule that ends an episode.
+#pragma once
+
+#include "mem_common.h"
+
+namespace nesle::mem {
+
+constexpr int kChunk = NESLE_DELTA_CHUNK;
+
+// exp(g) is zero in float32 below this (its smallest denormal is 2^-149, and
+// half of it exp(-103.97)): the state is dropped, not multiplied by zero, and
+// every gate that is multiplied keeps a finite logarithm.
+constexpr float kDropBelow = -104.0f;
+
+template <typename T>
+struct DeltaArgs {
+    Heads<T> q, k, v, dout;
+    const float *g, *beta;
+    const std::uint8_t* resets;
+    const float* state;
+    T* out;
+    float *state_out, *saved;
+    const float* dstate_out;
+    T *dq, *dk, *dv;
+    float *dg, *dbeta, *dstate, *scratch;
+    std::uint32_t steps, batch, hk, hv, group, dk_dim, dv_dim;     // group: value heads of a key head
+    float scale;
+};
+
+template <typename T>
+DeltaArgs<T> delta_args(const nesle_delta_args& a) {
+    DeltaArgs<T> d{};
+    d.q = heads<T>(a.q);
+    d.k = heads<T>(a.k);
+    d.v = heads<T>(a.v);
+    d.dout = heads<T>(a.dout);
+    d.g = a.g;
+    d.beta = a.beta;
+    d.resets = a.resets;
+    d.state = a.state;
+    d.out = static_cast<T*>(a.out);
+    d.state_out = a.state_out;
+    d.saved = a.saved;
+    d.dstate_out = a.dstate_out;
+    d.dq = static_cast<T*>(a.dq);
+    d.dk = static_cast<T*>(a.dk);
+    d.dv = static_cast<T*>(a.dv);
+    d.dg = a.dg;
+    d.dbeta = a.dbeta;
+    d.dstate = a.dstate;
+    d.scratch = a.scratch;
+    d.steps = a.steps;
+    d.batch = a.batch;
+    d.hk = a.k_heads;
+    d.hv = a.v_heads;
+    d.group = a.v_heads / a.k_heads;
+    d.dk_dim = a.k_dim;
+    d.dv_dim = a.v_dim;
+    d.scale = a.scale;
+    return d;
+}
+
+// Whether the state is dropped before a token.
+template <typename T>
+__device__ bool drops(const DeltaArgs<T>& a, std::uint32_t token, std::uint32_t env, std::uint32_t head) {
+    const std::size_t at = static_cast<std::size_t>(token) * a.batch + env;
+    return (a.resets != nullptr && a.resets[at] != 0) || a.g[at * a.hv + head] < kDropBelow;
+}
+
+inline std::uint32_t padded_dim(const nesle_delta_args& a) {
+    const std::uint32_t d = a.k_dim > a.v_dim ? a.k_dim : a.v_dim;
+    return d <= 32 ? 32 : d <= 64 ? 64 : 128;
+}
+
+// Arguments that no call may have; `step`: of nesle_delta_step.
+inline int check_delta(const char* who, const nesle_delta_args* a) {
+    if (a == nullptr) return refuse(who, "null arguments");
+    if (a->dtype != NESLE_MEM_F32 && a->dtype != NESLE_MEM_BF16) return refuse(who, "dtype must be NESLE_MEM_F32 or NESLE_MEM_BF16");
+    for (const std::uint32_t d : {a->k_dim, a->v_dim})
+        if (d == 0 || d % 8 != 0 || d > NESLE_DELTA_MAX_DIM)
+            return refuse(who, "k_dim and v_dim must be multiples of 8 up to " + std::to_string(NESLE_DELTA_MAX_DIM));
+    if (a->k_heads == 0 || a->v_heads == 0 || a->v_heads % a->k_heads != 0)
+        return refuse(who, "v_heads must be a multiple of k_heads");
+    if (static_cast<std::uint64_t>(a->batch) * a->v_heads > (1u << 22))
+        return refuse(who, "batch * v_heads must be at most 4,194,304");
+    if (a->steps > (1u << 30)) return refuse(who, "steps must be at most 2^30");
+    return NESLE_OK;
+}
+
+// The state tensors are read and written as 16-byte words.
+inline bool aligned16(const void* p) { return reinterpret_cast<std::uintptr_t>(p) % 16 == 0; }
+
+// Pointers that a call over at least one token and console needs.
+inline int check_delta_inputs(const char* who, const nesle_delta_args* a) {
+    if (!a->q.data || !a->k.data || !a->v.data || !a->g || !a->beta) return refuse(who, "null device pointer");
+    if (!aligned16(a->state) || !aligned16(a->state_out) || !aligned16(a->saved) || !aligned16(a->dstate_out) ||
+        !aligned16(a->dstate))
+        return refuse(who, "states must lie on 16-byte boundaries");
+    return NESLE_OK;
+}
+
+}  // namespace nesle::mem
