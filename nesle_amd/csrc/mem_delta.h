@@ -2,6 +2,10 @@
 // arguments and the rule that ends an episode.
 #pragma once
 
+#include <initializer_list>
+#include <type_traits>
+#include <utility>
+
 #include "mem_common.h"
 
 namespace nesle::mem {
@@ -61,16 +65,19 @@ DeltaArgs<T> delta_args(const nesle_delta_args& a) {
     return d;
 }
 
-// Whether the state is dropped before a token.
-template <typename T>
-__device__ bool drops(const DeltaArgs<T>& a, std::uint32_t token, std::uint32_t env, std::uint32_t head) {
-    const std::size_t at = static_cast<std::size_t>(token) * a.batch + env;
-    return (a.resets != nullptr && a.resets[at] != 0) || a.g[at * a.hv + head] < kDropBelow;
-}
-
 inline std::uint32_t padded_dim(const nesle_delta_args& a) {
     const std::uint32_t d = a.k_dim > a.v_dim ? a.k_dim : a.v_dim;
     return d <= 32 ? 32 : d <= 64 ? 64 : 128;
+}
+
+// Whether a chunk's rows of any tensor span 2^31 bytes or more, past what a
+// 32-bit offset reaches.
+inline bool wide_rows(const nesle_delta_args& a) {
+    const std::int64_t item = a.dtype == NESLE_MEM_F32 ? 4 : 2, limit = ((1ll << 31) - 4096) / kChunk;
+    for (const nesle_heads* x : {&a.q, &a.k, &a.v, &a.dout})
+        if (x->stride_t < 0 || x->stride_t * item >= limit) return true;
+    const std::int64_t heads = static_cast<std::int64_t>(a.batch) * a.v_heads;
+    return heads * (a.k_dim > a.v_dim ? a.k_dim : a.v_dim) * 4 >= limit;
 }
 
 // Arguments that no call may have; `step`: of nesle_delta_step.

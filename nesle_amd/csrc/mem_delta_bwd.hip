@@ -9,16 +9,17 @@
 //   dQ = scale gamma (dO S^T) + M1 K,                M1 = scale L dP
 //   dK = M1^T Q + E (U dS^T) - beta gamma (dR S^T) + M2 K + M2^T K,   M2 = beta L dA
 //   dbeta = dR . (V - gamma K S) + rowsum(dA L kk)
-// A gate enters through the G_i that include it.  dG_i is the row sum less the
-// column sum of dP P + dA A, plus gamma_i (scale dO.QS - beta dR.KS), less
-// e_i = E_i (K dS).U; the last G also has gamma_last <dS, S> + sum of e.
-// dg_t is the sum of dG_i over i >= t, and zero where the state is dropped.
+// The gate of token t scales what crosses from before t to t or later: dg_t is
+// the sum of E_ij = dP_ij P_ij + dA_ij A_ij over j < t <= i, of
+// gamma_i (scale dO.QS - beta dR.KS) over i >= t, of e_j = E_j (K dS)_j.U_j over
+// j < t, and of gamma_last <dS, S>.  (As sums of what crosses: the row sums less
+// the column sums over i >= t would be equal, but cancel where neighbouring
+// keys are alike.)  It is zero where the state is dropped.
 //
 // The part over value columns runs a wave per 16 columns, as in the forward;
 // the part that sums over the value dimension runs a wave per 16 key columns,
-// on U, dR, dO, S and dS written to LDS (the states in slabs of 64 columns).
-// No atomics: the sums over waves are added in a fixed order.
-#include "mem_delta.h"
+// on U, dR and dO left in LDS, S read again and dS passed through LDS 32
+// columns at a time.  No atomics: sums over waves are added in a fixed order.
 #include "mem_delta_tile.h"
 
 namespace nesle::mem {
@@ -27,272 +28,280 @@ namespace {
 template <typename T, int DP>
 struct GradTile : ChunkTile<T, DP> {
     using Base = ChunkTile<T, DP>;
-    static constexpr int kSlab = DP < 64 ? DP : 64;        // columns of a state slab
-    static constexpr int kSlabStride = kSlab + 4;
-    alignas(16) float dout[kChunk * Base::kStride];
-    alignas(16) float u[kChunk * Base::kStride];
-    alignas(16) float dr[kChunk * Base::kStride];
-    alignas(16) float slab[DP * kSlabStride];              // [key][value column]
-    alignas(16) float m1[kChunk * Base::kSmall];
-    alignas(16) float m2[kChunk * Base::kSmall];
-    float row_beta[Base::kWaves][kChunk], row_gate[Base::kWaves][kChunk];
-    float last_gate[Base::kWaves];
+    using M = typename Base::M;
+    // Transposed: [value column][token], [value column of 32][key].
+    typename M::template Tile<DP, kChunk, false> dout;
+    typename M::template Tile<DP, kChunk, true> u, dr;
+    typename M::template Tile<32, DP, true> slab;
+    float row_beta[Base::kWaves][kChunk], row_gate[Base::kWaves][kChunk], row_after[Base::kWaves][kChunk];
+    float place_beta[3][16], cross[4][16];     // of a tile: sums over columns; pairs that cross a token
+    float whole[Base::kWaves];
 };
 
-__device__ inline float sum16(float v) {
-    for (int d = 1; d < 16; d *= 2) v += __shfl_xor(v, d);
-    return v;
-}
-
-template <typename T, int DP>
+template <typename T, int DP, bool WIDE>
 __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> a) {
     using Tile = GradTile<T, DP>;
-    constexpr int KT = DP / 16, ST = Tile::kStride, SM = Tile::kSmall, SL = Tile::kSlabStride;
-    constexpr int kPerSlab = Tile::kSlab / 16;              // waves whose columns make a slab
+    using M = typename Tile::M;
+    using In = Rows<T, WIDE>;
+    constexpr int KT = Tile::KT, KP = Tile::KP, kWaves = Tile::kWaves, kPlaces = (3 + kWaves - 1) / kWaves;
     __shared__ Tile sh;
-    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, r = lane % 16, g4 = lane / 16;
+    const Lane<DP> first;
     const std::uint32_t env = blockIdx.x / a.hv, h = blockIdx.x % a.hv, hk = h / a.group;
-    const std::size_t head = blockIdx.x;
-    const unsigned col = 16 * wave + r;
-    const bool in_v = col < a.dv_dim, in_k = col < a.dk_dim;
+    const std::size_t head = blockIdx.x, state_size = static_cast<std::size_t>(a.dk_dim) * a.dv_dim;
+    const std::int64_t v_step = static_cast<std::int64_t>(a.batch) * a.hv * a.dv_dim;
     const f4 zero = {0, 0, 0, 0};
 
     f4 dS[KT];
-    Tile::load_state(a, a.dstate_out, head, col, g4, dS);
+    Tile::load_state(a, a.dstate_out, head, first, dS);
+    sh.start(first);
 
+    Ahead<T, DP, WIDE> in;
+    std::uint32_t dout[8];
+    const auto fetch = [&](std::uint32_t end, const Lane<DP>& at) {
+        const std::uint32_t start = (end - 1) / kChunk * kChunk;
+        in.fetch(a, start, static_cast<int>(end - start), env, h, at);
+        in.columns(a.dout, a.dv_dim, start, static_cast<int>(end - start), env, h, at, dout);
+    };
+    if (a.steps != 0) fetch(a.steps, first);
     for (std::uint32_t t1 = a.steps; t1 > 0;) {
-        // The chunk ends at t1; it starts at the last multiple of the chunk
-        // length, or at the last token after that which drops the state.
+        const Lane<DP> at = Lane<DP>::anew();
+        const int r = at.r, g = at.g;
+        const bool in_v = at.col < static_cast<int>(a.dv_dim), in_k = at.col < static_cast<int>(a.dk_dim);
+        // The tokens of this turn end at t1; they start at the last multiple of
+        // the chunk length, or at the last token after that which drops the
+        // state.  Row t of the tiles is token start + t: rows outside
+        // [lo, hi) are zero.
         const std::uint32_t start = (t1 - 1) / kChunk * kChunk;
-        const bool cut = lane < static_cast<int>(t1 - start) && drops(a, start + lane, env, h);
-        const unsigned long long cuts = __ballot(cut);
-        const bool dropped = cuts != 0;
-        const std::uint32_t t0 = dropped ? start + 63 - __clzll(static_cast<long long>(cuts)) : start;
-        const int n = static_cast<int>(t1 - t0);
-
+        const std::uint32_t drops = in.drops();
+        const bool dropped = drops != 0;
+        const int lo = dropped ? 31 - __clz(static_cast<int>(drops)) : 0, hi = static_cast<int>(t1 - start);
+        const float* from = dropped ? nullptr : start == 0 ? a.state
+                                              : a.saved + (start / kChunk - 1) * state_size * a.batch * a.hv;
         f4 S[KT];
-        if (dropped)
-#pragma unroll
-            for (int i = 0; i < KT; ++i) S[i] = zero;
-        else if (t0 == 0)
-            Tile::load_state(a, a.state, head, col, g4, S);
-        else
-            Tile::get_saved(a, t0 / kChunk - 1, head, wave, lane, S);
+        Tile::load_state(a, from, head, at, S);
 
-        sh.stage_keys(a, t0, n, env, hk, tid);
-        if (wave == 0) sh.stage_gates(a, t0, n, env, h, lane);
+        sh.stage_keys(in, lo, hi, at);
+        if (at.wave == 0) sh.stage_gates(in, lo, hi, at.lane);
         f4 V[2], dO[2];
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int e = 0; e < 8; ++e) {
+            const bool use = at.row(e) >= lo && at.row(e) < hi;
+            V[e / 4][e % 4] = use ? In::value_of(in.v[e]) : 0.0f;
+            dO[e / 4][e % 4] = use ? In::value_of(dout[e]) : 0.0f;
+        }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = 16 * m + 4 * g4 + i;
-                const bool in = row < n && in_v;
-                V[m][i] = in ? static_cast<float>(a.v.row(t0 + row, env, h)[col]) : 0.0f;
-                dO[m][i] = in ? static_cast<float>(a.dout.row(t0 + row, env, h)[col]) : 0.0f;
-                sh.dout[row * ST + col] = dO[m][i];
-            }
+        for (int m = 0; m < 2; ++m) sh.dout.put4(at.col, 16 * m + 4 * g, dO[m]);
+        t1 = start + lo;
+        if (t1 > 0) fetch(t1, at);
         __syncthreads();
-        sh.products(a.scale, wave, r, g4);
+        f4 kk[kPlaces], qk[kPlaces];
+#pragma unroll
+        for (int j = 0; j < kPlaces; ++j)
+            if (at.wave + j * kWaves < 3) sh.products(at.wave + j * kWaves, a.scale, at, kk[j], qk[j]);
         __syncthreads();
-        if (wave < 2) sh.invert(wave, r, g4);
+        if (at.wave == static_cast<int>(blockIdx.x % kWaves)) sh.invert(at);
 
         f4 ks[2] = {}, qs[2] = {}, kds[2] = {};
 #pragma unroll
-        for (int i = 0; i < KT; ++i)
+        for (int i = 0; i < KP; ++i) {
+            const auto s = M::full(S[2 * i], S[2 * i + 1]), ds = M::full(dS[2 * i], dS[2 * i + 1]);
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-                const f4 kk = along<ST>(sh.k, 16 * m, 16 * i, r, g4);
-                ks[m] = mma(kk, S[i], ks[m]);
-                kds[m] = mma(kk, dS[i], kds[m]);
-                qs[m] = mma(along<ST>(sh.q, 16 * m, 16 * i, r, g4), S[i], qs[m]);
+                const auto key = sh.k.rows(16 * m, i, r, g);
+                ks[m] = M::mul(key, s, ks[m]);
+                kds[m] = M::mul(key, ds, kds[m]);
+                qs[m] = M::mul(sh.q.rows(16 * m, i, r, g), s, qs[m]);
             }
-        f4 Y[2], R[2], U[2], dU[2], dR[2], gam[2], dec[2], beta[2];
+        }
+        f4 Y[2], gam[2], dec[2], beta[2];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            gam[m] = *reinterpret_cast<const f4*>(&sh.gamma[16 * m + 4 * g4]);
-            dec[m] = *reinterpret_cast<const f4*>(&sh.decay[16 * m + 4 * g4]);
-            beta[m] = *reinterpret_cast<const f4*>(&sh.beta[16 * m + 4 * g4]);
+            gam[m] = sh.of_rows(sh.gamma, m, g);
+            dec[m] = sh.of_rows(sh.decay, m, g);
+            beta[m] = sh.of_rows(sh.beta, m, g);
             Y[m] = V[m] - gam[m] * ks[m];
-            R[m] = beta[m] * Y[m];
         }
+        const auto right = M::full(beta[0] * Y[0], beta[1] * Y[1]);
+        const auto grad = M::exact(dO[0], dO[1]);
         __syncthreads();
-        sh.solve(R, U, r, g4);
-        dU[0] = mma(down<SM>(sh.p, 0, 0, r, g4), dO[0], dec[0] * kds[0]);
-        dU[0] = mma(down<SM>(sh.p, 16, 0, r, g4), dO[1], dU[0]);
-        dU[1] = mma(down<SM>(sh.p, 16, 16, r, g4), dO[1], dec[1] * kds[1]);
-        // (I + A)^T dR = dU, last tile first; the rows of A carry beta.
-        dR[1] = mma(down<20>(sh.t[1], 0, 0, r, g4), dU[1], zero);
-        const f4 above = mma(down<SM>(sh.a, 16, 0, r, g4) * beta[1], dR[1], zero);
-        dR[0] = mma(down<20>(sh.t[0], 0, 0, r, g4), dU[0] - above, zero);
+        f4 U[2], dU[2], dR[2], X[2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            U[m] = M::mul(sh.t.rows(16 * m, 0, r, g), right, zero);
+            dU[m] = M::mul(sh.p.cols(0, 16 * m, r, g), grad, dec[m] * kds[m]);
+        }
+        const auto du = M::full(dU[0], dU[1]);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            dR[m] = M::mul(sh.t.cols(0, 16 * m, r, g), du, zero);
+            X[m] = beta[m] * gam[m] * dR[m];
+            sh.u.put4(at.col, 16 * m + 4 * g, U[m]);
+            sh.dr.put4(at.col, 16 * m + 4 * g, dR[m]);
+        }
+        const In dv(a.dv + static_cast<std::int64_t>(start) * v_step + head * a.dv_dim, v_step);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            dv.put(in_v && at.row(e) >= lo && at.row(e) < hi, at.row(e), at.col, beta[e / 4][e % 4] * dR[e / 4][e % 4]);
 
         // Sums over the value dimension of dbeta and the gates, this wave's share.
         const float last = sh.gamma[kChunk - 1];
-        float last_gate = 0.0f;
+        float whole = 0.0f;
 #pragma unroll
         for (int i = 0; i < KT; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) last_gate += dS[i][j] * S[i][j];
-        last_gate *= last;
-        f4 X[2];
+            for (int j = 0; j < 4; ++j) whole += dS[i][j] * S[i][j];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            X[m] = beta[m] * gam[m] * dR[m];
             const f4 by_beta = dR[m] * Y[m];
             const f4 e = dec[m] * kds[m] * U[m];
-            const f4 by_gate = gam[m] * a.scale * dO[m] * qs[m] - X[m] * ks[m] - e;
+            const f4 by_gate = gam[m] * a.scale * dO[m] * qs[m] - X[m] * ks[m];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                last_gate += e[i];
-                const int row = 16 * m + 4 * g4 + i;
-                const float sb = sum16(by_beta[i]), sg = sum16(by_gate[i]);
+                const float sb = sum16(by_beta[i]), sg = sum16(by_gate[i]), se = sum16(e[i]);
                 if (r == 0) {
-                    sh.row_beta[wave][row] = sb;
-                    sh.row_gate[wave][row] = sg;
+                    sh.row_beta[at.wave][16 * m + 4 * g + i] = sb;
+                    sh.row_gate[at.wave][16 * m + 4 * g + i] = sg;
+                    sh.row_after[at.wave][16 * m + 4 * g + i] = se;
                 }
-                if (row < n && in_v)
-                    a.dv[((static_cast<std::size_t>(t0) + row) * a.batch + env) * a.hv * a.dv_dim + h * a.dv_dim + col] =
-                        static_cast<T>(beta[m][i] * dR[m][i]);
-                sh.u[row * ST + col] = U[m][i];
-                sh.dr[row * ST + col] = dR[m][i];
             }
         }
-        last_gate = sum16(last_gate);
-        last_gate += __shfl_xor(last_gate, 16);
-        last_gate += __shfl_xor(last_gate, 32);
-        if (lane == 0) sh.last_gate[wave] = last_gate;
+        whole = over_groups(sum16(whole)) * last;
+        if (at.lane == 0) sh.whole[at.wave] = whole;
 
         // The state's gradient before the chunk (dS itself is still needed).
         f4 before[KT];
+        {
+            const auto read = M::full(gam[0] * a.scale * dO[0], gam[1] * a.scale * dO[1]);
+            const auto held = M::full(-X[0], -X[1]);
 #pragma unroll
-        for (int i = 0; i < KT; ++i) {
-            f4 add = mma(down<ST>(sh.q, 0, 16 * i, r, g4), gam[0] * a.scale * dO[0], dS[i] * last);
-            add = mma(down<ST>(sh.q, 16, 16 * i, r, g4), gam[1] * a.scale * dO[1], add);
-            add = mma(down<ST>(sh.k, 0, 16 * i, r, g4), -X[0], add);
-            before[i] = mma(down<ST>(sh.k, 16, 16 * i, r, g4), -X[1], add);
+            for (int i = 0; i < KT; ++i) {
+                before[i] = M::mul(sh.q.cols(0, 16 * i, r, g), read, dS[i] * last);
+                before[i] = M::mul(sh.k.cols(0, 16 * i, r, g), held, before[i]);
+            }
         }
         __syncthreads();
 
-        // dP and dA by tiles; a and p become the gates' terms, m1 and m2 what
-        // multiplies K and Q.
-        for (int place = wave; place < 3; place += Tile::kWaves) {
-            const int mi = place != 0 ? 16 : 0, nj = place == 2 ? 16 : 0;
+        // dP and dA by tiles; P's space becomes M1 and the inverse's M2.
+#pragma unroll
+        for (int j = 0; j < kPlaces; ++j) {
+            const int place = at.wave + j * kWaves;
+            if (place >= 3) break;
+            const int mi = Tile::first_row(place), nj = Tile::first_col(place);
             f4 dP = zero, dA = zero;
 #pragma unroll
-            for (int i = 0; i < KT; ++i) {
-                const f4 uu = along<ST>(sh.u, nj, 16 * i, r, g4);
-                dP = mma(along<ST>(sh.dout, mi, 16 * i, r, g4), uu, dP);
-                dA = mma(along<ST>(sh.dr, mi, 16 * i, r, g4), uu, dA);
+            for (int i = 0; i < KP; ++i) {
+                const auto uu = sh.u.cols(32 * i, nj, r, g);
+                dP = M::mul(sh.dout.cols(32 * i, mi, r, g), uu, dP);
+                dA = M::mul(sh.dr.cols(32 * i, mi, r, g), uu, dA);
             }
+            // With token t = 16 x + r in lane r: pairs of this tile with
+            // j < t <= i.  Tile (16, 0) has them for both halves of t.
+            float cross = 0.0f, cross_below = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int row = mi + 4 * g4 + i, c = nj + r, at = row * SM + c;
-                const float L = c <= row ? sh.ratio(row, c) : 0.0f;
-                sh.m1[at] = c <= row ? a.scale * L * dP[i] : 0.0f;
-                sh.m2[at] = c < row ? -sh.beta[row] * L * dA[i] : 0.0f;
-                sh.p[at] = c <= row ? dP[i] * sh.p[at] : 0.0f;
-                sh.a[at] = c < row ? -dA[i] * sh.a[at] : 0.0f;
+                const int row = mi + 4 * g + i, c = nj + r;
+                const float L = sh.ratio(row, c), b = sh.beta[row];
+                sh.p.put(row, c, c <= row ? a.scale * L * dP[i] : 0.0f);
+                sh.t.put(row, c, c < row ? -b * L * dA[i] : 0.0f);
+                const float by_a = -dA[i] * kk[j][i];
+                const float before_t = sum_below(c < row ? dP[i] * qk[j][i] + b * by_a : 0.0f);
+                cross += place == 1 || row >= c ? before_t : 0.0f;
+                const float sb = sum16(by_a), all = sum16(c < row ? dP[i] * qk[j][i] + b * by_a : 0.0f);
+                if (4 * g + i >= r) cross_below += all;
+                if (r == 0) sh.place_beta[place][4 * g + i] = sb;
+            }
+            cross = over_groups(cross);
+            if (g == 0) sh.cross[place][r] = cross;
+            if (place == 1) {
+                cross_below = over_groups(cross_below);
+                if (g == 0) sh.cross[3][r] = cross_below;
             }
         }
-        // dO S^T, dR S^T, U dS^T: this wave's 16 key columns.
-        f4 dos[2] = {}, drs[2] = {}, uds[2] = {};
+        // dO S^T and dR S^T, then U dS^T: this wave's 16 key columns.
+        f4 dQ[2] = {}, dK[2] = {}, drs[2] = {};
+        if (from != nullptr) {
+            const Rows<float, false> states(from + head * state_size, a.dv_dim);
 #pragma unroll
-        for (int s = 0; s < 2 * KT / kPerSlab; ++s) {
-            const bool of_grad = s >= KT / kPerSlab;
-            const int first = (s % (KT / kPerSlab)) * kPerSlab;     // first wave of the slab's columns
-            if (wave >= first && wave < first + kPerSlab)
-#pragma unroll
-                for (int i = 0; i < KT; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        sh.slab[(16 * i + 4 * g4 + j) * SL + 16 * (wave - first) + r] = of_grad ? dS[i][j] : S[i][j];
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < kPerSlab; ++i) {
-                const f4 b = along<SL>(sh.slab, 16 * wave, 16 * i, r, g4);
+            for (int i = 0; i < KP; ++i) {
+                const auto s = M::full(states.get4(in_k && 32 * i + 4 * g < static_cast<int>(a.dv_dim), at.col, 32 * i + 4 * g),
+                                       states.get4(in_k && 32 * i + 16 + 4 * g < static_cast<int>(a.dv_dim), at.col, 32 * i + 16 + 4 * g));
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
-                    const int c = 16 * (first + i);
-                    if (of_grad) {
-                        uds[m] = mma(along<ST>(sh.u, 16 * m, c, r, g4), b, uds[m]);
-                    } else {
-                        dos[m] = mma(along<ST>(sh.dout, 16 * m, c, r, g4), b, dos[m]);
-                        drs[m] = mma(along<ST>(sh.dr, 16 * m, c, r, g4), b, drs[m]);
-                    }
+                    dQ[m] = M::mul(sh.dout.cols(32 * i, 16 * m, r, g), s, dQ[m]);
+                    drs[m] = M::mul(sh.dr.cols(32 * i, 16 * m, r, g), s, drs[m]);
                 }
             }
-            __syncthreads();
         }
-        f4 dQ[2], dK[2];
+#pragma unroll
+        for (int i = 0; i < KP; ++i) {
+            if (at.wave / 2 == i)
+#pragma unroll
+                for (int j = 0; j < KT; ++j) sh.slab.put4(16 * (at.wave % 2) + r, 16 * j + 4 * g, dS[j]);
+            __syncthreads();
+            const auto ds = sh.slab.cols(0, 16 * at.wave, r, g);
+#pragma unroll
+            for (int m = 0; m < 2; ++m) dK[m] = M::mul(sh.u.cols(32 * i, 16 * m, r, g), ds, dK[m]);
+            if (i + 1 < KP) __syncthreads();
+        }
+        const auto key = sh.k.cols(0, 16 * at.wave, r, g), query = sh.q.cols(0, 16 * at.wave, r, g);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            dQ[m] = gam[m] * a.scale * dos[m];
-            dK[m] = dec[m] * uds[m] - beta[m] * gam[m] * drs[m];
+            dQ[m] = M::mul(sh.p.rows(16 * m, 0, r, g), key, gam[m] * a.scale * dQ[m]);
+            dK[m] = M::mul(sh.p.cols(0, 16 * m, r, g), query, dec[m] * dK[m] - beta[m] * gam[m] * drs[m]);
+            dK[m] = M::mul(sh.t.rows(16 * m, 0, r, g), key, dK[m]);
+            dK[m] = M::mul(sh.t.cols(0, 16 * m, r, g), key, dK[m]);
         }
+        const std::int64_t token = static_cast<std::int64_t>(start) * a.batch + env;
+        if (a.group == 1) {
+            const std::int64_t step = static_cast<std::int64_t>(a.batch) * a.hk * a.dk_dim;
+            const In dq(a.dq + (token * a.hk + hk) * a.dk_dim, step), dk(a.dk + (token * a.hk + hk) * a.dk_dim, step);
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {                               // the tile of tokens summed over
-            const f4 kx = down<ST>(sh.k, 16 * x, 16 * wave, r, g4), qx = down<ST>(sh.q, 16 * x, 16 * wave, r, g4);
+            for (int e = 0; e < 8; ++e) {
+                const bool mine = in_k && at.row(e) >= lo && at.row(e) < hi;
+                dq.put(mine, at.row(e), at.col, dQ[e / 4][e % 4]);
+                dk.put(mine, at.row(e), at.col, dK[e / 4][e % 4]);
+            }
+        } else {            // one share a value head, added up afterwards
+            const std::int64_t step = static_cast<std::int64_t>(a.batch) * a.hv * a.dk_dim;
+            float* share = a.scratch + (token * a.hv + h) * a.dk_dim;
+            const Rows<float, WIDE> dq(share, step), dk(share + a.steps * step, step);
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                if (x <= m) {
-                    dQ[m] = mma(along<SM>(sh.m1, 16 * m, 16 * x, r, g4), kx, dQ[m]);
-                    dK[m] = mma(along<SM>(sh.m2, 16 * m, 16 * x, r, g4), kx, dK[m]);
-                }
-                if (x >= m) {
-                    dK[m] = mma(down<SM>(sh.m1, 16 * x, 16 * m, r, g4), qx, dK[m]);
-                    dK[m] = mma(down<SM>(sh.m2, 16 * x, 16 * m, r, g4), kx, dK[m]);
-                }
+            for (int e = 0; e < 8; ++e) {
+                const bool mine = in_k && at.row(e) >= lo && at.row(e) < hi;
+                dq.put(mine, at.row(e), at.col, dQ[e / 4][e % 4]);
+                dk.put(mine, at.row(e), at.col, dK[e / 4][e % 4]);
             }
         }
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = 16 * m + 4 * g4 + i;
-                if (row >= n || !in_k) continue;
-                const std::size_t at = (static_cast<std::size_t>(t0) + row) * a.batch + env;
-                if (a.group == 1) {
-                    a.dq[(at * a.hk + hk) * a.dk_dim + col] = static_cast<T>(dQ[m][i]);
-                    a.dk[(at * a.hk + hk) * a.dk_dim + col] = static_cast<T>(dK[m][i]);
-                } else {            // one share a value head, added up afterwards
-                    const std::size_t all = static_cast<std::size_t>(a.steps) * a.batch * a.hv * a.dk_dim;
-                    a.scratch[(at * a.hv + h) * a.dk_dim + col] = dQ[m][i];
-                    a.scratch[all + (at * a.hv + h) * a.dk_dim + col] = dK[m][i];
-                }
-            }
-        if (wave == 0) {            // one token a lane
-            const int t = lane % kChunk;
-            float db = 0.0f, gate = 0.0f;
-            for (int c = 0; c <= t; ++c) {
-                db += sh.a[t * SM + c];
-                gate += sh.p[t * SM + c];
-            }
-            gate += sh.beta[t] * db;
-            for (int c = t; c < kChunk; ++c) gate -= sh.p[c * SM + t] + sh.beta[c] * sh.a[c * SM + t];
-            for (int w = 0; w < Tile::kWaves; ++w) {
+        if (at.wave == 0) {            // one token a lane
+            const int t = at.lane % kChunk, i = t % 16;
+            float db = t < 16 ? sh.place_beta[0][i] : sh.place_beta[1][i] + sh.place_beta[2][i];
+            float dg = t < 16 ? sh.cross[0][i] + sh.cross[1][i] : sh.cross[2][i] + sh.cross[3][i];
+            float from_t = 0.0f, to_t = 0.0f;
+            for (int w = 0; w < kWaves; ++w) {
                 db += sh.row_beta[w][t];
-                gate += sh.row_gate[w][t];
+                from_t += sh.row_gate[w][t];
+                to_t += sh.row_after[w][t];
+                dg += sh.whole[w];
             }
-            if (t == kChunk - 1)
-                for (int w = 0; w < Tile::kWaves; ++w) gate += sh.last_gate[w];
-            double sum = gate;                                      // of the tokens from t on
 #pragma unroll
             for (int d = 1; d < kChunk; d *= 2) {
-                const double above = __shfl_down(sum, d);
-                if (t + d < kChunk) sum += above;
+                const float above = __shfl_down(from_t, d), below = __shfl_up(to_t, d);
+                if (t + d < kChunk) from_t += above;
+                if (t >= d) to_t += below;
             }
-            if (lane < n) {
-                const std::size_t at = ((static_cast<std::size_t>(t0) + t) * a.batch + env) * a.hv + h;
-                a.dbeta[at] = db;
-                a.dg[at] = dropped && t == 0 ? 0.0f : static_cast<float>(sum);
+            to_t = __shfl_up(to_t, 1);
+            dg += from_t + (t > 0 ? to_t : 0.0f);
+            if (at.lane >= lo && at.lane < hi) {
+                const std::size_t to = ((static_cast<std::size_t>(start) + t) * a.batch + env) * a.hv + h;
+                a.dbeta[to] = db;
+                a.dg[to] = dropped && t == lo ? 0.0f : dg;
             }
         }
 #pragma unroll
         for (int i = 0; i < KT; ++i) dS[i] = dropped ? zero : before[i];
-        t1 = t0;
         __syncthreads();
     }
-    if (a.dstate != nullptr) Tile::store_state(a, a.dstate, head, col, g4, dS);
+    if (a.dstate != nullptr) Tile::store_state(a, a.dstate, head, Lane<DP>::anew(), dS);
 }
 
 // dq and dk of a key head: the sum of its value heads' shares.
@@ -314,10 +323,12 @@ template <typename T>
 int backward(const char* who, const nesle_delta_args& x, hipStream_t s) {
     const DeltaArgs<T> a = delta_args<T>(x);
     const dim3 grid(a.batch * a.hv);
-    switch (padded_dim(x)) {
-        case 32: hipLaunchKernelGGL((delta_backward_kernel<T, 32>), grid, dim3(128), 0, s, a); break;
-        case 64: hipLaunchKernelGGL((delta_backward_kernel<T, 64>), grid, dim3(256), 0, s, a); break;
-        default: hipLaunchKernelGGL((delta_backward_kernel<T, 128>), grid, dim3(512), 0, s, a); break;
+    const std::uint32_t dim = wide_rows(x) ? 0 : padded_dim(x);
+    switch (dim) {
+        case 0: hipLaunchKernelGGL((delta_backward_kernel<T, 128, true>), grid, dim3(512), 0, s, a); break;
+        case 32: hipLaunchKernelGGL((delta_backward_kernel<T, 32, false>), grid, dim3(128), 0, s, a); break;
+        case 64: hipLaunchKernelGGL((delta_backward_kernel<T, 64, false>), grid, dim3(256), 0, s, a); break;
+        default: hipLaunchKernelGGL((delta_backward_kernel<T, 128, false>), grid, dim3(512), 0, s, a); break;
     }
     if (a.group > 1 && a.steps != 0) {
         const std::uint64_t quads = static_cast<std::uint64_t>(a.steps) * a.batch * a.hk * a.dk_dim / 4;

@@ -12,130 +12,138 @@
 // One workgroup walks one head of one console; a wave holds 16 columns of the
 // state, in registers for the whole rollout, and its 16 columns of R, U and O.
 // A result tile is the operand of the next product as it lies in the
-// registers (mem_common.h), so only what all columns share goes through LDS:
-// K, Q, A, P and the inverses of (I + A)'s two diagonal tiles.  Those are
-// found by substitution: neighbouring frames have nearly equal keys, where the
-// powers of A grow to thousands and a product form of the inverse cancels.
+// registers (mem_delta_math.h), so only what all columns share goes through
+// LDS: K, Q, P and (I + A)^-1.  That inverse is found by substitution:
+// neighbouring frames have nearly equal keys, where the powers of A grow to
+// thousands and a product form of the inverse cancels.
 //
-// Float32 throughout, products by v_mfma_f32_16x16x4_f32: the state and the
-// gates' gradients are float32 results whatever the inputs' type.
+// All products keep float32 precision: the state and the gates' gradients are
+// float32 results whatever the inputs' type.
 //
 // A chunk ends early at a token that drops the state (its episode ended) and
 // before one that holds a value that is not finite, so that neither reaches a
 // token it must not (a product with a masked zero would carry NaN).
-#include "mem_delta.h"
 #include "mem_delta_tile.h"
 
 namespace nesle::mem {
 namespace {
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(DP * 4) delta_forward_kernel(DeltaArgs<T> a) {
+template <typename T, int DP, bool WIDE>
+__global__ void __launch_bounds__(DP * 4, DP == 128 ? 2 : 4) delta_forward_kernel(DeltaArgs<T> a) {
     using Tile = ChunkTile<T, DP>;
-    constexpr int KT = DP / 16;                 // tiles of the key dimension
+    using M = typename Tile::M;
+    constexpr int KT = Tile::KT, KP = Tile::KP;
     __shared__ Tile sh;
-    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, r = lane % 16, g4 = lane / 16;
-    const std::uint32_t env = blockIdx.x / a.hv, h = blockIdx.x % a.hv, hk = h / a.group;
-    const std::size_t head = blockIdx.x;
-    const unsigned col = 16 * wave + r;
-    const bool in_col = col < a.dv_dim;
+    const Lane<DP> first;
+    const std::uint32_t env = blockIdx.x / a.hv, h = blockIdx.x % a.hv;
+    const std::size_t head = blockIdx.x, state_size = static_cast<std::size_t>(a.dk_dim) * a.dv_dim;
+    const std::int64_t out_step = static_cast<std::int64_t>(a.batch) * a.hv * a.dv_dim;
+    const f4 zero = {0, 0, 0, 0};
 
     f4 S[KT];
-    Tile::load_state(a, a.state, head, col, g4, S);
-    if (tid == 0) sh.bad = 0;
+    Tile::load_state(a, a.state, head, first, S);
+    sh.start(first);
     __syncthreads();
 
+    // Tokens from t0 to the next multiple of the chunk length or the end.
+    const auto width = [&](std::uint32_t t0) {
+        const std::uint32_t whole = kChunk - t0 % kChunk, left = a.steps - t0;
+        return static_cast<int>(whole < left ? whole : left);
+    };
+    Ahead<T, DP, WIDE> in;
+    if (a.steps != 0) in.fetch(a, 0, width(0), env, h, first);
     for (std::uint32_t t0 = 0; t0 < a.steps;) {
+        const Lane<DP> at = Lane<DP>::anew();
+        const int r = at.r, g = at.g;
+        const bool in_col = at.col < static_cast<int>(a.dv_dim);
         if (t0 != 0 && t0 % kChunk == 0 && a.saved != nullptr)
-            Tile::put_saved(a, t0 / kChunk - 1, head, wave, lane, S);
-        if (drops(a, t0, env, h))
+            Tile::store_state(a, a.saved + (t0 / kChunk - 1) * state_size * a.batch * a.hv, head, at, S);
+        const std::uint32_t drops = in.drops();
+        if (drops & 1u)
 #pragma unroll
-            for (int i = 0; i < KT; ++i) S[i] = f4{0, 0, 0, 0};
-        int n = Tile::extent(a, t0, env, h, lane);
+            for (int i = 0; i < KT; ++i) S[i] = zero;
+        int n = drops & ~1u ? __ffs(static_cast<int>(drops & ~1u)) - 1 : width(t0);
         f4 V[2];
         for (;;) {
-            sh.stage_keys(a, t0, n, env, hk, tid);
-            if (wave == 0) sh.stage_gates(a, t0, n, env, h, lane);
+            std::uint32_t odd = sh.stage_keys(in, 0, n, at);
+            if (at.wave == 0) odd |= sh.stage_gates(in, 0, n, at.lane);
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = 16 * m + 4 * g4 + i;
-                    float x = 0.0f;
-                    if (row < n && in_col) x = static_cast<float>(a.v.row(t0 + row, env, h)[col]);
-                    if (!(fabsf(x) < INFINITY)) atomicOr(&sh.bad, 1u << row);
-                    V[m][i] = x;
-                }
+            for (int e = 0; e < 8; ++e) {
+                const float x = at.row(e) < n ? Rows<T, WIDE>::value_of(in.v[e]) : 0.0f;
+                if (!(fabsf(x) < INFINITY)) odd |= 1u << at.row(e);
+                V[e / 4][e % 4] = x;
+            }
+            sh.report(odd);
             __syncthreads();
-            const unsigned bad = sh.bad;
+            const unsigned bad = __builtin_amdgcn_readfirstlane(sh.bad);
             if (bad == 0 || n == 1) break;
             // Rare: stage again, up to the first such token, or it alone.
-            n = (bad & 1u) ? 1 : __ffs(bad) - 1;
+            n = (bad & 1u) ? 1 : __ffs(static_cast<int>(bad)) - 1;
             __syncthreads();
-            if (tid == 0) sh.bad = 0;
+            if (at.tid == 0) sh.bad = 0;
             __syncthreads();
         }
-        sh.products(a.scale, wave, r, g4);
+        const std::uint32_t next = t0 + n;
+        if (next < a.steps) in.fetch(a, next, width(next), env, h, at);
+        for (int place = at.wave; place < 3; place += Tile::kWaves) {
+            f4 kk, qk;
+            sh.products(place, a.scale, at, kk, qk);
+        }
         __syncthreads();
-        if (tid == 0) sh.bad = 0;
-        if (wave < 2) sh.invert(wave, r, g4);
+        if (at.tid == 0) sh.bad = 0;
+        // A different wave each workgroup, as the waves of a compute unit's
+        // workgroups share its four SIMDs by their number.
+        if (at.wave == static_cast<int>(blockIdx.x % Tile::kWaves)) sh.invert(at);
 
         // K S and Q S for this wave's columns.
         f4 ks[2] = {}, qs[2] = {};
 #pragma unroll
-        for (int i = 0; i < KT; ++i)
+        for (int i = 0; i < KP; ++i) {
+            const auto s = M::full(S[2 * i], S[2 * i + 1]);
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-                ks[m] = mma(along<Tile::kStride>(sh.k, 16 * m, 16 * i, r, g4), S[i], ks[m]);
-                qs[m] = mma(along<Tile::kStride>(sh.q, 16 * m, 16 * i, r, g4), S[i], qs[m]);
+                ks[m] = M::mul(sh.k.rows(16 * m, i, r, g), s, ks[m]);
+                qs[m] = M::mul(sh.q.rows(16 * m, i, r, g), s, qs[m]);
             }
-        f4 R[2], gam[2], dec[2];
+        }
+        f4 R[2];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            gam[m] = *reinterpret_cast<const f4*>(&sh.gamma[16 * m + 4 * g4]);
-            dec[m] = *reinterpret_cast<const f4*>(&sh.decay[16 * m + 4 * g4]);
-            const f4 b = *reinterpret_cast<const f4*>(&sh.beta[16 * m + 4 * g4]);
-            R[m] = b * (V[m] - gam[m] * ks[m]);
+            const f4 gam = sh.of_rows(sh.gamma, m, g);
+            R[m] = sh.of_rows(sh.beta, m, g) * (V[m] - gam * ks[m]);
+            qs[m] *= gam * a.scale;
         }
+        const auto right = M::full(R[0], R[1]);
         __syncthreads();
-        f4 U[2];
-        sh.solve(R, U, r, g4);
-        const f4 zero = {0, 0, 0, 0};
-        f4 O[2];
-        O[0] = mma(along<Tile::kSmall>(sh.p, 0, 0, r, g4), U[0], qs[0] * gam[0] * a.scale);
-        O[1] = mma(along<Tile::kSmall>(sh.p, 16, 0, r, g4), U[0], qs[1] * gam[1] * a.scale);
-        O[1] = mma(along<Tile::kSmall>(sh.p, 16, 16, r, g4), U[1], O[1]);
+        f4 U[2], O[2];
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < 2; ++m) U[m] = M::mul(sh.t.rows(16 * m, 0, r, g), right, zero);
+        const auto u = M::full(U[0], U[1]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = 16 * m + 4 * g4 + i;
-                if (row < n && in_col)
-                    a.out[((static_cast<std::size_t>(t0) + row) * a.batch + env) * a.hv * a.dv_dim + h * a.dv_dim + col] =
-                        static_cast<T>(O[m][i]);
-            }
+        for (int m = 0; m < 2; ++m) O[m] = M::mul(sh.p.rows(16 * m, 0, r, g), u, qs[m]);
+        const Rows<T, WIDE> out(a.out + static_cast<std::int64_t>(t0) * out_step + head * a.dv_dim, out_step);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out.put(in_col && at.row(e) < n, at.row(e), at.col, O[e / 4][e % 4]);
         const float last = sh.gamma[kChunk - 1];
-        const f4 W[2] = {U[0] * dec[0], U[1] * dec[1]};
+        const auto w = M::full(U[0] * sh.of_rows(sh.decay, 0, g), U[1] * sh.of_rows(sh.decay, 1, g));
 #pragma unroll
-        for (int i = 0; i < KT; ++i) {
-            f4 add = mma(down<Tile::kStride>(sh.k, 0, 16 * i, r, g4), W[0], zero);
-            add = mma(down<Tile::kStride>(sh.k, 16, 16 * i, r, g4), W[1], add);
-            S[i] = S[i] * last + add;
-        }
-        t0 += n;
+        for (int i = 0; i < KT; ++i) S[i] = S[i] * last + M::mul(sh.k.cols(0, 16 * i, r, g), w, zero);
+        t0 = next;
         __syncthreads();
     }
-    Tile::store_state(a, a.state_out, head, col, g4, S);
+    Tile::store_state(a, a.state_out, head, Lane<DP>::anew(), S);
 }
 
 template <typename T>
 int forward(const char* who, const nesle_delta_args& x, hipStream_t s) {
     const DeltaArgs<T> a = delta_args<T>(x);
     const dim3 grid(a.batch * a.hv);
-    switch (padded_dim(x)) {
-        case 32: hipLaunchKernelGGL((delta_forward_kernel<T, 32>), grid, dim3(128), 0, s, a); break;
-        case 64: hipLaunchKernelGGL((delta_forward_kernel<T, 64>), grid, dim3(256), 0, s, a); break;
-        default: hipLaunchKernelGGL((delta_forward_kernel<T, 128>), grid, dim3(512), 0, s, a); break;
+    const std::uint32_t dim = wide_rows(x) ? 0 : padded_dim(x);
+    switch (dim) {
+        case 0: hipLaunchKernelGGL((delta_forward_kernel<T, 128, true>), grid, dim3(512), 0, s, a); break;
+        case 32: hipLaunchKernelGGL((delta_forward_kernel<T, 32, false>), grid, dim3(128), 0, s, a); break;
+        case 64: hipLaunchKernelGGL((delta_forward_kernel<T, 64, false>), grid, dim3(256), 0, s, a); break;
+        default: hipLaunchKernelGGL((delta_forward_kernel<T, 128, false>), grid, dim3(512), 0, s, a); break;
     }
     return launched(who);
 }
@@ -150,8 +158,7 @@ extern "C" {
 std::uint64_t nesle_delta_saved_floats(const nesle_delta_args* a) {
     if (a == nullptr || a->steps <= static_cast<std::uint32_t>(kChunk)) return 0;
     const std::uint64_t chunks = (static_cast<std::uint64_t>(a->steps) + kChunk - 1) / kChunk - 1;
-    const std::uint64_t d = padded_dim(*a);
-    return chunks * a->batch * a->v_heads * d * d;
+    return chunks * a->batch * a->v_heads * a->k_dim * a->v_dim;
 }
 
 int nesle_delta_forward(const nesle_delta_args* a, void* stream) {

@@ -27,7 +27,7 @@ __global__ void __launch_bounds__(64 * kWaves) delta_step_kernel(DeltaArgs<T> a,
     const bool in_cols = col < a.dv_dim;
     const std::size_t at = static_cast<std::size_t>(head_of_all);
     const float* S = a.state + at * a.dk_dim * a.dv_dim + col;
-    const bool keep = a.state != nullptr && !drops(a, 0, env, h);
+    const bool keep = a.state != nullptr && !(a.resets != nullptr && a.resets[env] != 0) && !(a.g[at] < kDropBelow);
     const float decay = expf(a.g[at]), beta = a.beta[at];
 
     const T* q = a.q.row(0, env, h / a.group);

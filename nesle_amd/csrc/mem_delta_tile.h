@@ -1,116 +1,239 @@
-// mem_delta_tile.h -- one chunk of the gated delta rule in LDS: what the
-// forward and the gradient kernels both make of it.
+// mem_delta_tile.h -- one chunk of the gated delta rule: its inputs on their
+// way through registers, and the tiles in LDS that the forward and the
+// gradient kernels both make of it.
 #pragma once
 
-#include "mem_delta.h"
+#include "mem_delta_math.h"
 
 namespace nesle::mem {
 
+// ---- strided rows of a chunk ------------------------------------------------------
+// Rows start .. start + 31 of a tensor whose row 0 is at `base`.  Loads go
+// through a buffer descriptor: one scalar base, 32-bit offsets, and an offset
+// past its range, which a row or column outside the tensor is given, reads as
+// zero and is not written.  WIDE: rows may lie 2^31 bytes apart, 64-bit
+// addresses.
+constexpr std::uint32_t kOutside = 0x80000000u, kRange = 0x7fffffffu;
+
+template <typename T, bool WIDE>
+struct Rows {
+    T* base;
+    std::int64_t step;          // elements from row to row
+    __amdgpu_buffer_rsrc_t rsrc;
+    __device__ Rows(const T* b, std::int64_t s) : base(const_cast<T*>(b)), step(s) {
+        if constexpr (!WIDE) rsrc = __builtin_amdgcn_make_buffer_rsrc(base, 0, static_cast<int>(kRange), 0x00027000);
+    }
+    __device__ std::uint32_t offset(bool in, int row, int col) const {
+        return in ? static_cast<std::uint32_t>(row * static_cast<int>(step) + col) * sizeof(T) : kOutside;
+    }
+    // An element's bits, upper half of the word for two-byte types once
+    // value_of() has it: nothing here waits for the load.
+    __device__ std::uint32_t get(bool in, int row, int col) const {
+        if constexpr (WIDE) {
+            if (!in) return 0u;
+            if constexpr (sizeof(T) == 4) return __builtin_bit_cast(std::uint32_t, base[row * step + col]);
+            else if constexpr (sizeof(T) == 2) return __builtin_bit_cast(std::uint16_t, base[row * step + col]);
+            else return base[row * step + col];
+        }
+        const int at = static_cast<int>(offset(in, row, col));
+        if constexpr (sizeof(T) == 4) return __builtin_amdgcn_raw_buffer_load_b32(rsrc, at, 0, 0);
+        else if constexpr (sizeof(T) == 1) return static_cast<std::uint8_t>(__builtin_amdgcn_raw_buffer_load_b8(rsrc, at, 0, 0));
+        else return static_cast<std::uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(rsrc, at, 0, 0));
+    }
+    static __device__ float value_of(std::uint32_t bits) {
+        return __builtin_bit_cast(float, sizeof(T) == 4 ? bits : bits << 16);
+    }
+    __device__ void put(bool in, int row, int col, float v) const {
+        const T x = static_cast<T>(v);
+        if constexpr (WIDE) {
+            if (in) base[row * step + col] = x;
+        } else {
+            const int at = static_cast<int>(offset(in, row, col));
+            if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, x), rsrc, at, 0, 0);
+            else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, x), rsrc, at, 0, 0);
+        }
+    }
+    // Four consecutive float32 elements on a 16-byte boundary.
+    __device__ f4 get4(bool in, int row, int col) const {
+        static_assert(sizeof(T) == 4 && !WIDE);
+        const auto x = __builtin_amdgcn_raw_buffer_load_b128(rsrc, static_cast<int>(offset(in, row, col)), 0, 0);
+        return __builtin_bit_cast(f4, x);
+    }
+    // Eight consecutive elements, as they lie in memory.
+    static constexpr int kWords = sizeof(T) * 8 / 4;
+    __device__ void get8(bool in, int row, int col, bool vec, std::uint32_t (&w)[kWords]) const {
+        if (!vec || WIDE) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const std::uint32_t x = get(in, row, col + i);
+                if constexpr (sizeof(T) == 4) w[i] = x;
+                else if (i % 2 == 0) w[i / 2] = x;
+                else w[i / 2] |= x << 16;
+            }
+            return;
+        }
+        const int at = static_cast<int>(offset(in, row, col));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {          // four elements at a time: their alignment is what `vec` says
+            if constexpr (sizeof(T) == 4) {
+                const auto x = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at + 16 * i, 0, 0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[4 * i + j] = x[j];
+            } else {
+                const auto x = __builtin_amdgcn_raw_buffer_load_b64(rsrc, at + 8 * i, 0, 0);
+                w[2 * i] = x[0];
+                w[2 * i + 1] = x[1];
+            }
+        }
+    }
+    // Elements 4 i .. 4 i + 3 of them.
+    static __device__ f4 four(const std::uint32_t (&w)[kWords], int i) {
+        const auto f = [&](int j) { return __builtin_bit_cast(float, w[j]); };
+        if constexpr (sizeof(T) == 4) return f4{f(4 * i), f(4 * i + 1), f(4 * i + 2), f(4 * i + 3)};
+        else return f4{lo_half(w[2 * i]), hi_half(w[2 * i]), lo_half(w[2 * i + 1]), hi_half(w[2 * i + 1])};
+    }
+};
+
+// Where a workgroup's lanes stand.
+template <int DP>
+struct Lane {
+    int tid, lane, r, g, wave, col, key_row, key_col;
+    __device__ explicit Lane(int id)
+        : tid(id), lane(tid % 64), r(lane % 16), g(lane / 16), wave(__builtin_amdgcn_readfirstlane(threadIdx.x / 64)),
+          col(16 * wave + r), key_row(tid / (DP / 8)), key_col(8 * (tid % (DP / 8))) {}
+    __device__ Lane() : Lane(static_cast<int>(threadIdx.x)) {}
+    // The same, made anew: addresses that follow from it are worked out where
+    // they are used, rather than all held in registers through a loop.
+    static __device__ Lane anew() {
+        int id = static_cast<int>(threadIdx.x);
+        asm volatile("" : "+v"(id));
+        return Lane(id);
+    }
+    // Token row e = 0..7 of a wave's columns.
+    __device__ int row(int e) const { return 16 * (e / 4) + 4 * g + e % 4; }
+};
+
+// The inputs of the tokens [start, start + width) of a chunk, loaded into
+// registers ahead of their use: a thread has eight elements of one token's
+// key and query, a wave its 16 columns of the values, every wave the gates,
+// one token a lane.
+template <typename T, int DP, bool WIDE>
+struct Ahead {
+    using In = Rows<T, WIDE>;
+    std::uint32_t k[In::kWords], q[In::kWords], v[8], g, beta, reset;
+
+    __device__ void fetch(const DeltaArgs<T>& x, std::uint32_t start, int width, std::uint32_t env, std::uint32_t h,
+                          const Lane<DP>& at) {
+        const std::uint32_t hk = h / x.group;
+        const bool in = at.key_row < width && at.key_col < static_cast<int>(x.dk_dim);
+        In(x.k.row(start, env, hk), x.k.t).get8(in, at.key_row, at.key_col, x.k.vec, k);
+        In(x.q.row(start, env, hk), x.q.t).get8(in, at.key_row, at.key_col, x.q.vec, q);
+        columns(x.v, x.dv_dim, start, width, env, h, at, v);
+        const std::size_t token = static_cast<std::size_t>(start) * x.batch + env;
+        const bool mine = at.lane < width;
+        const Rows<float, WIDE> gates(x.g + token * x.hv + h, static_cast<std::int64_t>(x.batch) * x.hv);
+        const Rows<float, WIDE> betas(x.beta + token * x.hv + h, static_cast<std::int64_t>(x.batch) * x.hv);
+        g = gates.get(mine, at.lane, 0);
+        beta = betas.get(mine, at.lane, 0);
+        reset = 0;
+        if (x.resets != nullptr) reset = Rows<std::uint8_t, WIDE>(x.resets + token, x.batch).get(mine, at.lane, 0);
+    }
+    // A wave's columns of a [tokens][value dimension] tensor.
+    static __device__ void columns(const Heads<T>& from, std::uint32_t dim, std::uint32_t start, int width,
+                                   std::uint32_t env, std::uint32_t h, const Lane<DP>& at, std::uint32_t (&to)[8]) {
+        const In rows(from.row(start, env, h), from.t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) to[e] = rows.get(at.row(e) < width && at.col < static_cast<int>(dim), at.row(e), at.col);
+    }
+    static __device__ float value(std::uint32_t bits) { return __builtin_bit_cast(float, bits); }
+    __device__ bool drop() const { return reset != 0 || value(g) < kDropBelow; }
+    // Bit t: the state is dropped before token start + t.
+    __device__ std::uint32_t drops() const { return static_cast<std::uint32_t>(__ballot(drop())); }
+};
+
 template <typename T, int DP>          // DP: head dimensions padded to 32, 64 or 128; DP / 16 waves
 struct ChunkTile {
-    static constexpr int kStride = DP + 4, kSmall = kChunk + 4;
-    static constexpr int KT = DP / 16, kWaves = DP / 16;
+    using M = typename MathOf<T>::type;
+    static constexpr int KT = DP / 16, KP = DP / 32, kWaves = DP / 16, kSmall = kChunk + 4;
 
-    alignas(16) float k[kChunk * kStride];
-    alignas(16) float q[kChunk * kStride];
+    typename M::template Tile<kChunk, DP, false> k, q;
+    typename M::template Tile<kChunk, kChunk, true> p;     // P: scale L_ij (q_i . k_j), j <= i; else 0
+    typename M::template Tile<kChunk, kChunk, true> t;     // (I + A)^-1
     alignas(16) float a[kChunk * kSmall];      // A without beta: L_ij (k_i . k_j), j < i; else 0
-    alignas(16) float p[kChunk * kSmall];      // P: scale L_ij (q_i . k_j), j <= i; else 0
-    alignas(16) float t[2][16 * 20];           // inverses of (I + A)'s diagonal tiles
     alignas(16) double G[kChunk];              // running sum of g: differences of it are taken
     alignas(16) float gamma[kChunk], decay[kChunk], beta[kChunk];
     unsigned bad;                              // tokens with a value that is not finite
 
-    // ---- states: lane (r, g4) of a wave holds S[16 i + 4 g4 + j][16 wave + r] ----
-    static __device__ void load_state(const DeltaArgs<T>& a, const float* from, std::size_t head, unsigned col, int g4,
+    // ---- states [k_dim][v_dim]: lane (r, g) of a wave holds S[16 i + 4 g + j][16 wave + r] ----
+    static __device__ void load_state(const DeltaArgs<T>& a, const float* from, std::size_t head, const Lane<DP>& at,
                                       f4 (&S)[KT]) {
+        if (from == nullptr) {
+#pragma unroll
+            for (int i = 0; i < KT; ++i) S[i] = f4{0, 0, 0, 0};
+            return;
+        }
+        const Rows<float, false> rows(from + head * a.dk_dim * a.dv_dim, a.dv_dim);
+        const bool in = at.col < static_cast<int>(a.dv_dim);
 #pragma unroll
         for (int i = 0; i < KT; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const unsigned row = 16 * i + 4 * g4 + j;
-                S[i][j] = from != nullptr && row < a.dk_dim && col < a.dv_dim
-                              ? from[(head * a.dk_dim + row) * a.dv_dim + col] : 0.0f;
+                const int row = 16 * i + 4 * at.g + j;
+                S[i][j] = rows.value_of(rows.get(in && row < static_cast<int>(a.dk_dim), row, at.col));
             }
     }
-    static __device__ void store_state(const DeltaArgs<T>& a, float* to, std::size_t head, unsigned col, int g4,
+    static __device__ void store_state(const DeltaArgs<T>& a, float* to, std::size_t head, const Lane<DP>& at,
                                        const f4 (&S)[KT]) {
+        const Rows<float, false> rows(to + head * a.dk_dim * a.dv_dim, a.dv_dim);
+        const bool in = at.col < static_cast<int>(a.dv_dim);
 #pragma unroll
         for (int i = 0; i < KT; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const unsigned row = 16 * i + 4 * g4 + j;
-                if (row < a.dk_dim && col < a.dv_dim) to[(head * a.dk_dim + row) * a.dv_dim + col] = S[i][j];
+                const int row = 16 * i + 4 * at.g + j;
+                rows.put(in && row < static_cast<int>(a.dk_dim), row, at.col, S[i][j]);
             }
     }
-    // The state before a chunk, kept for the gradient as the registers hold it.
-    static __device__ f4* saved_at(const DeltaArgs<T>& a, std::uint32_t slot, std::size_t head, int wave, int lane) {
-        const std::size_t state = static_cast<std::size_t>(slot) * a.batch * a.hv + head;
-        return reinterpret_cast<f4*>(a.saved + state * DP * DP) + static_cast<std::size_t>(wave) * KT * 64 + lane;
+
+    // The tiles' blocks above the diagonal, once.
+    __device__ void start(const Lane<DP>& at) {
+        if (at.tid == 0) bad = 0;
+        if (at.tid < 64)
+            for (int i = 0; i < 4; ++i) {
+                p.put(at.r, 16 + 4 * at.g + i, 0.0f);
+                t.put(at.r, 16 + 4 * at.g + i, 0.0f);
+            }
     }
-    static __device__ void put_saved(const DeltaArgs<T>& a, std::uint32_t slot, std::size_t head, int wave, int lane,
-                                     const f4 (&S)[KT]) {
-        f4* to = saved_at(a, slot, head, wave, lane);
+
+    // K and Q of the tokens [lo, hi) of the chunk, zeros in the other rows;
+    // bit t of the result: token t's key is not finite.
+    template <bool WIDE>
+    __device__ std::uint32_t stage_keys(const Ahead<T, DP, WIDE>& in, int lo, int hi, const Lane<DP>& at) {
+        const bool use = at.key_row >= lo && at.key_row < hi;
+        const f4 zero = {0, 0, 0, 0};
+        f4 odd = zero;
 #pragma unroll
-        for (int i = 0; i < KT; ++i) to[64 * i] = S[i];
-    }
-    static __device__ void get_saved(const DeltaArgs<T>& a, std::uint32_t slot, std::size_t head, int wave, int lane,
-                                     f4 (&S)[KT]) {
-        const f4* from = saved_at(a, slot, head, wave, lane);
-#pragma unroll
-        for (int i = 0; i < KT; ++i) S[i] = from[64 * i];
-    }
-
-    // Tokens of the chunk that starts at t0: up to the next multiple of the
-    // chunk length, the end, or the next token that drops the state.
-    static __device__ int extent(const DeltaArgs<T>& a, std::uint32_t t0, std::uint32_t env, std::uint32_t h, int lane) {
-        const std::uint32_t whole = kChunk - t0 % kChunk, left = a.steps - t0;
-        const int n = static_cast<int>(whole < left ? whole : left);
-        const bool drop = lane > 0 && lane < n && drops(a, t0 + lane, env, h);
-        const unsigned long long at = __ballot(drop);
-        return at == 0 ? n : __ffsll(static_cast<long long>(at)) - 1;
-    }
-
-    // Rows t0 .. t0 + n - 1 of K and Q, zeros below; marks keys that are not
-    // finite in `bad`.
-    __device__ void stage_keys(const DeltaArgs<T>& x, std::uint32_t t0, int n, std::uint32_t env, std::uint32_t hk,
-                               int tid) {
-        const int row = tid / (DP / 8), c = 8 * (tid % (DP / 8));
-        f4 k0 = {0, 0, 0, 0}, k1 = k0, q0 = k0, q1 = k0;
-        if (row < n && c < static_cast<int>(x.dk_dim)) {
-            const T* kp = x.k.row(t0 + row, env, hk) + c;
-            const T* qp = x.q.row(t0 + row, env, hk) + c;
-            k0 = load4(kp, x.k.vec);
-            k1 = load4(kp + 4, x.k.vec);
-            q0 = load4(qp, x.q.vec);
-            q1 = load4(qp + 4, x.q.vec);
+        for (int i = 0; i < 2; ++i) {
+            const f4 kx = use ? Rows<T, WIDE>::four(in.k, i) : zero;
+            k.put4(at.key_row, at.key_col + 4 * i, kx);
+            q.put4(at.key_row, at.key_col + 4 * i, use ? Rows<T, WIDE>::four(in.q, i) : zero);
+            odd += kx - kx;                                // 0, or NaN
         }
-        f4* kt = reinterpret_cast<f4*>(&k[row * kStride + c]);
-        f4* qt = reinterpret_cast<f4*>(&q[row * kStride + c]);
-        kt[0] = k0;
-        kt[1] = k1;
-        qt[0] = q0;
-        qt[1] = q1;
-        const f4 z = (k0 - k0) + (k1 - k1);                // 0, or NaN
-        if (!(z.x + z.y + z.z + z.w == 0.0f)) atomicOr(&bad, 1u << row);
+        return odd.x + odd.y + odd.z + odd.w == 0.0f ? 0u : 1u << at.key_row;
     }
 
-    // Gates and write strengths of the chunk's tokens (one wave); rows past
-    // the last token neither decay nor write.
-    __device__ void stage_gates(const DeltaArgs<T>& x, std::uint32_t t0, int n, std::uint32_t env, std::uint32_t h,
-                                int lane) {
-        float g = 0.0f, b = 0.0f;
-        if (lane < n) {
-            const std::size_t at = ((static_cast<std::size_t>(t0) + lane) * x.batch + env) * x.hv + h;
-            g = x.g[at];
-            b = x.beta[at];
-            if (!(fabsf(b) < INFINITY) || g != g || g == INFINITY) atomicOr(&bad, 1u << lane);
-            if (g < kDropBelow) g = 0.0f;                  // the chunk's first token: the state is dropped
-        }
+    // Gates and write strengths of the tokens [lo, hi) (one wave); other rows
+    // neither decay nor write.  The token at lo may be one that drops the
+    // state: nothing decays at it then.
+    template <bool WIDE>
+    __device__ std::uint32_t stage_gates(const Ahead<T, DP, WIDE>& in, int lo, int hi, int lane) {
+        const bool use = lane >= lo && lane < hi;
+        const float g = use && !in.drop() ? in.value(in.g) : 0.0f, b = use ? in.value(in.beta) : 0.0f;
         double sum = g;
 #pragma unroll
         for (int d = 1; d < kChunk; d *= 2) {
             const double below = __shfl_up(sum, d);
-            if (lane % kChunk >= d) sum += below;
+            if (lane >= d) sum += below;
         }
         const double end = __shfl(sum, kChunk - 1);
         if (lane < kChunk) {
@@ -119,53 +242,100 @@ struct ChunkTile {
             decay[lane] = expf(static_cast<float>(end - sum));
             beta[lane] = b;
         }
+        return fabsf(b) < INFINITY && g < INFINITY ? 0u : 1u << lane;
+    }
+    // Tokens with something that is not finite, from all waves.
+    __device__ void report(std::uint32_t bits) {
+        if (__any(bits != 0)) atomicOr(&bad, bits);
     }
 
-    // L_ij.
-    __device__ float ratio(int i, int j) const { return expf(static_cast<float>(G[i] - G[j])); }
+    // Of a wave's token rows.
+    __device__ f4 of_rows(const float* x, int m, int g) const { return *reinterpret_cast<const f4*>(x + 16 * m + 4 * g); }
 
-    // A and P: six tiles of products over the key dimension, spread over the
-    // waves; the tiles above the diagonal are not read.
-    __device__ void products(float scale, int wave, int r, int g4) {
-        for (int job = wave; job < 6; job += kWaves) {
-            const bool is_p = job >= 3;
-            const int place = job % 3, mi = place != 0 ? 16 : 0, nj = place == 2 ? 16 : 0;
-            const float* left = is_p ? q : k;
-            f4 c = {0, 0, 0, 0};
+    // L_ij.  exp2 of the rounded product is off by |x| 2^-24 of itself, which
+    // is 2^-25 of 1 at most where L <= 1.
+    __device__ float ratio(int i, int j) const {
+        return __builtin_amdgcn_exp2f(static_cast<float>(G[i] - G[j]) * 1.44269504f);
+    }
+
+    // A tile of 16x16 token pairs on or below the diagonal: place 0, 1, 2 starts
+    // at (0, 0), (16, 0), (16, 16).  `each(row, col, i, L_ij)` for the lane's four.
+    static __device__ int first_row(int place) { return place != 0 ? 16 : 0; }
+    static __device__ int first_col(int place) { return place == 2 ? 16 : 0; }
+
+    // k_i . k_j and q_i . k_j of a tile, times L_ij and zero where j is not
+    // before (not after) i; into A and P.
+    __device__ void products(int place, float scale, const Lane<DP>& at, f4& kk, f4& qk) {
+        const int mi = first_row(place), nj = first_col(place);
+        kk = qk = f4{0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < KT; ++i)
-                c = mma(along<kStride>(left, mi, 16 * i, r, g4), along<kStride>(k, nj, 16 * i, r, g4), c);
-            float* to = is_p ? p : a;
+        for (int i = 0; i < KP; ++i) {
+            const auto right = k.rows(nj, i, at.r, at.g);
+            kk = M::mul(k.rows(mi, i, at.r, at.g), right, kk);
+            qk = M::mul(q.rows(mi, i, at.r, at.g), right, qk);
+        }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = mi + 4 * g4 + i, col = nj + r;
-                float v = 0.0f;
-                if (is_p ? col <= row : col < row) v = c[i] * ratio(row, col) * (is_p ? scale : 1.0f);
-                to[row * kSmall + col] = v;
+        for (int i = 0; i < 4; ++i) {
+            const int row = mi + 4 * at.g + i, col = nj + at.r;
+            const float L = ratio(row, col);
+            kk[i] = col < row ? kk[i] * L : 0.0f;
+            qk[i] = col <= row ? qk[i] * L * scale : 0.0f;
+            a[row * kSmall + col] = kk[i];
+            p.put(row, col, qk[i]);
+        }
+    }
+
+    // (I + A)^-1 into t (one wave).  The two diagonal tiles by substitution,
+    // tile b in the lanes of rows b and b + 2 of 16, a column a lane: once an
+    // entry is known it is taken out of all below, and the lane of row m hands
+    // its A[m][i] to the others.  The block below the diagonal is
+    // -T1 (A10 T0), its factors read from where A's diagonal tiles were.
+    __device__ void invert(const Lane<DP>& at) {
+        const int b = at.g % 2, r = at.r, g = at.g;
+        float x[16], row[16];
+        const float* from = &a[(16 * b + r) * kSmall + 16 * b];
+        const float less = -beta[16 * b + r];
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const f4 w = *reinterpret_cast<const f4*>(from + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                row[i + j] = w[j] * less;
+                x[i + j] = i + j == r ? 1.0f : 0.0f;
             }
         }
-    }
-
-    // Inverse of diagonal tile b of I + A, one column a lane, by substitution.
-    __device__ void invert(int b, int r, int g4) {
-        float x[16];
+        // Two wait states between a register's write and its read by another
+        // lane, which the compiler does not see in the lines it reads below.
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float* row = &a[(16 * b + i) * kSmall + 16 * b];
-            float sum = 0.0f;
+        for (int i = 0; i < 16; i += 4) asm volatile("s_nop 1" : "+v"(row[i]), "+v"(row[i + 1]), "+v"(row[i + 2]), "+v"(row[i + 3]));
+        substitute(std::make_integer_sequence<int, 15>{}, row, x);
+        if (g < 2)
 #pragma unroll
-            for (int m = 0; m < i; ++m) sum += row[m] * x[m];
-            x[i] = (i == r ? 1.0f : 0.0f) - beta[16 * b + i] * sum;
-            if (g4 == 0) t[b][i * 20 + r] = x[i];
+            for (int i = 0; i < 16; ++i) a[(16 * b + i) * kSmall + 16 * b + r] = x[i];
+        __builtin_amdgcn_wave_barrier();       // in order within the wave
+        const f4 zero = {0, 0, 0, 0};
+        const f4 t0 = down<kSmall>(a, 0, 0, r, g), t1 = down<kSmall>(a, 16, 16, r, g);
+        const f4 w = mma(along<kSmall>(a, 16, 0, r, g) * beta[16 + r], t0, zero);
+        const f4 below = mma(along<kSmall>(a, 16, 16, r, g), w, zero);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            t.put(4 * g + i, r, t0[i]);
+            t.put(16 + 4 * g + i, 16 + r, t1[i]);
+            t.put(16 + 4 * g + i, r, -below[i]);
         }
     }
-
-    // U = (I + A)^-1 R for a wave's columns.
-    __device__ void solve(const f4 (&R)[2], f4 (&U)[2], int r, int g4) const {
-        const f4 zero = {0, 0, 0, 0};
-        U[0] = mma(along<20>(t[0], 0, 0, r, g4), R[0], zero);
-        const f4 below = mma(along<kSmall>(a, 16, 0, r, g4) * beta[16 + r], U[0], zero);
-        U[1] = mma(along<20>(t[1], 0, 0, r, g4), R[1] - below, zero);
+    // x += (row, in lane M of each 16) y.
+    template <int M1>
+    static __device__ void take_out_one(float& x, float row, float y) {
+        asm("v_fmac_f32_dpp %0, %1, %2 row_newbcast:%3 row_mask:0xf bank_mask:0xf" : "+v"(x) : "v"(row), "v"(y), "n"(M1));
+    }
+    template <int I, int... D>
+    static __device__ void take_out(std::integer_sequence<int, D...>, const float (&row)[16], float (&x)[16]) {
+        (take_out_one<I + 1 + D>(x[I + 1 + D], row[I], x[I]), ...);
+    }
+    template <int... I>
+    static __device__ void substitute(std::integer_sequence<int, I...>, const float (&row)[16], float (&x)[16]) {
+        (take_out<I>(std::make_integer_sequence<int, 15 - I>{}, row, x), ...);
     }
 };
 

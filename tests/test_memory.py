@@ -46,7 +46,7 @@ def test_delta_entries_refuse(entry):
 def test_delta_workspaces():
     L = abi.lib()
     assert L.nesle_delta_saved_floats(ctypes.byref(_delta(steps=32))) == 0
-    assert L.nesle_delta_saved_floats(ctypes.byref(_delta(steps=33, k_dim=40))) == 2 * 4 * 64 * 64
+    assert L.nesle_delta_saved_floats(ctypes.byref(_delta(steps=33, k_dim=40))) == 2 * 4 * 40 * 16
     assert L.nesle_delta_scratch_floats(ctypes.byref(_delta())) == 2 * 4 * 2 * 4 * 16
     assert L.nesle_delta_scratch_floats(ctypes.byref(_delta(k_heads=4))) == 0
 
