@@ -103,11 +103,13 @@ typedef struct nesle_delta_args {
     float* dg;
     float* dbeta;
     float* dstate;               /*           null: not wanted */
-    float* scratch;              /*           nesle_delta_scratch_floats() floats */
+    float* scratch;              /* nesle_delta_forward: nesle_delta_forward_scratch_floats() floats;
+                                    gradient: nesle_delta_scratch_floats(); unused where that is 0 */
 } nesle_delta_args;
 
-/* Floats of `saved`, and of `scratch` of the gradient. */
+/* Floats of `saved`, and of `scratch` of the forward and of the gradient. */
 uint64_t nesle_delta_saved_floats(const nesle_delta_args* args);
+uint64_t nesle_delta_forward_scratch_floats(const nesle_delta_args* args);
 uint64_t nesle_delta_scratch_floats(const nesle_delta_args* args);
 
 /* One token (steps 1) for every console; state_out may be state (in place). */

@@ -206,6 +206,7 @@ def lib():
         "nesle_qk_norm_rotate": (ctypes.c_int, [ctypes.POINTER(QkArgs), vp]),
         "nesle_qk_norm_rotate_grad": (ctypes.c_int, [ctypes.POINTER(QkArgs), vp]),
         "nesle_delta_saved_floats": (ctypes.c_uint64, [ctypes.POINTER(DeltaArgs)]),
+        "nesle_delta_forward_scratch_floats": (ctypes.c_uint64, [ctypes.POINTER(DeltaArgs)]),
         "nesle_delta_scratch_floats": (ctypes.c_uint64, [ctypes.POINTER(DeltaArgs)]),
         "nesle_delta_step": (ctypes.c_int, [ctypes.POINTER(DeltaArgs), vp]),
         "nesle_delta_forward": (ctypes.c_int, [ctypes.POINTER(DeltaArgs), vp]),

@@ -102,8 +102,8 @@ inline bool aligned16(const void* p) { return reinterpret_cast<std::uintptr_t>(p
 inline int check_delta_inputs(const char* who, const nesle_delta_args* a) {
     if (!a->q.data || !a->k.data || !a->v.data || !a->g || !a->beta) return refuse(who, "null device pointer");
     if (!aligned16(a->state) || !aligned16(a->state_out) || !aligned16(a->saved) || !aligned16(a->dstate_out) ||
-        !aligned16(a->dstate))
-        return refuse(who, "states must lie on 16-byte boundaries");
+        !aligned16(a->dstate) || !aligned16(a->scratch))
+        return refuse(who, "states and workspaces must lie on 16-byte boundaries");
     return NESLE_OK;
 }
 

@@ -23,16 +23,31 @@
 // A chunk ends early at a token that drops the state (its episode ended) and
 // before one that holds a value that is not finite, so that neither reaches a
 // token it must not (a product with a masked zero would carry NaN).
+//
+// A chunk takes its state to M S + B, with M [k_dim][k_dim] and B [k_dim][v_dim]
+// from its inputs alone.  Few heads over many tokens are cut into segments: one
+// launch finds each segment's M and B (the same walk over 2 DP columns, from
+// [0 | I], with values for the first half only), one takes the state through
+// the segments, one walks all segments from their states at once.
 #include "mem_delta_tile.h"
 
 namespace nesle::mem {
 namespace {
 
-template <typename T, int DP, bool WIDE>
-__global__ void __launch_bounds__(DP * 4, DP == 128 ? 2 : 4) delta_forward_kernel(DeltaArgs<T> a) {
+// Segments of `steps` tokens (a multiple of the chunk length).
+struct Segments {
+    std::uint32_t steps, count;
+    float* maps;           // [segment][head]: M, then B
+    float* states;         // [segment][head][k_dim][v_dim]: the state before it
+    std::uint32_t* dropped;    // [segment][head]: whether the state is dropped inside
+};
+
+// MAP: the segment's M and B; else outputs and states.
+template <typename T, int DP, bool WIDE, bool MAP>
+__global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_forward_kernel(DeltaArgs<T> a, Segments seg) {
     using Tile = ChunkTile<T, DP>;
     using M = typename Tile::M;
-    constexpr int KT = Tile::KT, KP = Tile::KP;
+    constexpr int KT = Tile::KT, KP = Tile::KP, kWaves = Tile::kWaves * (MAP ? 2 : 1);
     __shared__ Tile sh;
     const Lane<DP> first;
     const std::uint32_t env = blockIdx.x / a.hv, h = blockIdx.x % a.hv;
@@ -40,32 +55,48 @@ __global__ void __launch_bounds__(DP * 4, DP == 128 ? 2 : 4) delta_forward_kerne
     const std::int64_t out_step = static_cast<std::int64_t>(a.batch) * a.hv * a.dv_dim;
     const f4 zero = {0, 0, 0, 0};
 
+    const std::size_t slot = static_cast<std::size_t>(blockIdx.y) * gridDim.x + head;
+    const std::uint32_t begin = blockIdx.y * seg.steps;
+    const std::uint32_t end = a.steps - begin < seg.steps ? a.steps : begin + seg.steps;
+
     f4 S[KT];
-    Tile::load_state(a, a.state, head, first, S);
+    if constexpr (MAP) {
+#pragma unroll
+        for (int i = 0; i < KT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) S[i][j] = first.col - DP == 16 * i + 4 * first.g + j ? 1.0f : 0.0f;
+    } else if (seg.count > 1) {
+        Tile::load_state(a, seg.states, slot, first, S);
+    } else {
+        Tile::load_state(a, a.state, head, first, S);
+    }
     sh.start(first);
     __syncthreads();
 
     // Tokens from t0 to the next multiple of the chunk length or the end.
     const auto width = [&](std::uint32_t t0) {
-        const std::uint32_t whole = kChunk - t0 % kChunk, left = a.steps - t0;
+        const std::uint32_t whole = kChunk - t0 % kChunk, left = end - t0;
         return static_cast<int>(whole < left ? whole : left);
     };
     Ahead<T, DP, WIDE> in;
-    if (a.steps != 0) in.fetch(a, 0, width(0), env, h, first);
-    for (std::uint32_t t0 = 0; t0 < a.steps;) {
+    bool any_drop = false;
+    if (begin < end) in.template fetch<!MAP>(a, begin, width(begin), env, h, first);
+    for (std::uint32_t t0 = begin; t0 < end;) {
         const Lane<DP> at = Lane<DP>::anew();
         const int r = at.r, g = at.g;
         const bool in_col = at.col < static_cast<int>(a.dv_dim);
-        if (t0 != 0 && t0 % kChunk == 0 && a.saved != nullptr)
+        if (!MAP && t0 != 0 && t0 % kChunk == 0 && a.saved != nullptr)
             Tile::store_state(a, a.saved + (t0 / kChunk - 1) * state_size * a.batch * a.hv, head, at, S);
         const std::uint32_t drops = in.drops();
-        if (drops & 1u)
+        if (drops & 1u) {
+            any_drop = true;
 #pragma unroll
             for (int i = 0; i < KT; ++i) S[i] = zero;
+        }
         int n = drops & ~1u ? __ffs(static_cast<int>(drops & ~1u)) - 1 : width(t0);
         f4 V[2];
         for (;;) {
-            std::uint32_t odd = sh.stage_keys(in, 0, n, at);
+            std::uint32_t odd = sh.template stage_keys<!MAP>(in, 0, n, at);
             if (at.wave == 0) odd |= sh.stage_gates(in, 0, n, at.lane);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -84,16 +115,16 @@ __global__ void __launch_bounds__(DP * 4, DP == 128 ? 2 : 4) delta_forward_kerne
             __syncthreads();
         }
         const std::uint32_t next = t0 + n;
-        if (next < a.steps) in.fetch(a, next, width(next), env, h, at);
-        for (int place = at.wave; place < 3; place += Tile::kWaves) {
+        if (next < end) in.template fetch<!MAP>(a, next, width(next), env, h, at);
+        for (int place = at.wave; place < 3; place += kWaves) {
             f4 kk, qk;
-            sh.products(place, a.scale, at, kk, qk);
+            sh.template products<!MAP>(place, a.scale, at, kk, qk);
         }
         __syncthreads();
         if (at.tid == 0) sh.bad = 0;
         // A different wave each workgroup, as the waves of a compute unit's
         // workgroups share its four SIMDs by their number.
-        if (at.wave == static_cast<int>(blockIdx.x % Tile::kWaves)) sh.invert(at);
+        if (at.wave == static_cast<int>(blockIdx.x % kWaves)) sh.invert(at);
 
         // K S and Q S for this wave's columns.
         f4 ks[2] = {}, qs[2] = {};
@@ -103,7 +134,7 @@ __global__ void __launch_bounds__(DP * 4, DP == 128 ? 2 : 4) delta_forward_kerne
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 ks[m] = M::mul(sh.k.rows(16 * m, i, r, g), s, ks[m]);
-                qs[m] = M::mul(sh.q.rows(16 * m, i, r, g), s, qs[m]);
+                if constexpr (!MAP) qs[m] = M::mul(sh.q.rows(16 * m, i, r, g), s, qs[m]);
             }
         }
         f4 R[2];
@@ -118,12 +149,14 @@ __global__ void __launch_bounds__(DP * 4, DP == 128 ? 2 : 4) delta_forward_kerne
         f4 U[2], O[2];
 #pragma unroll
         for (int m = 0; m < 2; ++m) U[m] = M::mul(sh.t.rows(16 * m, 0, r, g), right, zero);
+        if constexpr (!MAP) {
         const auto u = M::full(U[0], U[1]);
 #pragma unroll
         for (int m = 0; m < 2; ++m) O[m] = M::mul(sh.p.rows(16 * m, 0, r, g), u, qs[m]);
         const Rows<T, WIDE> out(a.out + static_cast<std::int64_t>(t0) * out_step + head * a.dv_dim, out_step);
 #pragma unroll
         for (int e = 0; e < 8; ++e) out.put(in_col && at.row(e) < n, at.row(e), at.col, O[e / 4][e % 4]);
+        }
         const float last = sh.gamma[kChunk - 1];
         const auto w = M::full(U[0] * sh.of_rows(sh.decay, 0, g), U[1] * sh.of_rows(sh.decay, 1, g));
 #pragma unroll
@@ -131,19 +164,147 @@ __global__ void __launch_bounds__(DP * 4, DP == 128 ? 2 : 4) delta_forward_kerne
         t0 = next;
         __syncthreads();
     }
-    Tile::store_state(a, a.state_out, head, Lane<DP>::anew(), S);
+    const Lane<DP> at = Lane<DP>::anew();
+    const int rows = static_cast<int>(a.dk_dim), cols = static_cast<int>(a.dv_dim);
+    if constexpr (MAP) {
+        float* map = seg.maps + slot * a.dk_dim * (a.dk_dim + a.dv_dim);
+        if (at.wave < KT) Tile::store_columns(map + a.dk_dim * a.dk_dim, rows, cols, at.col, at.g, S);
+        else Tile::store_columns(map, rows, rows, at.col - DP, at.g, S);
+        if (at.tid == 0) seg.dropped[slot] = any_drop;
+    } else if (end == a.steps) {
+        Tile::store_state(a, a.state_out, head, at, S);
+    }
+}
+
+// The state before each segment, from one to the next: S <- M S + B.  A segment
+// that drops the state inside leaves B alone, whatever S held.  One workgroup
+// for 16 columns of a state, a wave for 16 of its rows: the steps are a chain,
+// so a step is kept short (one tile a wave by float32 matrix instructions, the
+// tiles exchanged through LDS) and M and B are loaded two to four steps ahead.
+template <int DP>
+__global__ void __launch_bounds__(DP * 4) delta_join_kernel(const float* state, Segments seg, int dk, int dv) {
+    constexpr int KT = DP / 16, kAhead = DP == 128 ? 2 : 4;
+    __shared__ f4 tiles[2][KT][64];
+    const int lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), col = 16 * blockIdx.y + r;
+    const std::size_t heads = gridDim.x, head = blockIdx.x, map_size = static_cast<std::size_t>(dk) * (dk + dv);
+    const auto tile = [&](const float* from) {             // rows 16 wave .., of this workgroup's columns
+        const Rows<float, false> x(from, dv);
+        f4 v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int row = 16 * wave + 4 * g + j;
+            v[j] = x.value_of(x.get(col < dv && row < dk, row, col));
+        }
+        return v;
+    };
+    f4 M[kAhead][KT], B[kAhead];
+    std::uint32_t dropped[kAhead];
+    const auto load = [&](int slot, std::uint32_t s) {
+        const float* map = seg.maps + (s * heads + head) * map_size;
+        const Rows<float, false> m(map, dk);
+#pragma unroll
+        for (int c = 0; c < KT; ++c)
+            M[slot][c] = m.get4(16 * wave + r < dk && 16 * c + 4 * g < dk, 16 * wave + r, 16 * c + 4 * g);
+        B[slot] = tile(map + static_cast<std::size_t>(dk) * dk);
+        // A vector load, counted in order with the others.
+        dropped[slot] = __builtin_amdgcn_raw_buffer_load_b32(
+            __builtin_amdgcn_make_buffer_rsrc(seg.dropped + s * heads + head, 0, 4, 0x00027000), 0, 0, 0);
+    };
+    f4 S = state == nullptr ? f4{0, 0, 0, 0} : tile(state + head * dk * dv);
+    const auto keep = [&](std::uint32_t s) {
+        const Rows<float, false> to(seg.states + (s * heads + head) * dk * dv, dv);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int row = 16 * wave + 4 * g + j;
+            to.put(col < dv && row < dk, row, col, S[j]);
+        }
+    };
+    const auto step = [&](int slot) {
+        tiles[slot % 2][wave][lane] = S;
+        __syncthreads();                                   // two buffers: the next write is a barrier later
+        f4 sum = {0, 0, 0, 0};
+        if (__builtin_amdgcn_readfirstlane(dropped[slot]) == 0)
+#pragma unroll
+            for (int c = 0; c < KT; ++c) sum = mma(M[slot][c], tiles[slot % 2][c][lane], sum);
+        S = sum + B[slot];
+    };
+    // Past the last map its loads are made again: without a condition around
+    // them they stay in flight through the steps before they are needed.
+    const std::uint32_t steps = seg.count - 1;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) load(i, min(static_cast<std::uint32_t>(i), steps - 1));
+    std::uint32_t s = 0;
+    for (; s + kAhead <= steps; s += kAhead)
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            keep(s + i);
+            step(i);
+            load(i, min(s + i + kAhead, steps - 1));
+        }
+#pragma unroll
+    for (int i = 0; i < kAhead - 1; ++i)
+        if (s + i < steps) {
+            keep(s + i);
+            step(i);
+        }
+    keep(steps);
+}
+
+// Segments for few heads over many tokens.  A walk of one chunk takes about the
+// same time whether a compute unit holds one head or two, and the three
+// launches walk every chunk twice.
+Segments segments(const nesle_delta_args& a) {
+    const std::uint64_t heads = static_cast<std::uint64_t>(a.batch) * a.v_heads;
+    const std::uint32_t chunks = (a.steps + kChunk - 1) / kChunk;
+    std::uint32_t count = 1;
+    if (chunks >= 8 && heads <= 128) {
+        count = static_cast<std::uint32_t>(512 / heads);
+        if (count > chunks / 4) count = chunks / 4;
+        if (count > 64) count = 64;
+    }
+    const std::uint32_t each = count < 2 ? chunks : (chunks + count - 1) / count;
+    Segments s{};
+    s.steps = each * kChunk;
+    s.count = chunks == 0 ? 1 : (chunks + each - 1) / each;
+    if (s.steps == 0) s.steps = kChunk;
+    return s;
+}
+
+std::uint64_t segment_floats(const nesle_delta_args& a, const Segments& s) {
+    if (s.count < 2) return 0;
+    const std::uint64_t slots = static_cast<std::uint64_t>(s.count) * a.batch * a.v_heads;
+    return slots * (static_cast<std::uint64_t>(a.k_dim) * (a.k_dim + 2 * a.v_dim) + 1);
+}
+
+template <typename T, int DP, bool WIDE>
+void launch_dim(const DeltaArgs<T>& a, const Segments& seg, hipStream_t s) {
+    const std::uint32_t heads = a.batch * a.hv;
+    if (seg.count > 1) {
+        // The last segment's M and B are not needed.
+        hipLaunchKernelGGL((delta_forward_kernel<T, DP, WIDE, true>), dim3(heads, seg.count - 1), dim3(DP * 8), 0, s, a, seg);
+        hipLaunchKernelGGL((delta_join_kernel<DP>), dim3(heads, (a.dv_dim + 15) / 16), dim3(DP * 4), 0, s, a.state, seg,
+                           static_cast<int>(a.dk_dim), static_cast<int>(a.dv_dim));
+    }
+    hipLaunchKernelGGL((delta_forward_kernel<T, DP, WIDE, false>), dim3(heads, seg.count), dim3(DP * 4), 0, s, a, seg);
 }
 
 template <typename T>
 int forward(const char* who, const nesle_delta_args& x, hipStream_t s) {
     const DeltaArgs<T> a = delta_args<T>(x);
-    const dim3 grid(a.batch * a.hv);
+    Segments seg = segments(x);
+    if (seg.count > 1) {
+        const std::size_t slots = static_cast<std::size_t>(seg.count) * a.batch * a.hv;
+        seg.maps = a.scratch;
+        seg.states = seg.maps + slots * a.dk_dim * (a.dk_dim + a.dv_dim);
+        seg.dropped = reinterpret_cast<std::uint32_t*>(seg.states + slots * a.dk_dim * a.dv_dim);
+    }
     const std::uint32_t dim = wide_rows(x) ? 0 : padded_dim(x);
     switch (dim) {
-        case 0: hipLaunchKernelGGL((delta_forward_kernel<T, 128, true>), grid, dim3(512), 0, s, a); break;
-        case 32: hipLaunchKernelGGL((delta_forward_kernel<T, 32, false>), grid, dim3(128), 0, s, a); break;
-        case 64: hipLaunchKernelGGL((delta_forward_kernel<T, 64, false>), grid, dim3(256), 0, s, a); break;
-        default: hipLaunchKernelGGL((delta_forward_kernel<T, 128, false>), grid, dim3(512), 0, s, a); break;
+        case 0: launch_dim<T, 128, true>(a, seg, s); break;
+        case 32: launch_dim<T, 32, false>(a, seg, s); break;
+        case 64: launch_dim<T, 64, false>(a, seg, s); break;
+        default: launch_dim<T, 128, false>(a, seg, s); break;
     }
     return launched(who);
 }
@@ -161,6 +322,11 @@ std::uint64_t nesle_delta_saved_floats(const nesle_delta_args* a) {
     return chunks * a->batch * a->v_heads * a->k_dim * a->v_dim;
 }
 
+std::uint64_t nesle_delta_forward_scratch_floats(const nesle_delta_args* a) {
+    if (a == nullptr || a->batch == 0 || a->v_heads == 0) return 0;
+    return segment_floats(*a, segments(*a));
+}
+
 int nesle_delta_forward(const nesle_delta_args* a, void* stream) {
     const char* who = "nesle_delta_forward";
     int rc = check_delta(who, a);
@@ -169,7 +335,7 @@ int nesle_delta_forward(const nesle_delta_args* a, void* stream) {
     if (a->steps != 0) {
         rc = check_delta_inputs(who, a);
         if (rc != NESLE_OK) return rc;
-        if (!a->out) return refuse(who, "null device pointer");
+        if (!a->out || (!a->scratch && nesle_delta_forward_scratch_floats(a) != 0)) return refuse(who, "null device pointer");
     }
     const auto s = static_cast<hipStream_t>(stream);
     return a->dtype == NESLE_MEM_F32 ? forward<float>(who, *a, s) : forward<bf16>(who, *a, s);

@@ -122,12 +122,13 @@ struct Ahead {
     using In = Rows<T, WIDE>;
     std::uint32_t k[In::kWords], q[In::kWords], v[8], g, beta, reset;
 
+    template <bool QUERIES = true>
     __device__ void fetch(const DeltaArgs<T>& x, std::uint32_t start, int width, std::uint32_t env, std::uint32_t h,
                           const Lane<DP>& at) {
         const std::uint32_t hk = h / x.group;
         const bool in = at.key_row < width && at.key_col < static_cast<int>(x.dk_dim);
         In(x.k.row(start, env, hk), x.k.t).get8(in, at.key_row, at.key_col, x.k.vec, k);
-        In(x.q.row(start, env, hk), x.q.t).get8(in, at.key_row, at.key_col, x.q.vec, q);
+        if constexpr (QUERIES) In(x.q.row(start, env, hk), x.q.t).get8(in, at.key_row, at.key_col, x.q.vec, q);
         columns(x.v, x.dv_dim, start, width, env, h, at, v);
         const std::size_t token = static_cast<std::size_t>(start) * x.batch + env;
         const bool mine = at.lane < width;
@@ -164,35 +165,41 @@ struct ChunkTile {
     alignas(16) float gamma[kChunk], decay[kChunk], beta[kChunk];
     unsigned bad;                              // tokens with a value that is not finite
 
-    // ---- states [k_dim][v_dim]: lane (r, g) of a wave holds S[16 i + 4 g + j][16 wave + r] ----
-    static __device__ void load_state(const DeltaArgs<T>& a, const float* from, std::size_t head, const Lane<DP>& at,
-                                      f4 (&S)[KT]) {
+    // ---- matrices [k_dim][cols] beside a head's keys (its state and its
+    // transition): lane (r, g) of a wave holds rows 16 i + 4 g + j of one column ----
+    static __device__ void load_columns(const float* from, int rows, int cols, int col, int g, f4 (&S)[KT]) {
         if (from == nullptr) {
 #pragma unroll
             for (int i = 0; i < KT; ++i) S[i] = f4{0, 0, 0, 0};
             return;
         }
-        const Rows<float, false> rows(from + head * a.dk_dim * a.dv_dim, a.dv_dim);
-        const bool in = at.col < static_cast<int>(a.dv_dim);
+        const Rows<float, false> x(from, cols);
 #pragma unroll
         for (int i = 0; i < KT; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int row = 16 * i + 4 * at.g + j;
-                S[i][j] = rows.value_of(rows.get(in && row < static_cast<int>(a.dk_dim), row, at.col));
+                const int row = 16 * i + 4 * g + j;
+                S[i][j] = x.value_of(x.get(col < cols && row < rows, row, col));
             }
+    }
+    static __device__ void store_columns(float* to, int rows, int cols, int col, int g, const f4 (&S)[KT]) {
+        const Rows<float, false> x(to, cols);
+#pragma unroll
+        for (int i = 0; i < KT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int row = 16 * i + 4 * g + j;
+                x.put(col < cols && row < rows, row, col, S[i][j]);
+            }
+    }
+    static __device__ void load_state(const DeltaArgs<T>& a, const float* from, std::size_t head, const Lane<DP>& at,
+                                      f4 (&S)[KT]) {
+        if (from != nullptr) from += head * a.dk_dim * a.dv_dim;
+        load_columns(from, static_cast<int>(a.dk_dim), static_cast<int>(a.dv_dim), at.col, at.g, S);
     }
     static __device__ void store_state(const DeltaArgs<T>& a, float* to, std::size_t head, const Lane<DP>& at,
                                        const f4 (&S)[KT]) {
-        const Rows<float, false> rows(to + head * a.dk_dim * a.dv_dim, a.dv_dim);
-        const bool in = at.col < static_cast<int>(a.dv_dim);
-#pragma unroll
-        for (int i = 0; i < KT; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int row = 16 * i + 4 * at.g + j;
-                rows.put(in && row < static_cast<int>(a.dk_dim), row, at.col, S[i][j]);
-            }
+        store_columns(to + head * a.dk_dim * a.dv_dim, static_cast<int>(a.dk_dim), static_cast<int>(a.dv_dim), at.col, at.g, S);
     }
 
     // The tiles' blocks above the diagonal, once.
@@ -207,8 +214,9 @@ struct ChunkTile {
 
     // K and Q of the tokens [lo, hi) of the chunk, zeros in the other rows;
     // bit t of the result: token t's key is not finite.
-    template <bool WIDE>
+    template <bool QUERIES = true, bool WIDE>
     __device__ std::uint32_t stage_keys(const Ahead<T, DP, WIDE>& in, int lo, int hi, const Lane<DP>& at) {
+        if (!QUERIES && at.key_row >= kChunk) return 0;        // more waves than the tile needs
         const bool use = at.key_row >= lo && at.key_row < hi;
         const f4 zero = {0, 0, 0, 0};
         f4 odd = zero;
@@ -216,7 +224,7 @@ struct ChunkTile {
         for (int i = 0; i < 2; ++i) {
             const f4 kx = use ? Rows<T, WIDE>::four(in.k, i) : zero;
             k.put4(at.key_row, at.key_col + 4 * i, kx);
-            q.put4(at.key_row, at.key_col + 4 * i, use ? Rows<T, WIDE>::four(in.q, i) : zero);
+            if constexpr (QUERIES) q.put4(at.key_row, at.key_col + 4 * i, use ? Rows<T, WIDE>::four(in.q, i) : zero);
             odd += kx - kx;                                // 0, or NaN
         }
         return odd.x + odd.y + odd.z + odd.w == 0.0f ? 0u : 1u << at.key_row;
@@ -265,6 +273,7 @@ struct ChunkTile {
 
     // k_i . k_j and q_i . k_j of a tile, times L_ij and zero where j is not
     // before (not after) i; into A and P.
+    template <bool QUERIES = true>
     __device__ void products(int place, float scale, const Lane<DP>& at, f4& kk, f4& qk) {
         const int mi = first_row(place), nj = first_col(place);
         kk = qk = f4{0, 0, 0, 0};
@@ -272,7 +281,7 @@ struct ChunkTile {
         for (int i = 0; i < KP; ++i) {
             const auto right = k.rows(nj, i, at.r, at.g);
             kk = M::mul(k.rows(mi, i, at.r, at.g), right, kk);
-            qk = M::mul(q.rows(mi, i, at.r, at.g), right, qk);
+            if constexpr (QUERIES) qk = M::mul(q.rows(mi, i, at.r, at.g), right, qk);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -281,7 +290,7 @@ struct ChunkTile {
             kk[i] = col < row ? kk[i] * L : 0.0f;
             qk[i] = col <= row ? qk[i] * L * scale : 0.0f;
             a[row * kSmall + col] = kk[i];
-            p.put(row, col, qk[i]);
+            if constexpr (QUERIES) p.put(row, col, qk[i]);
         }
     }
 

@@ -283,7 +283,11 @@ def _delta_forward(q, k, v, g, beta, state, resets, scale, keep: bool):
     out = _like(v)
     after = torch.empty((v.shape[1], v.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=v.device)
     a = _delta_args(q, k, v, g, beta, state, resets, scale, out.data_ptr(), after.data_ptr())
-    saved = None
+    saved = scratch = None
+    floats = abi.lib().nesle_delta_forward_scratch_floats(ctypes.byref(a))
+    if floats:
+        scratch = torch.empty(floats, dtype=torch.float32, device=v.device)
+        a.scratch = scratch.data_ptr()
     if keep:
         floats = int(abi.lib().nesle_delta_saved_floats(ctypes.byref(a)))
         if floats:

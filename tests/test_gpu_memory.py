@@ -189,6 +189,53 @@ def test_delta_offsets_past_32_bits():
     assert O.off(got[0], want[0]) <= tol(torch.bfloat16) and O.off(got[1], want[1]) <= F32
 
 
+def test_delta_gradient_with_wide_strides():
+    """Steps 2^26 elements apart: a chunk's rows span more than 2^31 bytes."""
+    say("[gpu] gated_delta wide strides, gradient")
+    far, T = (1 << 26) + 64, 34
+    buf = torch.empty((T - 1) * far + 8192, dtype=torch.bfloat16, device=dev())
+    x, resets, grads = make(T, 2, 1, 2, 32, 32, torch.bfloat16, 20)
+    at = iter((0, 512, 1024))
+
+    def move(t):
+        if t.dim() != 4 or t.shape[0] != T:
+            return t.to(dev())
+        cut = buf.as_strided(t.shape, (far, t.shape[2] * t.shape[3], t.shape[3], 1), next(at))
+        cut.copy_(t)
+        return cut.detach()
+
+    check_delta(x, resets, grads, move=move)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,resets", [((513, 1, 1, 1, 64, 64), 0.0), ((1025, 2, 1, 2, 32, 24), 0.004),
+                                          ((700, 1, 2, 2, 128, 128), 0.01), ((1500, 3, 1, 1, 16, 40), 0.5)])
+def test_delta_few_heads_over_many_tokens(shape, resets, dtype):
+    """Lengths at which the walk is cut into segments, with their gradient."""
+    say(f"[gpu] gated_delta long {shape} {dtype}")
+    check_delta(*make(*shape, dtype, seed=sum(shape), resets=resets))
+
+
+def test_delta_segments_keep_what_is_not_finite():
+    """A state of NaN, and tokens of NaN, end at the next reset also where it
+    lies inside a later segment, and not before."""
+    from nesle_amd import memory
+
+    say("[gpu] gated_delta long, not finite")
+    x, resets, _ = make(900, 2, 1, 1, 32, 32, torch.float32, 19, resets=0.0)
+    clean = O.delta(*(x[n] for n in NAMES), resets, 32 ** -0.5)[0]
+    resets[401, 0] = resets[777, 1] = True
+    x["state"][0] = float("nan")
+    x["k"][300, 1, 0, 0] = float("nan")
+    got = memory.gated_delta(*(x[n].to(dev()) for n in NAMES[:5]), state=x["state"].to(dev()), resets=resets.to(dev()))
+    out = got[0].cpu()
+    y = {n: torch.where(torch.isfinite(t), t, torch.zeros_like(t)) for n, t in x.items()}
+    want = O.delta(*(y[n] for n in NAMES), resets, 32 ** -0.5)[0]
+    assert torch.isnan(out[:401, 0]).all() and O.off(out[401:, 0], want[401:, 0]) <= F32
+    assert O.off(out[:300, 1], clean[:300, 1]) <= F32 and torch.isnan(out[300:777, 1]).all()
+    assert O.off(out[777:, 1], want[777:, 1]) <= F32 and torch.isfinite(got[1]).all()
+
+
 def test_delta_gradient_against_differences():
     """The kernel's gradient along a direction against central differences of
     the float64 definition: their own error is about h^2 = 1e-8 and 1e-16 / h =

@@ -49,6 +49,9 @@ def test_delta_workspaces():
     assert L.nesle_delta_saved_floats(ctypes.byref(_delta(steps=33, k_dim=40))) == 2 * 4 * 40 * 16
     assert L.nesle_delta_scratch_floats(ctypes.byref(_delta())) == 2 * 4 * 2 * 4 * 16
     assert L.nesle_delta_scratch_floats(ctypes.byref(_delta(k_heads=4))) == 0
+    assert L.nesle_delta_forward_scratch_floats(ctypes.byref(_delta(steps=128))) == 0
+    assert L.nesle_delta_forward_scratch_floats(ctypes.byref(_delta(steps=4096, batch=4096))) == 0
+    assert L.nesle_delta_forward_scratch_floats(ctypes.byref(_delta(steps=4096))) > 0
 
 
 @pytest.mark.parametrize("entry", ["nesle_qk_norm_rotate", "nesle_qk_norm_rotate_grad"])
