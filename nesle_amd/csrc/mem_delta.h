@@ -16,6 +16,10 @@ constexpr int kChunk = NESLE_DELTA_CHUNK;
 // half of it exp(-103.97)): the state is dropped, not multiplied by zero, and
 // every gate that is multiplied keeps a finite logarithm.
 constexpr float kDropBelow = -104.0f;
+// What a dropping token's gate counts for in the running sums: exp of any
+// difference across it is zero, and 32 of them leave a double 11 digits after
+// the point for the others.
+constexpr float kGone = -2000.0f;
 
 template <typename T>
 struct DeltaArgs {

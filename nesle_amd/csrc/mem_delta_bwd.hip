@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
     using Tile = GradTile<T, DP>;
     using M = typename Tile::M;
     using In = Rows<T, WIDE>;
-    constexpr int KT = Tile::KT, KP = Tile::KP, kWaves = Tile::kWaves, kPlaces = (3 + kWaves - 1) / kWaves;
+    constexpr int KT = Tile::KT, KP = Tile::KP, kWaves = Tile::kWaves, kPlaces = (3 + kWaves - 2) / (kWaves - 1);     // tiles of a wave
     __shared__ Tile sh;
     const Lane<DP> first;
     const std::uint32_t env = blockIdx.x / a.hv, h = blockIdx.x % a.hv, hk = h / a.group;
@@ -67,52 +67,56 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
         const Lane<DP> at = Lane<DP>::anew();
         const int r = at.r, g = at.g;
         const bool in_v = at.col < static_cast<int>(a.dv_dim), in_k = at.col < static_cast<int>(a.dk_dim);
-        // The tokens of this turn end at t1; they start at the last multiple of
-        // the chunk length, or at the last token after that which drops the
-        // state.  Row t of the tiles is token start + t: rows outside
-        // [lo, hi) are zero.
+        // A chunk from its start to t1.  Where it drops the state, gammas and
+        // decays are zero across that token, as in the forward.
         const std::uint32_t start = (t1 - 1) / kChunk * kChunk;
+        const int n = static_cast<int>(t1 - start);
         const std::uint32_t drops = in.drops();
-        const bool dropped = drops != 0;
-        const int lo = dropped ? 31 - __clz(static_cast<int>(drops)) : 0, hi = static_cast<int>(t1 - start);
-        const float* from = dropped ? nullptr : start == 0 ? a.state
-                                              : a.saved + (start / kChunk - 1) * state_size * a.batch * a.hv;
+        const float* from = (drops & 1u) ? nullptr : start == 0 ? a.state
+                                                   : a.saved + (start / kChunk - 1) * state_size * a.batch * a.hv;
         f4 S[KT];
         Tile::load_state(a, from, head, at, S);
 
-        sh.stage_keys(in, lo, hi, at);
-        if (at.wave == 0) sh.stage_gates(in, lo, hi, at.lane);
+        sh.stage_keys(in, at);
+        if (at.wave == 0) sh.stage_gates(in, n, at.lane);
         f4 V[2], dO[2];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const bool use = at.row(e) >= lo && at.row(e) < hi;
-            V[e / 4][e % 4] = use ? In::value_of(in.v[e]) : 0.0f;
-            dO[e / 4][e % 4] = use ? In::value_of(dout[e]) : 0.0f;
+            V[e / 4][e % 4] = In::value_of(in.v[e]);
+            dO[e / 4][e % 4] = In::value_of(dout[e]);
         }
 #pragma unroll
         for (int m = 0; m < 2; ++m) sh.dout.put4(at.col, 16 * m + 4 * g, dO[m]);
-        t1 = start + lo;
+        t1 = start;
         if (t1 > 0) fetch(t1, at);
         __syncthreads();
-        f4 kk[kPlaces], qk[kPlaces];
+        f4 kk[kPlaces], qk[kPlaces], ks[2] = {}, qs[2] = {}, kds[2] = {};
+        const auto read_states = [&] {
 #pragma unroll
-        for (int j = 0; j < kPlaces; ++j)
-            if (at.wave + j * kWaves < 3) sh.products(at.wave + j * kWaves, a.scale, at, kk[j], qk[j]);
-        __syncthreads();
-        if (at.wave == static_cast<int>(blockIdx.x % kWaves)) sh.invert(at);
-
-        f4 ks[2] = {}, qs[2] = {}, kds[2] = {};
+            for (int i = 0; i < KP; ++i) {
+                const auto s = M::full(S[2 * i], S[2 * i + 1]), ds = M::full(dS[2 * i], dS[2 * i + 1]);
 #pragma unroll
-        for (int i = 0; i < KP; ++i) {
-            const auto s = M::full(S[2 * i], S[2 * i + 1]), ds = M::full(dS[2 * i], dS[2 * i + 1]);
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                const auto key = sh.k.rows(16 * m, i, r, g);
-                ks[m] = M::mul(key, s, ks[m]);
-                kds[m] = M::mul(key, ds, kds[m]);
-                qs[m] = M::mul(sh.q.rows(16 * m, i, r, g), s, qs[m]);
+                for (int m = 0; m < 2; ++m) {
+                    const auto key = sh.k.rows(16 * m, i, r, g);
+                    ks[m] = M::mul(key, s, ks[m]);
+                    kds[m] = M::mul(key, ds, kds[m]);
+                    qs[m] = M::mul(sh.q.rows(16 * m, i, r, g), s, qs[m]);
+                }
             }
+        };
+        // As in the forward, the wave that inverts reads the states first and
+        // has no tile.
+        const int turn = (at.wave + static_cast<int>(blockIdx.x)) % kWaves;
+        if (turn == 0 || turn > 3) {
+            read_states();
+        } else {
+#pragma unroll
+            for (int j = 0; j < kPlaces; ++j)
+                if (turn - 1 + j * (kWaves - 1) < 3) sh.products(turn - 1 + j * (kWaves - 1), a.scale, at, kk[j], qk[j]);
         }
+        __syncthreads();
+        if (turn == 0) sh.invert(at);
+        else if (turn <= 3) read_states();
         f4 Y[2], gam[2], dec[2], beta[2];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
@@ -139,9 +143,7 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
             sh.dr.put4(at.col, 16 * m + 4 * g, dR[m]);
         }
         const In dv(a.dv + static_cast<std::int64_t>(start) * v_step + head * a.dv_dim, v_step);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            dv.put(in_v && at.row(e) >= lo && at.row(e) < hi, at.row(e), at.col, beta[e / 4][e % 4] * dR[e / 4][e % 4]);
+        put_columns(dv, in_v, n, at, [&](int e) { return beta[e / 4][e % 4] * dR[e / 4][e % 4]; });
 
         // Sums over the value dimension of dbeta and the gates, this wave's share.
         const float last = sh.gamma[kChunk - 1];
@@ -175,7 +177,7 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
             const auto held = M::full(-X[0], -X[1]);
 #pragma unroll
             for (int i = 0; i < KT; ++i) {
-                before[i] = M::mul(sh.q.cols(0, 16 * i, r, g), read, dS[i] * last);
+                before[i] = M::mul(sh.q.cols(0, 16 * i, r, g), read, drops != 0 ? zero : dS[i] * last);
                 before[i] = M::mul(sh.k.cols(0, 16 * i, r, g), held, before[i]);
             }
         }
@@ -184,8 +186,8 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
         // dP and dA by tiles; P's space becomes M1 and the inverse's M2.
 #pragma unroll
         for (int j = 0; j < kPlaces; ++j) {
-            const int place = at.wave + j * kWaves;
-            if (place >= 3) break;
+            const int place = turn - 1 + j * (kWaves - 1);
+            if (place < 0 || place >= 3) break;
             const int mi = Tile::first_row(place), nj = Tile::first_col(place);
             f4 dP = zero, dA = zero;
 #pragma unroll
@@ -255,22 +257,14 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
         if (a.group == 1) {
             const std::int64_t step = static_cast<std::int64_t>(a.batch) * a.hk * a.dk_dim;
             const In dq(a.dq + (token * a.hk + hk) * a.dk_dim, step), dk(a.dk + (token * a.hk + hk) * a.dk_dim, step);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const bool mine = in_k && at.row(e) >= lo && at.row(e) < hi;
-                dq.put(mine, at.row(e), at.col, dQ[e / 4][e % 4]);
-                dk.put(mine, at.row(e), at.col, dK[e / 4][e % 4]);
-            }
+            put_columns(dq, in_k, n, at, [&](int e) { return dQ[e / 4][e % 4]; });
+            put_columns(dk, in_k, n, at, [&](int e) { return dK[e / 4][e % 4]; });
         } else {            // one share a value head, added up afterwards
             const std::int64_t step = static_cast<std::int64_t>(a.batch) * a.hv * a.dk_dim;
             float* share = a.scratch + (token * a.hv + h) * a.dk_dim;
             const Rows<float, WIDE> dq(share, step), dk(share + a.steps * step, step);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const bool mine = in_k && at.row(e) >= lo && at.row(e) < hi;
-                dq.put(mine, at.row(e), at.col, dQ[e / 4][e % 4]);
-                dk.put(mine, at.row(e), at.col, dK[e / 4][e % 4]);
-            }
+            put_columns(dq, in_k, n, at, [&](int e) { return dQ[e / 4][e % 4]; });
+            put_columns(dk, in_k, n, at, [&](int e) { return dK[e / 4][e % 4]; });
         }
         if (at.wave == 0) {            // one token a lane
             const int t = at.lane % kChunk, i = t % 16;
@@ -291,14 +285,14 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
             }
             to_t = __shfl_up(to_t, 1);
             dg += from_t + (t > 0 ? to_t : 0.0f);
-            if (at.lane >= lo && at.lane < hi) {
+            if (at.lane < n) {
                 const std::size_t to = ((static_cast<std::size_t>(start) + t) * a.batch + env) * a.hv + h;
                 a.dbeta[to] = db;
-                a.dg[to] = dropped && t == lo ? 0.0f : dg;
+                a.dg[to] = drops >> t & 1u ? 0.0f : dg;
             }
         }
 #pragma unroll
-        for (int i = 0; i < KT; ++i) dS[i] = dropped ? zero : before[i];
+        for (int i = 0; i < KT; ++i) dS[i] = (drops & 1u) ? zero : before[i];
         __syncthreads();
     }
     if (a.dstate != nullptr) Tile::store_state(a, a.dstate, head, Lane<DP>::anew(), dS);

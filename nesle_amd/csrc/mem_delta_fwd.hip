@@ -20,9 +20,11 @@
 // All products keep float32 precision: the state and the gates' gradients are
 // float32 results whatever the inputs' type.
 //
-// A chunk ends early at a token that drops the state (its episode ended) and
-// before one that holds a value that is not finite, so that neither reaches a
-// token it must not (a product with a masked zero would carry NaN).
+// A token that drops the state counts as a gate that lets nothing through: L and
+// gamma across it are zero.  A product with a masked zero would still carry NaN,
+// so where a key, a value, a gate or (with a drop in the chunk) the state is
+// not finite, the chunk is cut before that token and at the drops: nothing of it
+// reaches a token it must not.
 //
 // A chunk takes its state to M S + B, with M [k_dim][k_dim] and B [k_dim][v_dim]
 // from its inputs alone.  Few heads over many tokens are cut into segments: one
@@ -88,55 +90,64 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_f
         if (!MAP && t0 != 0 && t0 % kChunk == 0 && a.saved != nullptr)
             Tile::store_state(a, a.saved + (t0 / kChunk - 1) * state_size * a.batch * a.hv, head, at, S);
         const std::uint32_t drops = in.drops();
-        if (drops & 1u) {
-            any_drop = true;
+        if (drops & 1u)
 #pragma unroll
             for (int i = 0; i < KT; ++i) S[i] = zero;
-        }
-        int n = drops & ~1u ? __ffs(static_cast<int>(drops & ~1u)) - 1 : width(t0);
-        f4 V[2];
+        int n = width(t0);
+        const std::uint32_t inside = drops & ~1u;
+        any_drop |= drops != 0;
         for (;;) {
-            std::uint32_t odd = sh.template stage_keys<!MAP>(in, 0, n, at);
-            if (at.wave == 0) odd |= sh.stage_gates(in, 0, n, at.lane);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float x = at.row(e) < n ? Rows<T, WIDE>::value_of(in.v[e]) : 0.0f;
-                if (!(fabsf(x) < INFINITY)) odd |= 1u << at.row(e);
-                V[e / 4][e % 4] = x;
-            }
+            sh.template stage_keys<!MAP>(in, at);
+            std::uint32_t odd = in.odd(at);
+            if (at.wave == 0) odd |= sh.stage_gates(in, n, at.lane);
+            if (inside != 0 && !Tile::finite(S)) odd |= inside;
             sh.report(odd);
             __syncthreads();
-            const unsigned bad = __builtin_amdgcn_readfirstlane(sh.bad);
+            const std::uint32_t bad = __builtin_amdgcn_readfirstlane(sh.bad) & ((n < 32 ? 1u << n : 0u) - 1u);
             if (bad == 0 || n == 1) break;
-            // Rare: stage again, up to the first such token, or it alone.
-            n = (bad & 1u) ? 1 : __ffs(static_cast<int>(bad)) - 1;
+            // Rare: stage again, up to the first such token or drop, or a first
+            // such token alone; what is left is the next turn's.
+            n = (bad & 1u) ? 1 : min(n, __ffs(static_cast<int>(bad | inside)) - 1);
+            in.cut(n, at);
             __syncthreads();
             if (at.tid == 0) sh.bad = 0;
             __syncthreads();
         }
+        f4 V[2];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) V[e / 4][e % 4] = Rows<T, WIDE>::value_of(in.v[e]);
         const std::uint32_t next = t0 + n;
         if (next < end) in.template fetch<!MAP>(a, next, width(next), env, h, at);
-        for (int place = at.wave; place < 3; place += kWaves) {
-            f4 kk, qk;
-            sh.template products<!MAP>(place, a.scale, at, kk, qk);
+        // K S and Q S for this wave's columns.
+        f4 ks[2] = {}, qs[2] = {};
+        const auto read_state = [&] {
+#pragma unroll
+            for (int i = 0; i < KP; ++i) {
+                const auto s = M::full(S[2 * i], S[2 * i + 1]);
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    ks[m] = M::mul(sh.k.rows(16 * m, i, r, g), s, ks[m]);
+                    if constexpr (!MAP) qs[m] = M::mul(sh.q.rows(16 * m, i, r, g), s, qs[m]);
+                }
+            }
+        };
+        // The inverse takes one wave as long as the rest of this part takes the
+        // others: that wave has no tile of A and P, and reads the state first.
+        // Another wave each workgroup, as the waves of a compute unit's
+        // workgroups share its four SIMDs by their number.
+        const int turn = (at.wave + static_cast<int>(blockIdx.x)) % kWaves;
+        if (turn == 0 || turn > 3) {
+            read_state();
+        } else {
+            for (int place = turn - 1; place < 3; place += kWaves - 1) {
+                f4 kk, qk;
+                sh.template products<!MAP>(place, a.scale, at, kk, qk);
+            }
         }
         __syncthreads();
         if (at.tid == 0) sh.bad = 0;
-        // A different wave each workgroup, as the waves of a compute unit's
-        // workgroups share its four SIMDs by their number.
-        if (at.wave == static_cast<int>(blockIdx.x % kWaves)) sh.invert(at);
-
-        // K S and Q S for this wave's columns.
-        f4 ks[2] = {}, qs[2] = {};
-#pragma unroll
-        for (int i = 0; i < KP; ++i) {
-            const auto s = M::full(S[2 * i], S[2 * i + 1]);
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                ks[m] = M::mul(sh.k.rows(16 * m, i, r, g), s, ks[m]);
-                if constexpr (!MAP) qs[m] = M::mul(sh.q.rows(16 * m, i, r, g), s, qs[m]);
-            }
-        }
+        if (turn == 0) sh.invert(at);
+        else if (turn <= 3) read_state();
         f4 R[2];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
@@ -150,12 +161,11 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_f
 #pragma unroll
         for (int m = 0; m < 2; ++m) U[m] = M::mul(sh.t.rows(16 * m, 0, r, g), right, zero);
         if constexpr (!MAP) {
-        const auto u = M::full(U[0], U[1]);
+            const auto u = M::full(U[0], U[1]);
 #pragma unroll
-        for (int m = 0; m < 2; ++m) O[m] = M::mul(sh.p.rows(16 * m, 0, r, g), u, qs[m]);
-        const Rows<T, WIDE> out(a.out + static_cast<std::int64_t>(t0) * out_step + head * a.dv_dim, out_step);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) out.put(in_col && at.row(e) < n, at.row(e), at.col, O[e / 4][e % 4]);
+            for (int m = 0; m < 2; ++m) O[m] = M::mul(sh.p.rows(16 * m, 0, r, g), u, qs[m]);
+            const Rows<T, WIDE> out(a.out + static_cast<std::int64_t>(t0) * out_step + head * a.dv_dim, out_step);
+            put_columns(out, in_col, n, at, [&](int e) { return O[e / 4][e % 4]; });
         }
         const float last = sh.gamma[kChunk - 1];
         const auto w = M::full(U[0] * sh.of_rows(sh.decay, 0, g), U[1] * sh.of_rows(sh.decay, 1, g));

@@ -34,6 +34,11 @@ struct F32Math {
         alignas(16) float d[ROWS * kRow];
         __device__ void put(int row, int col, float v) { d[row * kRow + col] = v; }
         __device__ void put4(int row, int col, f4 v) { *reinterpret_cast<f4*>(&d[row * kRow + col]) = v; }
+        // Eight columns as they lie in memory.
+        __device__ void put8(int row, int col, const std::uint32_t (&w)[8]) {
+            *reinterpret_cast<u4*>(&d[row * kRow + col]) = u4{w[0], w[1], w[2], w[3]};
+            *reinterpret_cast<u4*>(&d[row * kRow + col + 4]) = u4{w[4], w[5], w[6], w[7]};
+        }
         // Operand of the 16 rows from row0 over the inner columns 32 p ...
         __device__ Op rows(int row0, int p, int r, int g) const {
             const float* x = &d[(row0 + r) * kRow + 32 * p + 4 * g];
@@ -132,6 +137,11 @@ struct SplitMath {
                 *reinterpret_cast<u2*>(to + kPlane) = m;
                 *reinterpret_cast<u2*>(to + 2 * kPlane) = l;
             }
+        }
+        __device__ void put8(int row, int col, const std::uint32_t (&w)[4]) {
+            static_assert(!FULL);
+            *reinterpret_cast<u2*>(&d[row * kRow + place_of(col)]) = u2{w[0], w[1]};
+            *reinterpret_cast<u2*>(&d[row * kRow + place_of(col + 4)]) = u2{w[2], w[3]};
         }
         __device__ auto rows(int row0, int p, int r, int g) const {
             const auto at = [&](int plane) { return *reinterpret_cast<const u4*>(&d[plane * kPlane + (row0 + r) * kRow + 32 * p + 8 * g]); };

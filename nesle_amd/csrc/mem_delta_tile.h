@@ -40,6 +40,18 @@ struct Rows {
         else if constexpr (sizeof(T) == 1) return static_cast<std::uint8_t>(__builtin_amdgcn_raw_buffer_load_b8(rsrc, at, 0, 0));
         else return static_cast<std::uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(rsrc, at, 0, 0));
     }
+    // The same at a byte offset already made, plus a scalar one (from 0 to
+    // kRange, so that an offset outside stays outside).
+    __device__ std::uint32_t get_at(std::uint32_t at, std::uint32_t plus) const {
+        const int v = static_cast<int>(at), s = static_cast<int>(plus);
+        if constexpr (sizeof(T) == 4) return __builtin_amdgcn_raw_buffer_load_b32(rsrc, v, s, 0);
+        else return static_cast<std::uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(rsrc, v, s, 0));
+    }
+    __device__ void put_at(std::uint32_t at, std::uint32_t plus, float x) const {
+        const int v = static_cast<int>(at), s = static_cast<int>(plus);
+        if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, static_cast<T>(x)), rsrc, v, s, 0);
+        else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, static_cast<T>(x)), rsrc, v, s, 0);
+    }
     static __device__ float value_of(std::uint32_t bits) {
         return __builtin_bit_cast(float, sizeof(T) == 4 ? bits : bits << 16);
     }
@@ -85,12 +97,6 @@ struct Rows {
                 w[2 * i + 1] = x[1];
             }
         }
-    }
-    // Elements 4 i .. 4 i + 3 of them.
-    static __device__ f4 four(const std::uint32_t (&w)[kWords], int i) {
-        const auto f = [&](int j) { return __builtin_bit_cast(float, w[j]); };
-        if constexpr (sizeof(T) == 4) return f4{f(4 * i), f(4 * i + 1), f(4 * i + 2), f(4 * i + 3)};
-        else return f4{lo_half(w[2 * i]), hi_half(w[2 * i]), lo_half(w[2 * i + 1]), hi_half(w[2 * i + 1])};
     }
 };
 
@@ -143,14 +149,63 @@ struct Ahead {
     static __device__ void columns(const Heads<T>& from, std::uint32_t dim, std::uint32_t start, int width,
                                    std::uint32_t env, std::uint32_t h, const Lane<DP>& at, std::uint32_t (&to)[8]) {
         const In rows(from.row(start, env, h), from.t);
+        if (!WIDE && width == kChunk) {
+            const std::uint32_t base = rows.offset(at.col < static_cast<int>(dim), 4 * at.g, at.col);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) to[e] = rows.get_at(base, (16 * (e / 4) + e % 4) * static_cast<std::uint32_t>(rows.step) * sizeof(T));
+            return;
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) to[e] = rows.get(at.row(e) < width && at.col < static_cast<int>(dim), at.row(e), at.col);
+    }
+    // Zeros in the rows from n on.
+    __device__ void cut(int n, const Lane<DP>& at) {
+        const bool mine = at.key_row < n;
+#pragma unroll
+        for (int i = 0; i < In::kWords; ++i) {
+            k[i] = mine ? k[i] : 0;
+            q[i] = mine ? q[i] : 0;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = at.row(e) < n ? v[e] : 0;
+    }
+    // Tokens whose key or value holds something that is not finite.
+    __device__ std::uint32_t odd(const Lane<DP>& at) const {
+        using s2 = unsigned short __attribute__((ext_vector_type(2)));
+        constexpr std::uint32_t kInf = sizeof(T) == 4 ? 0x7f800000u : 0x7f80u, kSize = sizeof(T) == 4 ? 0x7fffffffu : 0x7fffu;
+        std::uint32_t most_v = 0, most_k = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most_v = max(most_v, v[e] & kSize);
+#pragma unroll
+        for (int i = 0; i < In::kWords; ++i)
+            if constexpr (sizeof(T) == 4) most_k = max(most_k, k[i] & kSize);
+            else most_k = __builtin_bit_cast(std::uint32_t, __builtin_elementwise_max(
+                              __builtin_bit_cast(s2, most_k), __builtin_bit_cast(s2, k[i] & 0x7fff7fffu)));
+        if constexpr (sizeof(T) == 2) most_k = max(most_k >> 16, most_k & 0xffffu);
+        if (!__any(max(most_v, most_k) >= kInf)) return 0;
+        std::uint32_t tokens = most_k >= kInf ? 1u << at.key_row : 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) tokens |= (v[e] & kSize) >= kInf ? 1u << at.row(e) : 0;
+        return tokens;
     }
     static __device__ float value(std::uint32_t bits) { return __builtin_bit_cast(float, bits); }
     __device__ bool drop() const { return reset != 0 || value(g) < kDropBelow; }
     // Bit t: the state is dropped before token start + t.
     __device__ std::uint32_t drops() const { return static_cast<std::uint32_t>(__ballot(drop())); }
 };
+
+// The first n rows of a wave's columns of a [tokens][dim] tensor.
+template <int DP, typename T, bool WIDE, typename F>
+__device__ void put_columns(const Rows<T, WIDE>& to, bool in, int n, const Lane<DP>& at, F value) {
+    if (!WIDE && n == kChunk) {
+        const std::uint32_t base = to.offset(in, 4 * at.g, at.col);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) to.put_at(base, (16 * (e / 4) + e % 4) * static_cast<std::uint32_t>(to.step) * sizeof(T), value(e));
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) to.put(in && at.row(e) < n, at.row(e), at.col, value(e));
+}
 
 template <typename T, int DP>          // DP: head dimensions padded to 32, 64 or 128; DP / 16 waves
 struct ChunkTile {
@@ -202,6 +257,13 @@ struct ChunkTile {
         store_columns(to + head * a.dk_dim * a.dv_dim, static_cast<int>(a.dk_dim), static_cast<int>(a.dv_dim), at.col, at.g, S);
     }
 
+    static __device__ bool finite(const f4 (&S)[KT]) {
+        f4 none = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < KT; ++i) none += S[i] - S[i];      // 0, or NaN
+        return none.x + none.y + none.z + none.w == 0.0f;
+    }
+
     // The tiles' blocks above the diagonal, once.
     __device__ void start(const Lane<DP>& at) {
         if (at.tid == 0) bad = 0;
@@ -212,31 +274,20 @@ struct ChunkTile {
             }
     }
 
-    // K and Q of the tokens [lo, hi) of the chunk, zeros in the other rows;
-    // bit t of the result: token t's key is not finite.
+    // K and Q.
     template <bool QUERIES = true, bool WIDE>
-    __device__ std::uint32_t stage_keys(const Ahead<T, DP, WIDE>& in, int lo, int hi, const Lane<DP>& at) {
-        if (!QUERIES && at.key_row >= kChunk) return 0;        // more waves than the tile needs
-        const bool use = at.key_row >= lo && at.key_row < hi;
-        const f4 zero = {0, 0, 0, 0};
-        f4 odd = zero;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const f4 kx = use ? Rows<T, WIDE>::four(in.k, i) : zero;
-            k.put4(at.key_row, at.key_col + 4 * i, kx);
-            if constexpr (QUERIES) q.put4(at.key_row, at.key_col + 4 * i, use ? Rows<T, WIDE>::four(in.q, i) : zero);
-            odd += kx - kx;                                // 0, or NaN
-        }
-        return odd.x + odd.y + odd.z + odd.w == 0.0f ? 0u : 1u << at.key_row;
+    __device__ void stage_keys(const Ahead<T, DP, WIDE>& in, const Lane<DP>& at) {
+        if (!QUERIES && at.key_row >= kChunk) return;          // more waves than the tile needs
+        k.put8(at.key_row, at.key_col, in.k);
+        if constexpr (QUERIES) q.put8(at.key_row, at.key_col, in.q);
     }
 
-    // Gates and write strengths of the tokens [lo, hi) (one wave); other rows
-    // neither decay nor write.  The token at lo may be one that drops the
-    // state: nothing decays at it then.
+    // Gates and write strengths of the tokens below n (one wave); other rows
+    // neither decay nor write.
     template <bool WIDE>
-    __device__ std::uint32_t stage_gates(const Ahead<T, DP, WIDE>& in, int lo, int hi, int lane) {
-        const bool use = lane >= lo && lane < hi;
-        const float g = use && !in.drop() ? in.value(in.g) : 0.0f, b = use ? in.value(in.beta) : 0.0f;
+    __device__ std::uint32_t stage_gates(const Ahead<T, DP, WIDE>& in, int n, int lane) {
+        const bool use = lane < n;
+        const float g = !use ? 0.0f : in.drop() ? kGone : in.value(in.g), b = use ? in.value(in.beta) : 0.0f;
         double sum = g;
 #pragma unroll
         for (int d = 1; d < kChunk; d *= 2) {
