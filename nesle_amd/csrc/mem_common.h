@@ -39,6 +39,15 @@ __device__ inline f4 load4(const bf16* p, bool vec) {
     }
     return f4{static_cast<float>(p[0]), static_cast<float>(p[1]), static_cast<float>(p[2]), static_cast<float>(p[3])};
 }
+// Eight consecutive elements of aligned ones.
+__device__ inline void load8(const bf16* p, f4& a, f4& b) {
+    const u4 w = *reinterpret_cast<const u4*>(p);
+    a = f4{lo_half(w.x), hi_half(w.x), lo_half(w.y), hi_half(w.y)};
+    b = f4{lo_half(w.z), hi_half(w.z), lo_half(w.w), hi_half(w.w)};
+}
+__device__ inline void store8(bf16* p, f4 a, f4 b) {
+    *reinterpret_cast<u4*>(p) = u4{pack_bf16(a.x, a.y), pack_bf16(a.z, a.w), pack_bf16(b.x, b.y), pack_bf16(b.z, b.w)};
+}
 __device__ inline void store4(float* p, f4 v) { *reinterpret_cast<f4*>(p) = v; }
 __device__ inline void store4(bf16* p, f4 v) {
     *reinterpret_cast<u2*>(p) = u2{pack_bf16(v.x, v.y), pack_bf16(v.z, v.w)};
@@ -50,7 +59,7 @@ template <typename T>
 struct Heads {
     const T* data;
     std::int64_t t, n, h;
-    bool vec;
+    bool vec, wide;      // wide: of eight
     __device__ const T* row(std::int64_t step, std::int64_t env, std::int64_t head) const {
         return data + step * t + env * n + head * h;
     }
@@ -58,10 +67,13 @@ struct Heads {
 
 template <typename T>
 Heads<T> heads(const nesle_heads& x) {
-    const std::uintptr_t group = 4 * sizeof(T);
-    const auto whole = [&](std::int64_t s) { return (s * static_cast<std::int64_t>(sizeof(T))) % static_cast<std::int64_t>(group) == 0; };
-    return {static_cast<const T*>(x.data), x.stride_t, x.stride_n, x.stride_h,
-            reinterpret_cast<std::uintptr_t>(x.data) % group == 0 && whole(x.stride_t) && whole(x.stride_n) && whole(x.stride_h)};
+    const auto aligned = [&](std::int64_t elements) {
+        const std::int64_t bytes = elements * static_cast<std::int64_t>(sizeof(T));
+        const auto whole = [&](std::int64_t stride) { return stride * static_cast<std::int64_t>(sizeof(T)) % bytes == 0; };
+        return reinterpret_cast<std::uintptr_t>(x.data) % static_cast<std::uintptr_t>(bytes) == 0 && whole(x.stride_t) &&
+               whole(x.stride_n) && whole(x.stride_h);
+    };
+    return {static_cast<const T*>(x.data), x.stride_t, x.stride_n, x.stride_h, aligned(4), aligned(8)};
 }
 
 inline int refuse(const char* who, const std::string& why) {

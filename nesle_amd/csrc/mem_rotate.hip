@@ -1,12 +1,13 @@
 // Norms of queries and keys for each head with the position rotation, and the
 // gradient (include/nesle_memory.h has the formulas).
 //
-// One pass: a group of lanes holds one head in registers, eight elements a
-// lane, so the sum of squares is a few lane exchanges and every element is
-// read and written once.  A lane's eight elements are four from the first
-// half of the rotated part and the four they are paired with in the second
-// half (two loads), so that a pair never crosses lanes in either layout;
-// lanes past the rotated part hold eight consecutive ones.
+// One pass: a group of lanes holds one head in registers, so the sum of squares
+// is a few lane exchanges and every element is read and written once.  A lane's
+// elements are PAIRS from the first half of the rotated part and the PAIRS they
+// are paired with in the second half, so that a pair never crosses lanes in
+// either layout; lanes past the rotated part hold 2 PAIRS consecutive ones.
+// PAIRS is what a 16-byte load holds, or four where the sizes or addresses do
+// not allow eight bfloat16.
 //
 // Bound by memory: about 10 operations an element.
 #include "mem_common.h"
@@ -15,9 +16,23 @@ namespace nesle::mem {
 namespace {
 
 constexpr unsigned kThreads = 256;
+// Heads a thread works on at once: their loads are in flight together, and
+// heads of one row share its position, cosines and sines.  One where the rows
+// do not fill the card: latency counts there.
+constexpr unsigned kTogether = 4, kGradTogether = 2;
 // Workgroups of the gradient with weights: each adds up its rows' share of
 // the weights' gradient, and one more launch adds the workgroups' in order.
-constexpr unsigned kGradBlocks = 1024;
+constexpr unsigned kGradBlocks = 2048;
+
+// x / d for x < 2^16 (d as it is) or x < 2 d (d of 2^15 or more).
+struct Divide {
+    std::uint32_t d, magic;
+    Divide(std::uint32_t by = 1) : d(by), magic(by > 1 ? static_cast<std::uint32_t>((0x100000000ull + by - 1) / by) : 0) {}
+    __device__ std::uint32_t operator()(std::uint32_t x) const {
+        if (d >= (1u << 15)) return x >= d ? 1u : 0u;
+        return d == 1 ? x : __umulhi(x, magic);
+    }
+};
 
 template <typename T>
 struct QkArgs {
@@ -27,49 +42,158 @@ struct QkArgs {
     const float* table;
     T *q_out, *k_out;        // forward: outputs; gradient: dq, dk
     float* partials;         // [blocks][2][dim]
-    std::uint32_t batch, hq, hk, dim, rotated, table_rows, lanes;   // lanes of one head: a power of two
+    Divide batch, per_row;   // rows of a step, heads of a row
+    std::uint32_t hq, hk, dim, rotated, table_rows, lanes;   // lanes of one head: a power of two
     std::uint64_t groups;    // heads of all rows
     float inv_count, eps;
     bool interleaved;
 };
 
-// The two element offsets of lane j's groups of four.
-template <typename T>
+// The two element offsets of lane j's groups.
+template <int PAIRS, typename T>
 __device__ void places(const QkArgs<T>& a, unsigned j, unsigned& first, unsigned& second) {
-    if (8 * j >= a.rotated || a.interleaved) {
-        first = 8 * j;
-        second = first + 4;
+    if (2 * PAIRS * j >= a.rotated || a.interleaved) {
+        first = 2 * PAIRS * j;
+        second = first + PAIRS;
     } else {
-        first = 4 * j;
+        first = PAIRS * j;
         second = a.rotated / 2 + first;
     }
 }
 
-// Cosines and sines of a lane's four pairs.
-template <typename T>
-__device__ void turns(const QkArgs<T>& a, std::uint64_t row, unsigned j, f4& c, f4& s) {
-    const std::int32_t p = a.positions[row];
-    if (p < 0 || static_cast<std::uint32_t>(p) >= a.table_rows) {
-        c = s = f4{NAN, NAN, NAN, NAN};
-        return;
+// A lane's elements of a head, or the angles of its pairs.
+template <int PAIRS>
+struct Part {
+    static constexpr int N = PAIRS / 4;
+    f4 a[N], b[N];
+    __device__ void clear() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) a[i] = b[i] = f4{0, 0, 0, 0};
     }
-    const float* t = a.table + static_cast<std::size_t>(p) * a.rotated + 4 * j;
-    c = *reinterpret_cast<const f4*>(t);
-    s = *reinterpret_cast<const f4*>(t + a.rotated / 2);
-}
+    template <typename T>
+    __device__ void load(const T* p, unsigned first, unsigned second, bool vec) {
+        if constexpr (PAIRS == 8) {
+            load8(p + first, a[0], a[1]);
+            load8(p + second, b[0], b[1]);
+        } else {
+            a[0] = load4(p + first, vec);
+            b[0] = load4(p + second, vec);
+        }
+    }
+    __device__ void load_floats(const float* p, unsigned first, unsigned second) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            a[i] = load4(p + first + 4 * i, true);
+            b[i] = load4(p + second + 4 * i, true);
+        }
+    }
+    template <typename T>
+    __device__ void store(T* p, unsigned first, unsigned second) const {
+        if constexpr (PAIRS == 8) {
+            store8(p + first, a[0], a[1]);
+            store8(p + second, b[0], b[1]);
+        } else {
+            store4(p + first, a[0]);
+            store4(p + second, b[0]);
+        }
+    }
+    __device__ float dot(const Part& o) const {
+        f4 v = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < N; ++i) v += a[i] * o.a[i] + b[i] * o.b[i];
+        return v.x + v.y + v.z + v.w;
+    }
+    __device__ void scale(float v) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            a[i] *= v;
+            b[i] *= v;
+        }
+    }
+    __device__ void scale(const Part& o) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            a[i] *= o.a[i];
+            b[i] *= o.b[i];
+        }
+    }
+    // Turn by the angles whose cosines are in t.a and sines in t.b, or back.
+    __device__ void turn(const Part& t, bool back, bool interleaved) {
+        if (interleaved) {
+            const auto pair = [&](float& x, float& y, int k) {
+                const float c = t.a[k / 4][k % 4], s = back ? -t.b[k / 4][k % 4] : t.b[k / 4][k % 4];
+                const float u = x * c - y * s;
+                y = x * s + y * c;
+                x = u;
+            };
+#pragma unroll
+            for (int k = 0; k < PAIRS / 2; ++k) {
+                float x = a[k / 2][2 * (k % 2)], y = a[k / 2][2 * (k % 2) + 1];
+                pair(x, y, k);
+                a[k / 2][2 * (k % 2)] = x;
+                a[k / 2][2 * (k % 2) + 1] = y;
+                x = b[k / 2][2 * (k % 2)], y = b[k / 2][2 * (k % 2) + 1];
+                pair(x, y, PAIRS / 2 + k);
+                b[k / 2][2 * (k % 2)] = x;
+                b[k / 2][2 * (k % 2) + 1] = y;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const f4 s = back ? -t.b[i] : t.b[i], u = a[i] * t.a[i] - b[i] * s;
+                b[i] = a[i] * s + b[i] * t.a[i];
+                a[i] = u;
+            }
+        }
+    }
+};
 
-// Turn (x, y), the lane's two groups, by the angles (c, s); sign -1 turns back.
-__device__ inline void turn(f4& x, f4& y, f4 c, f4 s, bool interleaved) {
-    if (interleaved) {
-        const f4 u = {x.x * c.x - x.y * s.x, x.x * s.x + x.y * c.x, x.z * c.y - x.w * s.y, x.z * s.y + x.w * c.y};
-        const f4 w = {y.x * c.z - y.y * s.z, y.x * s.z + y.y * c.z, y.z * c.w - y.w * s.w, y.z * s.w + y.w * c.w};
-        x = u;
-        y = w;
-    } else {
-        const f4 u = x * c - y * s;
-        y = x * s + y * c;
-        x = u;
+// Where a run of heads starts: divisions of 64-bit numbers once a workgroup,
+// small ones for each of its heads.
+struct Start {
+    std::uint64_t row, step;
+    std::uint32_t head, env;
+    template <typename T>
+    __device__ Start(const QkArgs<T>& a, std::uint64_t group)
+        : row(group / a.per_row.d), step(row / a.batch.d), head(static_cast<std::uint32_t>(group % a.per_row.d)),
+          env(static_cast<std::uint32_t>(row % a.batch.d)) {}
+};
+
+// One head: its tensors' kind, row and addresses.
+template <typename T>
+struct Spot {
+    bool is_q;
+    std::uint32_t h;
+    std::uint64_t row, step;
+    std::uint32_t env;
+    __device__ Spot(const QkArgs<T>& a, const Start& at, std::uint32_t plus) {
+        const std::uint32_t x = at.head + plus, down = a.per_row(x), head = x - down * a.per_row.d;
+        const std::uint32_t y = at.env + down, over = a.batch(y);
+        is_q = head < a.hq;
+        h = is_q ? head : head - a.hq;
+        row = at.row + down;
+        step = at.step + over;
+        env = y - over * a.batch.d;
     }
+    __device__ const T* in(const Heads<T>& q, const Heads<T>& k) const {
+        return is_q ? q.row(step, env, h) : k.row(step, env, h);
+    }
+    __device__ T* out(const QkArgs<T>& a) const {
+        return is_q ? a.q_out + (row * a.hq + h) * a.dim : a.k_out + (row * a.hk + h) * a.dim;
+    }
+};
+
+// Cosines and sines of a lane's pairs.
+template <int PAIRS, typename T>
+__device__ Part<PAIRS> turns(const QkArgs<T>& a, std::int32_t p, unsigned j) {
+    Part<PAIRS> t;
+    if (p < 0 || static_cast<std::uint32_t>(p) >= a.table_rows) {
+#pragma unroll
+        for (int i = 0; i < PAIRS / 4; ++i) t.a[i] = t.b[i] = f4{NAN, NAN, NAN, NAN};
+        return t;
+    }
+    t.load_floats(a.table + static_cast<std::size_t>(p) * a.rotated, PAIRS * j, PAIRS * j + a.rotated / 2);
+    return t;
 }
 
 __device__ inline float across(float v, unsigned lanes) {
@@ -77,117 +201,131 @@ __device__ inline float across(float v, unsigned lanes) {
     return v;
 }
 
-__device__ inline float dot(f4 a, f4 b) { return a.x * b.x + a.y * b.y + a.z * b.z + a.w * b.w; }
-
-template <typename T>
+template <typename T, int PAIRS, unsigned TOGETHER>
 __global__ void __launch_bounds__(kThreads) qk_forward(QkArgs<T> a) {
-    const unsigned j = threadIdx.x % a.lanes;
-    const std::uint64_t group = (static_cast<std::uint64_t>(blockIdx.x) * kThreads + threadIdx.x) / a.lanes;
-    const bool mine = group < a.groups && 8 * j < a.dim;
-    const std::uint32_t per_row = a.hq + a.hk;
-    const std::uint64_t row = mine ? group / per_row : 0;
-    const std::uint32_t head = mine ? static_cast<std::uint32_t>(group % per_row) : 0;
-    const bool is_q = head < a.hq;
-    const std::uint32_t h = is_q ? head : head - a.hq;
-    const Heads<T> in = is_q ? a.q : a.k;
+    const unsigned j = threadIdx.x % a.lanes, per = kThreads / a.lanes;
+    const std::uint64_t base = static_cast<std::uint64_t>(blockIdx.x) * per * TOGETHER;
+    const Start start(a, base);
+    const bool has = 2 * PAIRS * j < a.dim, rotates = 2 * PAIRS * j < a.rotated;
     unsigned first, second;
-    places(a, j, first, second);
-    f4 x = {0, 0, 0, 0}, y = x;
-    if (mine) {
-        const T* p = in.row(row / a.batch, row % a.batch, h);
-        x = load4(p + first, in.vec);
-        y = load4(p + second, in.vec);
+    places<PAIRS>(a, j, first, second);
+    Part<PAIRS> x[TOGETHER];
+    std::int32_t position[TOGETHER];
+#pragma unroll
+    for (unsigned i = 0; i < TOGETHER; ++i) {
+        const std::uint32_t plus = i * per + threadIdx.x / a.lanes;
+        x[i].clear();
+        position[i] = 0;
+        if (base + plus < a.groups && has) {
+            const Spot<T> at(a, start, plus);
+            x[i].load(at.in(a.q, a.k), first, second, at.is_q ? a.q.vec : a.k.vec);
+            if (rotates) position[i] = a.positions[at.row];
+        }
     }
-    const float inv = 1.0f / sqrtf(across(dot(x, x) + dot(y, y), a.lanes) * a.inv_count + a.eps);
-    if (!mine) return;
-    x *= inv;
-    y *= inv;
-    const float* w = is_q ? a.wq : a.wk;
-    if (w != nullptr) {
-        x *= load4(w + first, true);
-        y *= load4(w + second, true);
+#pragma unroll
+    for (unsigned i = 0; i < TOGETHER; ++i) {
+        const std::uint32_t plus = i * per + threadIdx.x / a.lanes;
+        const float inv = 1.0f / sqrtf(across(x[i].dot(x[i]), a.lanes) * a.inv_count + a.eps);
+        if (base + plus >= a.groups || !has) continue;
+        const Spot<T> at(a, start, plus);
+        x[i].scale(inv);
+        const float* w = at.is_q ? a.wq : a.wk;
+        if (w != nullptr) {
+            Part<PAIRS> weight;
+            weight.load_floats(w, first, second);
+            x[i].scale(weight);
+        }
+        if (rotates) x[i].turn(turns<PAIRS>(a, position[i], j), false, a.interleaved);
+        x[i].store(at.out(a), first, second);
     }
-    if (8 * j < a.rotated) {
-        f4 c, s;
-        turns(a, row, j, c, s);
-        turn(x, y, c, s, a.interleaved);
-    }
-    T* out = (is_q ? a.q_out : a.k_out) + (row * (is_q ? a.hq : a.hk) + h) * a.dim;
-    store4(out + first, x);
-    store4(out + second, y);
 }
 
 // dy = the output's gradient turned back; dx = inv w dy - x inv^3 <x, w dy> / count;
 // dw = sum over rows of x inv dy.
-template <typename T>
+template <typename T, int PAIRS>
 __global__ void __launch_bounds__(kThreads) qk_gradient(QkArgs<T> a) {
-    __shared__ f4 sums[kThreads / 64][2][2][32];       // [wave][q, k][first, second][lane of the head]
-    const unsigned j = threadIdx.x % a.lanes;
-    const std::uint32_t per_row = a.hq + a.hk;
+    constexpr int N = PAIRS / 4;
+    constexpr unsigned kTogether = kGradTogether / N;
+    __shared__ f4 sums[kThreads / 64][2][2 * N][32 / N];       // [wave][q, k][four of them][lane of the head]
+    const unsigned j = threadIdx.x % a.lanes, per = kThreads / a.lanes;
     unsigned first, second;
-    places(a, j, first, second);
-    const bool has = 8 * j < a.dim;
-    f4 dw[2][2] = {};
-    const std::uint64_t at_once = static_cast<std::uint64_t>(gridDim.x) * (kThreads / a.lanes);
+    places<PAIRS>(a, j, first, second);
+    const bool has = 2 * PAIRS * j < a.dim, rotates = 2 * PAIRS * j < a.rotated;
+    Part<PAIRS> dw[2];
+    dw[0].clear();
+    dw[1].clear();
+    const std::uint64_t at_once = static_cast<std::uint64_t>(gridDim.x) * per * kTogether;
     // Every lane of a workgroup takes every turn, as the lane exchanges need.
-    for (std::uint64_t base = static_cast<std::uint64_t>(blockIdx.x) * (kThreads / a.lanes); base < a.groups; base += at_once) {
-        const std::uint64_t group = base + threadIdx.x / a.lanes;
-        const bool mine = group < a.groups && has;
-        const std::uint64_t row = mine ? group / per_row : 0;
-        const std::uint32_t head = mine ? static_cast<std::uint32_t>(group % per_row) : 0;
-        const bool is_q = head < a.hq;
-        const std::uint32_t h = is_q ? head : head - a.hq;
-        const Heads<T> in = is_q ? a.q : a.k;
-        const Heads<T> grad = is_q ? a.dq_out : a.dk_out;
-        f4 x = {0, 0, 0, 0}, y = x, dx = x, dy = x;
-        if (mine) {
-            const std::uint64_t t = row / a.batch, n = row % a.batch;
-            const T* p = in.row(t, n, h);
-            const T* d = grad.row(t, n, h);
-            x = load4(p + first, in.vec);
-            y = load4(p + second, in.vec);
-            dx = load4(d + first, grad.vec);
-            dy = load4(d + second, grad.vec);
-            if (8 * j < a.rotated) {
-                f4 c, s;
-                turns(a, row, j, c, s);
-                turn(dx, dy, c, -s, a.interleaved);
+    for (std::uint64_t base = static_cast<std::uint64_t>(blockIdx.x) * per * kTogether; base < a.groups; base += at_once) {
+        const Start start(a, base);
+        Part<PAIRS> x[kTogether], d[kTogether];
+        std::int32_t position[kTogether];
+#pragma unroll
+        for (unsigned i = 0; i < kTogether; ++i) {
+            const std::uint32_t plus = i * per + threadIdx.x / a.lanes;
+            x[i].clear();
+            d[i].clear();
+            position[i] = 0;
+            if (base + plus < a.groups && has) {
+                const Spot<T> at(a, start, plus);
+                x[i].load(at.in(a.q, a.k), first, second, at.is_q ? a.q.vec : a.k.vec);
+                d[i].load(at.in(a.dq_out, a.dk_out), first, second, at.is_q ? a.dq_out.vec : a.dk_out.vec);
+                if (rotates) position[i] = a.positions[at.row];
             }
         }
-        const float inv = 1.0f / sqrtf(across(dot(x, x) + dot(y, y), a.lanes) * a.inv_count + a.eps);
-        const float* w = is_q ? a.wq : a.wk;
-        if (w != nullptr && mine) {
-            dw[is_q ? 0 : 1][0] += x * inv * dx;
-            dw[is_q ? 0 : 1][1] += y * inv * dy;
-            dx *= load4(w + first, true);
-            dy *= load4(w + second, true);
-        }
-        const float along = across(dot(x, dx) + dot(y, dy), a.lanes) * inv * inv * inv * a.inv_count;
-        if (mine) {
-            T* out = (is_q ? a.q_out : a.k_out) + (row * (is_q ? a.hq : a.hk) + h) * a.dim;
-            store4(out + first, dx * inv - x * along);
-            store4(out + second, dy * inv - y * along);
+#pragma unroll
+        for (unsigned i = 0; i < kTogether; ++i) {
+            const std::uint32_t plus = i * per + threadIdx.x / a.lanes;
+            const bool mine = base + plus < a.groups && has;
+            const Spot<T> at(a, start, mine ? plus : 0);
+            const float inv = 1.0f / sqrtf(across(x[i].dot(x[i]), a.lanes) * a.inv_count + a.eps);
+            if (mine && rotates) d[i].turn(turns<PAIRS>(a, position[i], j), true, a.interleaved);
+            const float* w = at.is_q ? a.wq : a.wk;
+            if (w != nullptr && mine) {
+                Part<PAIRS> weight;
+                weight.load_floats(w, first, second);
+#pragma unroll
+                for (int u = 0; u < N; ++u) {
+                    const f4 none = {0, 0, 0, 0}, one = x[i].a[u] * inv * d[i].a[u], two = x[i].b[u] * inv * d[i].b[u];
+                    dw[0].a[u] += at.is_q ? one : none;
+                    dw[0].b[u] += at.is_q ? two : none;
+                    dw[1].a[u] += at.is_q ? none : one;
+                    dw[1].b[u] += at.is_q ? none : two;
+                }
+                d[i].scale(weight);
+            }
+            const float along = across(x[i].dot(d[i]), a.lanes) * inv * inv * inv * a.inv_count;
+            if (mine) {
+#pragma unroll
+                for (int u = 0; u < N; ++u) {
+                    d[i].a[u] = d[i].a[u] * inv - x[i].a[u] * along;
+                    d[i].b[u] = d[i].b[u] * inv - x[i].b[u] * along;
+                }
+                d[i].store(at.out(a), first, second);
+            }
         }
     }
     if (a.partials == nullptr) return;
     // Lanes that hold the same elements, first within the wave, then over the
     // waves, in a fixed order.
     const unsigned lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+#pragma unroll
     for (int kind = 0; kind < 2; ++kind)
-        for (int half = 0; half < 2; ++half) {
-            f4 v = dw[kind][half];
+#pragma unroll
+        for (int u = 0; u < 2 * N; ++u) {
+            f4 v = u < N ? dw[kind].a[u] : dw[kind].b[u - N];
             for (unsigned d = a.lanes; d < 64; d *= 2)
                 v += f4{__shfl_xor(v.x, d), __shfl_xor(v.y, d), __shfl_xor(v.z, d), __shfl_xor(v.w, d)};
-            if (lane < a.lanes) sums[wave][kind][half][lane] = v;
+            if (lane < a.lanes) sums[wave][kind][u][lane] = v;
         }
     __syncthreads();
     if (threadIdx.x < a.lanes && has)
         for (int kind = 0; kind < 2; ++kind)
-            for (int half = 0; half < 2; ++half) {
-                f4 v = sums[0][kind][half][j];
-                for (unsigned u = 1; u < kThreads / 64; ++u) v += sums[u][kind][half][j];
+            for (int u = 0; u < 2 * N; ++u) {
+                f4 v = sums[0][kind][u][j];
+                for (unsigned o = 1; o < kThreads / 64; ++o) v += sums[o][kind][u][j];
                 float* p = a.partials + (static_cast<std::size_t>(blockIdx.x) * 2 + kind) * a.dim;
-                store4(p + (half ? second : first), v);
+                store4(p + (u < N ? first + 4 * u : second + 4 * (u - N)), v);
             }
 }
 
@@ -209,19 +347,19 @@ __global__ void __launch_bounds__(kThreads) qk_weight_sum(const float* partials,
     if (threadIdx.x == 0 && out != nullptr) out[e < dim ? e : e - dim] = sh[0];
 }
 
-std::uint32_t lanes_of(std::uint32_t dim) {
+std::uint32_t lanes_of(std::uint32_t dim, unsigned pairs) {
     std::uint32_t n = 1;
-    while (8 * n < dim) n *= 2;
+    while (2 * pairs * n < dim) n *= 2;
     return n;
 }
 
-std::uint64_t blocks_for(const nesle_qk_args& a) {
-    const std::uint64_t per = kThreads / lanes_of(a.dim);
+std::uint64_t blocks_for(const nesle_qk_args& a, unsigned pairs, unsigned together) {
+    const std::uint64_t per = kThreads / lanes_of(a.dim, pairs) * together;
     return (static_cast<std::uint64_t>(a.steps) * a.batch * (a.q_heads + a.k_heads) + per - 1) / per;
 }
 
 std::uint32_t grad_blocks(const nesle_qk_args& a) {
-    const std::uint64_t all = blocks_for(a);
+    const std::uint64_t all = blocks_for(a, 4, kGradTogether);     // of eight pairs: as many
     return static_cast<std::uint32_t>(all < kGradBlocks ? all : kGradBlocks);
 }
 
@@ -233,12 +371,12 @@ int check(const char* who, const nesle_qk_args* a) {
     if (a->dim == 0 || a->dim % 8 != 0 || a->dim > NESLE_QK_MAX_DIM)
         return refuse(who, "dim must be a multiple of 8 up to " + std::to_string(NESLE_QK_MAX_DIM));
     if (a->rotated % 8 != 0 || a->rotated > a->dim) return refuse(who, "rotated must be a multiple of 8 up to dim");
-    if (a->q_heads + static_cast<std::uint64_t>(a->k_heads) == 0 || a->q_heads > 65535u || a->k_heads > 65535u)
-        return refuse(who, "heads must be in 1..65535");
-    // One launch takes fewer than 2^32 threads of eight elements; the first
+    if (a->q_heads + static_cast<std::uint64_t>(a->k_heads) == 0 || a->q_heads > 4096u || a->k_heads > 4096u)
+        return refuse(who, "heads must be in 1..4096");
+    // One launch takes fewer than 2^32 threads of 32 elements; the first
     // test keeps the second one's product below 2^64.
-    if (static_cast<std::uint64_t>(a->steps) * a->batch > (1ull << 32) || blocks_for(*a) * kThreads > 0xffffffffull)
-        return refuse(who, "more than 2^35 elements");
+    if (static_cast<std::uint64_t>(a->steps) * a->batch > (1ull << 32) || blocks_for(*a, 4, kTogether) * kThreads > 0xffffffffull)
+        return refuse(who, "more than 2^37 elements");
     if (!(a->eps >= 0.0f)) return refuse(who, "eps must not be negative");
     if (a->rotated != 0 && !empty(a) && (a->positions == nullptr || a->table == nullptr || a->table_rows == 0))
         return refuse(who, "the rotation needs positions and a table");
@@ -246,7 +384,7 @@ int check(const char* who, const nesle_qk_args* a) {
 }
 
 template <typename T>
-QkArgs<T> pack(const nesle_qk_args& a) {
+QkArgs<T> pack(const nesle_qk_args& a, unsigned pairs) {
     QkArgs<T> k{};
     k.q = heads<T>(a.q);
     k.k = heads<T>(a.k);
@@ -254,13 +392,14 @@ QkArgs<T> pack(const nesle_qk_args& a) {
     k.wk = a.k_weight;
     k.positions = a.positions;
     k.table = a.table;
-    k.batch = a.batch;
+    k.batch = Divide(a.batch);
+    k.per_row = Divide(a.q_heads + a.k_heads);
     k.hq = a.q_heads;
     k.hk = a.k_heads;
     k.dim = a.dim;
     k.rotated = a.rotated;
     k.table_rows = a.table_rows;
-    k.lanes = lanes_of(a.dim);
+    k.lanes = lanes_of(a.dim, pairs);
     k.groups = static_cast<std::uint64_t>(a.steps) * a.batch * (a.q_heads + a.k_heads);
     k.inv_count = a.unit ? 1.0f : 1.0f / static_cast<float>(a.dim);
     k.eps = a.eps;
@@ -268,18 +407,37 @@ QkArgs<T> pack(const nesle_qk_args& a) {
     return k;
 }
 
-template <typename T>
-int forward(const char* who, const nesle_qk_args& a, hipStream_t s) {
-    QkArgs<T> k = pack<T>(a);
+// Eight bfloat16 a load where heads, halves and addresses allow it.
+bool by_eight(const nesle_qk_args& a, bool gradient) {
+    if (a.dtype != NESLE_MEM_BF16 || a.dim % 16 != 0 || a.rotated % 16 != 0) return false;
+    const auto wide = [](const nesle_heads& x, std::uint32_t n) { return n == 0 || heads<bf16>(x).wide; };
+    return wide(a.q, a.q_heads) && wide(a.k, a.k_heads) &&
+           (!gradient || (wide(a.dq_out, a.q_heads) && wide(a.dk_out, a.k_heads)));
+}
+
+template <typename T, int PAIRS>
+void launch_forward(const nesle_qk_args& a, hipStream_t s) {
+    QkArgs<T> k = pack<T>(a, PAIRS);
     k.q_out = static_cast<T*>(a.q_out);
     k.k_out = static_cast<T*>(a.k_out);
-    hipLaunchKernelGGL(qk_forward<T>, dim3(static_cast<std::uint32_t>(blocks_for(a))), dim3(kThreads), 0, s, k);
+    constexpr unsigned together = kTogether * 4 / PAIRS;
+    const auto blocks = static_cast<std::uint32_t>(blocks_for(a, PAIRS, together));
+    if (blocks < 1024)
+        hipLaunchKernelGGL((qk_forward<T, PAIRS, 1>), dim3(static_cast<std::uint32_t>(blocks_for(a, PAIRS, 1))), dim3(kThreads), 0, s, k);
+    else
+        hipLaunchKernelGGL((qk_forward<T, PAIRS, together>), dim3(blocks), dim3(kThreads), 0, s, k);
+}
+
+int forward(const char* who, const nesle_qk_args& a, hipStream_t s) {
+    if (a.dtype == NESLE_MEM_F32) launch_forward<float, 4>(a, s);
+    else if (by_eight(a, false)) launch_forward<bf16, 8>(a, s);
+    else launch_forward<bf16, 4>(a, s);
     return launched(who);
 }
 
-template <typename T>
-int gradient(const char* who, const nesle_qk_args& a, hipStream_t s) {
-    QkArgs<T> k = pack<T>(a);
+template <typename T, int PAIRS>
+void launch_gradient(const nesle_qk_args& a, hipStream_t s) {
+    QkArgs<T> k = pack<T>(a, PAIRS);
     k.dq_out = heads<T>(a.dq_out);
     k.dk_out = heads<T>(a.dk_out);
     k.q_out = static_cast<T*>(a.dq);
@@ -287,10 +445,16 @@ int gradient(const char* who, const nesle_qk_args& a, hipStream_t s) {
     const bool weights = a.q_weight != nullptr || a.k_weight != nullptr;
     k.partials = weights ? a.scratch : nullptr;
     const std::uint32_t blocks = grad_blocks(a);
-    hipLaunchKernelGGL(qk_gradient<T>, dim3(blocks), dim3(kThreads), 0, s, k);
+    hipLaunchKernelGGL((qk_gradient<T, PAIRS>), dim3(blocks), dim3(kThreads), 0, s, k);
     if (weights)
         hipLaunchKernelGGL(qk_weight_sum, dim3(2 * a.dim), dim3(kThreads), 0, s, a.scratch, blocks, a.dim, a.dq_weight,
                            a.dk_weight);
+}
+
+int gradient(const char* who, const nesle_qk_args& a, hipStream_t s) {
+    if (a.dtype == NESLE_MEM_F32) launch_gradient<float, 4>(a, s);
+    else if (by_eight(a, true)) launch_gradient<bf16, 8>(a, s);
+    else launch_gradient<bf16, 4>(a, s);
     return launched(who);
 }
 
@@ -314,7 +478,7 @@ int nesle_qk_norm_rotate(const nesle_qk_args* a, void* stream) {
         (a->k_heads != 0 && (a->k.data == nullptr || a->k_out == nullptr)))
         return refuse(who, "null device pointer");
     const auto s = static_cast<hipStream_t>(stream);
-    return a->dtype == NESLE_MEM_F32 ? forward<float>(who, *a, s) : forward<bf16>(who, *a, s);
+    return forward(who, *a, s);
 }
 
 int nesle_qk_norm_rotate_grad(const nesle_qk_args* a, void* stream) {
@@ -337,7 +501,7 @@ int nesle_qk_norm_rotate_grad(const nesle_qk_args* a, void* stream) {
                            a->dk_weight);
         return launched(who);
     }
-    return a->dtype == NESLE_MEM_F32 ? gradient<float>(who, *a, s) : gradient<bf16>(who, *a, s);
+    return gradient(who, *a, s);
 }
 
 }  // extern "C"
