@@ -6,9 +6,11 @@ Replaces the reference's nvcc build script (scripts/build_cuda_extension.py):
   for ``--offload-arch=gfx950``;
 * ``_cuda_core_native*.so`` -- the pybind11 drop-in for nesle._cuda_core
   (re-exported by nesle_amd/_cuda_core.py), host-only C++ linked against
-  libnesle_hip.so (rpath $ORIGIN).
+  libnesle_hip.so (rpath $ORIGIN);
+* ``_memory_native*.so`` -- tensor and autograd binding of the memory operators
+  (nesle_amd/memory.py), host-only C++ against PyTorch and libnesle_hip.so.
 
-Both land in-tree next to this file.  ``python -m nesle_amd.build`` rebuilds.
+All land in-tree next to this file.  ``python -m nesle_amd.build`` rebuilds.
 Environment: ``HIPCC`` (default: hipcc on PATH or /opt/rocm/bin/hipcc),
 ``NESLE_HIP_ARCH`` (default gfx950), ``CXX`` (default g++).
 """
@@ -34,6 +36,7 @@ HIP_SOURCES = [CSRC / "nes_step.hip", CSRC / "nes_step_full.hip", CSRC / "nes_st
                CSRC / "mem_rotate.hip", CSRC / "mem_delta_step.hip", CSRC / "mem_delta_fwd.hip",
                CSRC / "mem_delta_bwd.hip"]
 SHIM_SOURCE = CSRC / "cuda_core_module.cpp"
+MEMORY_SOURCE = CSRC / "memory_module.cpp"
 
 HIP_FLAGS = [
     # -O2: the step kernel runs about 1 % faster than at -O3 (65,536 consoles,
@@ -74,9 +77,17 @@ def _hipcc() -> str:
     return found or "/opt/rocm/bin/hipcc"
 
 
-def shim_path() -> Path:
+def _extension(name: str) -> Path:
     suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
-    return PKG / f"_cuda_core_native{suffix}"
+    return PKG / f"{name}{suffix}"
+
+
+def shim_path() -> Path:
+    return _extension("_cuda_core_native")
+
+
+def memory_path() -> Path:
+    return _extension("_memory_native")
 
 
 def _run(cmd: list[str]) -> None:
@@ -116,11 +127,41 @@ def build_shim() -> Path:
     return out
 
 
+def compile_memory(obj: Path) -> None:
+    """The object of MEMORY_SOURCE, against the installed PyTorch's headers."""
+    import torch
+
+    inc = Path(torch.__file__).parent / "include"
+    rocm = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
+    _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-w",
+          "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{inc}",
+          f"-I{inc / 'torch' / 'csrc' / 'api' / 'include'}", f"-I{rocm / 'include'}",
+          f"-I{sysconfig.get_paths()['include']}", "-c", str(MEMORY_SOURCE), "-o", str(obj)])
+
+
+def link_memory(obj: Path) -> Path:
+    import torch
+
+    libs = Path(torch.__file__).parent / "lib"
+    out = memory_path()
+    tmp = out.with_name(out.name + ".tmp")
+    _run([os.environ.get("CXX", "g++"), "-shared", "-o", str(tmp), str(obj), f"-L{PKG}", "-lnesle_hip", f"-L{libs}", "-lc10",
+          "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libs}"])
+    tmp.replace(out)
+    return out
+
+
 def build_all() -> None:
-    build_hip()
-    build_shim()
+    with tempfile.TemporaryDirectory(prefix="nesle_memory_") as work, concurrent.futures.ThreadPoolExecutor(1) as pool:
+        obj = Path(work) / "memory_module.o"
+        binding = pool.submit(compile_memory, obj)      # while hipcc compiles the kernels
+        build_hip()
+        build_shim()
+        binding.result()
+        link_memory(obj)
 
 
 if __name__ == "__main__":
     build_all()
-    print(f"built {LIB.name} and {shim_path().name}")
+    print(f"built {LIB.name}, {shim_path().name} and {memory_path().name}")

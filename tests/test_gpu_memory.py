@@ -539,6 +539,49 @@ def test_captured_in_a_graph():
             assert torch.equal(a, b), i
 
 
+def test_only_first_derivatives():
+    """The gradient's own gradient is refused where it is asked for; a backward
+    that keeps its graph for other reasons works."""
+    from nesle_amd import memory
+
+    x, resets, _ = make(4, 2, 1, 1, 16, 16, torch.float32, 21)
+    q, k, v, g, beta = (x[n].to(dev()).requires_grad_() for n in NAMES[:5])
+    w = torch.tensor(2.0, device=dev(), requires_grad=True)
+    for out in (memory.gated_delta(q, k, v, g, beta)[0], memory.qk_norm_rotate(q, k)[0]):
+        (d,) = torch.autograd.grad((out * w).square().sum(), [q], create_graph=True)
+        with pytest.raises(RuntimeError, match="second derivative"):
+            d.sum().backward()
+
+
+def test_unused_outputs_have_no_gradient():
+    """A loss that takes only the output, or only the state."""
+    from nesle_amd import memory
+
+    x, resets, grads = make(40, 2, 1, 2, 24, 16, torch.float32, 22)
+    for used in range(2):
+        ref = [x[n].double().requires_grad_() for n in NAMES]
+        want = O.delta(*ref, resets, 24 ** -0.5)[used]
+        dw = torch.autograd.grad(want, ref, grads[used].double(), allow_unused=True)
+        gpu = [x[n].to(dev()).requires_grad_() for n in NAMES]
+        got = memory.gated_delta(*gpu[:5], state=gpu[5], resets=resets.to(dev()))[used]
+        dg = torch.autograd.grad(got, gpu, grads[used].to(dev()))
+        for n, a, b in zip(NAMES, dg, dw):
+            assert O.off(a, torch.zeros(a.shape, dtype=torch.float64) if b is None else b) <= F32, (used, n)
+
+
+def test_step_marks_the_state_as_changed():
+    """A state that a graph saved and a step then overwrote is noticed."""
+    from nesle_amd import memory
+
+    x, _, _ = make(1, 2, 1, 1, 16, 16, torch.float32, 23)
+    q, k, v, g, beta, state = (x[n].to(dev()) for n in NAMES)
+    q.requires_grad_()
+    out, _ = memory.gated_delta(q, k, v, g, beta, state=state)
+    memory.gated_delta_step(q[0].detach(), k[0], v[0], g[0], beta[0], state)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        out.sum().backward()
+
+
 def test_refusals():
     from nesle_amd import memory
 
