@@ -26,13 +26,14 @@ namespace nesle::mem {
 namespace {
 
 template <typename T, int DP>
-struct GradTile : ChunkTile<T, DP> {
-    using Base = ChunkTile<T, DP>;
+struct GradTile : ChunkTile<T, DP, kFull> {
+    using Base = ChunkTile<T, DP, kFull>;
     using M = typename Base::M;
-    // Transposed: [value column][token], [value column of 32][key].
-    typename M::template Tile<DP, kChunk, false> dout;
-    typename M::template Tile<DP, kChunk, true> u, dr;
-    typename M::template Tile<32, DP, true> slab;
+    // Transposed: [value column][token], [value column of 32][key].  With rows of
+    // 18 and 42 words (mod 64) the transposing reads meet no bank twice.
+    typename M::template Tile<DP, kChunk, kExact, 4> dout;
+    typename M::template Tile<DP, kChunk, kFull, 4> u, dr;
+    typename M::template Tile<32, DP, kNear, DP == 32 ? 4 : 20> slab;
     float row_beta[Base::kWaves][kChunk], row_gate[Base::kWaves][kChunk], row_after[Base::kWaves][kChunk];
     float place_beta[3][16], cross[4][16];     // of a tile: sums over columns; pairs that cross a token
     float whole[Base::kWaves];
@@ -203,8 +204,8 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
             for (int i = 0; i < 4; ++i) {
                 const int row = mi + 4 * g + i, c = nj + r;
                 const float L = sh.ratio(row, c), b = sh.beta[row];
-                sh.p.put(row, c, c <= row ? a.scale * L * dP[i] : 0.0f);
-                sh.t.put(row, c, c < row ? -b * L * dA[i] : 0.0f);
+                sh.p.template put<kNear>(row, c, c <= row ? a.scale * L * dP[i] : 0.0f);
+                sh.t.template put<kNear>(row, c, c < row ? -b * L * dA[i] : 0.0f);
                 const float by_a = -dA[i] * kk[j][i];
                 const float before_t = sum_below(c < row ? dP[i] * qk[j][i] + b * by_a : 0.0f);
                 cross += place == 1 || row >= c ? before_t : 0.0f;
@@ -225,12 +226,12 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
             const Rows<float, false> states(from + head * state_size, a.dv_dim);
 #pragma unroll
             for (int i = 0; i < KP; ++i) {
-                const auto s = M::full(states.get4(in_k && 32 * i + 4 * g < static_cast<int>(a.dv_dim), at.col, 32 * i + 4 * g),
+                const auto s = M::near(states.get4(in_k && 32 * i + 4 * g < static_cast<int>(a.dv_dim), at.col, 32 * i + 4 * g),
                                        states.get4(in_k && 32 * i + 16 + 4 * g < static_cast<int>(a.dv_dim), at.col, 32 * i + 16 + 4 * g));
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
                     dQ[m] = M::mul(sh.dout.cols(32 * i, 16 * m, r, g), s, dQ[m]);
-                    drs[m] = M::mul(sh.dr.cols(32 * i, 16 * m, r, g), s, drs[m]);
+                    drs[m] = M::mul(sh.dr.template cols<kNear>(32 * i, 16 * m, r, g), s, drs[m]);
                 }
             }
         }
@@ -242,16 +243,16 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
             __syncthreads();
             const auto ds = sh.slab.cols(0, 16 * at.wave, r, g);
 #pragma unroll
-            for (int m = 0; m < 2; ++m) dK[m] = M::mul(sh.u.cols(32 * i, 16 * m, r, g), ds, dK[m]);
+            for (int m = 0; m < 2; ++m) dK[m] = M::mul(sh.u.template cols<kNear>(32 * i, 16 * m, r, g), ds, dK[m]);
             if (i + 1 < KP) __syncthreads();
         }
         const auto key = sh.k.cols(0, 16 * at.wave, r, g), query = sh.q.cols(0, 16 * at.wave, r, g);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            dQ[m] = M::mul(sh.p.rows(16 * m, 0, r, g), key, gam[m] * a.scale * dQ[m]);
-            dK[m] = M::mul(sh.p.cols(0, 16 * m, r, g), query, dec[m] * dK[m] - beta[m] * gam[m] * drs[m]);
-            dK[m] = M::mul(sh.t.rows(16 * m, 0, r, g), key, dK[m]);
-            dK[m] = M::mul(sh.t.cols(0, 16 * m, r, g), key, dK[m]);
+            dQ[m] = M::mul(sh.p.template rows<kNear>(16 * m, 0, r, g), key, gam[m] * a.scale * dQ[m]);
+            dK[m] = M::mul(sh.p.template cols<kNear>(0, 16 * m, r, g), query, dec[m] * dK[m] - beta[m] * gam[m] * drs[m]);
+            dK[m] = M::mul(sh.t.template rows<kNear>(16 * m, 0, r, g), key, dK[m]);
+            dK[m] = M::mul(sh.t.template cols<kNear>(0, 16 * m, r, g), key, dK[m]);
         }
         const std::int64_t token = static_cast<std::int64_t>(start) * a.batch + env;
         if (a.group == 1) {

@@ -47,7 +47,7 @@ struct Segments {
 // MAP: the segment's M and B; else outputs and states.
 template <typename T, int DP, bool WIDE, bool MAP>
 __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_forward_kernel(DeltaArgs<T> a, Segments seg) {
-    using Tile = ChunkTile<T, DP>;
+    using Tile = ChunkTile<T, DP, kNear>;
     using M = typename Tile::M;
     constexpr int KT = Tile::KT, KP = Tile::KP, kWaves = Tile::kWaves * (MAP ? 2 : 1);
     __shared__ Tile sh;
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_f
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
                     ks[m] = M::mul(sh.k.rows(16 * m, i, r, g), s, ks[m]);
-                    if constexpr (!MAP) qs[m] = M::mul(sh.q.rows(16 * m, i, r, g), s, qs[m]);
+                    if constexpr (!MAP) qs[m] = M::mul(sh.q.rows(16 * m, i, r, g), M::near(s), qs[m]);
                 }
             }
         };
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_f
 #pragma unroll
         for (int m = 0; m < 2; ++m) U[m] = M::mul(sh.t.rows(16 * m, 0, r, g), right, zero);
         if constexpr (!MAP) {
-            const auto u = M::full(U[0], U[1]);
+            const auto u = M::near(U[0], U[1]);
 #pragma unroll
             for (int m = 0; m < 2; ++m) O[m] = M::mul(sh.p.rows(16 * m, 0, r, g), u, qs[m]);
             const Rows<T, WIDE> out(a.out + static_cast<std::int64_t>(t0) * out_step + head * a.dv_dim, out_step);

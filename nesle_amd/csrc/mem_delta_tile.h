@@ -207,14 +207,15 @@ __device__ void put_columns(const Rows<T, WIDE>& to, bool in, int n, const Lane<
     for (int e = 0; e < 8; ++e) to.put(in && at.row(e) < n, at.row(e), at.col, value(e));
 }
 
-template <typename T, int DP>          // DP: head dimensions padded to 32, 64 or 128; DP / 16 waves
+// DP: head dimensions padded to 32, 64 or 128; DP / 16 waves.  P_PLANES: of P.
+template <typename T, int DP, int P_PLANES>
 struct ChunkTile {
     using M = typename MathOf<T>::type;
     static constexpr int KT = DP / 16, KP = DP / 32, kWaves = DP / 16, kSmall = kChunk + 4;
 
-    typename M::template Tile<kChunk, DP, false> k, q;
-    typename M::template Tile<kChunk, kChunk, true> p;     // P: scale L_ij (q_i . k_j), j <= i; else 0
-    typename M::template Tile<kChunk, kChunk, true> t;     // (I + A)^-1
+    typename M::template Tile<kChunk, DP, kExact, 8> k, q;
+    typename M::template Tile<kChunk, kChunk, P_PLANES, 8> p;     // P: scale L_ij (q_i . k_j), j <= i; else 0
+    typename M::template Tile<kChunk, kChunk, kFull, 8> t;     // (I + A)^-1
     alignas(16) float a[kChunk * kSmall];      // A without beta: L_ij (k_i . k_j), j < i; else 0
     alignas(16) double G[kChunk];              // running sum of g: differences of it are taken
     alignas(16) float gamma[kChunk], decay[kChunk], beta[kChunk];
