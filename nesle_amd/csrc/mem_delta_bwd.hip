@@ -75,8 +75,10 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
         const std::uint32_t drops = in.drops();
         const float* from = (drops & 1u) ? nullptr : start == 0 ? a.state
                                                    : a.saved + (start / kChunk - 1) * state_size * a.batch * a.hv;
+        const bool of_chunk = start != 0;          // kept by the forward as [v_dim][k_dim]; else the initial state
         f4 S[KT];
-        Tile::load_state(a, from, head, at, S);
+        if (of_chunk && from != nullptr) Tile::kept(a, from, head, at, S);
+        else Tile::load_state(a, from, head, at, S);
 
         sh.stage_keys(in, at);
         if (at.wave == 0) sh.stage_gates(in, n, at.lane);
@@ -223,11 +225,20 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
         // dO S^T and dR S^T, then U dS^T: this wave's 16 key columns.
         f4 dQ[2] = {}, dK[2] = {}, drs[2] = {};
         if (from != nullptr) {
-            const Rows<float, false> states(from + head * state_size, a.dv_dim);
+            const Rows<float, false> states(from + head * state_size, of_chunk ? a.dk_dim : a.dv_dim);
 #pragma unroll
             for (int i = 0; i < KP; ++i) {
-                const auto s = M::near(states.get4(in_k && 32 * i + 4 * g < static_cast<int>(a.dv_dim), at.col, 32 * i + 4 * g),
-                                       states.get4(in_k && 32 * i + 16 + 4 * g < static_cast<int>(a.dv_dim), at.col, 32 * i + 16 + 4 * g));
+                f4 part[2];
+#pragma unroll
+                for (int o = 0; o < 2; ++o) {
+                    const int v = 32 * i + 16 * o + 4 * g;
+                    const bool inside = in_k && v < static_cast<int>(a.dv_dim);
+                    if (!of_chunk) part[o] = states.get4(inside, at.col, v);
+                    else
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) part[o][j] = states.value_of(states.get(inside, v + j, at.col));
+                }
+                const auto s = M::near(part[0], part[1]);
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
                     dQ[m] = M::mul(sh.dout.cols(32 * i, 16 * m, r, g), s, dQ[m]);

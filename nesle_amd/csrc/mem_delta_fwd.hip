@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_f
         const int r = at.r, g = at.g;
         const bool in_col = at.col < static_cast<int>(a.dv_dim);
         if (!MAP && t0 != 0 && t0 % kChunk == 0 && a.saved != nullptr)
-            Tile::store_state(a, a.saved + (t0 / kChunk - 1) * state_size * a.batch * a.hv, head, at, S);
+            Tile::keep(a, a.saved + (t0 / kChunk - 1) * state_size * a.batch * a.hv, head, at, S);
         const std::uint32_t drops = in.drops();
         if (drops & 1u)
 #pragma unroll
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_f
         any_drop |= drops != 0;
         for (;;) {
             sh.template stage_keys<!MAP>(in, at);
-            std::uint32_t odd = in.odd(at);
+            std::uint32_t odd = in.odd();
             if (at.wave == 0) odd |= sh.stage_gates(in, n, at.lane);
             if (inside != 0 && !Tile::finite(S)) odd |= inside;
             sh.report(odd);
@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_f
             // Rare: stage again, up to the first such token or drop, or a first
             // such token alone; what is left is the next turn's.
             n = (bad & 1u) ? 1 : min(n, __ffs(static_cast<int>(bad | inside)) - 1);
-            in.cut(n, at);
+            in.cut(n);
             __syncthreads();
             if (at.tid == 0) sh.bad = 0;
             __syncthreads();

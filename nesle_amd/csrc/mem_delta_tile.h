@@ -71,6 +71,10 @@ struct Rows {
         const auto x = __builtin_amdgcn_raw_buffer_load_b128(rsrc, static_cast<int>(offset(in, row, col)), 0, 0);
         return __builtin_bit_cast(f4, x);
     }
+    __device__ void put4(bool in, int row, int col, f4 v) const {
+        static_assert(sizeof(T) == 4 && !WIDE);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), rsrc, static_cast<int>(offset(in, row, col)), 0, 0);
+    }
     // Eight consecutive elements, as they lie in memory.
     static constexpr int kWords = sizeof(T) * 8 / 4;
     __device__ void get8(bool in, int row, int col, bool vec, std::uint32_t (&w)[kWords]) const {
@@ -159,7 +163,8 @@ struct Ahead {
         for (int e = 0; e < 8; ++e) to[e] = rows.get(at.row(e) < width && at.col < static_cast<int>(dim), at.row(e), at.col);
     }
     // Zeros in the rows from n on.
-    __device__ void cut(int n, const Lane<DP>& at) {
+    __device__ void cut(int n) {
+        const Lane<DP> at = Lane<DP>::anew();
         const bool mine = at.key_row < n;
 #pragma unroll
         for (int i = 0; i < In::kWords; ++i) {
@@ -170,7 +175,7 @@ struct Ahead {
         for (int e = 0; e < 8; ++e) v[e] = at.row(e) < n ? v[e] : 0;
     }
     // Tokens whose key or value holds something that is not finite.
-    __device__ std::uint32_t odd(const Lane<DP>& at) const {
+    __device__ std::uint32_t odd() const {
         using s2 = unsigned short __attribute__((ext_vector_type(2)));
         constexpr std::uint32_t kInf = sizeof(T) == 4 ? 0x7f800000u : 0x7f80u, kSize = sizeof(T) == 4 ? 0x7fffffffu : 0x7fffu;
         std::uint32_t most_v = 0, most_k = 0;
@@ -183,6 +188,7 @@ struct Ahead {
                               __builtin_bit_cast(s2, most_k), __builtin_bit_cast(s2, k[i] & 0x7fff7fffu)));
         if constexpr (sizeof(T) == 2) most_k = max(most_k >> 16, most_k & 0xffffu);
         if (!__any(max(most_v, most_k) >= kInf)) return 0;
+        const Lane<DP> at = Lane<DP>::anew();
         std::uint32_t tokens = most_k >= kInf ? 1u << at.key_row : 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) tokens |= (v[e] & kSize) >= kInf ? 1u << at.row(e) : 0;
@@ -258,8 +264,24 @@ struct ChunkTile {
         store_columns(to + head * a.dk_dim * a.dv_dim, static_cast<int>(a.dk_dim), static_cast<int>(a.dv_dim), at.col, at.g, S);
     }
 
+    // A state before a chunk, kept for the gradient as [v_dim][k_dim]: the four
+    // rows a lane holds lie together.
+    static __device__ void keep(const DeltaArgs<T>& a, float* to, std::size_t head, const Lane<DP>& at, const f4 (&S)[KT]) {
+        const Rows<float, false> x(to + head * a.dk_dim * a.dv_dim, a.dk_dim);
+#pragma unroll
+        for (int i = 0; i < KT; ++i)
+            x.put4(at.col < static_cast<int>(a.dv_dim) && 16 * i + 4 * at.g < static_cast<int>(a.dk_dim), at.col, 16 * i + 4 * at.g, S[i]);
+    }
+    static __device__ void kept(const DeltaArgs<T>& a, const float* from, std::size_t head, const Lane<DP>& at, f4 (&S)[KT]) {
+        const Rows<float, false> x(from + head * a.dk_dim * a.dv_dim, a.dk_dim);
+#pragma unroll
+        for (int i = 0; i < KT; ++i)
+            S[i] = x.get4(at.col < static_cast<int>(a.dv_dim) && 16 * i + 4 * at.g < static_cast<int>(a.dk_dim), at.col, 16 * i + 4 * at.g);
+    }
+
     static __device__ bool finite(const f4 (&S)[KT]) {
         f4 none = {0, 0, 0, 0};
+        asm volatile("" : "+v"(none));         // here, not ahead of the condition around the call
 #pragma unroll
         for (int i = 0; i < KT; ++i) none += S[i] - S[i];      // 0, or NaN
         return none.x + none.y + none.z + none.w == 0.0f;
