@@ -9,7 +9,8 @@
  * Tensors are time-major: [steps][batch][heads][dim], a rollout of `batch`
  * consoles.  Queries, keys, values and gradients that the caller hands in may
  * be strided (a slice of one projection's output) as long as the elements of
- * a head lie next to each other; what a call writes is contiguous.
+ * a head lie next to each other; what a call writes is contiguous, and lies,
+ * as states and workspaces do, on 16-byte boundaries.
  */
 #ifndef NESLE_MEMORY_H
 #define NESLE_MEMORY_H

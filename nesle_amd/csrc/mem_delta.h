@@ -106,8 +106,9 @@ inline bool aligned16(const void* p) { return reinterpret_cast<std::uintptr_t>(p
 inline int check_delta_inputs(const char* who, const nesle_delta_args* a) {
     if (!a->q.data || !a->k.data || !a->v.data || !a->g || !a->beta) return refuse(who, "null device pointer");
     if (!aligned16(a->state) || !aligned16(a->state_out) || !aligned16(a->saved) || !aligned16(a->dstate_out) ||
-        !aligned16(a->dstate) || !aligned16(a->scratch))
-        return refuse(who, "states and workspaces must lie on 16-byte boundaries");
+        !aligned16(a->dstate) || !aligned16(a->scratch) || !aligned16(a->out) || !aligned16(a->dq) || !aligned16(a->dk) ||
+        !aligned16(a->dv))
+        return refuse(who, "states, outputs and workspaces must lie on 16-byte boundaries");
     return NESLE_OK;
 }
 

@@ -29,10 +29,14 @@ template <typename T, int DP>
 struct GradTile : ChunkTile<T, DP, kFull> {
     using Base = ChunkTile<T, DP, kFull>;
     using M = typename Base::M;
+    typename M::template Tile<kChunk, DP, kExact, 8> dout;
     // Transposed: [value column][token], [value column of 32][key].  With rows of
     // 18 and 42 words (mod 64) the transposing reads meet no bank twice.
-    typename M::template Tile<DP, kChunk, kExact, 4> dout;
-    typename M::template Tile<DP, kChunk, kFull, 4> u, dr;
+    typename M::template Tile<DP, kChunk, kFull, 4> u;
+    union {
+        typename M::template Tile<DP, kChunk, kFull, 4> dr;
+        Results<T, DP> keys[2];                            // dQ and dK, once dR has been read
+    };
     typename M::template Tile<32, DP, kNear, DP == 32 ? 4 : 20> slab;
     float row_beta[Base::kWaves][kChunk], row_gate[Base::kWaves][kChunk], row_after[Base::kWaves][kChunk];
     float place_beta[3][16], cross[4][16];     // of a tile: sums over columns; pairs that cross a token
@@ -57,17 +61,17 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
     sh.start(first);
 
     Ahead<T, DP, WIDE> in;
-    std::uint32_t dout[8];
+    std::uint32_t dout[In::kWords];
     const auto fetch = [&](std::uint32_t end, const Lane<DP>& at) {
         const std::uint32_t start = (end - 1) / kChunk * kChunk;
         in.fetch(a, start, static_cast<int>(end - start), env, h, at);
-        in.columns(a.dout, a.dv_dim, start, static_cast<int>(end - start), env, h, at, dout);
+        in.part(a.dout, a.dv_dim, start, static_cast<int>(end - start), env, h, at, dout);
     };
     if (a.steps != 0) fetch(a.steps, first);
     for (std::uint32_t t1 = a.steps; t1 > 0;) {
         const Lane<DP> at = Lane<DP>::anew();
         const int r = at.r, g = at.g;
-        const bool in_v = at.col < static_cast<int>(a.dv_dim), in_k = at.col < static_cast<int>(a.dk_dim);
+        const bool in_k = at.col < static_cast<int>(a.dk_dim);
         // A chunk from its start to t1.  Where it drops the state, gammas and
         // decays are zero across that token, as in the forward.
         const std::uint32_t start = (t1 - 1) / kChunk * kChunk;
@@ -80,16 +84,9 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
         if (of_chunk && from != nullptr) Tile::kept(a, from, head, at, S);
         else Tile::load_state(a, from, head, at, S);
 
-        sh.stage_keys(in, at);
+        sh.stage(in, at);
+        sh.dout.put8(at.key_row, at.key_col, dout);
         if (at.wave == 0) sh.stage_gates(in, n, at.lane);
-        f4 V[2], dO[2];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            V[e / 4][e % 4] = In::value_of(in.v[e]);
-            dO[e / 4][e % 4] = In::value_of(dout[e]);
-        }
-#pragma unroll
-        for (int m = 0; m < 2; ++m) sh.dout.put4(at.col, 16 * m + 4 * g, dO[m]);
         t1 = start;
         if (t1 > 0) fetch(t1, at);
         __syncthreads();
@@ -120,7 +117,10 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
         __syncthreads();
         if (turn == 0) sh.invert(at);
         else if (turn <= 3) read_states();
-        f4 Y[2], gam[2], dec[2], beta[2];
+        f4 V[2], dO[2], Y[2], gam[2], dec[2], beta[2];
+        M::values(sh.v.cols(0, 16 * at.wave, r, g), V);
+        const auto grad = sh.dout.cols(0, 16 * at.wave, r, g);
+        M::values(grad, dO);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             gam[m] = sh.of_rows(sh.gamma, m, g);
@@ -129,7 +129,6 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
             Y[m] = V[m] - gam[m] * ks[m];
         }
         const auto right = M::full(beta[0] * Y[0], beta[1] * Y[1]);
-        const auto grad = M::exact(dO[0], dO[1]);
         __syncthreads();
         f4 U[2], dU[2], dR[2], X[2];
 #pragma unroll
@@ -146,7 +145,8 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
             sh.dr.put4(at.col, 16 * m + 4 * g, dR[m]);
         }
         const In dv(a.dv + static_cast<std::int64_t>(start) * v_step + head * a.dv_dim, v_step);
-        put_columns(dv, in_v, n, at, [&](int e) { return beta[e / 4][e % 4] * dR[e / 4][e % 4]; });
+        const f4 dV[2] = {beta[0] * dR[0], beta[1] * dR[1]};
+        sh.results.put(dv, static_cast<int>(a.dv_dim), n, at, dV);
 
         // Sums over the value dimension of dbeta and the gates, this wave's share.
         const float last = sh.gamma[kChunk - 1];
@@ -185,6 +185,7 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
             }
         }
         __syncthreads();
+        sh.results.flush(dv, static_cast<int>(a.dv_dim), n, at);
 
         // dP and dA by tiles; P's space becomes M1 and the inverse's M2.
 #pragma unroll
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
 #pragma unroll
             for (int i = 0; i < KP; ++i) {
                 const auto uu = sh.u.cols(32 * i, nj, r, g);
-                dP = M::mul(sh.dout.cols(32 * i, mi, r, g), uu, dP);
+                dP = M::mul(sh.dout.rows(mi, i, r, g), uu, dP);
                 dA = M::mul(sh.dr.cols(32 * i, mi, r, g), uu, dA);
             }
             // With token t = 16 x + r in lane r: pairs of this tile with
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
                 const auto s = M::near(part[0], part[1]);
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
-                    dQ[m] = M::mul(sh.dout.cols(32 * i, 16 * m, r, g), s, dQ[m]);
+                    dQ[m] = M::mul(sh.dout.rows(16 * m, i, r, g), s, dQ[m]);
                     drs[m] = M::mul(sh.dr.template cols<kNear>(32 * i, 16 * m, r, g), s, drs[m]);
                 }
             }
@@ -266,17 +267,16 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
             dK[m] = M::mul(sh.t.template cols<kNear>(0, 16 * m, r, g), key, dK[m]);
         }
         const std::int64_t token = static_cast<std::int64_t>(start) * a.batch + env;
+        const std::int64_t key_step = static_cast<std::int64_t>(a.batch) * a.hk * a.dk_dim;
+        const In dq(a.dq + (token * a.hk + hk) * a.dk_dim, key_step), dk(a.dk + (token * a.hk + hk) * a.dk_dim, key_step);
         if (a.group == 1) {
-            const std::int64_t step = static_cast<std::int64_t>(a.batch) * a.hk * a.dk_dim;
-            const In dq(a.dq + (token * a.hk + hk) * a.dk_dim, step), dk(a.dk + (token * a.hk + hk) * a.dk_dim, step);
-            put_columns(dq, in_k, n, at, [&](int e) { return dQ[e / 4][e % 4]; });
-            put_columns(dk, in_k, n, at, [&](int e) { return dK[e / 4][e % 4]; });
+            sh.keys[0].put(dq, static_cast<int>(a.dk_dim), n, at, dQ);
+            sh.keys[1].put(dk, static_cast<int>(a.dk_dim), n, at, dK);
         } else {            // one share a value head, added up afterwards
             const std::int64_t step = static_cast<std::int64_t>(a.batch) * a.hv * a.dk_dim;
             float* share = a.scratch + (token * a.hv + h) * a.dk_dim;
-            const Rows<float, WIDE> dq(share, step), dk(share + a.steps * step, step);
-            put_columns(dq, in_k, n, at, [&](int e) { return dQ[e / 4][e % 4]; });
-            put_columns(dk, in_k, n, at, [&](int e) { return dK[e / 4][e % 4]; });
+            Results<float, DP>{}.put(Rows<float, WIDE>(share, step), static_cast<int>(a.dk_dim), n, at, dQ);
+            Results<float, DP>{}.put(Rows<float, WIDE>(share + a.steps * step, step), static_cast<int>(a.dk_dim), n, at, dK);
         }
         if (at.wave == 0) {            // one token a lane
             const int t = at.lane % kChunk, i = t % 16;
@@ -306,6 +306,10 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
 #pragma unroll
         for (int i = 0; i < KT; ++i) dS[i] = (drops & 1u) ? zero : before[i];
         __syncthreads();
+        if (a.group == 1) {
+            sh.keys[0].flush(dq, static_cast<int>(a.dk_dim), n, at);
+            sh.keys[1].flush(dk, static_cast<int>(a.dk_dim), n, at);
+        }
     }
     if (a.dstate != nullptr) Tile::store_state(a, a.dstate, head, Lane<DP>::anew(), dS);
 }

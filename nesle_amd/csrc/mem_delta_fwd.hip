@@ -86,7 +86,6 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_f
     for (std::uint32_t t0 = begin; t0 < end;) {
         const Lane<DP> at = Lane<DP>::anew();
         const int r = at.r, g = at.g;
-        const bool in_col = at.col < static_cast<int>(a.dv_dim);
         if (!MAP && t0 != 0 && t0 % kChunk == 0 && a.saved != nullptr)
             Tile::keep(a, a.saved + (t0 / kChunk - 1) * state_size * a.batch * a.hv, head, at, S);
         const std::uint32_t drops = in.drops();
@@ -97,7 +96,7 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_f
         const std::uint32_t inside = drops & ~1u;
         any_drop |= drops != 0;
         for (;;) {
-            sh.template stage_keys<!MAP>(in, at);
+            sh.template stage<!MAP>(in, at);
             std::uint32_t odd = in.odd();
             if (at.wave == 0) odd |= sh.stage_gates(in, n, at.lane);
             if (inside != 0 && !Tile::finite(S)) odd |= inside;
@@ -113,9 +112,6 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_f
             if (at.tid == 0) sh.bad = 0;
             __syncthreads();
         }
-        f4 V[2];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) V[e / 4][e % 4] = Rows<T, WIDE>::value_of(in.v[e]);
         const std::uint32_t next = t0 + n;
         if (next < end) in.template fetch<!MAP>(a, next, width(next), env, h, at);
         // K S and Q S for this wave's columns.
@@ -148,7 +144,8 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_f
         if (at.tid == 0) sh.bad = 0;
         if (turn == 0) sh.invert(at);
         else if (turn <= 3) read_state();
-        f4 R[2];
+        f4 R[2], V[2] = {};
+        if (!MAP || at.wave < KT) M::values(sh.v.cols(0, 16 * at.wave, r, g), V);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             const f4 gam = sh.of_rows(sh.gamma, m, g);
@@ -157,6 +154,7 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_f
         }
         const auto right = M::full(R[0], R[1]);
         __syncthreads();
+        const Rows<T, WIDE> out(a.out + static_cast<std::int64_t>(t0) * out_step + head * a.dv_dim, out_step);
         f4 U[2], O[2];
 #pragma unroll
         for (int m = 0; m < 2; ++m) U[m] = M::mul(sh.t.rows(16 * m, 0, r, g), right, zero);
@@ -164,8 +162,7 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_f
             const auto u = M::near(U[0], U[1]);
 #pragma unroll
             for (int m = 0; m < 2; ++m) O[m] = M::mul(sh.p.rows(16 * m, 0, r, g), u, qs[m]);
-            const Rows<T, WIDE> out(a.out + static_cast<std::int64_t>(t0) * out_step + head * a.dv_dim, out_step);
-            put_columns(out, in_col, n, at, [&](int e) { return O[e / 4][e % 4]; });
+            sh.results.put(out, static_cast<int>(a.dv_dim), n, at, O);
         }
         const float last = sh.gamma[kChunk - 1];
         const auto w = M::full(U[0] * sh.of_rows(sh.decay, 0, g), U[1] * sh.of_rows(sh.decay, 1, g));
@@ -173,6 +170,7 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_f
         for (int i = 0; i < KT; ++i) S[i] = S[i] * last + M::mul(sh.k.cols(0, 16 * i, r, g), w, zero);
         t0 = next;
         __syncthreads();
+        if constexpr (!MAP) sh.results.flush(out, static_cast<int>(a.dv_dim), n, at);
     }
     const Lane<DP> at = Lane<DP>::anew();
     const int rows = static_cast<int>(a.dk_dim), cols = static_cast<int>(a.dv_dim);

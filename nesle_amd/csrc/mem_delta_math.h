@@ -30,6 +30,11 @@ struct F32Math {
     static __device__ Op near(const Op& x) { return x; }
     static __device__ Op exact(f4 a, f4 b) { return {a, b}; }
     static __device__ f4 mul(const Op& x, const Op& y, f4 c) { return mma(x.b, y.b, mma(x.a, y.a, c)); }
+    // The two result tiles that an operand of inputs holds.
+    static __device__ void values(const Op& x, f4 (&to)[2]) {
+        to[0] = x.a;
+        to[1] = x.b;
+    }
 
     // [ROWS][COLS] of float.  A row is 4 words more than a multiple of 32, so
     // that 16 rows start at 16 different groups of four banks.
@@ -111,6 +116,12 @@ struct SplitMath {
     static __device__ Op<kNear> near(f4 a, f4 b) { return operand<kNear>(a, b); }
     static __device__ Op<kNear> near(const Op<kFull>& o) { return {{o.x[0], o.x[1]}}; }
     static __device__ Op<kExact> exact(f4 a, f4 b) { return operand<kExact>(a, b); }      // values that are bfloat16
+    // The two result tiles that an operand of inputs holds.
+    static __device__ void values(const Op<kExact>& o, f4 (&to)[2]) {
+        const u4 w = o.x[0];
+        to[0] = f4{lo_half(w.x), hi_half(w.x), lo_half(w.y), hi_half(w.y)};
+        to[1] = f4{lo_half(w.z), hi_half(w.z), lo_half(w.w), hi_half(w.w)};
+    }
     // The pairs of planes that together weigh no less than the wider operand's last.
     template <int P, int Q>
     static __device__ f4 mul(const Op<P>& x, const Op<Q>& y, f4 c) {

@@ -40,13 +40,8 @@ struct Rows {
         else if constexpr (sizeof(T) == 1) return static_cast<std::uint8_t>(__builtin_amdgcn_raw_buffer_load_b8(rsrc, at, 0, 0));
         else return static_cast<std::uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(rsrc, at, 0, 0));
     }
-    // The same at a byte offset already made, plus a scalar one (from 0 to
-    // kRange, so that an offset outside stays outside).
-    __device__ std::uint32_t get_at(std::uint32_t at, std::uint32_t plus) const {
-        const int v = static_cast<int>(at), s = static_cast<int>(plus);
-        if constexpr (sizeof(T) == 4) return __builtin_amdgcn_raw_buffer_load_b32(rsrc, v, s, 0);
-        else return static_cast<std::uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(rsrc, v, s, 0));
-    }
+    // At a byte offset already made, plus a scalar one (from 0 to kRange, so
+    // that an offset outside stays outside).
     __device__ void put_at(std::uint32_t at, std::uint32_t plus, float x) const {
         const int v = static_cast<int>(at), s = static_cast<int>(plus);
         if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, static_cast<T>(x)), rsrc, v, s, 0);
@@ -74,6 +69,15 @@ struct Rows {
     __device__ void put4(bool in, int row, int col, f4 v) const {
         static_assert(sizeof(T) == 4 && !WIDE);
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), rsrc, static_cast<int>(offset(in, row, col)), 0, 0);
+    }
+    // Eight consecutive bfloat16 on a 16-byte boundary.
+    __device__ void put8(bool in, int row, int col, u4 v) const {
+        static_assert(sizeof(T) == 2);
+        if constexpr (WIDE) {
+            if (in) *reinterpret_cast<u4*>(base + row * step + col) = v;
+        } else {
+            __builtin_amdgcn_raw_buffer_store_b128(v, rsrc, static_cast<int>(offset(in, row, col)), 0, 0);
+        }
     }
     // Eight consecutive elements, as they lie in memory.
     static constexpr int kWords = sizeof(T) * 8 / 4;
@@ -124,22 +128,24 @@ struct Lane {
 };
 
 // The inputs of the tokens [start, start + width) of a chunk, loaded into
-// registers ahead of their use: a thread has eight elements of one token's
-// key and query, a wave its 16 columns of the values, every wave the gates,
-// one token a lane.
+// registers ahead of their use: a thread has eight elements of one token's key,
+// query and value, every wave the gates, one token a lane.
 template <typename T, int DP, bool WIDE>
 struct Ahead {
     using In = Rows<T, WIDE>;
-    std::uint32_t k[In::kWords], q[In::kWords], v[8], g, beta, reset;
+    std::uint32_t k[In::kWords], q[In::kWords], v[In::kWords], g, beta, reset;
 
+    static __device__ void part(const Heads<T>& from, std::uint32_t dim, std::uint32_t start, int width, std::uint32_t env,
+                                std::uint32_t h, const Lane<DP>& at, std::uint32_t (&to)[In::kWords]) {
+        const bool in = at.key_row < width && at.key_col < static_cast<int>(dim);
+        In(from.row(start, env, h), from.t).get8(in, at.key_row, at.key_col, from.vec, to);
+    }
     template <bool QUERIES = true>
     __device__ void fetch(const DeltaArgs<T>& x, std::uint32_t start, int width, std::uint32_t env, std::uint32_t h,
                           const Lane<DP>& at) {
-        const std::uint32_t hk = h / x.group;
-        const bool in = at.key_row < width && at.key_col < static_cast<int>(x.dk_dim);
-        In(x.k.row(start, env, hk), x.k.t).get8(in, at.key_row, at.key_col, x.k.vec, k);
-        if constexpr (QUERIES) In(x.q.row(start, env, hk), x.q.t).get8(in, at.key_row, at.key_col, x.q.vec, q);
-        columns(x.v, x.dv_dim, start, width, env, h, at, v);
+        part(x.k, x.dk_dim, start, width, env, h / x.group, at, k);
+        if constexpr (QUERIES) part(x.q, x.dk_dim, start, width, env, h / x.group, at, q);
+        part(x.v, x.dv_dim, start, width, env, h, at, v);
         const std::size_t token = static_cast<std::size_t>(start) * x.batch + env;
         const bool mine = at.lane < width;
         const Rows<float, WIDE> gates(x.g + token * x.hv + h, static_cast<std::int64_t>(x.batch) * x.hv);
@@ -149,50 +155,31 @@ struct Ahead {
         reset = 0;
         if (x.resets != nullptr) reset = Rows<std::uint8_t, WIDE>(x.resets + token, x.batch).get(mine, at.lane, 0);
     }
-    // A wave's columns of a [tokens][value dimension] tensor.
-    static __device__ void columns(const Heads<T>& from, std::uint32_t dim, std::uint32_t start, int width,
-                                   std::uint32_t env, std::uint32_t h, const Lane<DP>& at, std::uint32_t (&to)[8]) {
-        const In rows(from.row(start, env, h), from.t);
-        if (!WIDE && width == kChunk) {
-            const std::uint32_t base = rows.offset(at.col < static_cast<int>(dim), 4 * at.g, at.col);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) to[e] = rows.get_at(base, (16 * (e / 4) + e % 4) * static_cast<std::uint32_t>(rows.step) * sizeof(T));
-            return;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) to[e] = rows.get(at.row(e) < width && at.col < static_cast<int>(dim), at.row(e), at.col);
-    }
     // Zeros in the rows from n on.
     __device__ void cut(int n) {
-        const Lane<DP> at = Lane<DP>::anew();
-        const bool mine = at.key_row < n;
+        const bool mine = Lane<DP>::anew().key_row < n;
 #pragma unroll
         for (int i = 0; i < In::kWords; ++i) {
             k[i] = mine ? k[i] : 0;
             q[i] = mine ? q[i] : 0;
+            v[i] = mine ? v[i] : 0;
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = at.row(e) < n ? v[e] : 0;
     }
     // Tokens whose key or value holds something that is not finite.
     __device__ std::uint32_t odd() const {
         using s2 = unsigned short __attribute__((ext_vector_type(2)));
-        constexpr std::uint32_t kInf = sizeof(T) == 4 ? 0x7f800000u : 0x7f80u, kSize = sizeof(T) == 4 ? 0x7fffffffu : 0x7fffu;
-        std::uint32_t most_v = 0, most_k = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) most_v = max(most_v, v[e] & kSize);
+        std::uint32_t most = 0;
 #pragma unroll
         for (int i = 0; i < In::kWords; ++i)
-            if constexpr (sizeof(T) == 4) most_k = max(most_k, k[i] & kSize);
-            else most_k = __builtin_bit_cast(std::uint32_t, __builtin_elementwise_max(
-                              __builtin_bit_cast(s2, most_k), __builtin_bit_cast(s2, k[i] & 0x7fff7fffu)));
-        if constexpr (sizeof(T) == 2) most_k = max(most_k >> 16, most_k & 0xffffu);
-        if (!__any(max(most_v, most_k) >= kInf)) return 0;
-        const Lane<DP> at = Lane<DP>::anew();
-        std::uint32_t tokens = most_k >= kInf ? 1u << at.key_row : 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) tokens |= (v[e] & kSize) >= kInf ? 1u << at.row(e) : 0;
-        return tokens;
+            for (const std::uint32_t w : {k[i], v[i]})
+                if constexpr (sizeof(T) == 4) most = max(most, w & 0x7fffffffu);
+                else most = __builtin_bit_cast(std::uint32_t, __builtin_elementwise_max(
+                                __builtin_bit_cast(s2, most), __builtin_bit_cast(s2, w & 0x7fff7fffu)));
+        if constexpr (sizeof(T) == 2) most = max(most >> 16, most & 0xffffu);
+        const bool bad = most >= (sizeof(T) == 4 ? 0x7f800000u : 0x7f80u);
+        if (!__any(bad)) return 0;
+        return bad ? 1u << Lane<DP>::anew().key_row : 0;
     }
     static __device__ float value(std::uint32_t bits) { return __builtin_bit_cast(float, bits); }
     __device__ bool drop() const { return reset != 0 || value(g) < kDropBelow; }
@@ -200,18 +187,50 @@ struct Ahead {
     __device__ std::uint32_t drops() const { return static_cast<std::uint32_t>(__ballot(drop())); }
 };
 
-// The first n rows of a wave's columns of a [tokens][dim] tensor.
-template <int DP, typename T, bool WIDE, typename F>
-__device__ void put_columns(const Rows<T, WIDE>& to, bool in, int n, const Lane<DP>& at, F value) {
-    if (!WIDE && n == kChunk) {
-        const std::uint32_t base = to.offset(in, 4 * at.g, at.col);
+// ---- results [tokens][dim] of the inputs' type, a wave's 16 columns at a time ----
+// Float32: from the registers, 64 bytes of a row together.
+template <typename T, int DP>
+struct Results {
+    template <bool WIDE>
+    __device__ void put(const Rows<T, WIDE>& to, int dim, int n, const Lane<DP>& at, const f4 (&x)[2]) {
+        const bool in = at.col < dim;
+        if (!WIDE && n == kChunk) {
+            const std::uint32_t base = to.offset(in, 4 * at.g, at.col);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) to.put_at(base, (16 * (e / 4) + e % 4) * static_cast<std::uint32_t>(to.step) * sizeof(T), value(e));
-        return;
+            for (int e = 0; e < 8; ++e) to.put_at(base, (16 * (e / 4) + e % 4) * static_cast<std::uint32_t>(to.step) * sizeof(T), x[e / 4][e % 4]);
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) to.put(in && at.row(e) < n, at.row(e), at.col, x[e / 4][e % 4]);
     }
+    template <bool WIDE>
+    __device__ void flush(const Rows<T, WIDE>&, int, int, const Lane<DP>&) const {}
+};
+// bfloat16: two bytes a lane would be 32 of a row, so through LDS ([column]
+// [token], rows of 18 words: no bank twice) and, after a barrier, eight elements
+// of a token a lane by transposing reads: a wave's block is 16 tokens of 32
+// columns.
+template <int DP>
+struct Results<bf16, DP> {
+    static constexpr int kRow = kChunk + 4;
+    alignas(16) std::uint16_t d[DP * kRow];
+    template <bool WIDE>
+    __device__ void put(const Rows<bf16, WIDE>&, int, int, const Lane<DP>& at, const f4 (&x)[2]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) to.put(in && at.row(e) < n, at.row(e), at.col, value(e));
-}
+        for (int m = 0; m < 2; ++m)
+            *reinterpret_cast<u2*>(&d[at.col * kRow + 16 * m + 4 * at.g]) = u2{pack_bf16(x[m].x, x[m].y), pack_bf16(x[m].z, x[m].w)};
+    }
+    template <bool WIDE>
+    __device__ void flush(const Rows<bf16, WIDE>& to, int dim, int n, const Lane<DP>& at) const {
+        using s4 = short __attribute__((ext_vector_type(4)));
+        using lds = __attribute__((address_space(3))) s4;
+        const int token = 16 * (at.wave % 2), col = 32 * (at.wave / 2) + 8 * at.g;
+        const std::uint16_t* from = &d[(col + at.r / 4) * kRow + token + 4 * (at.r % 4)];
+        const u2 a = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)from));
+        const u2 b = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)(from + 4 * kRow)));
+        to.put8(token + at.r < n && col < dim, token + at.r, col, u4{a.x, a.y, b.x, b.y});
+    }
+};
 
 // DP: head dimensions padded to 32, 64 or 128; DP / 16 waves.  P_PLANES: of P.
 template <typename T, int DP, int P_PLANES>
@@ -219,10 +238,13 @@ struct ChunkTile {
     using M = typename MathOf<T>::type;
     static constexpr int KT = DP / 16, KP = DP / 32, kWaves = DP / 16, kSmall = kChunk + 4;
 
-    typename M::template Tile<kChunk, DP, kExact, 8> k, q;
+    typename M::template Tile<kChunk, DP, kExact, 8> k, q, v;
     typename M::template Tile<kChunk, kChunk, P_PLANES, 8> p;     // P: scale L_ij (q_i . k_j), j <= i; else 0
     typename M::template Tile<kChunk, kChunk, kFull, 8> t;     // (I + A)^-1
-    alignas(16) float a[kChunk * kSmall];      // A without beta: L_ij (k_i . k_j), j < i; else 0
+    union {
+        alignas(16) float a[kChunk * kSmall];  // A without beta: L_ij (k_i . k_j), j < i; else 0
+        Results<T, DP> results;                // of the values, once A is inverted
+    };
     alignas(16) double G[kChunk];              // running sum of g: differences of it are taken
     alignas(16) float gamma[kChunk], decay[kChunk], beta[kChunk];
     unsigned bad;                              // tokens with a value that is not finite
@@ -297,12 +319,12 @@ struct ChunkTile {
             }
     }
 
-    // K and Q.
     template <bool QUERIES = true, bool WIDE>
-    __device__ void stage_keys(const Ahead<T, DP, WIDE>& in, const Lane<DP>& at) {
-        if (!QUERIES && at.key_row >= kChunk) return;          // more waves than the tile needs
+    __device__ void stage(const Ahead<T, DP, WIDE>& in, const Lane<DP>& at) {
+        if (!QUERIES && at.key_row >= kChunk) return;          // more waves than the tiles need
         k.put8(at.key_row, at.key_col, in.k);
         if constexpr (QUERIES) q.put8(at.key_row, at.key_col, in.q);
+        v.put8(at.key_row, at.key_col, in.v);
     }
 
     // Gates and write strengths of the tokens below n (one wave); other rows
