@@ -31,6 +31,8 @@
 // launch finds each segment's M and B (the same walk over 2 DP columns, from
 // [0 | I], with values for the first half only), one takes the state through
 // the segments, one walks all segments from their states at once.
+#include <algorithm>
+
 #include "mem_delta_tile.h"
 
 namespace nesle::mem {
@@ -259,17 +261,22 @@ __global__ void __launch_bounds__(DP * 4) delta_join_kernel(const float* state, 
     keep(steps);
 }
 
-// Segments for few heads over many tokens.  A walk of one chunk takes about the
-// same time whether a compute unit holds one head or two, and the three
-// launches walk every chunk twice.
+// Segments for few heads over many tokens.  The walk of one head through a chunk
+// takes 3.6 us by itself and 7 us beside another on its compute unit; a step of
+// the join takes 0.6 us, and the three launches walk every chunk twice.  So:
+// enough segments for two workgroups a compute unit, no more than balance the
+// join (its steps times 0.6 us against 2 x 5 us for a segment's chunks: the
+// square root of 16 chunks), two chunks or more in each.  Measured in bfloat16,
+// heads of 64, whole walk against segments: 1,024 tokens of 64 heads 120 / 59 us,
+// of 128 heads 122 / 97 us, of 256 heads 127 / 157 us; 256 tokens of 16 heads
+// 32 / 25 us; 8,191 tokens of 8 heads 923 / 91 us.
 Segments segments(const nesle_delta_args& a) {
     const std::uint64_t heads = static_cast<std::uint64_t>(a.batch) * a.v_heads;
     const std::uint32_t chunks = (a.steps + kChunk - 1) / kChunk;
     std::uint32_t count = 1;
     if (chunks >= 8 && heads <= 128) {
-        count = static_cast<std::uint32_t>(512 / heads);
-        if (count > chunks / 4) count = chunks / 4;
-        if (count > 64) count = 64;
+        while (static_cast<std::uint64_t>(count + 1) * (count + 1) <= 16ull * chunks) ++count;
+        count = std::min({count, static_cast<std::uint32_t>(512 / heads), chunks / 2, 4096u});
     }
     const std::uint32_t each = count < 2 ? chunks : (chunks + count - 1) / count;
     Segments s{};
