@@ -8,6 +8,9 @@
 * ``nesle_amd.env``         SB3/Gymnasium vector and single environments
   (``make_vec``, ``NesleVecEnv``, ``NesleEnv``), drop-in for ``nesle.env``;
 * ``nesle_amd.native_ppo``  GPU-resident PPO, drop-in for ``nesle.native_ppo``;
+* ``nesle_amd.memory``      operators of a policy with memory: per-head norm with
+  rotation, gated delta rule over a rollout and one token at a time;
+* ``nesle_amd.memory_ppo``  PPO with such a policy;
 * ``nesle_amd.actions``     controller masks and action sets.
 
 The native pieces are imported on first use, so importing the package never
