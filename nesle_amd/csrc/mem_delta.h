@@ -17,9 +17,9 @@ constexpr int kChunk = NESLE_DELTA_CHUNK;
 // every gate that is multiplied keeps a finite logarithm.
 constexpr float kDropBelow = -104.0f;
 // What a dropping token's gate counts for in the running sums: exp of any
-// difference across it is zero, and 32 of them leave a double 11 digits after
-// the point for the others.
-constexpr float kGone = -2000.0f;
+// difference across it is zero, and 32 of them leave a double 9 digits after the
+// point for the others.
+constexpr float kGone = -100000.0f;
 
 template <typename T>
 struct DeltaArgs {

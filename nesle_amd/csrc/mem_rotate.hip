@@ -10,6 +10,8 @@
 // not allow eight bfloat16.
 //
 // Bound by memory: about 10 operations an element.
+#include <initializer_list>
+
 #include "mem_common.h"
 
 namespace nesle::mem {
@@ -363,6 +365,12 @@ std::uint32_t grad_blocks(const nesle_qk_args& a) {
     return static_cast<std::uint32_t>(all < kGradBlocks ? all : kGradBlocks);
 }
 
+bool aligned(std::initializer_list<const void*> pointers) {
+    for (const void* p : pointers)
+        if (reinterpret_cast<std::uintptr_t>(p) % 16 != 0) return false;
+    return true;
+}
+
 bool empty(const nesle_qk_args* a) { return a->steps == 0 || a->batch == 0; }
 
 int check(const char* who, const nesle_qk_args* a) {
@@ -380,6 +388,8 @@ int check(const char* who, const nesle_qk_args* a) {
     if (!(a->eps >= 0.0f)) return refuse(who, "eps must not be negative");
     if (a->rotated != 0 && !empty(a) && (a->positions == nullptr || a->table == nullptr || a->table_rows == 0))
         return refuse(who, "the rotation needs positions and a table");
+    if (!aligned({a->q_weight, a->k_weight, a->table, a->q_out, a->k_out, a->dq, a->dk, a->scratch}))
+        return refuse(who, "weights, table, outputs and workspace must lie on 16-byte boundaries");
     return NESLE_OK;
 }
 

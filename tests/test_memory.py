@@ -68,7 +68,8 @@ def test_qk_entries_refuse(entry):
     for bad, why in (({"dtype": 2}, "dtype"), ({"dim": 12}, "dim"), ({"dim": 264}, "dim"), ({"rotated": 24}, "rotated"),
                      ({"rotated": 4}, "rotated"), ({"rotated": 8}, "positions"), ({"eps": -1.0}, "eps"),
                      ({"eps": math.nan}, "eps"), ({"q_heads": 0, "k_heads": 0}, "heads"),
-                     ({"steps": 1 << 31, "batch": 1 << 31}, "elements"), ({}, "null device pointer")):
+                     ({"steps": 1 << 31, "batch": 1 << 31}, "elements"), ({"q_out": 8}, "16-byte"),
+                     ({"q_heads": 5000}, "heads"), ({}, "null device pointer")):
         assert fn(ctypes.byref(args(**bad)), None) == abi.EINVAL, bad
         assert why in abi.lib().nesle_last_error().decode(), bad
     if entry.endswith("grad"):
