@@ -44,6 +44,10 @@ struct Segments {
     float* maps;           // [segment][head]: M, then B
     float* states;         // [segment][head][k_dim][v_dim]: the state before it
     std::uint32_t* dropped;    // [segment][head]: whether the state is dropped inside
+    // Of `per` segments each; one group: all.  The same of the groups.
+    std::uint32_t per, groups;
+    float *group_maps, *group_states;
+    std::uint32_t* group_dropped;
 };
 
 // MAP: the segment's M and B; else outputs and states.
@@ -186,71 +190,101 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_f
     }
 }
 
-// The state before each segment, from one to the next: S <- M S + B.  A segment
-// that drops the state inside leaves B alone, whatever S held.  One workgroup
-// for 16 columns of a state, a wave for 16 of its rows: the steps are a chain,
-// so a step is kept short (one tile a wave by float32 matrix instructions, the
-// tiles exchanged through LDS) and M and B are loaded two to four steps ahead.
-template <int DP>
-__global__ void __launch_bounds__(DP * 4) delta_join_kernel(const float* state, Segments seg, int dk, int dv) {
+// From segment to segment, S <- M S + B; a segment that drops the state inside
+// leaves B alone, whatever S held.  The steps are a chain, so where there are
+// many, the segments go in groups: COMPOSE takes [I | 0] through a group's
+// segments to the group's own M and B, a second launch takes the state through
+// the groups, a third takes it through the segments of every group at once.
+struct Chain {
+    const float* maps;             // [segment][head]: M, then B
+    const std::uint32_t* dropped;
+    const float* first;            // [group][head]: the state before it; null: zeros
+    float* to;                     // COMPOSE: the groups' maps; else [segment][head]: the state before it
+    std::uint32_t* to_dropped;     // COMPOSE: the groups'
+    std::uint32_t count, per;      // segments; of a group
+};
+
+// One workgroup for 16 columns, a wave for 16 rows of them: a step is kept short
+// (one tile a wave by float32 matrix instructions, the tiles exchanged through
+// LDS) and M and B are loaded two to four steps ahead.
+template <int DP, bool COMPOSE>
+__global__ void __launch_bounds__(DP * 4) delta_join_kernel(Chain x, int dk, int dv) {
     constexpr int KT = DP / 16, kAhead = DP == 128 ? 2 : 4;
     __shared__ f4 tiles[2][KT][64];
     const int lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), col = 16 * blockIdx.y + r;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const bool of_m = COMPOSE && blockIdx.y < KT;          // these columns are M's, else the state's
+    const int col = 16 * (of_m || !COMPOSE ? blockIdx.y : blockIdx.y - KT) + r, cols = of_m ? dk : dv;
     const std::size_t heads = gridDim.x, head = blockIdx.x, map_size = static_cast<std::size_t>(dk) * (dk + dv);
+    const std::uint32_t begin = blockIdx.z * x.per;
     const auto tile = [&](const float* from) {             // rows 16 wave .., of this workgroup's columns
-        const Rows<float, false> x(from, dv);
+        const Rows<float, false> rows(from, cols);
         f4 v;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int row = 16 * wave + 4 * g + j;
-            v[j] = x.value_of(x.get(col < dv && row < dk, row, col));
+            v[j] = rows.value_of(rows.get(col < cols && row < dk, row, col));
         }
         return v;
     };
     f4 M[kAhead][KT], B[kAhead];
     std::uint32_t dropped[kAhead];
     const auto load = [&](int slot, std::uint32_t s) {
-        const float* map = seg.maps + (s * heads + head) * map_size;
+        const std::size_t at = (begin + s) * heads + head;
+        const float* map = x.maps + at * map_size;
         const Rows<float, false> m(map, dk);
 #pragma unroll
         for (int c = 0; c < KT; ++c)
             M[slot][c] = m.get4(16 * wave + r < dk && 16 * c + 4 * g < dk, 16 * wave + r, 16 * c + 4 * g);
-        B[slot] = tile(map + static_cast<std::size_t>(dk) * dk);
+        B[slot] = of_m ? f4{0, 0, 0, 0} : tile(map + static_cast<std::size_t>(dk) * dk);
         // A vector load, counted in order with the others.
         dropped[slot] = __builtin_amdgcn_raw_buffer_load_b32(
-            __builtin_amdgcn_make_buffer_rsrc(seg.dropped + s * heads + head, 0, 4, 0x00027000), 0, 0, 0);
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<std::uint32_t*>(x.dropped) + at, 0, 4, 0x00027000), 0, 0, 0);
     };
-    f4 S = state == nullptr ? f4{0, 0, 0, 0} : tile(state + head * dk * dv);
-    const auto keep = [&](std::uint32_t s) {
-        const Rows<float, false> to(seg.states + (s * heads + head) * dk * dv, dv);
+    f4 S = {0, 0, 0, 0};
+    if constexpr (COMPOSE) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) S[j] = of_m && col == 16 * wave + 4 * g + j ? 1.0f : 0.0f;
+    } else if (x.first != nullptr) {
+        S = tile(x.first + (blockIdx.z * heads + head) * dk * dv);
+    }
+    const auto store = [&](float* to) {
+        const Rows<float, false> rows(to, cols);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int row = 16 * wave + 4 * g + j;
-            to.put(col < dv && row < dk, row, col, S[j]);
+            rows.put(col < cols && row < dk, row, col, S[j]);
         }
     };
+    const auto keep = [&](std::uint32_t s) {
+        if constexpr (!COMPOSE) store(x.to + ((begin + s) * heads + head) * dk * dv);
+    };
+    bool any_dropped = false;
     const auto step = [&](int slot) {
         tiles[slot % 2][wave][lane] = S;
         __syncthreads();                                   // two buffers: the next write is a barrier later
         f4 sum = {0, 0, 0, 0};
-        if (__builtin_amdgcn_readfirstlane(dropped[slot]) == 0)
+        if (__builtin_amdgcn_readfirstlane(dropped[slot]) == 0) {
 #pragma unroll
             for (int c = 0; c < KT; ++c) sum = mma(M[slot][c], tiles[slot % 2][c][lane], sum);
+        } else {
+            any_dropped = true;
+        }
         S = sum + B[slot];
     };
     // Past the last map its loads are made again: without a condition around
     // them they stay in flight through the steps before they are needed.
-    const std::uint32_t steps = seg.count - 1;
+    const std::uint32_t left = min(x.per, x.count - begin), steps = COMPOSE ? left : left - 1;
+    const std::uint32_t last = steps == 0 ? 0 : steps - 1;
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) load(i, min(static_cast<std::uint32_t>(i), steps - 1));
+    for (int i = 0; i < kAhead; ++i) load(i, min(static_cast<std::uint32_t>(i), last));
     std::uint32_t s = 0;
     for (; s + kAhead <= steps; s += kAhead)
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             keep(s + i);
             step(i);
-            load(i, min(s + i + kAhead, steps - 1));
+            load(i, min(s + i + kAhead, last));
         }
 #pragma unroll
     for (int i = 0; i < kAhead - 1; ++i)
@@ -258,37 +292,52 @@ __global__ void __launch_bounds__(DP * 4) delta_join_kernel(const float* state, 
             keep(s + i);
             step(i);
         }
-    keep(steps);
+    if constexpr (COMPOSE) {
+        const std::size_t at = blockIdx.z * heads + head;
+        store(x.to + at * map_size + (of_m ? 0 : static_cast<std::size_t>(dk) * dk));
+        if (threadIdx.x == 0 && blockIdx.y == 0) x.to_dropped[at] = any_dropped;
+    } else {
+        keep(steps);
+    }
 }
 
 // Segments for few heads over many tokens.  The walk of one head through a chunk
-// takes 3.6 us by itself and 7 us beside another on its compute unit; a step of
-// the join takes 0.6 us, and the three launches walk every chunk twice.  So:
-// enough segments for two workgroups a compute unit, no more than balance the
-// join (its steps times 0.6 us against 2 x 5 us for a segment's chunks: the
-// square root of 16 chunks), two chunks or more in each.  Measured in bfloat16,
-// heads of 64, whole walk against segments: 1,024 tokens of 64 heads 120 / 59 us,
-// of 128 heads 122 / 97 us, of 256 heads 127 / 157 us; 256 tokens of 16 heads
-// 32 / 25 us; 8,191 tokens of 8 heads 923 / 91 us.
+// takes 3.6 us by itself and 7 us beside another on its compute unit, a step of
+// a chain 0.6 us, a launch of one 5 us and more, and the launches walk every chunk
+// twice.  So: enough segments for two workgroups a compute unit, two chunks or
+// more in each, and no more than balance the chain's steps against the walks; in
+// groups, of as many segments as there are groups, once the chain would be longer
+// than 40.  Measured in bfloat16, heads of 64, whole walk against segments: 1,024
+// tokens of 64 heads 120 / 59 us, of 128 heads 122 / 97 us, of 256 heads 127 / 157
+// us; 256 tokens of 16 heads 32 / 25 us.  One chain against groups: 4,096 tokens of
+// 8 heads 60 / 63 us, 8,191 of 8 heads 91 / 82 us, 32,768 of 4 heads 167 / 127 us.
 Segments segments(const nesle_delta_args& a) {
     const std::uint64_t heads = static_cast<std::uint64_t>(a.batch) * a.v_heads;
     const std::uint32_t chunks = (a.steps + kChunk - 1) / kChunk;
+    const auto root = [](std::uint64_t x) {
+        std::uint32_t n = 1;
+        while (static_cast<std::uint64_t>(n + 1) * (n + 1) <= x) ++n;
+        return n;
+    };
     std::uint32_t count = 1;
     if (chunks >= 8 && heads <= 128) {
-        while (static_cast<std::uint64_t>(count + 1) * (count + 1) <= 16ull * chunks) ++count;
-        count = std::min({count, static_cast<std::uint32_t>(512 / heads), chunks / 2, 4096u});
+        const std::uint32_t most = std::min(static_cast<std::uint32_t>(512 / heads), chunks / 2);
+        count = std::min(root(8ull * chunks), most);
+        if (count > 40) count = std::min(root(64ull * chunks), most);
     }
     const std::uint32_t each = count < 2 ? chunks : (chunks + count - 1) / count;
     Segments s{};
     s.steps = each * kChunk;
     s.count = chunks == 0 ? 1 : (chunks + each - 1) / each;
     if (s.steps == 0) s.steps = kChunk;
+    s.per = s.count > 40 ? root(s.count) : s.count;
+    s.groups = (s.count + s.per - 1) / s.per;
     return s;
 }
 
 std::uint64_t segment_floats(const nesle_delta_args& a, const Segments& s) {
     if (s.count < 2) return 0;
-    const std::uint64_t slots = static_cast<std::uint64_t>(s.count) * a.batch * a.v_heads;
+    const std::uint64_t slots = (s.count + (s.groups > 1 ? s.groups : 0ull)) * a.batch * a.v_heads;
     return slots * (static_cast<std::uint64_t>(a.k_dim) * (a.k_dim + 2 * a.v_dim) + 1);
 }
 
@@ -298,8 +347,20 @@ void launch_dim(const DeltaArgs<T>& a, const Segments& seg, hipStream_t s) {
     if (seg.count > 1) {
         // The last segment's M and B are not needed.
         hipLaunchKernelGGL((delta_forward_kernel<T, DP, WIDE, true>), dim3(heads, seg.count - 1), dim3(DP * 8), 0, s, a, seg);
-        hipLaunchKernelGGL((delta_join_kernel<DP>), dim3(heads, (a.dv_dim + 15) / 16), dim3(DP * 4), 0, s, a.state, seg,
-                           static_cast<int>(a.dk_dim), static_cast<int>(a.dv_dim));
+        const int dk = static_cast<int>(a.dk_dim), dv = static_cast<int>(a.dv_dim);
+        const std::uint32_t slices = (a.dv_dim + 15) / 16;
+        const float* first = a.state;
+        if (seg.groups > 1) {                              // of the last group neither
+            const Chain in_groups{seg.maps, seg.dropped, nullptr, seg.group_maps, seg.group_dropped, seg.count, seg.per};
+            hipLaunchKernelGGL((delta_join_kernel<DP, true>), dim3(heads, DP / 16 + slices, seg.groups - 1), dim3(DP * 4), 0, s,
+                               in_groups, dk, dv);
+            const Chain of_groups{seg.group_maps, seg.group_dropped, first, seg.group_states, nullptr, seg.groups, seg.groups};
+            hipLaunchKernelGGL((delta_join_kernel<DP, false>), dim3(heads, slices), dim3(DP * 4), 0, s, of_groups, dk, dv);
+            first = seg.group_states;
+        }
+        const Chain of_segments{seg.maps, seg.dropped, first, seg.states, nullptr, seg.count, seg.per};
+        hipLaunchKernelGGL((delta_join_kernel<DP, false>), dim3(heads, slices, seg.groups), dim3(DP * 4), 0, s, of_segments, dk,
+                           dv);
     }
     hipLaunchKernelGGL((delta_forward_kernel<T, DP, WIDE, false>), dim3(heads, seg.count), dim3(DP * 4), 0, s, a, seg);
 }
@@ -309,10 +370,15 @@ int forward(const char* who, const nesle_delta_args& x, hipStream_t s) {
     const DeltaArgs<T> a = delta_args<T>(x);
     Segments seg = segments(x);
     if (seg.count > 1) {
-        const std::size_t slots = static_cast<std::size_t>(seg.count) * a.batch * a.hv;
+        const std::size_t heads = static_cast<std::size_t>(a.batch) * a.hv, slots = seg.count * heads;
+        const std::size_t groups = seg.groups > 1 ? seg.groups * heads : 0;
+        const std::size_t map_size = static_cast<std::size_t>(a.dk_dim) * (a.dk_dim + a.dv_dim), size = static_cast<std::size_t>(a.dk_dim) * a.dv_dim;
         seg.maps = a.scratch;
-        seg.states = seg.maps + slots * a.dk_dim * (a.dk_dim + a.dv_dim);
-        seg.dropped = reinterpret_cast<std::uint32_t*>(seg.states + slots * a.dk_dim * a.dv_dim);
+        seg.states = seg.maps + slots * map_size;
+        seg.group_maps = seg.states + slots * size;
+        seg.group_states = seg.group_maps + groups * map_size;
+        seg.dropped = reinterpret_cast<std::uint32_t*>(seg.group_states + groups * size);
+        seg.group_dropped = seg.dropped + slots;
     }
     const std::uint32_t dim = wide_rows(x) ? 0 : padded_dim(x);
     switch (dim) {

@@ -236,6 +236,34 @@ def test_delta_segments_keep_what_is_not_finite():
     assert O.off(out[777:, 1], want[777:, 1]) <= F32 and torch.isfinite(got[1]).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,resets", [((6753, 1, 1, 1, 64, 64), 0.0), ((6760, 1, 1, 2, 32, 24), 0.002),
+                                          ((6784, 2, 1, 1, 72, 128), 0.001)])
+def test_delta_segments_in_groups(shape, resets, dtype):
+    """Lengths whose segments are joined in groups, with their gradient."""
+    say(f"[gpu] gated_delta in groups {shape} {dtype}")
+    check_delta(*make(*shape, dtype, seed=sum(shape), resets=resets))
+
+
+def test_delta_groups_keep_what_is_not_finite():
+    """As above, with the resets in later groups of segments."""
+    from nesle_amd import memory
+
+    say("[gpu] gated_delta in groups, not finite")
+    x, resets, _ = make(6800, 2, 1, 1, 32, 32, torch.float32, 23, resets=0.0)
+    clean = O.delta(*(x[n] for n in NAMES), resets, 32 ** -0.5)[0]
+    resets[4501, 0] = resets[6377, 1] = True
+    x["state"][0] = float("nan")
+    x["v"][2300, 1, 0, 7] = float("inf")
+    got = memory.gated_delta(*(x[n].to(dev()) for n in NAMES[:5]), state=x["state"].to(dev()), resets=resets.to(dev()))
+    out = got[0].cpu()
+    y = {n: torch.where(torch.isfinite(t), t, torch.zeros_like(t)) for n, t in x.items()}
+    want = O.delta(*(y[n] for n in NAMES), resets, 32 ** -0.5)[0]
+    assert torch.isnan(out[:4501, 0]).all() and O.off(out[4501:, 0], want[4501:, 0]) <= F32
+    assert O.off(out[:2300, 1], clean[:2300, 1]) <= F32 and not torch.isfinite(out[2300:6377, 1, 0, 7]).any()
+    assert O.off(out[6377:, 1], want[6377:, 1]) <= F32 and torch.isfinite(got[1]).all()
+
+
 def test_delta_gradient_against_differences():
     """The kernel's gradient along a direction against central differences of
     the float64 definition: their own error is about h^2 = 1e-8 and 1e-16 / h =
