@@ -18,26 +18,30 @@
 //
 // The part over value columns runs a wave per 16 columns, as in the forward;
 // the part that sums over the value dimension runs a wave per 16 key columns,
-// on U, dR and dO left in LDS, S read again and dS passed through LDS 32
-// columns at a time.  No atomics: sums over waves are added in a fixed order.
+// on U, dR and dO left in LDS, S and dS passed through LDS 32 columns at a time.
+// No atomics: sums over waves are added in a fixed order.
 #include "mem_delta_tile.h"
 
 namespace nesle::mem {
 namespace {
 
+// 32 columns of a state or its gradient, transposed: [value column][key].
+template <typename T, int DP, int PAD>
+using Slab = typename MathOf<T>::type::template Tile<32, DP, kNear, PAD>;
+
 template <typename T, int DP>
-struct GradTile : ChunkTile<T, DP, kFull> {
-    using Base = ChunkTile<T, DP, kFull>;
+struct GradTile : ChunkTile<T, DP, kFull, Slab<T, DP, 8>> {
+    using Base = ChunkTile<T, DP, kFull, Slab<T, DP, 8>>;
     using M = typename Base::M;
     typename M::template Tile<kChunk, DP, kExact, 8> dout;
-    // Transposed: [value column][token], [value column of 32][key].  With rows of
-    // 18 and 42 words (mod 64) the transposing reads meet no bank twice.
+    // Transposed: [value column][token].  With rows of 18 and 42 words (mod 64)
+    // the transposing reads meet no bank twice.
     typename M::template Tile<DP, kChunk, kFull, 4> u;
     union {
         typename M::template Tile<DP, kChunk, kFull, 4> dr;
         Results<T, DP> keys[2];                            // dQ and dK, once dR has been read
     };
-    typename M::template Tile<32, DP, kNear, DP == 32 ? 4 : 20> slab;
+    Slab<T, DP, DP == 32 ? 4 : 20> slab;
     float row_beta[Base::kWaves][kChunk], row_gate[Base::kWaves][kChunk], row_after[Base::kWaves][kChunk];
     float place_beta[3][16], cross[4][16];     // of a tile: sums over columns; pairs that cross a token
     float whole[Base::kWaves];
@@ -71,7 +75,6 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
     for (std::uint32_t t1 = a.steps; t1 > 0;) {
         const Lane<DP> at = Lane<DP>::anew();
         const int r = at.r, g = at.g;
-        const bool in_k = at.col < static_cast<int>(a.dk_dim);
         // A chunk from its start to t1.  Where it drops the state, gammas and
         // decays are zero across that token, as in the forward.
         const std::uint32_t start = (t1 - 1) / kChunk * kChunk;
@@ -223,41 +226,38 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
                 if (g == 0) sh.cross[3][r] = cross_below;
             }
         }
-        // dO S^T and dR S^T, then U dS^T: this wave's 16 key columns.
+        // dO S^T and dR S^T, then U dS^T: this wave's 16 key columns.  The waves
+        // that hold 32 columns put them in one of two places in turn; the second
+        // is free once all have passed a barrier.
         f4 dQ[2] = {}, dK[2] = {}, drs[2] = {};
-        if (from != nullptr) {
-            const Rows<float, false> states(from + head * state_size, of_chunk ? a.dk_dim : a.dv_dim);
+        const auto pass = [&](const f4 (&x)[KT], int i, int turns, const auto& use) {
+            const auto put = [&](auto& to) {
+                if (at.wave / 2 == i)
 #pragma unroll
-            for (int i = 0; i < KP; ++i) {
-                f4 part[2];
+                    for (int j = 0; j < KT; ++j) to.put4(16 * (at.wave % 2) + r, 16 * j + 4 * g, x[j]);
+                __syncthreads();
+                use(i, to.cols(0, 16 * at.wave, r, g));
+            };
+            if (turns % 2 == 0) put(sh.slab);
+            else put(sh.later);
+        };
+        if (KP == 1 || from != nullptr) {
 #pragma unroll
-                for (int o = 0; o < 2; ++o) {
-                    const int v = 32 * i + 16 * o + 4 * g;
-                    const bool inside = in_k && v < static_cast<int>(a.dv_dim);
-                    if (!of_chunk) part[o] = states.get4(inside, at.col, v);
-                    else
+            for (int i = 0; i < KP; ++i)
+                pass(S, i, i, [&](int i, const auto& s) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) part[o][j] = states.value_of(states.get(inside, v + j, at.col));
-                }
-                const auto s = M::near(part[0], part[1]);
-#pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    dQ[m] = M::mul(sh.dout.rows(16 * m, i, r, g), s, dQ[m]);
-                    drs[m] = M::mul(sh.dr.template cols<kNear>(32 * i, 16 * m, r, g), s, drs[m]);
-                }
-            }
+                    for (int m = 0; m < 2; ++m) {
+                        dQ[m] = M::mul(sh.dout.rows(16 * m, i, r, g), s, dQ[m]);
+                        drs[m] = M::mul(sh.dr.template cols<kNear>(32 * i, 16 * m, r, g), s, drs[m]);
+                    }
+                });
         }
 #pragma unroll
-        for (int i = 0; i < KP; ++i) {
-            if (at.wave / 2 == i)
+        for (int i = 0; i < KP; ++i)
+            pass(dS, i, KP + i, [&](int i, const auto& ds) {
 #pragma unroll
-                for (int j = 0; j < KT; ++j) sh.slab.put4(16 * (at.wave % 2) + r, 16 * j + 4 * g, dS[j]);
-            __syncthreads();
-            const auto ds = sh.slab.cols(0, 16 * at.wave, r, g);
-#pragma unroll
-            for (int m = 0; m < 2; ++m) dK[m] = M::mul(sh.u.template cols<kNear>(32 * i, 16 * m, r, g), ds, dK[m]);
-            if (i + 1 < KP) __syncthreads();
-        }
+                for (int m = 0; m < 2; ++m) dK[m] = M::mul(sh.u.template cols<kNear>(32 * i, 16 * m, r, g), ds, dK[m]);
+            });
         const auto key = sh.k.cols(0, 16 * at.wave, r, g), query = sh.q.cols(0, 16 * at.wave, r, g);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {

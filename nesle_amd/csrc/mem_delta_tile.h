@@ -233,17 +233,24 @@ struct Results<bf16, DP> {
 };
 
 // DP: head dimensions padded to 32, 64 or 128; DP / 16 waves.  P_PLANES: of P.
-template <typename T, int DP, int P_PLANES>
+// Later: what takes the place of the values, A and the results afterwards.
+template <typename T, int DP, int P_PLANES, typename Later = char>
 struct ChunkTile {
     using M = typename MathOf<T>::type;
     static constexpr int KT = DP / 16, KP = DP / 32, kWaves = DP / 16, kSmall = kChunk + 4;
 
-    typename M::template Tile<kChunk, DP, kExact, 8> k, q, v;
+    typename M::template Tile<kChunk, DP, kExact, 8> k, q;
     typename M::template Tile<kChunk, kChunk, P_PLANES, 8> p;     // P: scale L_ij (q_i . k_j), j <= i; else 0
     typename M::template Tile<kChunk, kChunk, kFull, 8> t;     // (I + A)^-1
     union {
-        alignas(16) float a[kChunk * kSmall];  // A without beta: L_ij (k_i . k_j), j < i; else 0
-        Results<T, DP> results;                // of the values, once A is inverted
+        struct {
+            typename M::template Tile<kChunk, DP, kExact, 8> v;
+            union {
+                alignas(16) float a[kChunk * kSmall];  // A without beta: L_ij (k_i . k_j), j < i; else 0
+                Results<T, DP> results;                // of the values, once A is inverted
+            };
+        };
+        Later later;
     };
     alignas(16) double G[kChunk];              // running sum of g: differences of it are taken
     alignas(16) float gamma[kChunk], decay[kChunk], beta[kChunk];
