@@ -84,7 +84,7 @@ inline bool wide_rows(const nesle_delta_args& a) {
     return heads * (a.k_dim > a.v_dim ? a.k_dim : a.v_dim) * 4 >= limit;
 }
 
-// Arguments that no call may have; `step`: of nesle_delta_step.
+// Arguments that no call may have.
 inline int check_delta(const char* who, const nesle_delta_args* a) {
     if (a == nullptr) return refuse(who, "null arguments");
     if (a->dtype != NESLE_MEM_F32 && a->dtype != NESLE_MEM_BF16) return refuse(who, "dtype must be NESLE_MEM_F32 or NESLE_MEM_BF16");

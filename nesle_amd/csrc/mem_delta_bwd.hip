@@ -20,6 +20,16 @@
 // the part that sums over the value dimension runs a wave per 16 key columns,
 // on U, dR and dO left in LDS, S and dS passed through LDS 32 columns at a time.
 // No atomics: sums over waves are added in a fixed order.
+//
+// Bound by neither memory nor the matrix units: 128 steps of 512 consoles of 4 heads
+// of 64 in bfloat16 take 230 us, where the 0.30 GB they move take 61 us at a large
+// copy's rate and the products' instructions 40 us.  79 KB of LDS and 246 registers
+// leave two waves a SIMD, whose vector units are busy half the time (with cutting
+// float32 values in three, masks, and addresses), in a chain of eight parts
+// between barriers.  With the parts left out one at a time: tiles of dP and dA
+// -15 us, the sums over columns -10, loads ahead -7, the inverse -8, the gates' end
+// -4, results -1.  64 consoles in float32: 66 us, of which the float32 matrix
+// instructions are 21.
 #include "mem_delta_tile.h"
 
 namespace nesle::mem {
@@ -71,10 +81,18 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
         in.fetch(a, start, static_cast<int>(end - start), env, h, at);
         in.part(a.dout, a.dv_dim, start, static_cast<int>(end - start), env, h, at, dout);
     };
-    if (a.steps != 0) fetch(a.steps, first);
+    // As in the forward, the wave that inverts (turn 0) reads the states first
+    // and has no tile; the last one stages the next chunk's gates meanwhile.
+    const int turn = (first.wave + static_cast<int>(blockIdx.x)) % kWaves;
+    if (a.steps != 0) {
+        fetch(a.steps, first);
+        if (turn == kWaves - 1) sh.gates[0].stage(in, static_cast<int>((a.steps - 1) % kChunk) + 1, first.lane);
+    }
+    int which = 0;
     for (std::uint32_t t1 = a.steps; t1 > 0;) {
         const Lane<DP> at = Lane<DP>::anew();
         const int r = at.r, g = at.g;
+        Gates& now = sh.gates[which];
         // A chunk from its start to t1.  Where it drops the state, gammas and
         // decays are zero across that token, as in the forward.
         const std::uint32_t start = (t1 - 1) / kChunk * kChunk;
@@ -89,7 +107,6 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
 
         sh.stage(in, at);
         sh.dout.put8(at.key_row, at.key_col, dout);
-        if (at.wave == 0) sh.stage_gates(in, n, at.lane);
         t1 = start;
         if (t1 > 0) fetch(t1, at);
         __syncthreads();
@@ -107,28 +124,27 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
                 }
             }
         };
-        // As in the forward, the wave that inverts reads the states first and
-        // has no tile.
-        const int turn = (at.wave + static_cast<int>(blockIdx.x)) % kWaves;
         if (turn == 0 || turn > 3) {
             read_states();
         } else {
 #pragma unroll
             for (int j = 0; j < kPlaces; ++j)
-                if (turn - 1 + j * (kWaves - 1) < 3) sh.products(turn - 1 + j * (kWaves - 1), a.scale, at, kk[j], qk[j]);
+                if (turn - 1 + j * (kWaves - 1) < 3) sh.products(turn - 1 + j * (kWaves - 1), a.scale, now, at, kk[j], qk[j]);
         }
         __syncthreads();
-        if (turn == 0) sh.invert(at);
+        if (turn == 0) sh.invert(now, at);
         else if (turn <= 3) read_states();
+        which ^= 1;
+        if (turn == kWaves - 1 && t1 > 0) sh.gates[which].stage(in, kChunk, at.lane);
         f4 V[2], dO[2], Y[2], gam[2], dec[2], beta[2];
         M::values(sh.v.cols(0, 16 * at.wave, r, g), V);
         const auto grad = sh.dout.cols(0, 16 * at.wave, r, g);
         M::values(grad, dO);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            gam[m] = sh.of_rows(sh.gamma, m, g);
-            dec[m] = sh.of_rows(sh.decay, m, g);
-            beta[m] = sh.of_rows(sh.beta, m, g);
+            gam[m] = now.of_rows(now.gamma, m, g);
+            dec[m] = now.of_rows(now.decay, m, g);
+            beta[m] = now.of_rows(now.beta, m, g);
             Y[m] = V[m] - gam[m] * ks[m];
         }
         const auto right = M::full(beta[0] * Y[0], beta[1] * Y[1]);
@@ -152,7 +168,7 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
         sh.results.put(dv, static_cast<int>(a.dv_dim), n, at, dV);
 
         // Sums over the value dimension of dbeta and the gates, this wave's share.
-        const float last = sh.gamma[kChunk - 1];
+        const float last = now.gamma[kChunk - 1];
         float whole = 0.0f;
 #pragma unroll
         for (int i = 0; i < KT; ++i)
@@ -209,7 +225,7 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int row = mi + 4 * g + i, c = nj + r;
-                const float L = sh.ratio(row, c), b = sh.beta[row];
+                const float L = now.ratio(row, c), b = now.beta[row];
                 sh.p.template put<kNear>(row, c, c <= row ? a.scale * L * dP[i] : 0.0f);
                 sh.t.template put<kNear>(row, c, c < row ? -b * L * dA[i] : 0.0f);
                 const float by_a = -dA[i] * kk[j][i];

@@ -50,9 +50,25 @@ struct Segments {
     std::uint32_t* group_dropped;
 };
 
+// What LDS leaves room for.
+template <typename T, int DP>
+constexpr int kWavesPerSimd = DP == 128 ? 2 : DP == 64 && sizeof(T) == 2 ? 4 : 3;
+
 // MAP: the segment's M and B; else outputs and states.
+//
+// Bound by memory where there are many heads: 128 steps of 512 consoles of 4 heads
+// of 64 in bfloat16 move 0.30 GB (inputs, outputs, the states in and out and the
+// ones kept for the gradient) in 82 us, 3.7 TB/s against a large copy's 4.9.  With
+// the parts left out one at a time: kept states -19 us, first and last states -20,
+// loads of the inputs -17, outputs -14, the inverse -4.  With one workgroup a compute
+// unit a chunk takes 3.6 us, a chain of short parts: inverse 0.7, loads 0.2,
+// products and the tests of what is not finite 0.1 each; in float32 4.8 us (28 us
+// for 64 consoles, of which the float32 matrix instructions are the most).  A
+// chunk of 32 tokens is one inner step of the bfloat16 instruction and the
+// largest whose inverse one wave finds in registers; its tile leaves room for
+// four workgroups a compute unit.
 template <typename T, int DP, bool WIDE, bool MAP>
-__global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_forward_kernel(DeltaArgs<T> a, Segments seg) {
+__global__ void __launch_bounds__(DP * (MAP ? 8 : 4), (kWavesPerSimd<T, DP>)) delta_forward_kernel(DeltaArgs<T> a, Segments seg) {
     using Tile = ChunkTile<T, DP, kNear>;
     using M = typename Tile::M;
     constexpr int KT = Tile::KT, KP = Tile::KP, kWaves = Tile::kWaves * (MAP ? 2 : 1);
@@ -86,12 +102,24 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_f
         const std::uint32_t whole = kChunk - t0 % kChunk, left = end - t0;
         return static_cast<int>(whole < left ? whole : left);
     };
+    // The inverse takes one wave as long as the rest of its part takes the
+    // others: that wave (turn 0) has no tile of A and P, and reads the state
+    // first.  The last one stages the next chunk's gates meanwhile.  Other waves
+    // each workgroup, as the waves of a compute unit's workgroups share its four
+    // SIMDs by their number.
+    const int turn = (first.wave + static_cast<int>(blockIdx.x)) % kWaves;
     Ahead<T, DP, WIDE> in;
     bool any_drop = false;
-    if (begin < end) in.template fetch<!MAP>(a, begin, width(begin), env, h, first);
+    std::uint32_t odd_gates = 0;
+    if (begin < end) {
+        in.template fetch<!MAP>(a, begin, width(begin), env, h, first);
+        if (turn == kWaves - 1) odd_gates = sh.gates[0].stage(in, width(begin), first.lane);
+    }
+    int which = 0;
     for (std::uint32_t t0 = begin; t0 < end;) {
         const Lane<DP> at = Lane<DP>::anew();
         const int r = at.r, g = at.g;
+        Gates& now = sh.gates[which];
         if (!MAP && t0 != 0 && t0 % kChunk == 0 && a.saved != nullptr)
             Tile::keep(a, a.saved + (t0 / kChunk - 1) * state_size * a.batch * a.hv, head, at, S);
         const std::uint32_t drops = in.drops();
@@ -104,7 +132,7 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_f
         for (;;) {
             sh.template stage<!MAP>(in, at);
             std::uint32_t odd = in.odd();
-            if (at.wave == 0) odd |= sh.stage_gates(in, n, at.lane);
+            odd |= odd_gates;
             if (inside != 0 && !Tile::finite(S)) odd |= inside;
             sh.report(odd);
             __syncthreads();
@@ -116,6 +144,7 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_f
             in.cut(n);
             __syncthreads();
             if (at.tid == 0) sh.bad = 0;
+            if (turn == kWaves - 1) odd_gates = now.stage(in, n, at.lane);
             __syncthreads();
         }
         const std::uint32_t next = t0 + n;
@@ -133,29 +162,26 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_f
                 }
             }
         };
-        // The inverse takes one wave as long as the rest of this part takes the
-        // others: that wave has no tile of A and P, and reads the state first.
-        // Another wave each workgroup, as the waves of a compute unit's
-        // workgroups share its four SIMDs by their number.
-        const int turn = (at.wave + static_cast<int>(blockIdx.x)) % kWaves;
         if (turn == 0 || turn > 3) {
             read_state();
         } else {
             for (int place = turn - 1; place < 3; place += kWaves - 1) {
                 f4 kk, qk;
-                sh.template products<!MAP>(place, a.scale, at, kk, qk);
+                sh.template products<!MAP>(place, a.scale, now, at, kk, qk);
             }
         }
         __syncthreads();
         if (at.tid == 0) sh.bad = 0;
-        if (turn == 0) sh.invert(at);
+        if (turn == 0) sh.invert(now, at);
         else if (turn <= 3) read_state();
+        which ^= 1;
+        if (turn == kWaves - 1 && next < end) odd_gates = sh.gates[which].stage(in, width(next), at.lane);
         f4 R[2], V[2] = {};
         if (!MAP || at.wave < KT) M::values(sh.v.cols(0, 16 * at.wave, r, g), V);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            const f4 gam = sh.of_rows(sh.gamma, m, g);
-            R[m] = sh.of_rows(sh.beta, m, g) * (V[m] - gam * ks[m]);
+            const f4 gam = now.of_rows(now.gamma, m, g);
+            R[m] = now.of_rows(now.beta, m, g) * (V[m] - gam * ks[m]);
             qs[m] *= gam * a.scale;
         }
         const auto right = M::full(R[0], R[1]);
@@ -170,8 +196,8 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), DP == 128 ? 2 : 4) delta_f
             for (int m = 0; m < 2; ++m) O[m] = M::mul(sh.p.rows(16 * m, 0, r, g), u, qs[m]);
             sh.results.put(out, static_cast<int>(a.dv_dim), n, at, O);
         }
-        const float last = sh.gamma[kChunk - 1];
-        const auto w = M::full(U[0] * sh.of_rows(sh.decay, 0, g), U[1] * sh.of_rows(sh.decay, 1, g));
+        const float last = now.gamma[kChunk - 1];
+        const auto w = M::full(U[0] * now.of_rows(now.decay, 0, g), U[1] * now.of_rows(now.decay, 1, g));
 #pragma unroll
         for (int i = 0; i < KT; ++i) S[i] = S[i] * last + M::mul(sh.k.cols(0, 16 * i, r, g), w, zero);
         t0 = next;

@@ -28,7 +28,6 @@ struct F32Math {
     static __device__ Op full(f4 a, f4 b) { return {a, b}; }
     static __device__ Op near(f4 a, f4 b) { return {a, b}; }
     static __device__ Op near(const Op& x) { return x; }
-    static __device__ Op exact(f4 a, f4 b) { return {a, b}; }
     static __device__ f4 mul(const Op& x, const Op& y, f4 c) { return mma(x.b, y.b, mma(x.a, y.a, c)); }
     // The two result tiles that an operand of inputs holds.
     static __device__ void values(const Op& x, f4 (&to)[2]) {
@@ -115,7 +114,6 @@ struct SplitMath {
     static __device__ Op<kFull> full(f4 a, f4 b) { return operand<kFull>(a, b); }
     static __device__ Op<kNear> near(f4 a, f4 b) { return operand<kNear>(a, b); }
     static __device__ Op<kNear> near(const Op<kFull>& o) { return {{o.x[0], o.x[1]}}; }
-    static __device__ Op<kExact> exact(f4 a, f4 b) { return operand<kExact>(a, b); }      // values that are bfloat16
     // The two result tiles that an operand of inputs holds.
     static __device__ void values(const Op<kExact>& o, f4 (&to)[2]) {
         const u4 w = o.x[0];

@@ -1,11 +1,14 @@
 // One token of the gated delta rule for every console (acting): each state is
 // read once and written once, which is all the work there is (8 bytes an
 // element against 7 operations), so the kernel is bound by memory, and by
-// latency for a few consoles.
+// latency for a few consoles.  Measured against a large copy's 4.9 TB/s: 8,192
+// consoles of 4 heads of 64 x 64, 1.09 GB in 207 us (5.3 TB/s); 1,000 of 6 heads
+// of 48 x 40 in float32, 95 MB in 22.6 us (4.2 TB/s); one console 3.9 us, a launch.
 //
 // A wave holds all k_dim rows of COLS columns of one state in registers, four
-// columns a lane: 64 / (COLS / 4) lanes share the rows of a column group.
-// Columns do not interact, so nothing crosses a wave and the state may be
+// columns a lane: 64 / (COLS / 4) lanes share the rows of a column group.  With 16
+// columns a row's loads are 64 bytes together, and one console's 4 heads of 64 are
+// 16 waves.  Columns do not interact, so nothing crosses a wave and the state may be
 // updated in place.  With D = a S (S^T k and S^T q read in one pass):
 //   u = beta (v - D^T k),  out = scale (D^T q + (k . q) u),  S <- D + k u^T
 #include "mem_delta.h"

@@ -232,6 +232,41 @@ struct Results<bf16, DP> {
     }
 };
 
+// What a chunk's gates come to: two of these, one staged while the other is used.
+struct Gates {
+    alignas(16) double G[kChunk];              // running sum of g: differences of it are taken
+    alignas(16) float gamma[kChunk], decay[kChunk], beta[kChunk];
+
+    // Of the tokens below n (one wave); other rows neither decay nor write.
+    // Returns the bits of tokens whose gate or write strength is not finite.
+    template <typename T, int DP, bool WIDE>
+    __device__ std::uint32_t stage(const Ahead<T, DP, WIDE>& in, int n, int lane) {
+        const bool use = lane < n;
+        const float g = !use ? 0.0f : in.drop() ? kGone : in.value(in.g), b = use ? in.value(in.beta) : 0.0f;
+        double sum = g;
+#pragma unroll
+        for (int d = 1; d < kChunk; d *= 2) {
+            const double below = __shfl_up(sum, d);
+            if (lane >= d) sum += below;
+        }
+        const double end = __shfl(sum, kChunk - 1);
+        if (lane < kChunk) {
+            G[lane] = sum;
+            gamma[lane] = expf(static_cast<float>(sum));
+            decay[lane] = expf(static_cast<float>(end - sum));
+            beta[lane] = b;
+        }
+        return fabsf(b) < INFINITY && g < INFINITY ? 0u : 1u << lane;
+    }
+    // Of a wave's token rows.
+    static __device__ f4 of_rows(const float* x, int m, int g) { return *reinterpret_cast<const f4*>(x + 16 * m + 4 * g); }
+    // L_ij.  exp2 of the rounded product is off by |x| 2^-24 of itself, which
+    // is 2^-25 of 1 at most where L <= 1.
+    __device__ float ratio(int i, int j) const {
+        return __builtin_amdgcn_exp2f(static_cast<float>(G[i] - G[j]) * 1.44269504f);
+    }
+};
+
 // DP: head dimensions padded to 32, 64 or 128; DP / 16 waves.  P_PLANES: of P.
 // Later: what takes the place of the values, A and the results afterwards.
 template <typename T, int DP, int P_PLANES, typename Later = char>
@@ -252,8 +287,7 @@ struct ChunkTile {
         };
         Later later;
     };
-    alignas(16) double G[kChunk];              // running sum of g: differences of it are taken
-    alignas(16) float gamma[kChunk], decay[kChunk], beta[kChunk];
+    Gates gates[2];
     unsigned bad;                              // tokens with a value that is not finite
 
     // ---- matrices [k_dim][cols] beside a head's keys (its state and its
@@ -334,39 +368,9 @@ struct ChunkTile {
         v.put8(at.key_row, at.key_col, in.v);
     }
 
-    // Gates and write strengths of the tokens below n (one wave); other rows
-    // neither decay nor write.
-    template <bool WIDE>
-    __device__ std::uint32_t stage_gates(const Ahead<T, DP, WIDE>& in, int n, int lane) {
-        const bool use = lane < n;
-        const float g = !use ? 0.0f : in.drop() ? kGone : in.value(in.g), b = use ? in.value(in.beta) : 0.0f;
-        double sum = g;
-#pragma unroll
-        for (int d = 1; d < kChunk; d *= 2) {
-            const double below = __shfl_up(sum, d);
-            if (lane >= d) sum += below;
-        }
-        const double end = __shfl(sum, kChunk - 1);
-        if (lane < kChunk) {
-            G[lane] = sum;
-            gamma[lane] = expf(static_cast<float>(sum));
-            decay[lane] = expf(static_cast<float>(end - sum));
-            beta[lane] = b;
-        }
-        return fabsf(b) < INFINITY && g < INFINITY ? 0u : 1u << lane;
-    }
     // Tokens with something that is not finite, from all waves.
     __device__ void report(std::uint32_t bits) {
         if (__any(bits != 0)) atomicOr(&bad, bits);
-    }
-
-    // Of a wave's token rows.
-    __device__ f4 of_rows(const float* x, int m, int g) const { return *reinterpret_cast<const f4*>(x + 16 * m + 4 * g); }
-
-    // L_ij.  exp2 of the rounded product is off by |x| 2^-24 of itself, which
-    // is 2^-25 of 1 at most where L <= 1.
-    __device__ float ratio(int i, int j) const {
-        return __builtin_amdgcn_exp2f(static_cast<float>(G[i] - G[j]) * 1.44269504f);
     }
 
     // A tile of 16x16 token pairs on or below the diagonal: place 0, 1, 2 starts
@@ -377,7 +381,7 @@ struct ChunkTile {
     // k_i . k_j and q_i . k_j of a tile, times L_ij and zero where j is not
     // before (not after) i; into A and P.
     template <bool QUERIES = true>
-    __device__ void products(int place, float scale, const Lane<DP>& at, f4& kk, f4& qk) {
+    __device__ void products(int place, float scale, const Gates& now, const Lane<DP>& at, f4& kk, f4& qk) {
         const int mi = first_row(place), nj = first_col(place);
         kk = qk = f4{0, 0, 0, 0};
 #pragma unroll
@@ -389,7 +393,7 @@ struct ChunkTile {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int row = mi + 4 * at.g + i, col = nj + at.r;
-            const float L = ratio(row, col);
+            const float L = now.ratio(row, col);
             kk[i] = col < row ? kk[i] * L : 0.0f;
             qk[i] = col <= row ? qk[i] * L * scale : 0.0f;
             a[row * kSmall + col] = kk[i];
@@ -402,11 +406,11 @@ struct ChunkTile {
     // entry is known it is taken out of all below, and the lane of row m hands
     // its A[m][i] to the others.  The block below the diagonal is
     // -T1 (A10 T0), its factors read from where A's diagonal tiles were.
-    __device__ void invert(const Lane<DP>& at) {
+    __device__ void invert(const Gates& now, const Lane<DP>& at) {
         const int b = at.g % 2, r = at.r, g = at.g;
         float x[16], row[16];
         const float* from = &a[(16 * b + r) * kSmall + 16 * b];
-        const float less = -beta[16 * b + r];
+        const float less = -now.beta[16 * b + r];
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
             const f4 w = *reinterpret_cast<const f4*>(from + i);
@@ -427,7 +431,7 @@ struct ChunkTile {
         __builtin_amdgcn_wave_barrier();       // in order within the wave
         const f4 zero = {0, 0, 0, 0};
         const f4 t0 = down<kSmall>(a, 0, 0, r, g), t1 = down<kSmall>(a, 16, 16, r, g);
-        const f4 w = mma(along<kSmall>(a, 16, 0, r, g) * beta[16 + r], t0, zero);
+        const f4 w = mma(along<kSmall>(a, 16, 0, r, g) * now.beta[16 + r], t0, zero);
         const f4 below = mma(along<kSmall>(a, 16, 16, r, g), w, zero);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

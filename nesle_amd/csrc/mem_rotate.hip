@@ -9,7 +9,14 @@
 // PAIRS is what a 16-byte load holds, or four where the sizes or addresses do
 // not allow eight bfloat16.
 //
-// Bound by memory: about 10 operations an element.
+// Bound by memory: about 10 operations an element.  Measured against a large
+// copy's 4.9 TB/s, bfloat16: 1.08 GB of 128 steps of 4,096 rows and 8 heads of 64
+// in 222 us (4.9 TB/s); 128 steps of 512 rows, forward 134 MB in 29 us (4.6 TB/s),
+// gradient 134 MB more in 55 us (3.7 TB/s: twice the tensors in flight, and sums
+// over lanes) and the weights' sum 5 us.  One load of 8 bytes a lane for each
+// operand in place of 16 took 309 us for the first; heads of one row side by side
+// in a thread, which share a row of the table, 338 us.  Below about 100 rows a call
+// is a launch: 3.4 us.
 #include <initializer_list>
 
 #include "mem_common.h"
