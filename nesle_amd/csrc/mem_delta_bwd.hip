@@ -179,14 +179,11 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
             const f4 by_beta = dR[m] * Y[m];
             const f4 e = dec[m] * kds[m] * U[m];
             const f4 by_gate = gam[m] * a.scale * dO[m] * qs[m] - X[m] * ks[m];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float sb = sum16(by_beta[i]), sg = sum16(by_gate[i]), se = sum16(e[i]);
-                if (r == 0) {
-                    sh.row_beta[at.wave][16 * m + 4 * g + i] = sb;
-                    sh.row_gate[at.wave][16 * m + 4 * g + i] = sg;
-                    sh.row_after[at.wave][16 * m + 4 * g + i] = se;
-                }
+            const float sb = sum16_of(by_beta), sg = sum16_of(by_gate), se = sum16_of(e);
+            if (r % 4 == 0) {
+                sh.row_beta[at.wave][16 * m + 4 * g + r / 4] = sb;
+                sh.row_gate[at.wave][16 * m + 4 * g + r / 4] = sg;
+                sh.row_after[at.wave][16 * m + 4 * g + r / 4] = se;
             }
         }
         whole = over_groups(sum16(whole)) * last;
@@ -222,22 +219,28 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
             // With token t = 16 x + r in lane r: pairs of this tile with
             // j < t <= i.  Tile (16, 0) has them for both halves of t.
             float cross = 0.0f, cross_below = 0.0f;
+            f4 by_a, pairs;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int row = mi + 4 * g + i, c = nj + r;
                 const float L = now.ratio(row, c), b = now.beta[row];
                 sh.p.template put<kNear>(row, c, c <= row ? a.scale * L * dP[i] : 0.0f);
                 sh.t.template put<kNear>(row, c, c < row ? -b * L * dA[i] : 0.0f);
-                const float by_a = -dA[i] * kk[j][i];
-                const float before_t = sum_below(c < row ? dP[i] * qk[j][i] + b * by_a : 0.0f);
+                by_a[i] = -dA[i] * kk[j][i];
+                pairs[i] = c < row ? dP[i] * qk[j][i] + b * by_a[i] : 0.0f;
+                const float before_t = sum_below(pairs[i]);
                 cross += place == 1 || row >= c ? before_t : 0.0f;
-                const float sb = sum16(by_a), all = sum16(c < row ? dP[i] * qk[j][i] + b * by_a : 0.0f);
-                if (4 * g + i >= r) cross_below += all;
-                if (r == 0) sh.place_beta[place][4 * g + i] = sb;
             }
+            const float sb = sum16_of(by_a);
+            if (r % 4 == 0) sh.place_beta[place][4 * g + r / 4] = sb;
             cross = over_groups(cross);
             if (g == 0) sh.cross[place][r] = cross;
             if (place == 1) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float all = sum16(pairs[i]);
+                    if (4 * g + i >= r) cross_below += all;
+                }
                 cross_below = over_groups(cross_below);
                 if (g == 0) sh.cross[3][r] = cross_below;
             }

@@ -218,6 +218,25 @@ __device__ inline float sum16(float v) {
     v += moved<kRowRor + 2>(v);
     return v + moved<kRowRor + 1>(v);
 }
+// Four such sums at once, that of v[i] in the i-th four of the 16 lanes: as soon
+// as half the lanes hold a sum they take another's.
+template <int BANKS>
+__device__ float taken(float v, float from) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, v), __builtin_bit_cast(int, from), 0xe4, 0xf, BANKS, false));
+}
+__device__ inline float sum16_of(f4 v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float x = v[i];
+        v[i] = x + moved<kRowRor + 8>(x);
+    }
+    float x = taken<0xc>(v[0], v[2]), y = taken<0xc>(v[1], v[3]);
+    x += moved<kRowRor + 12>(x);
+    y += moved<kRowRor + 4>(y);
+    x = taken<0xa>(x, y);
+    x += moved<0xb1>(x);           // the other of two, then of two pairs
+    return x + moved<0x4e>(x);
+}
 // Sum over the lanes below in a row of 16.
 __device__ inline float sum_below(float v) {
     v += moved<kRowShr + 1>(v);
