@@ -74,6 +74,8 @@ void check_heads(const Common& c, const Tensor& t, const char* name) {
     }
 }
 
+bool on_16_bytes(const Tensor& t) { return reinterpret_cast<std::uintptr_t>(t.const_data_ptr()) % 16 == 0; }
+
 void check_plain(const Common& c, const Tensor& t, const char* name, at::ScalarType type, at::IntArrayRef sizes,
                  bool aligned = false) {
     if (t.scalar_type() != type || t.device() != c.device || t.sizes() != sizes || !t.is_contiguous()) {
@@ -81,7 +83,7 @@ void check_plain(const Common& c, const Tensor& t, const char* name, at::ScalarT
         want << "a contiguous " << type << " tensor of shape " << sizes << " on " << c.device;
         refuse(c.who, name, want.str(), t);
     }
-    if (aligned && reinterpret_cast<std::uintptr_t>(t.const_data_ptr()) % 16 != 0)
+    if (aligned && !on_16_bytes(t))
         refuse(c.who, name, "on a 16-byte boundary", t);
 }
 
@@ -109,8 +111,14 @@ Tensor floats(const Tensor& beside, uint64_t n) {
     return n == 0 ? Tensor() : at::empty({static_cast<int64_t>(n)}, beside.options().dtype(at::kFloat));
 }
 
-// A gradient as autograd hands it over, made readable where it is not.
+// Gradients as autograd hands them over, made readable where they are not: of
+// heads, and of states (a slice of a longer gradient may start anywhere).
 Tensor unit_last(const Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
+Tensor whole(const Tensor& t) {
+    const Tensor c = t.contiguous();
+    return on_16_bytes(c) ? c : c.clone();
+}
+Tensor zeros(const Tensor& t) { return at::zeros_like(t, t.options(), at::MemoryFormat::Contiguous); }
 
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
@@ -195,8 +203,8 @@ struct QkNormRotate : torch::autograd::Function<QkNormRotate> {
         {
             const at::AutoGradMode none(false);
             nesle_qk_args a = qk_args(q, k, wq, wk, saved[4], saved[5], ctx->saved_data["eps"].toDouble(), how & 1, how & 2);
-            const Tensor dq_out = grads[0].defined() ? unit_last(grads[0]) : at::zeros_like(q);
-            const Tensor dk_out = grads[1].defined() ? unit_last(grads[1]) : at::zeros_like(k);
+            const Tensor dq_out = grads[0].defined() ? unit_last(grads[0]) : zeros(q);
+            const Tensor dk_out = grads[1].defined() ? unit_last(grads[1]) : zeros(k);
             a.dq_out = heads(dq_out);
             a.dk_out = heads(dk_out);
             const Tensor dq = like(q), dk = like(k), dwq = wq.defined() ? like(wq) : Tensor(),
@@ -326,8 +334,8 @@ struct GatedDelta : torch::autograd::Function<GatedDelta> {
             const at::AutoGradMode none(false);
             nesle_delta_args a = delta_args(q, saved[1], v, saved[3], saved[4], state, saved[6],
                                             ctx->saved_data["scale"].toDouble());
-            const Tensor dout = grads[0].defined() ? unit_last(grads[0]) : at::zeros_like(v);
-            const Tensor dafter = grads[1].defined() ? grads[1].contiguous() : Tensor();
+            const Tensor dout = grads[0].defined() ? unit_last(grads[0]) : zeros(v);
+            const Tensor dafter = grads[1].defined() ? whole(grads[1]) : Tensor();
             const Tensor dq = like(q), dk = like(q), dv = like(v), dg = like(saved[3]), dbeta = like(saved[4]);
             const Tensor dstate = state.defined() && state.requires_grad() ? like(state) : Tensor();
             const Tensor scratch = floats(q, nesle_delta_scratch_floats(&a));
@@ -375,8 +383,8 @@ Tensor gated_delta_step(const Tensor& q, const Tensor& k, const Tensor& v, const
     const Tensor out = like(v);
     a.out = ptr(out);
     a.state_out = ptr<float>(*state);
-    check(nesle_delta_step(&a, stream_of(q)));
     state->unsafeGetTensorImpl()->bump_version();          // autograd sees the state change
+    check(nesle_delta_step(&a, stream_of(q)));
     return out;
 }
 

@@ -264,6 +264,23 @@ def test_delta_groups_keep_what_is_not_finite():
     assert O.off(out[6377:, 1], want[6377:, 1]) <= F32 and torch.isfinite(got[1]).all()
 
 
+def test_delta_gradient_of_a_state_that_starts_anywhere():
+    """The state's gradient may come as a slice of a longer one, off every
+    boundary: the same as by itself."""
+    from nesle_amd import memory
+
+    say("[gpu] gated_delta gradient of a slice")
+    x, resets, grads = make(40, 2, 1, 2, 24, 16, torch.float32, 29)
+    gpu = [x[n].to(dev()).requires_grad_() for n in NAMES]
+    out, state = memory.gated_delta(*gpu[:5], state=gpu[5], resets=resets.to(dev()))
+    whole = torch.cat((out.flatten()[:3], state.flatten()))
+    weight = torch.cat((torch.zeros(3), grads[1].flatten())).to(dev())
+    got = torch.autograd.grad(whole, gpu, weight, retain_graph=True)
+    want = torch.autograd.grad((out, state), gpu, (torch.zeros_like(out), grads[1].to(dev())))
+    for n, a, b in zip(NAMES, got, want):
+        assert torch.equal(a, b), n
+
+
 def test_delta_gradient_against_differences():
     """The kernel's gradient along a direction against central differences of
     the float64 definition: their own error is about h^2 = 1e-8 and 1e-16 / h =
