@@ -77,11 +77,12 @@ inline std::uint32_t padded_dim(const nesle_delta_args& a) {
 // Whether a chunk's rows of any tensor span 2^31 bytes or more, past what a
 // 32-bit offset reaches.
 inline bool wide_rows(const nesle_delta_args& a) {
-    const std::int64_t item = a.dtype == NESLE_MEM_F32 ? 4 : 2, limit = ((1ll << 31) - 4096) / kChunk;
+    const std::int64_t item = a.dtype == NESLE_MEM_F32 ? 4 : 2, limit = ((1ll << 31) - 4096) / (kChunk - 1);
     for (const nesle_heads* x : {&a.q, &a.k, &a.v, &a.dout})
         if (x->stride_t < 0 || x->stride_t * item >= limit) return true;
+    // What the kernels write: of the inputs' type, and shares of key heads' gradients in float32.
     const std::int64_t heads = static_cast<std::int64_t>(a.batch) * a.v_heads;
-    return heads * (a.k_dim > a.v_dim ? a.k_dim : a.v_dim) * 4 >= limit;
+    return heads * (a.k_dim > a.v_dim ? a.k_dim : a.v_dim) * (a.v_heads > a.k_heads ? 4 : item) >= limit;
 }
 
 // Arguments that no call may have.

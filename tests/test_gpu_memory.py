@@ -207,6 +207,24 @@ def test_delta_gradient_with_wide_strides():
     check_delta(x, resets, grads, move=move)
 
 
+@pytest.mark.parametrize("far", [((1 << 31) - 4096) // 62 // 8 * 8, ((1 << 31) - 4096) // 62 // 8 * 8 + 8])
+def test_delta_gradient_at_the_last_32_bit_stride(far):
+    """The largest steps whose chunks' rows a 32-bit offset reaches, and the next."""
+    say(f"[gpu] gated_delta steps of {far} elements, gradient")
+    buf = torch.empty(33 * far + 8192, dtype=torch.bfloat16, device=dev())
+    x, resets, grads = make(34, 2, 1, 2, 32, 32, torch.bfloat16, 30)
+    at = iter((0, 512, 1024))
+
+    def move(t):
+        if t.dim() != 4 or t.shape[0] != 34:
+            return t.to(dev())
+        cut = buf.as_strided(t.shape, (far, t.shape[2] * t.shape[3], t.shape[3], 1), next(at))
+        cut.copy_(t)
+        return cut.detach()
+
+    check_delta(x, resets, grads, move=move)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("shape,resets", [((513, 1, 1, 1, 64, 64), 0.0), ((1025, 2, 1, 2, 32, 24), 0.004),
                                           ((700, 1, 2, 2, 128, 128), 0.01), ((1500, 3, 1, 1, 16, 40), 0.5)])
