@@ -52,7 +52,7 @@ struct Segments {
 
 // What LDS leaves room for.
 template <typename T, int DP>
-constexpr int kWavesPerSimd = DP == 128 ? 2 : DP == 64 && sizeof(T) == 2 ? 4 : 3;
+constexpr int kWavesPerSimd = DP == 32 ? 3 : DP == 64 && sizeof(T) == 2 ? 4 : 2;
 
 // MAP: the segment's M and B; else outputs and states.
 //
@@ -69,7 +69,7 @@ constexpr int kWavesPerSimd = DP == 128 ? 2 : DP == 64 && sizeof(T) == 2 ? 4 : 3
 // four workgroups a compute unit.
 template <typename T, int DP, bool WIDE, bool MAP>
 __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), (kWavesPerSimd<T, DP>)) delta_forward_kernel(DeltaArgs<T> a, Segments seg) {
-    using Tile = ChunkTile<T, DP, kNear>;
+    using Tile = ChunkTile<T, typename MathOf<T, DP>::forward, DP, MathOf<T, DP>::forward::kNear>;
     using M = typename Tile::M;
     constexpr int KT = Tile::KT, KP = Tile::KP, kWaves = Tile::kWaves * (MAP ? 2 : 1);
     __shared__ Tile sh;

@@ -9,6 +9,8 @@
 // elements 4g + i and 16 + 4g + i.  Operands from LDS follow that order.
 #pragma once
 
+#include <type_traits>
+
 #include "mem_delta.h"
 
 namespace nesle::mem {
@@ -16,12 +18,14 @@ namespace nesle::mem {
 // Place of an inner element within 32 so that a lane's eight lie together.
 __device__ constexpr int place_of(int c) { return (c & ~31) | ((c >> 2) & 3) << 3 | ((c >> 4) & 1) << 2 | (c & 3); }
 
-// Planes of an operand or a tile: an input as it is, a result that is rounded to
-// the inputs' type next, float32.
-constexpr int kExact = 1, kNear = 2, kFull = 3;
+// Planes of an operand or a tile that hold float32.  Each kind of products has
+// planes of its own for the inputs, kIn, and for a result that is rounded to the
+// inputs' type next, kNear.
+constexpr int kFull = 3;
 
-// ---- float32 inputs: v_mfma_f32_16x16x4_f32 -----------------------------------
+// ---- v_mfma_f32_16x16x4_f32 ------------------------------------------------------
 struct F32Math {
+    static constexpr int kIn = 1, kNear = 1;
     struct Op {
         f4 a, b;
     };
@@ -65,20 +69,22 @@ struct F32Math {
     };
 };
 
-// ---- bfloat16 inputs: v_mfma_f32_16x16x32_bf16 ----------------------------------
+// ---- v_mfma_f32_16x16x32_bf16 ----------------------------------------------------
 // A float32 value is the sum of three bfloat16 values, its 24 significant bits
 // cut in three (by truncation, so nothing is lost).  A product of two such
 // operands takes the six instructions of the pairs that weigh 2^-16 or more
-// against the first; the rest is below 2^-24, where float32 rounds.  Against an
-// input, which is one bfloat16 value, three instructions give the product
-// whole.  At 16 cycles for 32 inner elements that is 48 or 96 cycles where
-// float32's instructions take 256.
+// against the first; the rest is below 2^-24, where float32 rounds.  Against a
+// bfloat16 input, which is one such value (IN = 1, else 3), three instructions
+// give the product whole.  At 16 cycles for 32 inner elements that is 48 or 96
+// cycles where float32's instructions take 256.
 //
 // Where a product's result is rounded to bfloat16 next and goes nowhere else
 // (the outputs; the gradients of queries and keys), two of the three are enough:
 // they leave out 2^-16 of an operand where the rounding takes 2^-9 of the
 // result, for half the instructions (`near`).
+template <int IN>
 struct SplitMath {
+    static constexpr int kIn = IN, kNear = IN == 1 ? 2 : kFull;
     using b8 = bf16 __attribute__((ext_vector_type(8)));
     template <int PLANES>
     struct Op {
@@ -113,12 +119,19 @@ struct SplitMath {
     }
     static __device__ Op<kFull> full(f4 a, f4 b) { return operand<kFull>(a, b); }
     static __device__ Op<kNear> near(f4 a, f4 b) { return operand<kNear>(a, b); }
-    static __device__ Op<kNear> near(const Op<kFull>& o) { return {{o.x[0], o.x[1]}}; }
+    static __device__ Op<kNear> near(const Op<kFull>& o) {
+        if constexpr (kNear == kFull) return o;
+        else return {{o.x[0], o.x[1]}};
+    }
     // The two result tiles that an operand of inputs holds.
-    static __device__ void values(const Op<kExact>& o, f4 (&to)[2]) {
-        const u4 w = o.x[0];
-        to[0] = f4{lo_half(w.x), hi_half(w.x), lo_half(w.y), hi_half(w.y)};
-        to[1] = f4{lo_half(w.z), hi_half(w.z), lo_half(w.w), hi_half(w.w)};
+    static __device__ void values(const Op<kIn>& o, f4 (&to)[2]) {
+        to[0] = to[1] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int p = kIn - 1; p >= 0; --p) {
+            const u4 w = o.x[p];
+            to[0] += f4{lo_half(w.x), hi_half(w.x), lo_half(w.y), hi_half(w.y)};
+            to[1] += f4{lo_half(w.z), hi_half(w.z), lo_half(w.w), hi_half(w.w)};
+        }
     }
     // The pairs of planes that together weigh no less than the wider operand's last.
     template <int P, int Q>
@@ -159,9 +172,13 @@ struct SplitMath {
         }
         // Eight columns as they lie in memory.
         __device__ void put8(int row, int col, const std::uint32_t (&w)[4]) {
-            static_assert(PLANES == kExact);
+            static_assert(PLANES == 1);
             *reinterpret_cast<u2*>(&d[row * kRow + place_of(col)]) = u2{w[0], w[1]};
             *reinterpret_cast<u2*>(&d[row * kRow + place_of(col + 4)]) = u2{w[2], w[3]};
+        }
+        __device__ void put8(int row, int col, const std::uint32_t (&w)[8]) {
+            put4(row, col, __builtin_bit_cast(f4, u4{w[0], w[1], w[2], w[3]}));
+            put4(row, col + 4, __builtin_bit_cast(f4, u4{w[4], w[5], w[6], w[7]}));
         }
         // Operand of the 16 rows from row0 over the inner columns 32 p ...
         template <int USED = PLANES>
@@ -193,15 +210,19 @@ struct SplitMath {
     };
 };
 
-template <typename T>
-struct MathOf;
-template <>
-struct MathOf<float> {
-    using type = F32Math;
+// Float32 inputs in three planes take up to twice the LDS of a tile of float32:
+// quicker in the forward of 64 dimensions (64 consoles of 4 heads 28.4 -> 27.0 us, 256
+// 73.9 -> 67.5) and 128 (64 consoles 62.5 -> 51.9), not of 32 (512 consoles 76 -> 86);
+// in the gradient they would leave one workgroup a compute unit, or none.
+template <typename T, int DP>
+struct MathOf {
+    using forward = SplitMath<1>;
+    using gradient = SplitMath<1>;
 };
-template <>
-struct MathOf<bf16> {
-    using type = SplitMath;
+template <int DP>
+struct MathOf<float, DP> {
+    using forward = std::conditional_t<DP == 32, F32Math, SplitMath<3>>;
+    using gradient = F32Math;
 };
 
 // v as lane r - N (ROW_SHR: zero where there is none) or r + N around (ROW_ROR)
