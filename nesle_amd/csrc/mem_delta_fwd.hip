@@ -58,15 +58,14 @@ constexpr int kWavesPerSimd = DP == 32 ? 3 : DP == 64 && sizeof(T) == 2 ? 4 : 2;
 //
 // Bound by memory where there are many heads: 128 steps of 512 consoles of 4 heads
 // of 64 in bfloat16 move 0.30 GB (inputs, outputs, the states in and out and the
-// ones kept for the gradient) in 82 us, 3.7 TB/s against a large copy's 4.9.  With
+// ones kept for the gradient) in 81 us, 3.7 TB/s against a large copy's 4.9.  With
 // the parts left out one at a time: kept states -19 us, first and last states -20,
 // loads of the inputs -17, outputs -14, the inverse -4.  With one workgroup a compute
-// unit a chunk takes 3.6 us, a chain of short parts: inverse 0.7, loads 0.2,
-// products and the tests of what is not finite 0.1 each; in float32 4.8 us (28 us
-// for 64 consoles, of which the float32 matrix instructions are the most).  A
-// chunk of 32 tokens is one inner step of the bfloat16 instruction and the
-// largest whose inverse one wave finds in registers; its tile leaves room for
-// four workgroups a compute unit.
+// unit a chunk takes 3.4 us, a chain of short parts: inverse 0.7, loads 0.2,
+// products and the tests of what is not finite 0.1 each (64 consoles 21 us, in
+// float32 27).  A chunk of 32 tokens is one inner step of the bfloat16 instruction
+// and the largest whose inverse one wave finds in registers; its tile leaves room
+// for four workgroups a compute unit.
 template <typename T, int DP, bool WIDE, bool MAP>
 __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), (kWavesPerSimd<T, DP>)) delta_forward_kernel(DeltaArgs<T> a, Segments seg) {
     using Tile = ChunkTile<T, typename MathOf<T, DP>::forward, DP, MathOf<T, DP>::forward::kNear>;
@@ -328,14 +327,14 @@ __global__ void __launch_bounds__(DP * 4) delta_join_kernel(Chain x, int dk, int
 }
 
 // Segments for few heads over many tokens.  The walk of one head through a chunk
-// takes 3.6 us by itself and 7 us beside another on its compute unit, a step of
+// takes 3.4 us by itself and 6 us beside another on its compute unit, a step of
 // a chain 0.6 us, a launch of one 5 us and more, and the launches walk every chunk
 // twice.  So: enough segments for two workgroups a compute unit, two chunks or
 // more in each, and no more than balance the chain's steps against the walks; in
 // groups, of as many segments as there are groups, once the chain would be longer
 // than 40.  Measured in bfloat16, heads of 64, whole walk against segments: 1,024
-// tokens of 64 heads 120 / 59 us, of 128 heads 122 / 97 us, of 256 heads 127 / 157
-// us; 256 tokens of 16 heads 32 / 25 us.  One chain against groups: 4,096 tokens of
+// tokens of 64 heads 111 / 58 us, of 128 heads 113 / 95 us, of 256 heads 127 / 157
+// us; 256 tokens of 16 heads 30 / 25 us.  One chain against groups: 4,096 tokens of
 // 8 heads 60 / 63 us, 8,191 of 8 heads 91 / 82 us, 32,768 of 4 heads 167 / 127 us.
 Segments segments(const nesle_delta_args& a) {
     const std::uint64_t heads = static_cast<std::uint64_t>(a.batch) * a.v_heads;

@@ -9,11 +9,12 @@ import math
 import re
 import shutil
 import subprocess
+from pathlib import Path
 
 import pytest
 import torch
 
-from nesle_amd import abi, memory
+from nesle_amd import abi, build, memory
 
 
 def _delta(**kw):
@@ -125,3 +126,20 @@ def test_cpu_tensors_are_refused():
         memory.qk_norm_rotate(q, q)
     with pytest.raises(ValueError, match="GPU"):
         memory.gated_delta_step(q, q, q, q[..., 0], q[..., 0], torch.zeros(3, 2, 16, 16))
+
+
+def test_delta_kernels_share_a_compute_unit(tmp_path):
+    """The gradient's LDS leaves room for two workgroups of heads of 64 on a
+    compute unit's 160 KB, the bfloat16 forward's for four; up to 64 dimensions
+    nothing spills."""
+    from test_kernel_resources import HIPCC, _kernels
+
+    if not Path(HIPCC).exists():
+        pytest.skip("hipcc not available")
+    for source, lds in (("mem_delta_fwd.hip", {"IDF16bLi64": 40, "IfLi64": 80}),
+                        ("mem_delta_bwd.hip", {"IDF16bLi64": 80, "IfLi64": 80})):
+        kernels = {k: v for k, v in _kernels(build.CSRC / source, tmp_path).items() if "ward_kernel" in k}
+        for kind, most in lds.items():
+            of_kind = [v for k, v in kernels.items() if kind in k]
+            assert of_kind and all(v["group_segment_fixed_size"] <= most << 10 for v in of_kind), source
+        assert all(v["private_segment_fixed_size"] == 0 for k, v in kernels.items() if "Li128" not in k), source
