@@ -251,7 +251,9 @@ __global__ void __launch_bounds__(kThreads) qk_forward(QkArgs<T> a) {
 
 // dy = the output's gradient turned back; dx = inv w dy - x inv^3 <x, w dy> / count;
 // dw = sum over rows of x inv dy.
-template <typename T, int PAIRS>
+// KINDS: kinds of heads that a lane meets, 1 where the heads of a row divide those
+// of a workgroup.
+template <typename T, int PAIRS, int KINDS>
 __global__ void __launch_bounds__(kThreads) qk_gradient(QkArgs<T> a) {
     constexpr int N = PAIRS / 4;
     constexpr unsigned kTogether = kGradTogether / N;
@@ -260,9 +262,8 @@ __global__ void __launch_bounds__(kThreads) qk_gradient(QkArgs<T> a) {
     unsigned first, second;
     places<PAIRS>(a, j, first, second);
     const bool has = 2 * PAIRS * j < a.dim, rotates = 2 * PAIRS * j < a.rotated;
-    Part<PAIRS> dw[2];
-    dw[0].clear();
-    dw[1].clear();
+    Part<PAIRS> dw[KINDS];
+    for (auto& d : dw) d.clear();
     const std::uint64_t at_once = static_cast<std::uint64_t>(gridDim.x) * per * kTogether;
     // Every lane of a workgroup takes every turn, as the lane exchanges need.
     for (std::uint64_t base = static_cast<std::uint64_t>(blockIdx.x) * per * kTogether; base < a.groups; base += at_once) {
@@ -296,10 +297,12 @@ __global__ void __launch_bounds__(kThreads) qk_gradient(QkArgs<T> a) {
 #pragma unroll
                 for (int u = 0; u < N; ++u) {
                     const f4 none = {0, 0, 0, 0}, one = x[i].a[u] * inv * d[i].a[u], two = x[i].b[u] * inv * d[i].b[u];
-                    dw[0].a[u] += at.is_q ? one : none;
-                    dw[0].b[u] += at.is_q ? two : none;
-                    dw[1].a[u] += at.is_q ? none : one;
-                    dw[1].b[u] += at.is_q ? none : two;
+                    dw[0].a[u] += KINDS == 1 || at.is_q ? one : none;
+                    dw[0].b[u] += KINDS == 1 || at.is_q ? two : none;
+                    if constexpr (KINDS == 2) {
+                        dw[1].a[u] += at.is_q ? none : one;
+                        dw[1].b[u] += at.is_q ? none : two;
+                    }
                 }
                 d[i].scale(weight);
             }
@@ -318,11 +321,13 @@ __global__ void __launch_bounds__(kThreads) qk_gradient(QkArgs<T> a) {
     // Lanes that hold the same elements, first within the wave, then over the
     // waves, in a fixed order.
     const unsigned lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const bool of_k = threadIdx.x / a.lanes % a.per_row.d >= a.hq;          // KINDS == 1: this lane's kind
 #pragma unroll
     for (int kind = 0; kind < 2; ++kind)
 #pragma unroll
         for (int u = 0; u < 2 * N; ++u) {
-            f4 v = u < N ? dw[kind].a[u] : dw[kind].b[u - N];
+            f4 v = u < N ? dw[kind % KINDS].a[u] : dw[kind % KINDS].b[u - N];
+            if (KINDS == 1 && of_k != (kind == 1)) v = f4{0, 0, 0, 0};
             for (unsigned d = a.lanes; d < 64; d *= 2)
                 v += f4{__shfl_xor(v.x, d), __shfl_xor(v.y, d), __shfl_xor(v.z, d), __shfl_xor(v.w, d)};
             if (lane < a.lanes) sums[wave][kind][u][lane] = v;
@@ -462,7 +467,10 @@ void launch_gradient(const nesle_qk_args& a, hipStream_t s) {
     const bool weights = a.q_weight != nullptr || a.k_weight != nullptr;
     k.partials = weights ? a.scratch : nullptr;
     const std::uint32_t blocks = grad_blocks(a);
-    hipLaunchKernelGGL((qk_gradient<T, PAIRS>), dim3(blocks), dim3(kThreads), 0, s, k);
+    if (kThreads / k.lanes % (a.q_heads + a.k_heads) == 0)
+        hipLaunchKernelGGL((qk_gradient<T, PAIRS, 1>), dim3(blocks), dim3(kThreads), 0, s, k);
+    else
+        hipLaunchKernelGGL((qk_gradient<T, PAIRS, 2>), dim3(blocks), dim3(kThreads), 0, s, k);
     if (weights)
         hipLaunchKernelGGL(qk_weight_sum, dim3(2 * a.dim), dim3(kThreads), 0, s, a.scratch, blocks, a.dim, a.dq_weight,
                            a.dk_weight);
