@@ -11,12 +11,12 @@
 //
 // Bound by memory: about 10 operations an element.  Measured against a large
 // copy's 4.9 TB/s, bfloat16: 1.08 GB of 128 steps of 4,096 rows and 8 heads of 64
-// in 222 us (4.9 TB/s); 128 steps of 512 rows, forward 134 MB in 29 us (4.6 TB/s),
-// gradient 134 MB more in 55 us (3.7 TB/s: twice the tensors in flight, and sums
-// over lanes) and the weights' sum 5 us.  One load of 8 bytes a lane for each
-// operand in place of 16 took 309 us for the first; heads of one row side by side
-// in a thread, which share a row of the table, 338 us.  Below about 100 rows a call
-// is a launch: 3.4 us.
+// in 221 us (4.9 TB/s); 128 steps of 512 rows, forward 134 MB in 29 us (4.6 TB/s),
+// gradient 202 MB in 40 us (5.0 TB/s) and the weights' sum 4 us.  Loads of 8 bytes a
+// lane in place of 16 took 309 us for the first; heads of one row side by side in a
+// thread, which share a row of the table, 338 us.  Below about 100 rows a call is a
+// launch: 3.6 us.
+#include <algorithm>
 #include <initializer_list>
 
 #include "mem_common.h"
@@ -29,9 +29,10 @@ constexpr unsigned kThreads = 256;
 // heads of one row share its position, cosines and sines.  One where the rows
 // do not fill the card: latency counts there.
 constexpr unsigned kTogether = 4, kGradTogether = 2;
-// Workgroups of the gradient with weights: each adds up its rows' share of
-// the weights' gradient, and one more launch adds the workgroups' in order.
-constexpr unsigned kGradBlocks = 2048;
+// Workgroups of the gradient, four a compute unit, which their registers leave
+// room for (twice as many: 47 us for 43): each adds up its rows' share of a
+// weight's gradient, and one more launch adds the workgroups' in order.
+constexpr unsigned kGradBlocks = 1024;
 
 // x / d for x < 2^16 (d as it is) or x < 2 d (d of 2^15 or more).
 struct Divide {
@@ -50,9 +51,10 @@ struct QkArgs {
     const std::int32_t* positions;
     const float* table;
     T *q_out, *k_out;        // forward: outputs; gradient: dq, dk
-    float* partials;         // [blocks][2][dim]
-    Divide batch, per_row;   // rows of a step, heads of a row
+    float* partials;         // [blocks][dim]
+    Divide batch, per_row, per_q, per_k;   // rows of a step, heads of a row, of either kind
     std::uint32_t hq, hk, dim, rotated, table_rows, lanes;   // lanes of one head: a power of two
+    std::uint32_t q_blocks;  // gradient: the workgroups that take queries
     std::uint64_t groups;    // heads of all rows
     float inv_count, eps;
     bool interleaved;
@@ -162,30 +164,32 @@ struct Part {
 struct Start {
     std::uint64_t row, step;
     std::uint32_t head, env;
-    template <typename T>
-    __device__ Start(const QkArgs<T>& a, std::uint64_t group)
-        : row(group / a.per_row.d), step(row / a.batch.d), head(static_cast<std::uint32_t>(group % a.per_row.d)),
-          env(static_cast<std::uint32_t>(row % a.batch.d)) {}
+    __device__ Start(const Divide& batch, const Divide& per_row, std::uint64_t group)
+        : row(group / per_row.d), step(row / batch.d), head(static_cast<std::uint32_t>(group % per_row.d)),
+          env(static_cast<std::uint32_t>(row % batch.d)) {}
 };
 
-// One head: its tensors' kind, row and addresses.
-template <typename T>
+// One head of those of a row.
 struct Spot {
-    bool is_q;
-    std::uint32_t h;
+    std::uint32_t h, env;
     std::uint64_t row, step;
-    std::uint32_t env;
-    __device__ Spot(const QkArgs<T>& a, const Start& at, std::uint32_t plus) {
-        const std::uint32_t x = at.head + plus, down = a.per_row(x), head = x - down * a.per_row.d;
-        const std::uint32_t y = at.env + down, over = a.batch(y);
-        is_q = head < a.hq;
-        h = is_q ? head : head - a.hq;
+    __device__ Spot(const Divide& batch, const Divide& per_row, const Start& at, std::uint32_t plus) {
+        const std::uint32_t x = at.head + plus, down = per_row(x), y = at.env + down, over = batch(y);
+        h = x - down * per_row.d;
         row = at.row + down;
         step = at.step + over;
-        env = y - over * a.batch.d;
+        env = y - over * batch.d;
     }
-    __device__ const T* in(const Heads<T>& q, const Heads<T>& k) const {
-        return is_q ? q.row(step, env, h) : k.row(step, env, h);
+    template <typename T>
+    __device__ const T* in(const Heads<T>& x) const { return x.row(step, env, h); }
+};
+// One of all: its kind too.
+template <typename T>
+struct AnySpot : Spot {
+    bool is_q;
+    __device__ AnySpot(const QkArgs<T>& a, const Start& at, std::uint32_t plus) : Spot(a.batch, a.per_row, at, plus) {
+        is_q = h < a.hq;
+        h = is_q ? h : h - a.hq;
     }
     __device__ T* out(const QkArgs<T>& a) const {
         return is_q ? a.q_out + (row * a.hq + h) * a.dim : a.k_out + (row * a.hk + h) * a.dim;
@@ -214,7 +218,7 @@ template <typename T, int PAIRS, unsigned TOGETHER>
 __global__ void __launch_bounds__(kThreads) qk_forward(QkArgs<T> a) {
     const unsigned j = threadIdx.x % a.lanes, per = kThreads / a.lanes;
     const std::uint64_t base = static_cast<std::uint64_t>(blockIdx.x) * per * TOGETHER;
-    const Start start(a, base);
+    const Start start(a.batch, a.per_row, base);
     const bool has = 2 * PAIRS * j < a.dim, rotates = 2 * PAIRS * j < a.rotated;
     unsigned first, second;
     places<PAIRS>(a, j, first, second);
@@ -226,8 +230,8 @@ __global__ void __launch_bounds__(kThreads) qk_forward(QkArgs<T> a) {
         x[i].clear();
         position[i] = 0;
         if (base + plus < a.groups && has) {
-            const Spot<T> at(a, start, plus);
-            x[i].load(at.in(a.q, a.k), first, second, at.is_q ? a.q.vec : a.k.vec);
+            const AnySpot<T> at(a, start, plus);
+            x[i].load(at.is_q ? at.in(a.q) : at.in(a.k), first, second, at.is_q ? a.q.vec : a.k.vec);
             if (rotates) position[i] = a.positions[at.row];
         }
     }
@@ -236,7 +240,7 @@ __global__ void __launch_bounds__(kThreads) qk_forward(QkArgs<T> a) {
         const std::uint32_t plus = i * per + threadIdx.x / a.lanes;
         const float inv = 1.0f / sqrtf(across(x[i].dot(x[i]), a.lanes) * a.inv_count + a.eps);
         if (base + plus >= a.groups || !has) continue;
-        const Spot<T> at(a, start, plus);
+        const AnySpot<T> at(a, start, plus);
         x[i].scale(inv);
         const float* w = at.is_q ? a.wq : a.wk;
         if (w != nullptr) {
@@ -250,24 +254,33 @@ __global__ void __launch_bounds__(kThreads) qk_forward(QkArgs<T> a) {
 }
 
 // dy = the output's gradient turned back; dx = inv w dy - x inv^3 <x, w dy> / count;
-// dw = sum over rows of x inv dy.
-// KINDS: kinds of heads that a lane meets, 1 where the heads of a row divide those
-// of a workgroup.
-template <typename T, int PAIRS, int KINDS>
+// dw = sum over rows of x inv dy.  A workgroup takes heads of one kind, so that a
+// lane adds up one weight's gradient and reads neighbouring heads: both kinds' took
+// 130 registers for 116, three waves a SIMD for four, and 55 us for 40 in the case
+// above.
+template <typename T, int PAIRS>
 __global__ void __launch_bounds__(kThreads) qk_gradient(QkArgs<T> a) {
     constexpr int N = PAIRS / 4;
     constexpr unsigned kTogether = kGradTogether / N;
-    __shared__ f4 sums[kThreads / 64][2][2 * N][32 / N];       // [wave][q, k][four of them][lane of the head]
+    __shared__ f4 sums[kThreads / 64][2 * N][32 / N];       // [wave][four of them][lane of the head]
+    const bool is_q = blockIdx.x < a.q_blocks;
+    const std::uint32_t block = is_q ? blockIdx.x : blockIdx.x - a.q_blocks;
+    const std::uint32_t blocks = is_q ? a.q_blocks : gridDim.x - a.q_blocks;
+    const Heads<T> in = is_q ? a.q : a.k, dy = is_q ? a.dq_out : a.dk_out;
+    const Divide per_row = is_q ? a.per_q : a.per_k;
+    const std::uint64_t groups = a.groups / a.per_row.d * per_row.d;
+    const float* w = is_q ? a.wq : a.wk;
+    T* out = is_q ? a.q_out : a.k_out;
     const unsigned j = threadIdx.x % a.lanes, per = kThreads / a.lanes;
     unsigned first, second;
     places<PAIRS>(a, j, first, second);
     const bool has = 2 * PAIRS * j < a.dim, rotates = 2 * PAIRS * j < a.rotated;
-    Part<PAIRS> dw[KINDS];
-    for (auto& d : dw) d.clear();
-    const std::uint64_t at_once = static_cast<std::uint64_t>(gridDim.x) * per * kTogether;
+    Part<PAIRS> dw;
+    dw.clear();
+    const std::uint64_t at_once = static_cast<std::uint64_t>(blocks) * per * kTogether;
     // Every lane of a workgroup takes every turn, as the lane exchanges need.
-    for (std::uint64_t base = static_cast<std::uint64_t>(blockIdx.x) * per * kTogether; base < a.groups; base += at_once) {
-        const Start start(a, base);
+    for (std::uint64_t base = static_cast<std::uint64_t>(block) * per * kTogether; base < groups; base += at_once) {
+        const Start start(a.batch, per_row, base);
         Part<PAIRS> x[kTogether], d[kTogether];
         std::int32_t position[kTogether];
 #pragma unroll
@@ -276,33 +289,26 @@ __global__ void __launch_bounds__(kThreads) qk_gradient(QkArgs<T> a) {
             x[i].clear();
             d[i].clear();
             position[i] = 0;
-            if (base + plus < a.groups && has) {
-                const Spot<T> at(a, start, plus);
-                x[i].load(at.in(a.q, a.k), first, second, at.is_q ? a.q.vec : a.k.vec);
-                d[i].load(at.in(a.dq_out, a.dk_out), first, second, at.is_q ? a.dq_out.vec : a.dk_out.vec);
+            if (base + plus < groups && has) {
+                const Spot at(a.batch, per_row, start, plus);
+                x[i].load(at.in(in), first, second, in.vec);
+                d[i].load(at.in(dy), first, second, dy.vec);
                 if (rotates) position[i] = a.positions[at.row];
             }
         }
 #pragma unroll
         for (unsigned i = 0; i < kTogether; ++i) {
             const std::uint32_t plus = i * per + threadIdx.x / a.lanes;
-            const bool mine = base + plus < a.groups && has;
-            const Spot<T> at(a, start, mine ? plus : 0);
+            const bool mine = base + plus < groups && has;
             const float inv = 1.0f / sqrtf(across(x[i].dot(x[i]), a.lanes) * a.inv_count + a.eps);
             if (mine && rotates) d[i].turn(turns<PAIRS>(a, position[i], j), true, a.interleaved);
-            const float* w = at.is_q ? a.wq : a.wk;
             if (w != nullptr && mine) {
                 Part<PAIRS> weight;
                 weight.load_floats(w, first, second);
 #pragma unroll
                 for (int u = 0; u < N; ++u) {
-                    const f4 none = {0, 0, 0, 0}, one = x[i].a[u] * inv * d[i].a[u], two = x[i].b[u] * inv * d[i].b[u];
-                    dw[0].a[u] += KINDS == 1 || at.is_q ? one : none;
-                    dw[0].b[u] += KINDS == 1 || at.is_q ? two : none;
-                    if constexpr (KINDS == 2) {
-                        dw[1].a[u] += at.is_q ? none : one;
-                        dw[1].b[u] += at.is_q ? none : two;
-                    }
+                    dw.a[u] += x[i].a[u] * inv * d[i].a[u];
+                    dw.b[u] += x[i].b[u] * inv * d[i].b[u];
                 }
                 d[i].scale(weight);
             }
@@ -313,7 +319,7 @@ __global__ void __launch_bounds__(kThreads) qk_gradient(QkArgs<T> a) {
                     d[i].a[u] = d[i].a[u] * inv - x[i].a[u] * along;
                     d[i].b[u] = d[i].b[u] * inv - x[i].b[u] * along;
                 }
-                d[i].store(at.out(a), first, second);
+                d[i].store(out + (base + plus) * a.dim, first, second);
             }
         }
     }
@@ -321,44 +327,40 @@ __global__ void __launch_bounds__(kThreads) qk_gradient(QkArgs<T> a) {
     // Lanes that hold the same elements, first within the wave, then over the
     // waves, in a fixed order.
     const unsigned lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const bool of_k = threadIdx.x / a.lanes % a.per_row.d >= a.hq;          // KINDS == 1: this lane's kind
 #pragma unroll
-    for (int kind = 0; kind < 2; ++kind)
-#pragma unroll
-        for (int u = 0; u < 2 * N; ++u) {
-            f4 v = u < N ? dw[kind % KINDS].a[u] : dw[kind % KINDS].b[u - N];
-            if (KINDS == 1 && of_k != (kind == 1)) v = f4{0, 0, 0, 0};
-            for (unsigned d = a.lanes; d < 64; d *= 2)
-                v += f4{__shfl_xor(v.x, d), __shfl_xor(v.y, d), __shfl_xor(v.z, d), __shfl_xor(v.w, d)};
-            if (lane < a.lanes) sums[wave][kind][u][lane] = v;
-        }
+    for (int u = 0; u < 2 * N; ++u) {
+        f4 v = u < N ? dw.a[u] : dw.b[u - N];
+        for (unsigned d = a.lanes; d < 64; d *= 2)
+            v += f4{__shfl_xor(v.x, d), __shfl_xor(v.y, d), __shfl_xor(v.z, d), __shfl_xor(v.w, d)};
+        if (lane < a.lanes) sums[wave][u][lane] = v;
+    }
     __syncthreads();
     if (threadIdx.x < a.lanes && has)
-        for (int kind = 0; kind < 2; ++kind)
-            for (int u = 0; u < 2 * N; ++u) {
-                f4 v = sums[0][kind][u][j];
-                for (unsigned o = 1; o < kThreads / 64; ++o) v += sums[o][kind][u][j];
-                float* p = a.partials + (static_cast<std::size_t>(blockIdx.x) * 2 + kind) * a.dim;
-                store4(p + (u < N ? first + 4 * u : second + 4 * (u - N)), v);
-            }
+        for (int u = 0; u < 2 * N; ++u) {
+            f4 v = sums[0][u][j];
+            for (unsigned o = 1; o < kThreads / 64; ++o) v += sums[o][u][j];
+            float* p = a.partials + static_cast<std::size_t>(blockIdx.x) * a.dim;
+            store4(p + (u < N ? first + 4 * u : second + 4 * (u - N)), v);
+        }
 }
 
-// One element of one weight's gradient a workgroup: the partials of all
+// One element of one weight's gradient a workgroup: the partials of the kind's
 // workgroups, added in a fixed order.
-__global__ void __launch_bounds__(kThreads) qk_weight_sum(const float* partials, std::uint32_t blocks,
+__global__ void __launch_bounds__(kThreads) qk_weight_sum(const float* partials, std::uint32_t q_blocks, std::uint32_t blocks,
                                                           std::uint32_t dim, float* dwq, float* dwk) {
     __shared__ float sh[kThreads];
-    const std::uint32_t e = blockIdx.x;                // 0 .. 2 dim - 1
+    const bool is_q = blockIdx.x < dim;
+    const std::uint32_t e = is_q ? blockIdx.x : blockIdx.x - dim, end = is_q ? q_blocks : blocks;
     float v = 0.0f;
-    for (std::uint32_t b = threadIdx.x; b < blocks; b += kThreads) v += partials[static_cast<std::size_t>(b) * 2 * dim + e];
+    for (std::uint32_t b = (is_q ? 0 : q_blocks) + threadIdx.x; b < end; b += kThreads) v += partials[static_cast<std::size_t>(b) * dim + e];
     sh[threadIdx.x] = v;
     __syncthreads();
     for (unsigned s = kThreads / 2; s > 0; s /= 2) {
         if (threadIdx.x < s) sh[threadIdx.x] += sh[threadIdx.x + s];
         __syncthreads();
     }
-    float* out = e < dim ? dwq : dwk;
-    if (threadIdx.x == 0 && out != nullptr) out[e < dim ? e : e - dim] = sh[0];
+    float* out = is_q ? dwq : dwk;
+    if (threadIdx.x == 0 && out != nullptr) out[e] = sh[0];
 }
 
 std::uint32_t lanes_of(std::uint32_t dim, unsigned pairs) {
@@ -372,9 +374,13 @@ std::uint64_t blocks_for(const nesle_qk_args& a, unsigned pairs, unsigned togeth
     return (static_cast<std::uint64_t>(a.steps) * a.batch * (a.q_heads + a.k_heads) + per - 1) / per;
 }
 
-std::uint32_t grad_blocks(const nesle_qk_args& a) {
-    const std::uint64_t all = blocks_for(a, 4, kGradTogether);     // of eight pairs: as many
-    return static_cast<std::uint32_t>(all < kGradBlocks ? all : kGradBlocks);
+// Workgroups of the gradient for heads of one kind.
+std::uint32_t grad_blocks(const nesle_qk_args& a, std::uint32_t kind_heads) {
+    if (kind_heads == 0) return 0;
+    const std::uint64_t per = kThreads / lanes_of(a.dim, 4) * kGradTogether;      // of eight pairs: as many
+    const std::uint64_t all = (static_cast<std::uint64_t>(a.steps) * a.batch * kind_heads + per - 1) / per;
+    const std::uint64_t most = std::max(1u, kGradBlocks * kind_heads / (a.q_heads + a.k_heads));
+    return static_cast<std::uint32_t>(std::min(all, most));
 }
 
 bool aligned(std::initializer_list<const void*> pointers) {
@@ -416,6 +422,8 @@ QkArgs<T> pack(const nesle_qk_args& a, unsigned pairs) {
     k.table = a.table;
     k.batch = Divide(a.batch);
     k.per_row = Divide(a.q_heads + a.k_heads);
+    k.per_q = Divide(a.q_heads);
+    k.per_k = Divide(a.k_heads);
     k.hq = a.q_heads;
     k.hk = a.k_heads;
     k.dim = a.dim;
@@ -466,14 +474,12 @@ void launch_gradient(const nesle_qk_args& a, hipStream_t s) {
     k.k_out = static_cast<T*>(a.dk);
     const bool weights = a.q_weight != nullptr || a.k_weight != nullptr;
     k.partials = weights ? a.scratch : nullptr;
-    const std::uint32_t blocks = grad_blocks(a);
-    if (kThreads / k.lanes % (a.q_heads + a.k_heads) == 0)
-        hipLaunchKernelGGL((qk_gradient<T, PAIRS, 1>), dim3(blocks), dim3(kThreads), 0, s, k);
-    else
-        hipLaunchKernelGGL((qk_gradient<T, PAIRS, 2>), dim3(blocks), dim3(kThreads), 0, s, k);
+    k.q_blocks = grad_blocks(a, a.q_heads);
+    const std::uint32_t blocks = k.q_blocks + grad_blocks(a, a.k_heads);
+    hipLaunchKernelGGL((qk_gradient<T, PAIRS>), dim3(blocks), dim3(kThreads), 0, s, k);
     if (weights)
-        hipLaunchKernelGGL(qk_weight_sum, dim3(2 * a.dim), dim3(kThreads), 0, s, a.scratch, blocks, a.dim, a.dq_weight,
-                           a.dk_weight);
+        hipLaunchKernelGGL(qk_weight_sum, dim3(2 * a.dim), dim3(kThreads), 0, s, a.scratch, k.q_blocks, blocks, a.dim,
+                           a.dq_weight, a.dk_weight);
 }
 
 int gradient(const char* who, const nesle_qk_args& a, hipStream_t s) {
@@ -492,7 +498,7 @@ extern "C" {
 
 std::uint64_t nesle_qk_scratch_floats(const nesle_qk_args* a) {
     if (a == nullptr || (a->q_weight == nullptr && a->k_weight == nullptr)) return 0;
-    return static_cast<std::uint64_t>(grad_blocks(*a)) * 2 * a->dim;
+    return (static_cast<std::uint64_t>(grad_blocks(*a, a->q_heads)) + grad_blocks(*a, a->k_heads)) * a->dim;
 }
 
 int nesle_qk_norm_rotate(const nesle_qk_args* a, void* stream) {
@@ -522,8 +528,8 @@ int nesle_qk_norm_rotate_grad(const nesle_qk_args* a, void* stream) {
     const auto s = static_cast<hipStream_t>(stream);
     if (empty(a)) {       // no rows: the weights' gradient is zero
         if (!weights) return NESLE_OK;
-        hipLaunchKernelGGL(qk_weight_sum, dim3(2 * a->dim), dim3(kThreads), 0, s, nullptr, 0u, a->dim, a->dq_weight,
-                           a->dk_weight);
+        hipLaunchKernelGGL(qk_weight_sum, dim3(2 * a->dim), dim3(kThreads), 0, s, nullptr, 0u, 0u, a->dim,
+                           a->dq_weight, a->dk_weight);
         return launched(who);
     }
     return gradient(who, *a, s);
