@@ -35,13 +35,14 @@
 namespace nesle::mem {
 namespace {
 
-// 32 columns of a state or its gradient, transposed: [value column][key].
-template <typename T, int DP, int PAD>
-using Slab = typename MathOf<T, DP>::gradient::template Tile<32, DP, MathOf<T, DP>::gradient::kNear, PAD>;
+// 32 columns of a state or its gradient, transposed: [value column][key].  In
+// float32, which takes less room than three planes; a reader cuts its own.
+template <int DP>
+using Slab = F32Math::Tile<32, DP, 1>;
 
 template <typename T, int DP>
-struct GradTile : ChunkTile<T, typename MathOf<T, DP>::gradient, DP, kFull, Slab<T, DP, 8>> {
-    using Base = ChunkTile<T, typename MathOf<T, DP>::gradient, DP, kFull, Slab<T, DP, 8>>;
+struct GradTile : ChunkTile<T, typename MathOf<T, DP>::gradient, DP, Slab<DP>> {
+    using Base = ChunkTile<T, typename MathOf<T, DP>::gradient, DP, Slab<DP>>;
     using M = typename Base::M;
     typename M::template Tile<kChunk, DP, M::kIn, 8> dout;
     // Transposed: [value column][token].  With rows of 18 and 42 words (mod 64)
@@ -51,7 +52,7 @@ struct GradTile : ChunkTile<T, typename MathOf<T, DP>::gradient, DP, kFull, Slab
         typename M::template Tile<DP, kChunk, kFull, 4> dr;
         Results<T, DP> keys[2];                            // dQ and dK, once dR has been read
     };
-    Slab<T, DP, DP == 32 ? 4 : 20> slab;
+    Slab<DP> slab;
     float row_beta[Base::kWaves][kChunk], row_gate[Base::kWaves][kChunk], row_after[Base::kWaves][kChunk];
     float place_beta[3][16], cross[4][16];     // of a tile: sums over columns; pairs that cross a token
     float whole[Base::kWaves];
@@ -224,8 +225,8 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
             for (int i = 0; i < 4; ++i) {
                 const int row = mi + 4 * g + i, c = nj + r;
                 const float L = now.ratio(row, c), b = now.beta[row];
-                sh.p.template put<M::kNear>(row, c, c <= row ? a.scale * L * dP[i] : 0.0f);
-                sh.t.template put<M::kNear>(row, c, c < row ? -b * L * dA[i] : 0.0f);
+                sh.p.put(row, c, c <= row ? a.scale * L * dP[i] : 0.0f);
+                sh.t.put(row, c, c < row ? -b * L * dA[i] : 0.0f);
                 by_a[i] = -dA[i] * kk[j][i];
                 pairs[i] = c < row ? dP[i] * qk[j][i] + b * by_a[i] : 0.0f;
                 const float before_t = sum_below(pairs[i]);
@@ -255,7 +256,8 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
 #pragma unroll
                     for (int j = 0; j < KT; ++j) to.put4(16 * (at.wave % 2) + r, 16 * j + 4 * g, x[j]);
                 __syncthreads();
-                use(i, to.cols(0, 16 * at.wave, r, g));
+                const auto held = to.cols(0, 16 * at.wave, r, g);
+                use(i, M::full(held.a, held.b));
             };
             if (turns % 2 == 0) put(sh.slab);
             else put(sh.later);
@@ -267,7 +269,7 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
                         dQ[m] = M::mul(sh.dout.rows(16 * m, i, r, g), s, dQ[m]);
-                        drs[m] = M::mul(sh.dr.template cols<M::kNear>(32 * i, 16 * m, r, g), s, drs[m]);
+                        drs[m] = M::mul(sh.dr.cols(32 * i, 16 * m, r, g), s, drs[m]);
                     }
                 });
         }
@@ -275,15 +277,15 @@ __global__ void __launch_bounds__(DP * 4, 2) delta_backward_kernel(DeltaArgs<T> 
         for (int i = 0; i < KP; ++i)
             pass(dS, i, KP + i, [&](int i, const auto& ds) {
 #pragma unroll
-                for (int m = 0; m < 2; ++m) dK[m] = M::mul(sh.u.template cols<M::kNear>(32 * i, 16 * m, r, g), ds, dK[m]);
+                for (int m = 0; m < 2; ++m) dK[m] = M::mul(sh.u.cols(32 * i, 16 * m, r, g), ds, dK[m]);
             });
         const auto key = sh.k.cols(0, 16 * at.wave, r, g), query = sh.q.cols(0, 16 * at.wave, r, g);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            dQ[m] = M::mul(sh.p.template rows<M::kNear>(16 * m, 0, r, g), key, gam[m] * a.scale * dQ[m]);
-            dK[m] = M::mul(sh.p.template cols<M::kNear>(0, 16 * m, r, g), query, dec[m] * dK[m] - beta[m] * gam[m] * drs[m]);
-            dK[m] = M::mul(sh.t.template rows<M::kNear>(16 * m, 0, r, g), key, dK[m]);
-            dK[m] = M::mul(sh.t.template cols<M::kNear>(0, 16 * m, r, g), key, dK[m]);
+            dQ[m] = M::mul(sh.p.rows(16 * m, 0, r, g), key, gam[m] * a.scale * dQ[m]);
+            dK[m] = M::mul(sh.p.cols(0, 16 * m, r, g), query, dec[m] * dK[m] - beta[m] * gam[m] * drs[m]);
+            dK[m] = M::mul(sh.t.rows(16 * m, 0, r, g), key, dK[m]);
+            dK[m] = M::mul(sh.t.cols(0, 16 * m, r, g), key, dK[m]);
         }
         const std::int64_t token = static_cast<std::int64_t>(start) * a.batch + env;
         const std::int64_t key_step = static_cast<std::int64_t>(a.batch) * a.hk * a.dk_dim;

@@ -68,7 +68,7 @@ constexpr int kWavesPerSimd = DP == 32 ? 3 : DP == 64 && sizeof(T) == 2 ? 4 : 2;
 // for four workgroups a compute unit.
 template <typename T, int DP, bool WIDE, bool MAP>
 __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), (kWavesPerSimd<T, DP>)) delta_forward_kernel(DeltaArgs<T> a, Segments seg) {
-    using Tile = ChunkTile<T, typename MathOf<T, DP>::forward, DP, MathOf<T, DP>::forward::kNear>;
+    using Tile = ChunkTile<T, typename MathOf<T, DP>::forward, DP>;
     using M = typename Tile::M;
     constexpr int KT = Tile::KT, KP = Tile::KP, kWaves = Tile::kWaves * (MAP ? 2 : 1);
     __shared__ Tile sh;
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), (kWavesPerSimd<T, DP>)) de
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
                     ks[m] = M::mul(sh.k.rows(16 * m, i, r, g), s, ks[m]);
-                    if constexpr (!MAP) qs[m] = M::mul(sh.q.rows(16 * m, i, r, g), M::near(s), qs[m]);
+                    if constexpr (!MAP) qs[m] = M::mul(sh.q.rows(16 * m, i, r, g), s, qs[m]);
                 }
             }
         };
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(DP * (MAP ? 8 : 4), (kWavesPerSimd<T, DP>)) de
 #pragma unroll
         for (int m = 0; m < 2; ++m) U[m] = M::mul(sh.t.rows(16 * m, 0, r, g), right, zero);
         if constexpr (!MAP) {
-            const auto u = M::near(U[0], U[1]);
+            const auto u = M::full(U[0], U[1]);
 #pragma unroll
             for (int m = 0; m < 2; ++m) O[m] = M::mul(sh.p.rows(16 * m, 0, r, g), u, qs[m]);
             sh.results.put(out, static_cast<int>(a.dv_dim), n, at, O);

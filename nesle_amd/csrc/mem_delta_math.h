@@ -19,19 +19,16 @@ namespace nesle::mem {
 __device__ constexpr int place_of(int c) { return (c & ~31) | ((c >> 2) & 3) << 3 | ((c >> 4) & 1) << 2 | (c & 3); }
 
 // Planes of an operand or a tile that hold float32.  Each kind of products has
-// planes of its own for the inputs, kIn, and for a result that is rounded to the
-// inputs' type next, kNear.
+// planes of its own for the inputs, kIn.
 constexpr int kFull = 3;
 
 // ---- v_mfma_f32_16x16x4_f32 ------------------------------------------------------
 struct F32Math {
-    static constexpr int kIn = 1, kNear = 1;
+    static constexpr int kIn = 1;
     struct Op {
         f4 a, b;
     };
     static __device__ Op full(f4 a, f4 b) { return {a, b}; }
-    static __device__ Op near(f4 a, f4 b) { return {a, b}; }
-    static __device__ Op near(const Op& x) { return x; }
     static __device__ f4 mul(const Op& x, const Op& y, f4 c) { return mma(x.b, y.b, mma(x.a, y.a, c)); }
     // The two result tiles that an operand of inputs holds.
     static __device__ void values(const Op& x, f4 (&to)[2]) {
@@ -45,7 +42,6 @@ struct F32Math {
     struct Tile {
         static constexpr int kRow = COLS + 4;
         alignas(16) float d[ROWS * kRow];
-        template <int USED = PLANES>
         __device__ void put(int row, int col, float v) { d[row * kRow + col] = v; }
         __device__ void put4(int row, int col, f4 v) { *reinterpret_cast<f4*>(&d[row * kRow + col]) = v; }
         // Eight columns as they lie in memory.
@@ -54,13 +50,11 @@ struct F32Math {
             *reinterpret_cast<u4*>(&d[row * kRow + col + 4]) = u4{w[4], w[5], w[6], w[7]};
         }
         // Operand of the 16 rows from row0 over the inner columns 32 p ...
-        template <int USED = PLANES>
         __device__ Op rows(int row0, int p, int r, int g) const {
             const float* x = &d[(row0 + r) * kRow + 32 * p + 4 * g];
             return {*reinterpret_cast<const f4*>(x), *reinterpret_cast<const f4*>(x + 16)};
         }
         // Operand of the 16 columns from col0 over the inner rows row0 ...
-        template <int USED = PLANES>
         __device__ Op cols(int row0, int col0, int r, int g) const {
             const float* x = &d[(row0 + 4 * g) * kRow + col0 + r];
             return {f4{x[0], x[kRow], x[2 * kRow], x[3 * kRow]},
@@ -70,58 +64,41 @@ struct F32Math {
 };
 
 // ---- v_mfma_f32_16x16x32_bf16 ----------------------------------------------------
-// A float32 value is the sum of three bfloat16 values, its 24 significant bits
-// cut in three (by truncation, so nothing is lost).  A product of two such
-// operands takes the six instructions of the pairs that weigh 2^-16 or more
-// against the first; the rest is below 2^-24, where float32 rounds.  Against a
-// bfloat16 input, which is one such value (IN = 1, else 3), three instructions
-// give the product whole.  At 16 cycles for 32 inner elements that is 48 or 96
-// cycles where float32's instructions take 256.
-//
-// Where a product's result is rounded to bfloat16 next and goes nowhere else
-// (the outputs; the gradients of queries and keys), two of the three are enough:
-// they leave out 2^-16 of an operand where the rounding takes 2^-9 of the
-// result, for half the instructions (`near`).
+// A float32 value is the sum of three bfloat16 values: itself rounded to nearest,
+// at most 2^-8 of it away, what that leaves rounded again, 2^-17, and the rest,
+// which fits (the 24 significant bits are 8 and 8 and 8).  A product of two such
+// operands takes the six instructions of the pairs that weigh 2^-17 or more
+// against the first; the three left out are at most 2^-24 of the product, where
+// float32 rounds, and of either sign (planes cut off instead of rounded would leave
+// out up to 2^-21, always toward zero).  Against a bfloat16 input, which is one such
+// value (IN = 1, else 3), three instructions give the product whole.  At 16 cycles
+// for 32 inner elements that is 48 or 96 cycles where float32's instructions take
+// 256.  Values above bfloat16's largest, within 2^-9 of float32's, come out not
+// finite.
 template <int IN>
 struct SplitMath {
-    static constexpr int kIn = IN, kNear = IN == 1 ? 2 : kFull;
+    static constexpr int kIn = IN;
     using b8 = bf16 __attribute__((ext_vector_type(8)));
     template <int PLANES>
     struct Op {
         u4 x[PLANES];          // from the most significant on
     };
-    static __device__ std::uint32_t tops(std::uint32_t low, std::uint32_t high) {      // the upper halves of two words
-        return __builtin_amdgcn_perm(high, low, 0x07060302u);
-    }
     template <int PLANES>
     static __device__ void split(f4 x, u2 (&to)[PLANES]) {
-        std::uint32_t w[4];
 #pragma unroll
         for (int p = 0; p < PLANES; ++p) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float v = x[i];              // bit casts of a vector's element itself take its first
-                w[i] = __builtin_bit_cast(std::uint32_t, v);
-                if (p + 1 < PLANES) x[i] = v - __builtin_bit_cast(float, w[i] & 0xffff0000u);
-            }
-            to[p] = u2{tops(w[0], w[1]), tops(w[2], w[3])};
+            to[p] = u2{pack_bf16(x.x, x.y), pack_bf16(x.z, x.w)};
+            if (p + 1 < PLANES) x -= f4{lo_half(to[p].x), hi_half(to[p].x), lo_half(to[p].y), hi_half(to[p].y)};
         }
     }
-    template <int PLANES>
-    static __device__ Op<PLANES> operand(f4 a, f4 b) {
-        u2 x[PLANES], y[PLANES];
+    static __device__ Op<kFull> full(f4 a, f4 b) {
+        u2 x[kFull], y[kFull];
         split(a, x);
         split(b, y);
-        Op<PLANES> o;
+        Op<kFull> o;
 #pragma unroll
-        for (int p = 0; p < PLANES; ++p) o.x[p] = u4{x[p].x, x[p].y, y[p].x, y[p].y};
+        for (int p = 0; p < kFull; ++p) o.x[p] = u4{x[p].x, x[p].y, y[p].x, y[p].y};
         return o;
-    }
-    static __device__ Op<kFull> full(f4 a, f4 b) { return operand<kFull>(a, b); }
-    static __device__ Op<kNear> near(f4 a, f4 b) { return operand<kNear>(a, b); }
-    static __device__ Op<kNear> near(const Op<kFull>& o) {
-        if constexpr (kNear == kFull) return o;
-        else return {{o.x[0], o.x[1]}};
     }
     // The two result tiles that an operand of inputs holds.
     static __device__ void values(const Op<kIn>& o, f4 (&to)[2]) {
@@ -154,14 +131,13 @@ struct SplitMath {
     struct Tile {
         static constexpr int kRow = COLS + PAD, kPlane = ROWS * kRow;
         alignas(16) std::uint16_t d[PLANES * kPlane];
-        template <int USED = PLANES>
         __device__ void put(int row, int col, float v) {
             std::uint16_t* to = &d[row * kRow + place_of(col)];
 #pragma unroll
-            for (int p = 0; p < USED; ++p) {
-                const std::uint32_t w = __builtin_bit_cast(std::uint32_t, v);
-                to[p * kPlane] = static_cast<std::uint16_t>(w >> 16);
-                v -= __builtin_bit_cast(float, w & 0xffff0000u);
+            for (int p = 0; p < PLANES; ++p) {
+                const bf16 top = static_cast<bf16>(v);
+                to[p * kPlane] = __builtin_bit_cast(std::uint16_t, top);
+                v -= static_cast<float>(top);
             }
         }
         __device__ void put4(int row, int col, f4 v) {
@@ -181,26 +157,24 @@ struct SplitMath {
             put4(row, col + 4, __builtin_bit_cast(f4, u4{w[4], w[5], w[6], w[7]}));
         }
         // Operand of the 16 rows from row0 over the inner columns 32 p ...
-        template <int USED = PLANES>
-        __device__ Op<USED> rows(int row0, int p, int r, int g) const {
+        __device__ Op<PLANES> rows(int row0, int p, int r, int g) const {
             static_assert(PAD % 8 == 0);
-            Op<USED> o;
+            Op<PLANES> o;
 #pragma unroll
-            for (int i = 0; i < USED; ++i)
+            for (int i = 0; i < PLANES; ++i)
                 o.x[i] = *reinterpret_cast<const u4*>(&d[i * kPlane + (row0 + r) * kRow + 32 * p + 8 * g]);
             return o;
         }
         // Operand of the 16 columns from col0 over the inner rows row0 ...  The
         // transposing read hands 16 lanes a block of 4 rows and 16 columns: lane
         // 4 j + q fetches columns 4 q .. of row j, lane r gets column r.
-        template <int USED = PLANES>
-        __device__ Op<USED> cols(int row0, int col0, int r, int g) const {
+        __device__ Op<PLANES> cols(int row0, int col0, int r, int g) const {
             using s4 = short __attribute__((ext_vector_type(4)));
             using lds = __attribute__((address_space(3))) s4;
             const std::uint16_t* from = &d[(row0 + 4 * g + r / 4) * kRow + place_of(col0 + 4 * (r % 4))];
-            Op<USED> o;
+            Op<PLANES> o;
 #pragma unroll
-            for (int i = 0; i < USED; ++i) {
+            for (int i = 0; i < PLANES; ++i) {
                 const u2 a = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)(from + i * kPlane)));
                 const u2 b = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)(from + i * kPlane + 16 * kRow)));
                 o.x[i] = u4{a.x, a.y, b.x, b.y};

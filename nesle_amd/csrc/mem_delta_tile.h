@@ -267,15 +267,15 @@ struct Gates {
     }
 };
 
-// Math: the kind of products.  DP: head dimensions padded to 32, 64 or 128; DP / 16 waves.  P_PLANES: of P.
+// Math: the kind of products.  DP: head dimensions padded to 32, 64 or 128; DP / 16 waves.
 // Later: what takes the place of the values, A and the results afterwards.
-template <typename T, typename Math, int DP, int P_PLANES, typename Later = char>
+template <typename T, typename Math, int DP, typename Later = char>
 struct ChunkTile {
     using M = Math;
     static constexpr int KT = DP / 16, KP = DP / 32, kWaves = DP / 16, kSmall = kChunk + 4;
 
     typename M::template Tile<kChunk, DP, M::kIn, 8> k, q;
-    typename M::template Tile<kChunk, kChunk, P_PLANES, 8> p;     // P: scale L_ij (q_i . k_j), j <= i; else 0
+    typename M::template Tile<kChunk, kChunk, kFull, 8> p;     // P: scale L_ij (q_i . k_j), j <= i; else 0
     typename M::template Tile<kChunk, kChunk, kFull, 8> t;     // (I + A)^-1
     union {
         struct {

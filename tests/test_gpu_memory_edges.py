@@ -1,0 +1,56 @@
+"""The memory operators where they can go wrong: what bfloat16 results hold, and
+equal keys on every kind of products (32, 64 and 128 dimensions of either type)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests import memory_oracle as O
+from tests import test_gpu_memory as M
+from tests.helpers import say
+
+pytestmark = pytest.mark.gpu
+
+F32, NAMES = M.F32, M.NAMES
+BOTH = [torch.float32, torch.bfloat16]
+DIMS = [32, 64, 128]
+
+
+def dev():
+    return torch.device("cuda")
+
+
+# A float32 result that is off by F32 of its norm and then rounded to bfloat16
+# (steps of at most 2^-7 of an element): an element comes out a step away with
+# the chance error / step, so the squares add up to at most |error| |steps| =
+# F32 2^-7 of the result's.
+ROUNDED = (F32 * 2.0 ** -7) ** 0.5
+
+
+@pytest.mark.parametrize("shape", [(128, 16, 4, 4, 64, 64), (96, 16, 2, 4, 32, 32), (96, 8, 2, 2, 128, 128),
+                                   (1024, 2, 2, 2, 64, 64)])
+def test_bfloat16_results_are_float32_results_rounded(shape):
+    """Outputs and the gradients of queries, keys and values hold what float32
+    products give, rounded once."""
+    from nesle_amd import memory
+
+    say(f"[gpu] gated_delta bfloat16 results {shape}")
+    x, resets, grads = M.make(*shape, torch.bfloat16, 31, resets=0.005)
+    ref = [x[n].double().requires_grad_() for n in NAMES]
+    want = O.delta(*ref, resets, shape[-2] ** -0.5)
+    gpu = [x[n].to(dev()).requires_grad_() for n in NAMES]
+    got = memory.gated_delta(*gpu[:5], state=gpu[5], resets=resets.to(dev()))
+    dw = torch.autograd.grad(want, ref, [t.double() for t in grads])
+    dg = torch.autograd.grad(got, gpu, [t.to(dev()) for t in grads])
+    off = {"out": O.off(got[0], want[0]), **{f"d{n}": O.off(a, b) for n, a, b in zip("qkv", dg, dw)}}
+    assert all(v <= ROUNDED for v in off.values()), off
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("dim", DIMS)
+def test_equal_keys_of_every_size(dim, dtype):
+    say(f"[gpu] gated_delta equal keys, {dim} {dtype}")
+    x, resets, grads = M.make(96, 2, 1, 1, dim, dim, dtype, 7, resets=0.0, alike=1.0)
+    x["beta"][:] = 1.0
+    M.check_delta(x, resets, grads)
