@@ -30,6 +30,12 @@ struct F32Math {
     };
     static __device__ Op full(f4 a, f4 b) { return {a, b}; }
     static __device__ f4 mul(const Op& x, const Op& y, f4 c) { return mma(x.b, y.b, mma(x.a, y.a, c)); }
+    // The same, summed by itself, 16 inner elements at a time, and then added: for
+    // sums that cancel later, where the roundings of one long chain would show.
+    static __device__ f4 mul_apart(const Op& x, const Op& y, f4 c) {
+        const f4 zero = {0, 0, 0, 0};
+        return c + (mma(x.a, y.a, zero) + mma(x.b, y.b, zero));
+    }
     // The two result tiles that an operand of inputs holds.
     static __device__ void values(const Op& x, f4 (&to)[2]) {
         to[0] = x.a;
@@ -123,6 +129,9 @@ struct SplitMath {
                                                                 __builtin_bit_cast(b8, y.x[sum - p]), c, 0, 0, 0);
         return c;
     }
+
+    template <int P, int Q>
+    static __device__ f4 mul_apart(const Op<P>& x, const Op<Q>& y, f4 c) { return c + mul(x, y, f4{0, 0, 0, 0}); }
 
     // [ROWS][COLS] of values in planes of bfloat16, columns in place_of order.
     // A row is PAD elements longer: 8 (16 bytes) for a tile that is read by rows,
