@@ -12,10 +12,11 @@ namespace nesle::mem {
 
 constexpr int kChunk = NESLE_DELTA_CHUNK;
 
-// exp(g) is zero in float32 below this (its smallest denormal is 2^-149, and
-// half of it exp(-103.97)): the state is dropped, not multiplied by zero, and
-// every gate that is multiplied keeps a finite logarithm.
-constexpr float kDropBelow = -104.0f;
+// exp(g) is zero in float32 below this: its smallest value is 2^-149, and half of
+// that, which rounds to zero, is exp(-103.9720771), between this number and the next
+// lower one.  The state is dropped there, not multiplied by zero, and every gate that
+// is multiplied keeps a finite logarithm.
+constexpr float kDropBelow = -103.972076f;
 // What a dropping token's gate counts for in the running sums: exp of any
 // difference across it is zero, and 32 of them leave a double 9 digits after the
 // point for the others.

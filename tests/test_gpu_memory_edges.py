@@ -1,5 +1,6 @@
-"""The memory operators where they can go wrong: what bfloat16 results hold, and
-equal keys on every kind of products (32, 64 and 128 dimensions of either type)."""
+"""The memory operators where they can go wrong: what bfloat16 results hold, equal
+keys on every kind of products (32, 64 and 128 dimensions of either type), gates
+that leave nothing."""
 
 from __future__ import annotations
 
@@ -54,3 +55,41 @@ def test_equal_keys_of_every_size(dim, dtype):
     x, resets, grads = M.make(96, 2, 1, 1, dim, dim, dtype, 7, resets=0.0, alike=1.0)
     x["beta"][:] = 1.0
     M.check_delta(x, resets, grads)
+
+
+# exp of the first is zero in float32 (half its smallest value is 2^-150 =
+# exp(-103.97208)), exp of the second is not.
+GONE, HELD = -103.9721, -103.95
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("dim", [32, 64])
+@pytest.mark.parametrize("T", [1, 40, 600])
+def test_gate_whose_exponential_is_zero_drops_the_state(T, dim, dtype):
+    """By selection: a state of NaN reaches nothing after it.  The gradient of
+    the state is zero there, and the gate's."""
+    from nesle_amd import memory
+
+    say(f"[gpu] gated_delta gate of {GONE}, {T} x {dim} {dtype}")
+    assert float(torch.tensor(GONE).exp()) == 0.0 and float(torch.tensor(HELD).exp()) > 0.0
+    x, _, grads = M.make(T, 2, 1, 1, dim, dim, dtype, 14)
+    at = T // 2
+    x["g"][at, 0], x["g"][at, 1] = GONE, HELD
+    y = {n: t.clone() for n, t in x.items()}
+    x["state"][:] = float("nan")
+    y["state"][:] = 0.0
+    got = memory.gated_delta(*(x[n].to(dev()) for n in NAMES[:5]), state=x["state"].to(dev()))
+    y["g"][at, 0] = -float("inf")
+    want = O.delta(*(y[n] for n in NAMES), None, dim ** -0.5)
+    assert O.off(got[0][at:, 0], want[0][at:, 0]) <= M.tol(dtype) and O.off(got[1][0], want[1][0]) <= F32
+    assert torch.isnan(got[0][:, 1]).all() and torch.isnan(got[1][1]).all()
+    if T == 1:
+        state = x["state"].to(dev())
+        out = memory.gated_delta_step(*(x[n][0].to(dev()) for n in NAMES[:5]), state)
+        assert O.off(out[0], want[0][0, 0]) <= M.tol(dtype) and O.off(state[0], want[1][0]) <= F32
+        assert torch.isnan(out[1]).all() and torch.isnan(state[1]).all()
+    y["state"] = torch.randn(y["state"].shape, generator=torch.Generator().manual_seed(1))
+    y["g"][at, 0] = GONE
+    gpu = [y[n].to(dev()).requires_grad_() for n in NAMES]
+    d = torch.autograd.grad(memory.gated_delta(*gpu[:5], state=gpu[5]), gpu, [t.to(dev()) for t in grads])
+    assert float(d[3][at, 0].abs().sum()) == 0.0 and (T > 1 or float(d[5][0].abs().sum()) == 0.0)
