@@ -77,9 +77,9 @@ template <int PAIRS>
 struct Part {
     static constexpr int N = PAIRS / 4;
     f4 a[N], b[N];
-    __device__ void clear() {
+    __device__ void fill(float v) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) a[i] = b[i] = f4{0, 0, 0, 0};
+        for (int i = 0; i < N; ++i) a[i] = b[i] = f4{v, v, v, v};
     }
     template <typename T>
     __device__ void load(const T* p, unsigned first, unsigned second, bool vec) {
@@ -196,17 +196,18 @@ struct AnySpot : Spot {
     }
 };
 
-// Cosines and sines of a lane's pairs.
+// Lane j's part of a head, turned (back) by its row of the table; where the table
+// has no such row all of the head is NaN, its elements past the rotated ones too.
 template <int PAIRS, typename T>
-__device__ Part<PAIRS> turns(const QkArgs<T>& a, std::int32_t p, unsigned j) {
-    Part<PAIRS> t;
-    if (p < 0 || static_cast<std::uint32_t>(p) >= a.table_rows) {
-#pragma unroll
-        for (int i = 0; i < PAIRS / 4; ++i) t.a[i] = t.b[i] = f4{NAN, NAN, NAN, NAN};
-        return t;
+__device__ void rotate(const QkArgs<T>& a, std::int32_t p, unsigned j, bool rotates, bool back, Part<PAIRS>& x) {
+    if (a.rotated == 0) return;
+    if (static_cast<std::uint32_t>(p) >= a.table_rows || p < 0) {
+        x.fill(NAN);
+    } else if (rotates) {
+        Part<PAIRS> t;
+        t.load_floats(a.table + static_cast<std::size_t>(p) * a.rotated, PAIRS * j, PAIRS * j + a.rotated / 2);
+        x.turn(t, back, a.interleaved);
     }
-    t.load_floats(a.table + static_cast<std::size_t>(p) * a.rotated, PAIRS * j, PAIRS * j + a.rotated / 2);
-    return t;
 }
 
 __device__ inline float across(float v, unsigned lanes) {
@@ -227,12 +228,12 @@ __global__ void __launch_bounds__(kThreads) qk_forward(QkArgs<T> a) {
 #pragma unroll
     for (unsigned i = 0; i < TOGETHER; ++i) {
         const std::uint32_t plus = i * per + threadIdx.x / a.lanes;
-        x[i].clear();
+        x[i].fill(0.0f);
         position[i] = 0;
         if (base + plus < a.groups && has) {
             const AnySpot<T> at(a, start, plus);
             x[i].load(at.is_q ? at.in(a.q) : at.in(a.k), first, second, at.is_q ? a.q.vec : a.k.vec);
-            if (rotates) position[i] = a.positions[at.row];
+            if (a.rotated != 0) position[i] = a.positions[at.row];
         }
     }
 #pragma unroll
@@ -248,7 +249,7 @@ __global__ void __launch_bounds__(kThreads) qk_forward(QkArgs<T> a) {
             weight.load_floats(w, first, second);
             x[i].scale(weight);
         }
-        if (rotates) x[i].turn(turns<PAIRS>(a, position[i], j), false, a.interleaved);
+        rotate(a, position[i], j, rotates, false, x[i]);
         x[i].store(at.out(a), first, second);
     }
 }
@@ -276,7 +277,7 @@ __global__ void __launch_bounds__(kThreads) qk_gradient(QkArgs<T> a) {
     places<PAIRS>(a, j, first, second);
     const bool has = 2 * PAIRS * j < a.dim, rotates = 2 * PAIRS * j < a.rotated;
     Part<PAIRS> dw;
-    dw.clear();
+    dw.fill(0.0f);
     const std::uint64_t at_once = static_cast<std::uint64_t>(blocks) * per * kTogether;
     // Every lane of a workgroup takes every turn, as the lane exchanges need.
     for (std::uint64_t base = static_cast<std::uint64_t>(block) * per * kTogether; base < groups; base += at_once) {
@@ -286,14 +287,14 @@ __global__ void __launch_bounds__(kThreads) qk_gradient(QkArgs<T> a) {
 #pragma unroll
         for (unsigned i = 0; i < kTogether; ++i) {
             const std::uint32_t plus = i * per + threadIdx.x / a.lanes;
-            x[i].clear();
-            d[i].clear();
+            x[i].fill(0.0f);
+            d[i].fill(0.0f);
             position[i] = 0;
             if (base + plus < groups && has) {
                 const Spot at(a.batch, per_row, start, plus);
                 x[i].load(at.in(in), first, second, in.vec);
                 d[i].load(at.in(dy), first, second, dy.vec);
-                if (rotates) position[i] = a.positions[at.row];
+                if (a.rotated != 0) position[i] = a.positions[at.row];
             }
         }
 #pragma unroll
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(kThreads) qk_gradient(QkArgs<T> a) {
             const std::uint32_t plus = i * per + threadIdx.x / a.lanes;
             const bool mine = base + plus < groups && has;
             const float inv = 1.0f / sqrtf(across(x[i].dot(x[i]), a.lanes) * a.inv_count + a.eps);
-            if (mine && rotates) d[i].turn(turns<PAIRS>(a, position[i], j), true, a.interleaved);
+            if (mine) rotate(a, position[i], j, rotates, true, d[i]);
             if (w != nullptr && mine) {
                 Part<PAIRS> weight;
                 weight.load_floats(w, first, second);

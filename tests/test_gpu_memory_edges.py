@@ -1,6 +1,6 @@
 """The memory operators where they can go wrong: what bfloat16 results hold, equal
 keys on every kind of products (32, 64 and 128 dimensions of either type), gates
-that leave nothing."""
+that leave nothing, positions outside the table."""
 
 from __future__ import annotations
 
@@ -93,3 +93,20 @@ def test_gate_whose_exponential_is_zero_drops_the_state(T, dim, dtype):
     gpu = [y[n].to(dev()).requires_grad_() for n in NAMES]
     d = torch.autograd.grad(memory.gated_delta(*gpu[:5], state=gpu[5]), gpu, [t.to(dev()) for t in grads])
     assert float(d[3][at, 0].abs().sum()) == 0.0 and (T > 1 or float(d[5][0].abs().sum()) == 0.0)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("rotated", [16, 32])
+def test_position_outside_the_table_makes_the_whole_head_nan(rotated, dtype):
+    from nesle_amd import memory
+
+    say(f"[gpu] qk_norm_rotate positions outside, {rotated} of 32 {dtype}")
+    q, k, wq, wk, pos, table, dq, dk = (t.to(dev()) for t in M.make_rotate((6, 5), 2, 3, 32, rotated, dtype, 6))
+    pos[0, 0], pos[3, 2], pos[5, 4] = -1, 50, 1 << 30
+    bad = (pos < 0) | (pos >= 50)
+    leaves = [t.requires_grad_() for t in (q, k, wq, wk)]
+    got = memory.qk_norm_rotate(*leaves, positions=pos, table=table)
+    d = torch.autograd.grad(got, leaves, [dq, dk])
+    for t in (*got, *d[:2]):
+        assert torch.isnan(t[bad]).all() and torch.isfinite(t[~bad]).all()
+    assert all(torch.isnan(t).all() for t in d[2:])
