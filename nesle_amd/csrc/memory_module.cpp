@@ -131,6 +131,13 @@ bool wants_grad(std::initializer_list<const Tensor*> tensors) {
     return false;
 }
 
+// Forward-mode derivatives are not there either: a tangent would be lost.
+void refuse_tangents(const char* who, std::initializer_list<const Tensor*> tensors) {
+    for (const Tensor* t : tensors)
+        if (t->defined() && t->_fw_grad(/*level=*/0).defined())
+            throw py::value_error(std::string(who) + " has no forward-mode derivative");
+}
+
 // The gradients of a node whose own gradient is not there: asking for it is an
 // error, where it is asked for.
 variable_list first_order(const char* who, const variable_list& outputs, const variable_list& grads) {
@@ -225,11 +232,12 @@ struct QkNormRotate : torch::autograd::Function<QkNormRotate> {
 
 py::tuple qk_norm_rotate(const Tensor& q, const Tensor& k, const MaybeTensor& q_weight, const MaybeTensor& k_weight,
                          const MaybeTensor& positions, const MaybeTensor& table, double eps, bool unit, bool interleaved) {
+    const Tensor wq = some(q_weight), wk = some(k_weight), turns = some(table);
+    refuse_tangents("qk_norm_rotate", {&q, &k, &wq, &wk, &turns});
     const Common c = common_of("qk_norm_rotate", q, 1, 2);
     check_heads(c, k, "k");
     const int64_t dim = q.size(-1);
     if (k.size(-1) != dim) refuse(c.who, "k", "of q's head dimension " + std::to_string(dim), k);
-    const Tensor wq = some(q_weight), wk = some(k_weight), turns = some(table);
     if (wq.defined()) check_plain(c, wq, "q_weight", at::kFloat, {dim}, true);
     if (wk.defined()) check_plain(c, wk, "k_weight", at::kFloat, {dim}, true);
     Tensor at_step;
@@ -360,8 +368,9 @@ struct GatedDelta : torch::autograd::Function<GatedDelta> {
 
 py::tuple gated_delta(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta,
                       const MaybeTensor& state, const MaybeTensor& resets, const std::optional<double>& scale) {
-    const Common c = common_of("gated_delta", q, 2, 2);
     const Tensor start = some(state), ends = some(resets);
+    refuse_tangents("gated_delta", {&q, &k, &v, &g, &beta, &start});
+    const Common c = common_of("gated_delta", q, 2, 2);
     check_delta(c, q, k, v, g, beta, start, ends);
     const double s = scale_or_default(scale, q);
     const variable_list out = wants_grad({&q, &k, &v, &g, &beta, &start})
@@ -372,8 +381,9 @@ py::tuple gated_delta(const Tensor& q, const Tensor& k, const Tensor& v, const T
 
 Tensor gated_delta_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta,
                         const MaybeTensor& state, const MaybeTensor& resets, const std::optional<double>& scale) {
-    const Common c = common_of("gated_delta_step", q, 1, 1);
     if (!given(state)) throw py::value_error("gated_delta_step: state must be a tensor");
+    refuse_tangents("gated_delta_step", {&q, &k, &v, &g, &beta, &*state});
+    const Common c = common_of("gated_delta_step", q, 1, 1);
     const Tensor ends = some(resets);
     check_delta(c, q, k, v, g, beta, *state, ends);
     if (wants_grad({&q, &k, &v, &g, &beta, &*state}))

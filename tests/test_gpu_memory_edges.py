@@ -1,11 +1,12 @@
 """The memory operators where they can go wrong: what bfloat16 results hold, equal
 keys on every kind of products (32, 64 and 128 dimensions of either type), gates
-that leave nothing, positions outside the table."""
+that leave nothing, positions outside the table, calls that cannot be answered."""
 
 from __future__ import annotations
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from tests import memory_oracle as O
 from tests import test_gpu_memory as M
@@ -110,3 +111,38 @@ def test_position_outside_the_table_makes_the_whole_head_nan(rotated, dtype):
     for t in (*got, *d[:2]):
         assert torch.isnan(t[bad]).all() and torch.isfinite(t[~bad]).all()
     assert all(torch.isnan(t).all() for t in d[2:])
+
+
+# ---- calls that cannot be answered --------------------------------------------------------
+
+def _calls():
+    """Each operator as a function of its inputs, with those inputs."""
+    from nesle_amd import memory
+
+    x, _, _ = M.make(4, 2, 1, 1, 16, 16, torch.float32, 21)
+    q, k, v, g, beta, state = (x[n].to(dev()) for n in NAMES)
+    w, table = torch.ones(16, device=dev()), memory.rotation_table(10, 16)
+    pos = torch.zeros(4, 2, dtype=torch.int32, device=dev())
+    return {
+        "qk_norm_rotate": (lambda q, k, w, u, t: memory.qk_norm_rotate(q, k, w, u, positions=pos, table=t)[0],
+                           [q, k, w, w.clone(), table]),
+        "gated_delta": (lambda q, k, v, g, b, s: memory.gated_delta(q, k, v, g, b, state=s)[0], [q, k, v, g, beta, state]),
+        "gated_delta_step": (lambda q, k, v, g, b, s: memory.gated_delta_step(q, k, v, g, b, s),
+                             [q[0], k[0], v[0], g[0], beta[0], state.clone()]),
+    }
+
+
+@pytest.mark.parametrize("name", ["qk_norm_rotate", "gated_delta", "gated_delta_step"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_derivatives_are_refused(name, grad):
+    """A tangent would be lost."""
+    fn, inputs = _calls()[name]
+    for i, t in enumerate(inputs):
+        with fwAD.dual_level():
+            args = list(inputs)
+            args[i] = fwAD.make_dual(t.clone(), torch.ones_like(t))
+            if grad and name != "gated_delta_step":
+                args[(i + 1) % len(args)] = args[(i + 1) % len(args)].clone().requires_grad_(i + 2 < len(args))
+            with pytest.raises(ValueError, match=f"{name}.*forward"):
+                fn(*args)
+    fn(*inputs)

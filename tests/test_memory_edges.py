@@ -1,0 +1,39 @@
+"""The memory operators' binding and entry points without a GPU: calls that cannot
+be answered are refused."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+from nesle_amd import memory
+
+
+def calls():
+    """Each operator as a function of its tensors, and those tensors (on the CPU,
+    which is refused last)."""
+    q, g, state = torch.zeros(2, 3, 1, 16), torch.zeros(2, 3, 1), torch.zeros(3, 1, 16, 16)
+    w, table = torch.ones(16), memory.rotation_table(4, 16, device="cpu")
+    pos = torch.zeros(2, 3, dtype=torch.int32)
+    return {
+        "qk_norm_rotate": (lambda q, k, w, u, t: memory.qk_norm_rotate(q, k, w, u, positions=pos, table=t)[0],
+                           [q, q.clone(), w, w.clone(), table]),
+        "gated_delta": (lambda q, k, v, g, b, s: memory.gated_delta(q, k, v, g, b, state=s)[0],
+                        [q, q.clone(), q.clone(), g, g.clone(), state]),
+        "gated_delta_step": (lambda q, k, v, g, b, s: memory.gated_delta_step(q, k, v, g, b, s),
+                             [q[0], q[1], q[0].clone(), g[0], g[1], state.clone()]),
+    }
+
+
+@pytest.mark.parametrize("name", ["qk_norm_rotate", "gated_delta", "gated_delta_step"])
+def test_forward_derivatives_are_refused(name):
+    fn, inputs = calls()[name]
+    with pytest.raises(ValueError, match="GPU"):
+        fn(*inputs)
+    for i, t in enumerate(inputs):
+        with fwAD.dual_level():
+            args = list(inputs)
+            args[i] = fwAD.make_dual(t.clone(), torch.ones_like(t))
+            with pytest.raises(ValueError, match=f"{name} has no forward-mode derivative"):
+                fn(*args)
