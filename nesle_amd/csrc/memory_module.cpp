@@ -5,11 +5,13 @@
 // own: the same work in Python took 15 us a call and 80 us a backward, several
 // times the kernels.
 #include <ATen/ATen.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
@@ -138,6 +140,15 @@ void refuse_tangents(const char* who, std::initializer_list<const Tensor*> tenso
             throw py::value_error(std::string(who) + " has no forward-mode derivative");
 }
 
+// A trace records the allocation of the outputs but no launch: what it replays
+// would be memory that nobody wrote.
+void refuse_tracing(const char* who) {
+    using c10::impl::TorchDispatchModeKey;
+    using c10::impl::TorchDispatchModeTLS;
+    if (torch::jit::tracer::isTracing() || TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY).has_value())
+        throw py::value_error(std::string(who) + " cannot be traced");
+}
+
 // The gradients of a node whose own gradient is not there: asking for it is an
 // error, where it is asked for.
 variable_list first_order(const char* who, const variable_list& outputs, const variable_list& grads) {
@@ -233,6 +244,7 @@ struct QkNormRotate : torch::autograd::Function<QkNormRotate> {
 py::tuple qk_norm_rotate(const Tensor& q, const Tensor& k, const MaybeTensor& q_weight, const MaybeTensor& k_weight,
                          const MaybeTensor& positions, const MaybeTensor& table, double eps, bool unit, bool interleaved) {
     const Tensor wq = some(q_weight), wk = some(k_weight), turns = some(table);
+    refuse_tracing("qk_norm_rotate");
     refuse_tangents("qk_norm_rotate", {&q, &k, &wq, &wk, &turns});
     const Common c = common_of("qk_norm_rotate", q, 1, 2);
     check_heads(c, k, "k");
@@ -369,6 +381,7 @@ struct GatedDelta : torch::autograd::Function<GatedDelta> {
 py::tuple gated_delta(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta,
                       const MaybeTensor& state, const MaybeTensor& resets, const std::optional<double>& scale) {
     const Tensor start = some(state), ends = some(resets);
+    refuse_tracing("gated_delta");
     refuse_tangents("gated_delta", {&q, &k, &v, &g, &beta, &start});
     const Common c = common_of("gated_delta", q, 2, 2);
     check_delta(c, q, k, v, g, beta, start, ends);
@@ -382,6 +395,7 @@ py::tuple gated_delta(const Tensor& q, const Tensor& k, const Tensor& v, const T
 Tensor gated_delta_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta,
                         const MaybeTensor& state, const MaybeTensor& resets, const std::optional<double>& scale) {
     if (!given(state)) throw py::value_error("gated_delta_step: state must be a tensor");
+    refuse_tracing("gated_delta_step");
     refuse_tangents("gated_delta_step", {&q, &k, &v, &g, &beta, &*state});
     const Common c = common_of("gated_delta_step", q, 1, 1);
     const Tensor ends = some(resets);

@@ -16,7 +16,9 @@ or bfloat16, on the GPU.  Queries, keys and values may be slices of one
 projection's output: only the elements of a head have to lie next to each
 other.  Arguments that do not fit raise ValueError.  Work is enqueued on the
 current stream; nothing synchronises, so calls may be captured in a graph.
-First derivatives in reverse mode only: forward-mode derivatives are refused.
+First derivatives in reverse mode only: forward-mode derivatives are refused,
+and so is a call under a tracer (``torch.jit.trace``, ``make_fx``), whose record
+would hold the outputs without the launch.
 """
 
 from __future__ import annotations

@@ -146,3 +146,15 @@ def test_forward_derivatives_are_refused(name, grad):
             with pytest.raises(ValueError, match=f"{name}.*forward"):
                 fn(*args)
     fn(*inputs)
+
+
+@pytest.mark.parametrize("name", ["qk_norm_rotate", "gated_delta", "gated_delta_step"])
+def test_tracing_is_refused(name):
+    """A trace would hold an output that nobody wrote."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    fn, inputs = _calls()[name]
+    with pytest.raises(ValueError, match=f"{name} cannot be traced"):
+        torch.jit.trace(fn, tuple(inputs), check_trace=False)
+    with pytest.raises(ValueError, match=f"{name} cannot be traced"):
+        make_fx(fn)(*inputs)

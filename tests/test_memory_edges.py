@@ -37,3 +37,14 @@ def test_forward_derivatives_are_refused(name):
             args[i] = fwAD.make_dual(t.clone(), torch.ones_like(t))
             with pytest.raises(ValueError, match=f"{name} has no forward-mode derivative"):
                 fn(*args)
+
+
+@pytest.mark.parametrize("name", ["qk_norm_rotate", "gated_delta", "gated_delta_step"])
+def test_tracing_is_refused(name):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    fn, inputs = calls()[name]
+    with pytest.raises(ValueError, match=f"{name} cannot be traced"):
+        torch.jit.trace(fn, tuple(inputs), check_trace=False)
+    with pytest.raises(ValueError, match=f"{name} cannot be traced"):
+        make_fx(fn)(*inputs)
