@@ -150,12 +150,10 @@ void refuse_tracing(const char* who) {
 }
 
 // The gradients of a node whose own gradient is not there: asking for it is an
-// error, where it is asked for.
-variable_list first_order(const char* who, const variable_list& outputs, const variable_list& grads) {
+// error, where it is asked for.  They depend on the inputs whatever gradient came
+// in, also one that requires none.
+variable_list first_order(const char* who, const variable_list& outputs) {
     if (!at::GradMode::is_enabled()) return outputs;
-    bool asked = false;
-    for (const Tensor& g : grads) asked |= g.defined() && g.requires_grad();
-    if (!asked) return outputs;
     variable_list fakes;
     for (const Tensor& t : outputs) fakes.push_back(t.defined() ? t.detach().requires_grad_() : t);
     auto error = std::make_shared<torch::autograd::DelayedError>(
@@ -235,7 +233,7 @@ struct QkNormRotate : torch::autograd::Function<QkNormRotate> {
             check(nesle_qk_norm_rotate_grad(&a, stream_of(q)));
             out = {dq, dk, dwq, dwk};
         }
-        out = first_order("qk_norm_rotate", out, grads);
+        out = first_order("qk_norm_rotate", out);
         out.resize(9);
         return out;
     }
@@ -372,7 +370,7 @@ struct GatedDelta : torch::autograd::Function<GatedDelta> {
             check(nesle_delta_backward(&a, stream_of(q)));
             out = {dq, dk, dv, dg, dbeta, dstate};
         }
-        out = first_order("gated_delta", out, grads);
+        out = first_order("gated_delta", out);
         out.resize(8);
         return out;
     }

@@ -158,3 +158,14 @@ def test_tracing_is_refused(name):
         torch.jit.trace(fn, tuple(inputs), check_trace=False)
     with pytest.raises(ValueError, match=f"{name} cannot be traced"):
         make_fx(fn)(*inputs)
+
+
+def test_second_derivatives_are_refused_whatever_the_gradients_are():
+    """Also where the gradient handed in needs none: the result depends on the
+    inputs all the same."""
+    for name in ("qk_norm_rotate", "gated_delta"):
+        fn, inputs = _calls()[name]
+        leaves = [t.requires_grad_() for t in inputs[:2]]
+        (d,) = torch.autograd.grad(fn(*inputs).sum(), leaves[:1], create_graph=True)
+        with pytest.raises(RuntimeError, match="second derivative"):
+            d.square().sum().backward()
