@@ -14,6 +14,7 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <limits>
 #include <optional>
 #include <sstream>
 #include <string>
@@ -54,7 +55,14 @@ struct Common {
     int64_t batch() const { return sizes[lead - 1]; }
 };
 
+// The C entries take sizes of 32 bits, and have limits of their own below that.
+void check_sizes(const char* who, const char* name, const Tensor& t) {
+    for (const int64_t n : t.sizes())
+        if (n > std::numeric_limits<uint32_t>::max()) refuse(who, name, "of sizes below 2^32", t);
+}
+
 Common common_of(const char* who, const Tensor& q, int64_t least, int64_t most) {
+    check_sizes(who, "q", q);
     const int64_t lead = q.dim() - 2;
     if (!q.is_cuda() || (q.scalar_type() != at::kFloat && q.scalar_type() != at::kBFloat16) || lead < least ||
         lead > most || q.stride(-1) != 1)
@@ -66,6 +74,7 @@ Common common_of(const char* who, const Tensor& q, int64_t least, int64_t most) 
 
 // [lead..., heads, dim], elements of a head next to each other.
 void check_heads(const Common& c, const Tensor& t, const char* name) {
+    check_sizes(c.who, name, t);
     bool ok = t.scalar_type() == c.type && t.device() == c.device && t.dim() == c.lead + 2 && t.stride(-1) == 1;
     for (int64_t i = 0; ok && i < c.lead; ++i) ok = t.size(i) == c.sizes[i];
     if (!ok) {
@@ -252,6 +261,7 @@ py::tuple qk_norm_rotate(const Tensor& q, const Tensor& k, const MaybeTensor& q_
     if (wk.defined()) check_plain(c, wk, "k_weight", at::kFloat, {dim}, true);
     Tensor at_step;
     if (turns.defined()) {
+        check_sizes(c.who, "table", turns);
         if (turns.dim() != 2 || turns.size(0) < 1 || turns.size(1) < 8 || turns.size(1) % 8 != 0 || turns.size(1) > dim)
             refuse(c.who, "table", "a float32 tensor [rows, R], R a multiple of 8 up to " + std::to_string(dim), turns);
         check_plain(c, turns, "table", at::kFloat, turns.sizes(), true);

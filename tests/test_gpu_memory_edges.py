@@ -169,3 +169,18 @@ def test_second_derivatives_are_refused_whatever_the_gradients_are():
         (d,) = torch.autograd.grad(fn(*inputs).sum(), leaves[:1], create_graph=True)
         with pytest.raises(RuntimeError, match="second derivative"):
             d.square().sum().backward()
+
+
+def test_sizes_of_more_than_32_bits_are_refused():
+    """Of the other tensors too: heads of keys, heads of values."""
+    from nesle_amd import memory
+
+    x, _, _ = M.make(4, 2, 1, 1, 16, 16, torch.float32, 21)
+    q, k, v, g, beta, state = (x[n].to(dev()) for n in NAMES)
+    many = q.expand(4, 2, (1 << 32) + 1, 16)
+    with pytest.raises(ValueError, match="k must be of sizes below"):
+        memory.qk_norm_rotate(q, many)
+    with pytest.raises(ValueError, match="v must be of sizes below"):
+        memory.gated_delta(q, k, many, g, beta, state=state)
+    with pytest.raises(ValueError, match="v must be of sizes below"):
+        memory.gated_delta_step(q[0], k[0], many[0], g[0], beta[0], state)

@@ -48,3 +48,16 @@ def test_tracing_is_refused(name):
         torch.jit.trace(fn, tuple(inputs), check_trace=False)
     with pytest.raises(ValueError, match=f"{name} cannot be traced"):
         make_fx(fn)(*inputs)
+
+
+@pytest.mark.parametrize("name", ["qk_norm_rotate", "gated_delta", "gated_delta_step"])
+def test_sizes_of_more_than_32_bits_are_refused(name):
+    """An expanded tensor takes no memory, so such a size is within reach; cut to
+    32 bits it would pass every later check."""
+    fn, inputs = calls()[name]
+    for size in (1 << 32, (1 << 32) + 2):
+        for dim in range(inputs[0].dim() - 1):
+            q = inputs[0][tuple(slice(0, 1) if d == dim else slice(None) for d in range(inputs[0].dim()))]
+            q = q.expand(*(size if d == dim else n for d, n in enumerate(q.shape)))
+            with pytest.raises(ValueError, match=f"{name}: q must be of sizes below 2\\^32"):
+                fn(q, q, *inputs[2:])
