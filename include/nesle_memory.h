@@ -70,6 +70,7 @@ typedef struct nesle_qk_args {
     float* scratch;              /*           nesle_qk_scratch_floats() floats */
 } nesle_qk_args;
 
+/* 0 where no scratch is needed, and for dimensions that the calls refuse. */
 uint64_t nesle_qk_scratch_floats(const nesle_qk_args* args);
 int nesle_qk_norm_rotate(const nesle_qk_args* args, void* stream);
 int nesle_qk_norm_rotate_grad(const nesle_qk_args* args, void* stream);

@@ -499,6 +499,7 @@ extern "C" {
 
 std::uint64_t nesle_qk_scratch_floats(const nesle_qk_args* a) {
     if (a == nullptr || (a->q_weight == nullptr && a->k_weight == nullptr)) return 0;
+    if (a->dim == 0 || a->dim > NESLE_QK_MAX_DIM) return 0;        // no call takes it, and no workgroup a head of it
     return (static_cast<std::uint64_t>(grad_blocks(*a, a->q_heads)) + grad_blocks(*a, a->k_heads)) * a->dim;
 }
 

@@ -3,11 +3,17 @@ be answered are refused."""
 
 from __future__ import annotations
 
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
 
 from nesle_amd import memory
+
+ROOT = Path(__file__).resolve().parents[1]
 
 
 def calls():
@@ -61,3 +67,13 @@ def test_sizes_of_more_than_32_bits_are_refused(name):
             q = q.expand(*(size if d == dim else n for d, n in enumerate(q.shape)))
             with pytest.raises(ValueError, match=f"{name}: q must be of sizes below 2\\^32"):
                 fn(q, q, *inputs[2:])
+
+
+@pytest.mark.parametrize("dim", [0, 264, 3000, 4096, 0xffffffff])
+def test_scratch_of_dimensions_that_are_refused(dim):
+    """The size asked for ends, and is nothing, where the call itself refuses (in a
+    process of its own: it did not return for the largest)."""
+    code = ("import ctypes; from nesle_amd import abi; a = abi.QkArgs(abi.MEM_F32, 4, 2, 2, 2, %d, 0, 0, 0, 1e-6, "
+            "q_weight=16); print(abi.lib().nesle_qk_scratch_floats(ctypes.byref(a)))" % dim)
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=60, cwd=ROOT)
+    assert done.returncode == 0 and done.stdout.strip() == "0", done
