@@ -8,7 +8,8 @@ Replaces the reference's nvcc build script (scripts/build_cuda_extension.py):
   (re-exported by nesle_amd/_cuda_core.py), host-only C++ linked against
   libnesle_hip.so (rpath $ORIGIN);
 * ``_memory_native*.so`` -- tensor and autograd binding of the memory operators
-  (nesle_amd/memory.py), host-only C++ against PyTorch and libnesle_hip.so.
+  (nesle_amd/memory.py), host-only C++ against PyTorch and libnesle_hip.so; left
+  out where PyTorch is not importable, as the console and its batch need none.
 
 All land in-tree next to this file.  ``python -m nesle_amd.build`` rebuilds.
 Environment: ``HIPCC`` (default: hipcc on PATH or /opt/rocm/bin/hipcc),
@@ -18,6 +19,7 @@ Environment: ``HIPCC`` (default: hipcc on PATH or /opt/rocm/bin/hipcc),
 from __future__ import annotations
 
 import concurrent.futures
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -152,7 +154,15 @@ def link_memory(obj: Path) -> Path:
     return out
 
 
+def has_torch() -> bool:
+    return importlib.util.find_spec("torch") is not None
+
+
 def build_all() -> None:
+    if not has_torch():
+        build_hip()
+        build_shim()
+        return
     with tempfile.TemporaryDirectory(prefix="nesle_memory_") as work, concurrent.futures.ThreadPoolExecutor(1) as pool:
         obj = Path(work) / "memory_module.o"
         binding = pool.submit(compile_memory, obj)      # while hipcc compiles the kernels
@@ -164,4 +174,5 @@ def build_all() -> None:
 
 if __name__ == "__main__":
     build_all()
-    print(f"built {LIB.name}, {shim_path().name} and {memory_path().name}")
+    print(f"built {LIB.name}, {shim_path().name}" + (f" and {memory_path().name}" if has_torch() else
+                                                    "; no PyTorch, so no memory operators"))

@@ -77,3 +77,15 @@ def test_scratch_of_dimensions_that_are_refused(dim):
             "q_weight=16); print(abi.lib().nesle_qk_scratch_floats(ctypes.byref(a)))" % dim)
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=60, cwd=ROOT)
     assert done.returncode == 0 and done.stdout.strip() == "0", done
+
+
+def test_the_console_builds_without_pytorch(monkeypatch):
+    from nesle_amd import build
+
+    made = []
+    monkeypatch.setitem(sys.modules, "torch", None)        # not importable
+    monkeypatch.setattr(build, "build_hip", lambda: made.append("hip"))
+    monkeypatch.setattr(build, "build_shim", lambda: made.append("shim"))
+    monkeypatch.setattr(build, "_run", lambda cmd: made.append(cmd))
+    build.build_all()
+    assert made == ["hip", "shim"]
