@@ -135,7 +135,7 @@ def train_memory_ppo(config: MemoryPPOConfig, *, rom_bytes: bytes | None = None,
     actions = torch.empty((T, n), dtype=torch.long, device=dev)
     logprobs, rewards, dones, values = (torch.empty((T, n), device=dev) for _ in range(4))
     steps, resets = torch.empty((T, n), dtype=torch.int32, device=dev), torch.empty((T, n), dtype=torch.bool, device=dev)
-    state, step = model.new_state(n), torch.zeros(n, dtype=torch.int32, device=dev)
+    state, length = model.new_state(n), torch.zeros(n, dtype=torch.int32, device=dev)      # steps of the episode so far
     done = torch.ones(n, dtype=torch.bool, device=dev)      # every console starts an episode
     last = model.table.shape[0] - 1
     stats = {"global_step": 0, "updates": 0, "log": [], "model": model}
@@ -143,7 +143,7 @@ def train_memory_ppo(config: MemoryPPOConfig, *, rom_bytes: bytes | None = None,
     for update in range(1, math.ceil(config.total_timesteps / (n * T)) + 1):
         before = state.clone()
         for t in range(T):
-            step = torch.where(done, 0, torch.clamp(step + 1, max=last)).to(torch.int32)
+            step = torch.clamp(length, max=last)
             obs[t], dones[t], steps[t], resets[t] = ram, done.float(), step, done
             logits, values[t] = model.act(ram, step, done, state)
             logp = torch.log_softmax(logits, -1)
@@ -152,9 +152,14 @@ def train_memory_ppo(config: MemoryPPOConfig, *, rom_bytes: bytes | None = None,
             batch.step_device(mask_table[action], auto_reset=True, synchronize=False)
             rewards[t] = rewards_view
             done = dones_view.bool()
+            length += 1
+            if config.max_episode_steps > 0:
+                timeout = (length >= config.max_episode_steps) & ~done
+                batch.reset_envs_device(timeout.to(torch.uint8))       # consoles not in the mask are untouched
+                done = done | timeout
+            length.masked_fill_(done, 0)
         with torch.no_grad():
-            _, next_value = model.act(ram, torch.where(done, 0, torch.clamp(step + 1, max=last)).to(torch.int32), done,
-                                      state.clone())
+            _, next_value = model.act(ram, torch.clamp(length, max=last), done, state.clone())
             advantages, returns = P.compute_gae(rewards, dones, values, done.float(), next_value, config.gamma,
                                                 config.gae_lambda)
         if on_rollout is not None:
@@ -196,12 +201,14 @@ def main(argv=None) -> None:
     p.add_argument("--action-space", default="simple_with_start",
                    choices=["right_only", "simple", "simple_with_start", "complex", "mario", "raw"])
     p.add_argument("--reset-state-path", default=None)
+    p.add_argument("--max-episode-steps", type=int, default=0)
     p.add_argument("--seed", type=int, default=1)
     a = p.parse_args(argv)
     train_memory_ppo(MemoryPPOConfig(
         rom_path=a.rom_path, num_envs=a.num_envs, total_timesteps=a.total_timesteps, n_steps=a.n_steps,
         batch_size=a.batch_size, heads=a.heads, head_dim=a.head_dim, memory_dtype=a.memory_dtype,
-        action_space=a.action_space, reset_state_path=a.reset_state_path, seed=a.seed))
+        action_space=a.action_space, reset_state_path=a.reset_state_path,
+        max_episode_steps=a.max_episode_steps, seed=a.seed))
 
 
 if __name__ == "__main__":

@@ -1,0 +1,65 @@
+"""Options of the trainer of a policy with memory (nesle_amd.memory_ppo) that it
+shares with native_ppo's: each is honoured."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from nesle_amd import synthrom
+from oracle import oracle as O
+from tests.helpers import OracleBatch, say, warm_snapshots
+
+pytestmark = pytest.mark.gpu
+
+REWARD = dict(kind="x_delta", x_lo=synthrom.X_LO, x_hi=synthrom.X_HI, done_addr=synthrom.DONE_BYTE, clip=15,
+              time_penalty=0.25)
+
+
+def trainer(**kw):
+    """(config, ROM, snapshots) of a small run on the synthetic game."""
+    from nesle_amd import memory_ppo as M
+
+    rom = synthrom.make_rom(5).rom
+    snaps = warm_snapshots(rom, [100, 150, 200, 250], seed=55)
+    for i, s in enumerate(snaps):
+        s[O.OFF["ram"] + synthrom.DONE_BYTE] = 3 + 4 * i
+    return M.MemoryPPOConfig("synthetic.nes", **{**dict(
+        num_envs=16, n_steps=12, batch_size=96, update_epochs=1, total_timesteps=2 * 16 * 12, action_space="complex",
+        reward=REWARD, seed=4, save_checkpoints=False), **kw}), rom, [bytes(s) for s in snaps]
+
+
+@pytest.mark.parametrize("most", [0, 5])
+def test_episodes_end_at_the_step_limit(most):
+    """Consoles, steps of the episode and resets are those of oracle consoles under
+    the same actions, put back where an episode ended by itself or by the limit."""
+    from nesle_amd import memory_ppo as M
+
+    say(f"[gpu] memory ppo, max_episode_steps={most}")
+    cfg, rom, snaps = trainer(max_episode_steps=most)
+    seen = []
+    M.train_memory_ppo(cfg, rom_bytes=rom, snapshot_bytes=snaps, on_rollout=lambda u, b: seen.append(
+        {k: b[k].cpu().numpy().copy() for k in ("actions", "rewards", "steps", "resets", "obs")}))
+    run = {k: np.concatenate([s[k] for s in seen]) for k in seen[0]}
+    masks = np.asarray(M._actions.action_masks("complex"), dtype=np.uint8)
+    n, levels = cfg.num_envs, np.arange(cfg.num_envs) % len(snaps)
+    ob = OracleBatch(rom, list(range(n)), reward=dict(REWARD, kind=1))
+    for e, c in enumerate(ob.cons):
+        c.load(np.frombuffer(snaps[levels[e]], dtype=np.uint8))
+    first_ram = np.stack([np.frombuffer(s, dtype=np.uint8)[O.OFF["ram"]:O.OFF["ram"] + 2048] for s in snaps])[levels]
+    done, length, by_limit = np.ones(n, dtype=bool), np.zeros(n, dtype=np.int64), 0
+    for t in range(len(run["steps"])):
+        length = np.where(done, 0, length)
+        np.testing.assert_array_equal(run["resets"][t], done, err_msg=f"step {t}")
+        np.testing.assert_array_equal(run["steps"][t], length, err_msg=f"step {t}")
+        np.testing.assert_array_equal(run["obs"][t][done], first_ram[done], err_msg=f"step {t}")
+        _, want, ended = ob.step(masks[run["actions"][t]], 4)
+        np.testing.assert_array_equal(run["rewards"][t], want, err_msg=f"step {t}")
+        length += 1
+        late = (length >= most) & ~ended.astype(bool) if most else np.zeros(n, dtype=bool)
+        by_limit += int(late.sum())
+        done = ended.astype(bool) | late
+        for e in np.nonzero(done)[0]:
+            ob.cons[e].load(np.frombuffer(snaps[levels[e]], dtype=np.uint8))
+    assert (by_limit > 0) == (most > 0)
