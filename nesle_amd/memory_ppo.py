@@ -102,11 +102,13 @@ class MemoryPPOConfig(P.NativePPOConfig):
     heads: int = 4
     head_dim: int = 64
     memory_dtype: str = "float32"
+    checkpoint_path: str = "nesle_memory_ppo.pt"
 
 
-def train_memory_ppo(config: MemoryPPOConfig, *, rom_bytes: bytes | None = None, snapshot_bytes=None, batch=None,
+def train_memory_ppo(config: MemoryPPOConfig, resume_from: str | None = None, *, rom_bytes: bytes | None = None, snapshot_bytes=None, batch=None,
                      on_rollout=None) -> dict:
-    """Train; returns {"global_step", "updates", "log", "model"}.
+    """Train; returns {"global_step", "updates", "log", "model"}.  Checkpoints, and
+    ``resume_from`` one of them, as ``native_ppo``'s trainer has them.
     ``on_rollout(update, buffers)`` receives each rollout's buffers (tests)."""
     if config.reward_mode != "minimal":
         raise ValueError("the memory trainer takes reward_mode 'minimal'")
@@ -130,6 +132,7 @@ def train_memory_ppo(config: MemoryPPOConfig, *, rom_bytes: bytes | None = None,
     model = MemoryActorCritic(len(masks), width=config.hidden_size, heads=config.heads, head_dim=config.head_dim,
                               dtype=getattr(torch, config.memory_dtype))
     optimizer = torch.optim.Adam(model.parameters(), lr=config.learning_rate, eps=1e-5, fused=True)
+    global_step = P._load_checkpoint(resume_from, model, optimizer)
 
     obs = torch.empty((T, n, 2048), dtype=torch.uint8, device=dev)
     actions = torch.empty((T, n), dtype=torch.long, device=dev)
@@ -138,9 +141,9 @@ def train_memory_ppo(config: MemoryPPOConfig, *, rom_bytes: bytes | None = None,
     state, length = model.new_state(n), torch.zeros(n, dtype=torch.int32, device=dev)      # steps of the episode so far
     done = torch.ones(n, dtype=torch.bool, device=dev)      # every console starts an episode
     last = model.table.shape[0] - 1
-    stats = {"global_step": 0, "updates": 0, "log": [], "model": model}
+    stats = {"global_step": global_step, "updates": 0, "log": [], "model": model}
 
-    for update in range(1, math.ceil(config.total_timesteps / (n * T)) + 1):
+    for update in range(1, math.ceil(max(0, config.total_timesteps - global_step) / (n * T)) + 1):
         before = state.clone()
         for t in range(T):
             step = torch.clamp(length, max=last)
@@ -185,6 +188,8 @@ def train_memory_ppo(config: MemoryPPOConfig, *, rom_bytes: bytes | None = None,
                 "reward_mean": float(rewards.mean()), "episodes": int(dones.sum())}
         stats["log"].append(line)
         print(" ".join(f"{k}={v:.4f}" if isinstance(v, float) else f"{k}={v}" for k, v in line.items()), flush=True)
+        if config.save_checkpoints:
+            P._save_checkpoint(config.checkpoint_path, model, optimizer, config, stats["global_step"])
     return stats
 
 
@@ -203,12 +208,14 @@ def main(argv=None) -> None:
     p.add_argument("--reset-state-path", default=None)
     p.add_argument("--max-episode-steps", type=int, default=0)
     p.add_argument("--seed", type=int, default=1)
+    p.add_argument("--checkpoint-path", default="nesle_memory_ppo.pt")
+    p.add_argument("--resume-from", default=None)
     a = p.parse_args(argv)
     train_memory_ppo(MemoryPPOConfig(
         rom_path=a.rom_path, num_envs=a.num_envs, total_timesteps=a.total_timesteps, n_steps=a.n_steps,
         batch_size=a.batch_size, heads=a.heads, head_dim=a.head_dim, memory_dtype=a.memory_dtype,
         action_space=a.action_space, reset_state_path=a.reset_state_path,
-        max_episode_steps=a.max_episode_steps, seed=a.seed))
+        max_episode_steps=a.max_episode_steps, seed=a.seed, checkpoint_path=a.checkpoint_path), a.resume_from)
 
 
 if __name__ == "__main__":

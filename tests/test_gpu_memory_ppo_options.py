@@ -63,3 +63,25 @@ def test_episodes_end_at_the_step_limit(most):
         for e in np.nonzero(done)[0]:
             ob.cons[e].load(np.frombuffer(snaps[levels[e]], dtype=np.uint8))
     assert (by_limit > 0) == (most > 0)
+
+
+def test_checkpoints_are_written_and_read(tmp_path):
+    """The model and optimizer of the last update, and a run that goes on from them."""
+    from nesle_amd import memory_ppo as M
+
+    say("[gpu] memory ppo, checkpoints")
+    path = tmp_path / "made" / "memory.pt"
+    cfg, rom, snaps = trainer(save_checkpoints=True, checkpoint_path=str(path))
+    stats = M.train_memory_ppo(cfg, rom_bytes=rom, snapshot_bytes=snaps)
+    kept = torch.load(path, weights_only=True)
+    assert kept["global_step"] == stats["global_step"] == 2 * 16 * 12 and kept["config"]["heads"] == cfg.heads
+    want = stats["model"].state_dict()
+    assert kept["model"].keys() == want.keys() and all(torch.equal(kept["model"][k], want[k]) for k in want)
+
+    seen = []
+    cfg, _, _ = trainer(total_timesteps=3 * 16 * 12)
+    after = M.train_memory_ppo(cfg, str(path), rom_bytes=rom, snapshot_bytes=snaps, on_rollout=lambda u, b: seen.append(
+        {k: v.clone() for k, v in b["model"].state_dict().items()}))
+    assert len(seen) == after["updates"] == 1 and after["global_step"] == 3 * 16 * 12
+    assert all(torch.equal(seen[0][k], want[k].to(seen[0][k].device)) for k in want)
+    assert torch.load(path, weights_only=True)["global_step"] == 2 * 16 * 12        # the second run saved nothing
