@@ -39,8 +39,10 @@ class MemoryActorCritic(nn.Module):
     tanh -> action logits + value."""
 
     def __init__(self, action_dim: int, obs_dim: int = 2048, width: int = 256, heads: int = 4, head_dim: int = 64,
-                 max_steps: int = 4096, dtype: torch.dtype = torch.float32, device=None) -> None:
+                 max_steps: int = 4096, dtype: torch.dtype = torch.float32, init: str = "orthogonal", device=None) -> None:
         super().__init__()
+        if init not in ("orthogonal", "xavier"):
+            raise ValueError(f"unknown init {init!r}: 'orthogonal' or 'xavier'")
         dev = device if device is not None else torch.device("cuda")
         self.heads, self.head_dim, self.dtype = heads, head_dim, dtype
         inner = heads * head_dim
@@ -54,7 +56,7 @@ class MemoryActorCritic(nn.Module):
         self.critic = nn.Linear(width, 1, device=dev)
         for layer, gain in ((self.encode, math.sqrt(2.0)), (self.project, 1.0), (self.gates, 0.1), (self.merge, 1.0),
                             (self.actor, 0.01), (self.critic, 1.0)):
-            nn.init.orthogonal_(layer.weight, gain)
+            (nn.init.orthogonal_ if init == "orthogonal" else nn.init.xavier_uniform_)(layer.weight, gain)
             nn.init.zeros_(layer.bias)
         # Half lives of about 10 to 300 steps to begin with, one for each head.
         with torch.no_grad():
@@ -98,20 +100,25 @@ class MemoryActorCritic(nn.Module):
 @dataclass
 class MemoryPPOConfig(P.NativePPOConfig):
     """``native_ppo``'s configuration; ``batch_size`` counts samples and is
-    rounded down to whole consoles.  Rewards are the batch's in-kernel rule."""
+    rounded down to whole consoles.  Rewards are the batch's in-kernel rule, so the
+    shaped reward's options are refused.  Rollouts and updates run eagerly, whatever
+    ``cuda_graph`` says."""
     heads: int = 4
     head_dim: int = 64
     memory_dtype: str = "float32"
     checkpoint_path: str = "nesle_memory_ppo.pt"
 
 
-def train_memory_ppo(config: MemoryPPOConfig, resume_from: str | None = None, *, rom_bytes: bytes | None = None, snapshot_bytes=None, batch=None,
-                     on_rollout=None) -> dict:
+def train_memory_ppo(config: MemoryPPOConfig, resume_from: str | None = None, *, rom_bytes: bytes | None = None,
+                     snapshot_bytes=None, batch=None, on_rollout=None) -> dict:
     """Train; returns {"global_step", "updates", "log", "model"}.  Checkpoints, and
     ``resume_from`` one of them, as ``native_ppo``'s trainer has them.
     ``on_rollout(update, buffers)`` receives each rollout's buffers (tests)."""
     if config.reward_mode != "minimal":
         raise ValueError("the memory trainer takes reward_mode 'minimal'")
+    for name in ("flag_bonus", "finish_zone_bonus", "death_penalty"):
+        if getattr(config, name) is not None:
+            raise ValueError(f"{name} belongs to reward_mode 'smart', which the memory trainer does not take")
     n, T = config.num_envs, config.n_steps
     consoles = config.batch_size // T
     if consoles < 1 or consoles > n:
@@ -130,7 +137,7 @@ def train_memory_ppo(config: MemoryPPOConfig, resume_from: str | None = None, *,
     ram, rewards_view, dones_view = (from_dlpack(v()) for v in (batch.ram_device, batch.rewards_device,
                                                                 batch.last_done_device))
     model = MemoryActorCritic(len(masks), width=config.hidden_size, heads=config.heads, head_dim=config.head_dim,
-                              dtype=getattr(torch, config.memory_dtype))
+                              dtype=getattr(torch, config.memory_dtype), init=config.init)
     optimizer = torch.optim.Adam(model.parameters(), lr=config.learning_rate, eps=1e-5, fused=True)
     global_step = P._load_checkpoint(resume_from, model, optimizer)
 
@@ -143,7 +150,9 @@ def train_memory_ppo(config: MemoryPPOConfig, resume_from: str | None = None, *,
     last = model.table.shape[0] - 1
     stats = {"global_step": global_step, "updates": 0, "log": [], "model": model}
 
-    for update in range(1, math.ceil(max(0, config.total_timesteps - global_step) / (n * T)) + 1):
+    num_updates = math.ceil(max(0, config.total_timesteps - global_step) / (n * T))
+    progress = P._progress_bar(config.progress_bar, global_step + num_updates * n * T, global_step)
+    for update in range(1, num_updates + 1):
         before = state.clone()
         for t in range(T):
             step = torch.clamp(length, max=last)
@@ -183,6 +192,10 @@ def train_memory_ppo(config: MemoryPPOConfig, resume_from: str | None = None, *,
                 count += 1
         stats["global_step"] += n * T
         stats["updates"] = update
+        if progress is not None:
+            progress.update(n * T)
+        if update % max(1, config.log_interval) != 0 and update != num_updates:
+            continue
         loss, clipfrac = (sums / count).tolist()
         line = {"update": update, "step": stats["global_step"], "loss": loss, "clipfrac": clipfrac,
                 "reward_mean": float(rewards.mean()), "episodes": int(dones.sum())}
@@ -190,6 +203,8 @@ def train_memory_ppo(config: MemoryPPOConfig, resume_from: str | None = None, *,
         print(" ".join(f"{k}={v:.4f}" if isinstance(v, float) else f"{k}={v}" for k, v in line.items()), flush=True)
         if config.save_checkpoints:
             P._save_checkpoint(config.checkpoint_path, model, optimizer, config, stats["global_step"])
+    if progress is not None:
+        progress.close()
     return stats
 
 
@@ -207,7 +222,10 @@ def main(argv=None) -> None:
                    choices=["right_only", "simple", "simple_with_start", "complex", "mario", "raw"])
     p.add_argument("--reset-state-path", default=None)
     p.add_argument("--max-episode-steps", type=int, default=0)
+    p.add_argument("--init", default="orthogonal", choices=["orthogonal", "xavier"])
     p.add_argument("--seed", type=int, default=1)
+    p.add_argument("--log-interval", type=int, default=1)
+    p.add_argument("--progress-bar", action="store_true")
     p.add_argument("--checkpoint-path", default="nesle_memory_ppo.pt")
     p.add_argument("--resume-from", default=None)
     a = p.parse_args(argv)
@@ -215,7 +233,8 @@ def main(argv=None) -> None:
         rom_path=a.rom_path, num_envs=a.num_envs, total_timesteps=a.total_timesteps, n_steps=a.n_steps,
         batch_size=a.batch_size, heads=a.heads, head_dim=a.head_dim, memory_dtype=a.memory_dtype,
         action_space=a.action_space, reset_state_path=a.reset_state_path,
-        max_episode_steps=a.max_episode_steps, seed=a.seed, checkpoint_path=a.checkpoint_path), a.resume_from)
+        max_episode_steps=a.max_episode_steps, init=a.init, seed=a.seed, log_interval=a.log_interval,
+        progress_bar=a.progress_bar, checkpoint_path=a.checkpoint_path), a.resume_from)
 
 
 if __name__ == "__main__":

@@ -85,3 +85,37 @@ def test_checkpoints_are_written_and_read(tmp_path):
     assert len(seen) == after["updates"] == 1 and after["global_step"] == 3 * 16 * 12
     assert all(torch.equal(seen[0][k], want[k].to(seen[0][k].device)) for k in want)
     assert torch.load(path, weights_only=True)["global_step"] == 2 * 16 * 12        # the second run saved nothing
+
+
+@pytest.mark.parametrize("init", ["orthogonal", "xavier"])
+def test_weights_start_as_asked(init):
+    """Orthogonal rows, or values that reach xavier's bound and no further."""
+    from nesle_amd import memory_ppo as M
+
+    torch.manual_seed(0)
+    model = M.MemoryActorCritic(12, init=init)
+    w = model.encode.weight.detach().double()               # 256 x 2,048, gain sqrt(2)
+    bound = 2.0 ** 0.5 * (6 / (256 + 2048)) ** 0.5
+    assert (float(w.abs().max()) <= bound * (1 + 1e-6)) == (init == "xavier")
+    square = w @ w.T
+    square.diagonal().sub_(2.0)
+    assert (float(square.abs().max()) < 1e-4) == (init == "orthogonal")
+
+
+def test_log_lines_at_the_interval_and_the_end():
+    from nesle_amd import memory_ppo as M
+
+    say("[gpu] memory ppo, log_interval")
+    cfg, rom, snaps = trainer(log_interval=2, total_timesteps=5 * 16 * 12, init="xavier")
+    stats = M.train_memory_ppo(cfg, rom_bytes=rom, snapshot_bytes=snaps)
+    assert stats["updates"] == 5 and [x["update"] for x in stats["log"]] == [2, 4, 5]
+
+
+def test_options_that_would_have_no_effect_are_refused():
+    from nesle_amd import memory_ppo as M
+
+    for option in ("flag_bonus", "finish_zone_bonus", "death_penalty"):
+        with pytest.raises(ValueError, match=option):
+            M.train_memory_ppo(M.MemoryPPOConfig("x", **{option: 1.0}))
+    with pytest.raises(ValueError, match="init"):
+        M.MemoryActorCritic(12, init="zeros")
