@@ -69,7 +69,7 @@ class MemoryActorCritic(nn.Module):
 
     def _tokens(self, obs, steps):
         """(features, q, k, v, g, beta) of observations [..., obs_dim]."""
-        x = torch.tanh(self.encode(obs.float().div_(255.0)))
+        x = torch.tanh(self.encode((obs / 255.0).float()))
         q, k, v = self.project(x).to(self.dtype).unflatten(-1, (3, self.heads, self.head_dim)).unbind(-3)
         # Unit norms (the rule wants keys of about unit length); the weights
         # scale the directions against each other.

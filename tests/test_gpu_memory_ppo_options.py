@@ -119,3 +119,18 @@ def test_options_that_would_have_no_effect_are_refused():
             M.train_memory_ppo(M.MemoryPPOConfig("x", **{option: 1.0}))
     with pytest.raises(ValueError, match="init"):
         M.MemoryActorCritic(12, init="zeros")
+
+
+def test_observations_are_left_as_they_are():
+    """Float observations too, which a cast would hand on as they lie; the policy
+    sees the same."""
+    from nesle_amd import memory_ppo as M
+
+    model = M.MemoryActorCritic(12)
+    ram = torch.randint(0, 256, (4, 2048), dtype=torch.uint8, generator=torch.Generator().manual_seed(1)).cuda()
+    steps, resets = torch.zeros(4, dtype=torch.int32).cuda(), torch.ones(4, dtype=torch.bool).cuda()
+    want = model.act(ram, steps, resets, model.new_state(4))
+    obs = ram.float()
+    got = model.act(obs, steps, resets, model.new_state(4))
+    assert torch.equal(obs, ram.float())
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
