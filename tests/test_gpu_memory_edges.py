@@ -1,6 +1,7 @@
-"""The memory operators where they can go wrong: what bfloat16 results hold, equal
-keys on every kind of products (32, 64 and 128 dimensions of either type), gates
-that leave nothing, positions outside the table, calls that cannot be answered."""
+"""The memory operators where they can go wrong: what bfloat16 results hold; equal
+keys, ended episodes, gates and values that are not finite on every kind of
+products (32, 64 and 128 dimensions of either type); gates that leave nothing,
+positions outside the table, calls that cannot be answered."""
 
 from __future__ import annotations
 
@@ -184,3 +185,73 @@ def test_sizes_of_more_than_32_bits_are_refused():
         memory.gated_delta(q, k, many, g, beta, state=state)
     with pytest.raises(ValueError, match="v must be of sizes below"):
         memory.gated_delta_step(q[0], k[0], many[0], g[0], beta[0], state)
+
+
+# ---- ended episodes, gates ------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("dim", DIMS)
+@pytest.mark.parametrize("where", ["all", "first", "edges", "last"])
+def test_resets_of_every_size(where, dim, dtype):
+    say(f"[gpu] gated_delta resets {where}, {dim} {dtype}")
+    x, resets, grads = M.make(70, 3, 1, 2, dim, dim, dtype, 5, resets=0.0)
+    resets[:] = where == "all"
+    if where == "first":
+        resets[0] = True
+    if where == "last":
+        resets[-1] = True
+    if where == "edges":
+        for n, t in enumerate((31, 32, 33)):
+            resets[t, n] = True
+            resets[t + 1, n] = n == 2
+    M.check_delta(x, resets, grads)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("dim", DIMS)
+@pytest.mark.parametrize("gate", ["zero", "strong", "off", "growing"])
+def test_gates_of_every_size(gate, dim, dtype):
+    say(f"[gpu] gated_delta gates {gate}, {dim} {dtype}")
+    x, resets, grads = M.make(70, 2, 1, 2, dim, dim, dtype, 6, resets=0.0)
+    if gate == "zero":
+        x["g"].zero_()
+    elif gate == "strong":
+        x["g"] = x["g"] * 250
+    elif gate == "growing":
+        x["g"] = x["g"] * -0.1
+    else:
+        x["g"][5, 0, 0], x["g"][40, 1, 1], x["g"][32, 0, 1] = -float("inf"), -200.0, -float("inf")
+    M.check_delta(x, resets, grads)
+
+
+# ---- what is not finite ------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("dim", DIMS)
+@pytest.mark.parametrize("T", [70, 900])
+def test_what_is_not_finite_stays_where_it_belongs(T, dim, dtype):
+    """A state of NaN ends at a reset; a NaN or infinite token reaches neither
+    earlier tokens, nor other consoles, nor the next episode.  900 steps of 4
+    heads are walked in segments."""
+    from nesle_amd import memory
+
+    say(f"[gpu] gated_delta not finite, {T} x {dim} {dtype}")
+    x, resets, _ = M.make(T, 4, 1, 1, dim, dim, dtype, 13, resets=0.0)
+    s, at, tol = dim ** -0.5, T - 70, M.tol(dtype)
+    clean = O.delta(*(x[n] for n in NAMES), resets, s)[0]
+    resets[at, 0] = True
+    x["state"][0] = float("nan")
+    x["v"][at + 20, 1, 0, 3] = float("nan")
+    x["k"][at + 41, 2, 0, 5] = float("inf")
+    resets[at + 50, 1], resets[at + 45, 2] = True, True
+    x["beta"][at + 10, 3], x["g"][at + 12, 3], resets[at + 13, 3] = float("nan"), float("nan"), True
+    got = memory.gated_delta(*(x[n].to(dev()) for n in NAMES[:5]), state=x["state"].to(dev()), resets=resets.to(dev()))
+    out = got[0].cpu()
+    y = {n: torch.where(torch.isfinite(t), t, torch.zeros_like(t)) for n, t in x.items()}
+    want = O.delta(*(y[n] for n in NAMES), resets, s)[0]
+    assert O.off(out[at:, 0], want[at:, 0]) <= tol and torch.isnan(out[:at, 0]).all()
+    assert O.off(out[:at + 20, 1], clean[:at + 20, 1]) <= tol and O.off(out[at + 50:, 1], want[at + 50:, 1]) <= tol
+    assert O.off(out[:at + 41, 2], clean[:at + 41, 2]) <= tol and O.off(out[at + 45:, 2], want[at + 45:, 2]) <= tol
+    assert O.off(out[:at + 10, 3], clean[:at + 10, 3]) <= tol and O.off(out[at + 13:, 3], want[at + 13:, 3]) <= tol
+    assert torch.isnan(out[at + 20:at + 50, 1, 0, 3]).all() and torch.isnan(out[at + 10:at + 13, 3]).all()
+    assert torch.isfinite(got[1]).all()
