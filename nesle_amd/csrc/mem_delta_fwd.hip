@@ -326,16 +326,24 @@ __global__ void __launch_bounds__(DP * 4) delta_join_kernel(Chain x, int dk, int
     }
 }
 
-// Segments for few heads over many tokens.  The walk of one head through a chunk
-// takes 3.4 us by itself and 6 us beside another on its compute unit, a step of
+// Segments for few heads over many tokens.  The walk of one head of 64 through a
+// chunk takes 3.5 us by itself and 6 us beside another on its compute unit, a step of
 // a chain 0.6 us, a launch of one 5 us and more, and the launches walk every chunk
-// twice.  So: enough segments for two workgroups a compute unit, two chunks or
-// more in each, and no more than balance the chain's steps against the walks; in
-// groups, of as many segments as there are groups, once the chain would be longer
-// than 40.  Measured in bfloat16, heads of 64, whole walk against segments: 1,024
-// tokens of 64 heads 111 / 58 us, of 128 heads 113 / 95 us, of 256 heads 127 / 157
-// us; 256 tokens of 16 heads 30 / 25 us.  One chain against groups: 4,096 tokens of
-// 8 heads 60 / 63 us, 8,191 of 8 heads 91 / 82 us, 32,768 of 4 heads 167 / 127 us.
+// twice.  So: as many segments as the card holds workgroups of the maps at once (DP / 8
+// waves each, 16 waves a compute unit: 1,024, 512 or 256 of them), four at least to
+// make up for the second walk, two chunks or more in each, or four chunks where there
+// are only four to seven segments, and no more than balance the chain's steps against
+// the walks; in groups, of as many segments as there are groups, once the chain would
+// be longer than 40.
+// Whole walk against segments, us, bfloat16 / float32 (* where the rule walks whole):
+//   32 dimensions, 256 tokens of 128 heads 37 / 39, 27 / 30; 1,024 of 256 heads 137 /
+//   143, 89 / 102; 64 dimensions, 256 of 64 heads 32 / 41, 27 / 31; 256 of 128 heads*
+//   32 / 41, 38 / 44; 512 of 128 heads 61 / 78, 57 / 69; 1,024 of 256 heads* 127, 157 in
+//   bfloat16; 128 dimensions, 256 of 32 heads 46 / 70, 47 / 57; 256 of 64 heads* 48 / 71,
+//   58 / 71; 512 of 64 heads 90 / 137, 81 / 105; 1,024 of 128 heads* 174 / 279, 215 / 309.
+// One chain against groups, heads of 64 in bfloat16: 4,096 tokens of 8 heads 60 / 63
+// us, 8,192 of 8 heads 94 / 79, 32,768 of 4 heads 175 / 121; of 32 and 128 dimensions,
+// 16,384 of 4 heads 84 / 55 and 236 / 191.
 Segments segments(const nesle_delta_args& a) {
     const std::uint64_t heads = static_cast<std::uint64_t>(a.batch) * a.v_heads;
     const std::uint32_t chunks = (a.steps + kChunk - 1) / kChunk;
@@ -345,8 +353,9 @@ Segments segments(const nesle_delta_args& a) {
         return n;
     };
     std::uint32_t count = 1;
-    if (chunks >= 8 && heads <= 128) {
-        const std::uint32_t most = std::min(static_cast<std::uint32_t>(512 / heads), chunks / 2);
+    const std::uint64_t at_once = (1u << 15) / padded_dim(a);
+    if (4 * heads <= at_once && chunks >= (8 * heads <= at_once ? 8 : 16)) {
+        const std::uint32_t most = std::min(static_cast<std::uint32_t>(at_once / heads), chunks / 2);
         count = std::min(root(8ull * chunks), most);
         if (count > 40) count = std::min(root(64ull * chunks), most);
     }
