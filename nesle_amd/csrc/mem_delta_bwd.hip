@@ -24,14 +24,13 @@
 // No atomics: sums over waves are added in a fixed order.
 //
 // Bound by neither memory nor the matrix units: 128 steps of 512 consoles of 4 heads
-// of 64 in bfloat16 take 221 us, where the 0.30 GB they move take 61 us at a large
-// copy's rate and the products' instructions 34 us.  80 KB of LDS and 252 registers
-// leave two waves a SIMD (one: 342 us), whose vector units are busy half the time
-// (with cutting float32 values in three, masks, and addresses), in a chain of eight
-// parts between barriers.  With the parts left out one at a time: tiles of dP and
-// dA -15 us, loads ahead -7, the inverse -8, the gates' end -4, results -1; LDS rows
-// of other lengths, 1 % either way.  64 consoles in float32: 63 us, of which the
-// float32 matrix instructions are 21.
+// of 64 in bfloat16 take 250 us, where the 0.30 GB they move take 61 us at a large
+// copy's rate and the products' instructions 41 us.  78 KB of LDS and 229 registers
+// leave two waves a SIMD, whose vector units are busy half the time (with cutting
+// float32 values in three, masks, and addresses), in a chain of eight parts between
+// barriers.  With the parts left out one at a time: tiles of dP and dA -19 us, the
+// inverse -16, results -12, loads ahead -10, the gates' end -5.  64 consoles in
+// float32: 64 us, of which the float32 matrix instructions are 21.
 #include "mem_delta_tile.h"
 
 namespace nesle::mem {

@@ -58,12 +58,11 @@ constexpr int kWavesPerSimd = DP == 32 ? 3 : DP == 64 && sizeof(T) == 2 ? 4 : 2;
 //
 // Bound by memory where there are many heads: 128 steps of 512 consoles of 4 heads
 // of 64 in bfloat16 move 0.30 GB (inputs, outputs, the states in and out and the
-// ones kept for the gradient) in 81 us, 3.7 TB/s against a large copy's 4.9.  With
-// the parts left out one at a time: kept states -19 us, first and last states -20,
-// loads of the inputs -17, outputs -14, the inverse -4.  With one workgroup a compute
-// unit a chunk takes 3.4 us, a chain of short parts: inverse 0.7, loads 0.2,
-// products and the tests of what is not finite 0.1 each (64 consoles 21 us, in
-// float32 27).  A chunk of 32 tokens is one inner step of the bfloat16 instruction
+// ones kept for the gradient) in 88 us, 3.4 TB/s against a large copy's 4.9.  With
+// the parts left out one at a time: kept states -19 us, first and last states -19,
+// loads of the inputs -16, outputs -13, the inverse -3.  With one workgroup a compute
+// unit a chunk takes 3.6 us, a chain of short parts of which the inverse is 0.4 (64
+// consoles 22 us, in float32 28).  A chunk of 32 tokens is one inner step of the bfloat16 instruction
 // and the largest whose inverse one wave finds in registers; its tile leaves room
 // for four workgroups a compute unit.
 template <typename T, int DP, bool WIDE, bool MAP>
@@ -327,7 +326,7 @@ __global__ void __launch_bounds__(DP * 4) delta_join_kernel(Chain x, int dk, int
 }
 
 // Segments for few heads over many tokens.  The walk of one head of 64 through a
-// chunk takes 3.5 us by itself and 6 us beside another on its compute unit, a step of
+// chunk takes 3.6 us by itself and 6 us beside another on its compute unit, a step of
 // a chain 0.6 us, a launch of one 5 us and more, and the launches walk every chunk
 // twice.  So: as many segments as the card holds workgroups of the maps at once (DP / 8
 // waves each, 16 waves a compute unit: 1,024, 512 or 256 of them), four at least to

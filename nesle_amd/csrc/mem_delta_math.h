@@ -194,9 +194,10 @@ struct SplitMath {
 };
 
 // Float32 inputs in three planes take up to twice the LDS of a tile of float32:
-// quicker in the forward of 64 dimensions (64 consoles of 4 heads 28.4 -> 27.0 us, 256
-// 73.9 -> 67.5) and 128 (64 consoles 62.5 -> 51.9), not of 32 (512 consoles 76 -> 86);
-// in the gradient they would leave one workgroup a compute unit, or none.
+// quicker in the forward of 64 dimensions (128 steps of 128 consoles of 4 heads, by
+// float32 instructions 38, by planes 34 us; of 256 consoles 64 and 60) and of 128 (64
+// consoles 52 and 44, 256 207 and 178), not of 32 (256 consoles 32 and 51, 512 69 and
+// 83); in the gradient they would leave one workgroup a compute unit, or none.
 template <typename T, int DP>
 struct MathOf {
     using forward = SplitMath<1>;

@@ -11,8 +11,10 @@
 //
 // Bound by memory: about 10 operations an element.  Measured against a large
 // copy's 4.9 TB/s, bfloat16: 1.08 GB of 128 steps of 4,096 rows and 8 heads of 64
-// in 221 us (4.9 TB/s); 128 steps of 512 rows, forward 134 MB in 29 us (4.6 TB/s),
-// gradient 202 MB in 40 us (5.0 TB/s) and the weights' sum 4 us.  Loads of 8 bytes a
+// in 222 us (4.9 TB/s); 128 steps of 512 rows, forward 134 MB in 29 us (4.6 TB/s),
+// gradient 202 MB in 41 us (4.9 TB/s) and the weights' sum 4 us.  A head has a power of
+// two lanes: of 40 float32 elements 5 of 8 work (23,177 rows of 8 such heads: forward
+// 59 MB in 16 us, 3.7 TB/s).  Loads of 8 bytes a
 // lane in place of 16 took 309 us for the first; heads of one row side by side in a
 // thread, which share a row of the table, 338 us.  Below about 100 rows a call is a
 // launch: 3.6 us.
@@ -25,9 +27,11 @@ namespace nesle::mem {
 namespace {
 
 constexpr unsigned kThreads = 256;
-// Heads a thread works on at once: their loads are in flight together, and
-// heads of one row share its position, cosines and sines.  One where the rows
-// do not fill the card: latency counts there.
+// Heads a thread works on at once, rows apart: their loads are in flight together.
+// One where the rows do not fill the card, fewer than 1,024 workgroups: latency
+// counts there.  In float32, 4 + 4 heads of 64, together / one: 1,024 rows 6.1 / 3.4
+// us, 8,192 rows 9.0 / 7.5, 16,384 rows (the first together) 13.9 / 13.9, 65,536 rows
+// 45.4 / 46.5.
 constexpr unsigned kTogether = 4, kGradTogether = 2;
 // Workgroups of the gradient, four a compute unit, which their registers leave
 // room for (twice as many: 47 us for 43): each adds up its rows' share of a

@@ -98,5 +98,7 @@ def gated_delta(q, k, v, g, beta, *, state=None, resets=None, scale: float | Non
     float32, a tensor of its own.  Differentiable in q, k, v, g, beta and
     state.  No value of a dropped state, and nothing that is not finite in a
     later token, reaches an output it does not belong to; the gradient of
-    inputs that are not finite is unspecified."""
+    inputs that are not finite is unspecified, and so is a chunk of 32 tokens of a
+    head in which finite inputs overflow float32.  Products keep float32 precision
+    for either type: bfloat16 results are rounded once."""
     return _called(_native.gated_delta, q, k, v, g, beta, state, resets, scale)
