@@ -120,6 +120,113 @@ int nesle_delta_step(const nesle_delta_args* args, void* stream);
 int nesle_delta_forward(const nesle_delta_args* args, void* stream);
 int nesle_delta_backward(const nesle_delta_args* args, void* stream);
 
+/* ---- linear attention with a decay for each head ------------------------------
+ *
+ * Each head of each console holds a state S [k_dim][v_dim] in float32.  One
+ * token, with a = exp(g) of its head:
+ *   S <- a S                                  (S <- 0 where resets != 0)
+ *   S <- S + k v^T
+ *   out = scale S^T q
+ * A reset, and a decay whose exp(g) is zero in float32, drop the state by
+ * selection.  Value head h uses query and key head h / (v_heads / k_heads). */
+#define NESLE_DECAY_MAX_DIM 128u
+
+typedef struct nesle_decay_args {
+    uint32_t dtype;
+    uint32_t steps, batch, k_heads, v_heads, k_dim, v_dim;
+    float scale;
+    nesle_heads q, k, v;
+    const float* g;              /* [v_heads] */
+    const uint8_t* resets;       /* [steps][batch], or null */
+    const float* state;          /* [batch][v_heads][k_dim][v_dim], or null: zeros */
+    void* out;                   /* [steps][batch][v_heads][v_dim] */
+    float* state_out;            /* as state; nesle_decay_step: may be state itself */
+    float* saved;                /* forward writes, gradient reads; null where no gradient follows */
+    nesle_heads dout;            /* gradient: of out, in */
+    const float* dstate_out;     /*           of state_out, in; null: zeros */
+    void* dq;                    /*           out */
+    void* dk;
+    void* dv;
+    float* dg;                   /*           [v_heads]; null: not wanted */
+    float* dstate;               /*           null: not wanted */
+    float* scratch;              /* nesle_decay_forward: nesle_decay_forward_scratch_floats() floats;
+                                    gradient: nesle_decay_scratch_floats(); unused where that is 0 */
+} nesle_decay_args;
+
+/* Floats of `saved`, and of `scratch` of the forward and of the gradient. */
+uint64_t nesle_decay_saved_floats(const nesle_decay_args* args);
+uint64_t nesle_decay_forward_scratch_floats(const nesle_decay_args* args);
+uint64_t nesle_decay_scratch_floats(const nesle_decay_args* args);
+
+/* One token (steps 1) for every console; state_out may be state (in place). */
+int nesle_decay_step(const nesle_decay_args* args, void* stream);
+/* A rollout in chunks, and its gradient. */
+int nesle_decay_forward(const nesle_decay_args* args, void* stream);
+int nesle_decay_backward(const nesle_decay_args* args, void* stream);
+
+/* ---- layer norm ------------------------------------------------------------------
+ *
+ * For each row x of `dim` elements, with statistics in float32:
+ *   y = (x - mean) / sqrt(mean((x - mean)^2) + eps) * weight + bias
+ * (null: 1 and 0), rounded once on output.  Rows are [steps][batch][heads]. */
+#define NESLE_NORM_MAX_DIM 16384u
+
+typedef struct nesle_norm_args {
+    uint32_t dtype;
+    uint32_t steps, batch, heads, dim;
+    float eps;
+    nesle_heads x;
+    const float* weight;         /* [dim], or null */
+    const float* bias;           /* [dim], or null */
+    void* y;                     /* forward */
+    nesle_heads dy;              /* gradient: of y, in */
+    void* dx;                    /*           of x, out */
+    float* dweight;              /*           [dim] each; null: not wanted */
+    float* dbias;
+    float* scratch;              /*           nesle_norm_scratch_floats() floats */
+} nesle_norm_args;
+
+/* 0 where no scratch is needed, and for sizes that the calls refuse. */
+uint64_t nesle_norm_scratch_floats(const nesle_norm_args* args);
+int nesle_layer_norm(const nesle_norm_args* args, void* stream);
+int nesle_layer_norm_grad(const nesle_norm_args* args, void* stream);
+
+/* ---- sampling of actions from given random numbers --------------------------------
+ *
+ * For each row of `actions` scores, in float64 throughout:
+ *   s = logits / temperature,  w = exp(s - max s)
+ *   of the rows' actions in order of falling s, equal ones by rising index, w is
+ *   set to 0 from the top_k-th on (top_k 0: nowhere); then where the sum of those
+ *   before is no less than top_p times the sum of all; and where w < min_p
+ *   action = the first, by index, at which the running sum of w exceeds
+ *            uniform times the sum of all
+ *   logprob = log(w[action] / sum w)
+ * Temperature 0 takes the largest logit (the lowest index of equal ones), with
+ * logprob 0.  A row without an answer gets action -1 and logprob NaN: one whose
+ * logits hold NaN or +infinity or nothing above -infinity, whose uniform is NaN,
+ * or whose own temperature, top_k, top_p or min_p is out of its range.  A uniform
+ * below 0 counts as 0, one of 1 or more picks the last action that is left. */
+#define NESLE_SAMPLE_MAX_ACTIONS 1024u
+
+typedef struct nesle_sample_args {
+    uint32_t dtype;
+    uint32_t steps, batch, actions;
+    nesle_heads logits;          /* [steps][batch][actions]; stride_h is not used */
+    const float* uniform;        /* [steps][batch] */
+    double temperature;          /* 0 or more, finite */
+    double top_p;                /* above 0, up to 1 */
+    double min_p;                /* 0 to 1 */
+    uint32_t top_k;              /* 0 or as many actions as there are, or more: all */
+    const float* temperatures;   /* [steps][batch] each, or null: the row's own */
+    const int32_t* top_ks;
+    const float* top_ps;
+    const float* min_ps;
+    int64_t* action;             /* [steps][batch] */
+    float* logprob;
+} nesle_sample_args;
+
+int nesle_sample(const nesle_sample_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

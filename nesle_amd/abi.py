@@ -31,6 +31,7 @@ VIEW_PRESENT = 14   # presentation records [n][16 + video memory block]
 SHAPED_STATE_WORDS = 11   # NESLE_SMB_SHAPED_STATE_WORDS
 MEM_F32, MEM_BF16 = 0, 1
 QK_MAX_DIM, DELTA_MAX_DIM, DELTA_CHUNK = 256, 128, 32
+DECAY_MAX_DIM, NORM_MAX_DIM, SAMPLE_MAX_ACTIONS = 128, 16384, 1024
 # Step-kernel census slots (nesle_amd/csrc/nes_layout.h, namespace census).
 CENSUS_FIELDS = ("waves", "iterations", "rare", "rare_io_write", "rare_side", "rare_idle", "rare_illegal",
                  "rare_timing", "rare_budget", "rare_outside", "rare_only_io_write", "dma", "present", "io_read",
@@ -111,6 +112,35 @@ class DeltaArgs(ctypes.Structure):
                 + [("dout", Heads)]
                 + [(name, ctypes.c_void_p) for name in ("dstate_out", "dq", "dk", "dv", "dg", "dbeta", "dstate",
                                                         "scratch")])
+
+
+class DecayArgs(ctypes.Structure):
+    """nesle_decay_args (include/nesle_memory.h)."""
+    _fields_ = ([(name, ctypes.c_uint32) for name in ("dtype", "steps", "batch", "k_heads", "v_heads", "k_dim",
+                                                      "v_dim")]
+                + [("scale", ctypes.c_float), ("q", Heads), ("k", Heads), ("v", Heads)]
+                + [(name, ctypes.c_void_p) for name in ("g", "resets", "state", "out", "state_out", "saved")]
+                + [("dout", Heads)]
+                + [(name, ctypes.c_void_p) for name in ("dstate_out", "dq", "dk", "dv", "dg", "dstate", "scratch")])
+
+
+class NormArgs(ctypes.Structure):
+    """nesle_norm_args (include/nesle_memory.h)."""
+    _fields_ = ([(name, ctypes.c_uint32) for name in ("dtype", "steps", "batch", "heads", "dim")]
+                + [("eps", ctypes.c_float), ("x", Heads)]
+                + [(name, ctypes.c_void_p) for name in ("weight", "bias", "y")]
+                + [("dy", Heads)]
+                + [(name, ctypes.c_void_p) for name in ("dx", "dweight", "dbias", "scratch")])
+
+
+class SampleArgs(ctypes.Structure):
+    """nesle_sample_args (include/nesle_memory.h)."""
+    _fields_ = ([(name, ctypes.c_uint32) for name in ("dtype", "steps", "batch", "actions")]
+                + [("logits", Heads), ("uniform", ctypes.c_void_p)]
+                + [(name, ctypes.c_double) for name in ("temperature", "top_p", "min_p")]
+                + [("top_k", ctypes.c_uint32)]
+                + [(name, ctypes.c_void_p) for name in ("temperatures", "top_ks", "top_ps", "min_ps", "action",
+                                                        "logprob")])
 
 
 class RomInfo(ctypes.Structure):
@@ -211,6 +241,16 @@ def lib():
         "nesle_delta_step": (ctypes.c_int, [ctypes.POINTER(DeltaArgs), vp]),
         "nesle_delta_forward": (ctypes.c_int, [ctypes.POINTER(DeltaArgs), vp]),
         "nesle_delta_backward": (ctypes.c_int, [ctypes.POINTER(DeltaArgs), vp]),
+        "nesle_decay_saved_floats": (ctypes.c_uint64, [ctypes.POINTER(DecayArgs)]),
+        "nesle_decay_forward_scratch_floats": (ctypes.c_uint64, [ctypes.POINTER(DecayArgs)]),
+        "nesle_decay_scratch_floats": (ctypes.c_uint64, [ctypes.POINTER(DecayArgs)]),
+        "nesle_decay_step": (ctypes.c_int, [ctypes.POINTER(DecayArgs), vp]),
+        "nesle_decay_forward": (ctypes.c_int, [ctypes.POINTER(DecayArgs), vp]),
+        "nesle_decay_backward": (ctypes.c_int, [ctypes.POINTER(DecayArgs), vp]),
+        "nesle_norm_scratch_floats": (ctypes.c_uint64, [ctypes.POINTER(NormArgs)]),
+        "nesle_layer_norm": (ctypes.c_int, [ctypes.POINTER(NormArgs), vp]),
+        "nesle_layer_norm_grad": (ctypes.c_int, [ctypes.POINTER(NormArgs), vp]),
+        "nesle_sample": (ctypes.c_int, [ctypes.POINTER(SampleArgs), vp]),
         "nesle_smb_shaped_defaults": (None, [ctypes.POINTER(ShapedParams)]),
         "nesle_smb_shaped_reset": (ctypes.c_int, [vp, vp, ctypes.c_uint32, vp, vp]),
         "nesle_smb_shaped_reward": (ctypes.c_int, [vp, vp, vp, ctypes.c_uint32, ctypes.POINTER(ShapedParams), vp,

@@ -36,7 +36,8 @@ HIP_SOURCES = [CSRC / "nes_step.hip", CSRC / "nes_step_full.hip", CSRC / "nes_st
                CSRC / "nes_kernels.hip",
                CSRC / "nes_render.hip", CSRC / "nes_host.hip", CSRC / "ppo_head.hip", CSRC / "smb_shaped.hip",
                CSRC / "mem_rotate.hip", CSRC / "mem_delta_step.hip", CSRC / "mem_delta_fwd.hip",
-               CSRC / "mem_delta_bwd.hip"]
+               CSRC / "mem_delta_bwd.hip", CSRC / "mem_decay_step.hip", CSRC / "mem_decay_fwd.hip", CSRC / "mem_decay_bwd.hip",
+               CSRC / "mem_norm.hip", CSRC / "mem_sample.hip"]
 SHIM_SOURCE = CSRC / "cuda_core_module.cpp"
 MEMORY_SOURCE = CSRC / "memory_module.cpp"
 

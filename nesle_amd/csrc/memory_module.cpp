@@ -11,9 +11,11 @@
 #include <pybind11/stl.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <limits>
 #include <optional>
 #include <sstream>
@@ -420,6 +422,278 @@ Tensor gated_delta_step(const Tensor& q, const Tensor& k, const Tensor& v, const
     return out;
 }
 
+// ---- linear attention with a decay for each head --------------------------------------
+
+nesle_decay_args decay_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& state,
+                            const Tensor& resets, double scale) {
+    nesle_decay_args a{};
+    const int64_t d = q.dim();
+    a.dtype = dtype_of(q);
+    a.steps = d == 4 ? static_cast<uint32_t>(q.size(0)) : 1u;
+    a.batch = static_cast<uint32_t>(q.size(d - 3));
+    a.k_heads = static_cast<uint32_t>(q.size(d - 2));
+    a.v_heads = static_cast<uint32_t>(v.size(d - 2));
+    a.k_dim = static_cast<uint32_t>(q.size(d - 1));
+    a.v_dim = static_cast<uint32_t>(v.size(d - 1));
+    a.scale = static_cast<float>(scale);
+    a.q = heads(q);
+    a.k = heads(k);
+    a.v = heads(v);
+    a.g = ptr<float>(g);
+    a.resets = ptr<uint8_t>(resets);
+    a.state = ptr<float>(state);
+    return a;
+}
+
+void check_decay(const Common& c, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& state,
+                 const Tensor& resets) {
+    check_heads(c, k, "k");
+    check_heads(c, v, "v");
+    if (k.sizes() != q.sizes()) refuse(c.who, "k", "of q's shape", k);
+    const int64_t hk = q.size(-2), dk = q.size(-1), hv = v.size(-2), dv = v.size(-1);
+    if (hk == 0 || hv == 0 || hv % hk != 0) refuse(c.who, "v", "of a multiple of " + std::to_string(hk) + " heads", v);
+    constexpr int64_t most = NESLE_DECAY_MAX_DIM;
+    if (dk % 8 != 0 || dv % 8 != 0 || dk < 8 || dv < 8 || dk > most || dv > most)
+        throw py::value_error(std::string(c.who) + ": head dimensions must be multiples of 8 up to " + std::to_string(most) +
+                              ", got " + std::to_string(dk) + " and " + std::to_string(dv));
+    check_plain(c, g, "g", at::kFloat, {hv});
+    if (state.defined()) check_plain(c, state, "state", at::kFloat, {c.batch(), hv, dk, dv}, true);
+    if (resets.defined())
+        check_plain(c, resets, "resets", resets.scalar_type() == at::kByte ? at::kByte : at::kBool, c.sizes.slice(0, c.lead));
+}
+
+struct DecayAttention : torch::autograd::Function<DecayAttention> {
+    // Output, state after it and, to keep for the gradient, the states before
+    // the chunks.
+    static variable_list run(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& state,
+                             const Tensor& resets, double scale, bool keep) {
+        const c10::OptionalDeviceGuard guard(q.device());
+        nesle_decay_args a = decay_args(q, k, v, g, state, resets, scale);
+        const Tensor out = like(v), after = at::empty({v.size(1), v.size(2), q.size(3), v.size(3)}, g.options());
+        const Tensor saved = floats(q, keep ? nesle_decay_saved_floats(&a) : 0);
+        const Tensor scratch = floats(q, nesle_decay_forward_scratch_floats(&a));
+        a.out = ptr(out);
+        a.state_out = ptr<float>(after);
+        a.saved = ptr<float>(saved);
+        a.scratch = ptr<float>(scratch);
+        check(nesle_decay_forward(&a, stream_of(q)));
+        return {out, after, saved};
+    }
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
+                                 const MaybeTensor& start, const MaybeTensor& ends, double scale) {
+        const Tensor state = some(start), resets = some(ends);
+        variable_list out = run(q, k, v, g, state, resets, scale, true);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({q, k, v, g, state, resets, out[2]});
+        ctx->saved_data["scale"] = scale;
+        out.pop_back();
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &q = saved[0], &v = saved[2], &g = saved[3], &state = saved[4];
+        const c10::OptionalDeviceGuard guard(q.device());
+        variable_list out;
+        {
+            const at::AutoGradMode none(false);
+            nesle_decay_args a = decay_args(q, saved[1], v, g, state, saved[5], ctx->saved_data["scale"].toDouble());
+            const Tensor dout = grads[0].defined() ? unit_last(grads[0]) : zeros(v);
+            const Tensor dafter = grads[1].defined() ? whole(grads[1]) : Tensor();
+            const Tensor dq = like(q), dk = like(q), dv = like(v), dg = g.requires_grad() ? like(g) : Tensor();
+            const Tensor dstate = state.defined() && state.requires_grad() ? like(state) : Tensor();
+            const Tensor scratch = floats(q, nesle_decay_scratch_floats(&a));
+            a.saved = ptr<float>(saved[6]);
+            a.dout = heads(dout);
+            a.dstate_out = ptr<float>(dafter);
+            a.dq = ptr(dq);
+            a.dk = ptr(dk);
+            a.dv = ptr(dv);
+            a.dg = ptr<float>(dg);
+            a.dstate = ptr<float>(dstate);
+            a.scratch = ptr<float>(scratch);
+            check(nesle_decay_backward(&a, stream_of(q)));
+            out = {dq, dk, dv, dg, dstate};
+        }
+        out = first_order("decay_attention", out);
+        out.resize(7);
+        return out;
+    }
+};
+
+py::tuple decay_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const MaybeTensor& state,
+                          const MaybeTensor& resets, const std::optional<double>& scale) {
+    const Tensor start = some(state), ends = some(resets);
+    refuse_tracing("decay_attention");
+    refuse_tangents("decay_attention", {&q, &k, &v, &g, &start});
+    const Common c = common_of("decay_attention", q, 2, 2);
+    check_decay(c, q, k, v, g, start, ends);
+    const double s = scale_or_default(scale, q);
+    const variable_list out = wants_grad({&q, &k, &v, &g, &start})
+        ? DecayAttention::apply(q, k, v, g, state, resets, s)
+        : DecayAttention::run(q, k, v, g, start, ends, s, false);
+    return py::make_tuple(out[0], out[1]);
+}
+
+Tensor decay_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const MaybeTensor& state,
+                            const MaybeTensor& resets, const std::optional<double>& scale) {
+    if (!given(state)) throw py::value_error("decay_attention_step: state must be a tensor");
+    refuse_tracing("decay_attention_step");
+    refuse_tangents("decay_attention_step", {&q, &k, &v, &g, &*state});
+    const Common c = common_of("decay_attention_step", q, 1, 1);
+    const Tensor ends = some(resets);
+    check_decay(c, q, k, v, g, *state, ends);
+    if (wants_grad({&q, &k, &v, &g, &*state}))
+        throw py::value_error("decay_attention_step has no gradient: use decay_attention, or torch.no_grad()");
+    const c10::OptionalDeviceGuard guard(q.device());
+    nesle_decay_args a = decay_args(q, k, v, g, *state, ends, scale_or_default(scale, q));
+    const Tensor out = like(v);
+    a.out = ptr(out);
+    a.state_out = ptr<float>(*state);
+    state->unsafeGetTensorImpl()->bump_version();          // autograd sees the state change
+    check(nesle_decay_step(&a, stream_of(q)));
+    return out;
+}
+
+// ---- layer norm ----------------------------------------------------------------------------
+
+// Up to three leading dimensions as [steps][batch][heads], from the right.
+nesle_heads rows(const Tensor& t) {
+    const int64_t d = t.dim();
+    return {t.const_data_ptr(), d > 3 ? t.stride(0) : 0, d > 2 ? t.stride(d - 3) : 0, d > 1 ? t.stride(d - 2) : t.size(0)};
+}
+
+nesle_norm_args norm_args(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps) {
+    nesle_norm_args a{};
+    const int64_t d = x.dim();
+    a.dtype = dtype_of(x);
+    a.steps = d > 3 ? static_cast<uint32_t>(x.size(0)) : 1u;
+    a.batch = d > 2 ? static_cast<uint32_t>(x.size(d - 3)) : 1u;
+    a.heads = d > 1 ? static_cast<uint32_t>(x.size(d - 2)) : 1u;
+    a.dim = static_cast<uint32_t>(x.size(d - 1));
+    a.eps = static_cast<float>(eps);
+    a.x = rows(x);
+    a.weight = ptr<float>(weight);
+    a.bias = ptr<float>(bias);
+    return a;
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+    static Tensor run(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps) {
+        const c10::OptionalDeviceGuard guard(x.device());
+        nesle_norm_args a = norm_args(x, weight, bias, eps);
+        const Tensor y = like(x);
+        a.y = ptr(y);
+        check(nesle_layer_norm(&a, stream_of(x)));
+        return y;
+    }
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, double eps) {
+        const Tensor w = some(weight), b = some(bias);
+        ctx->save_for_backward({x, w, b});
+        ctx->saved_data["eps"] = eps;
+        return run(x, w, b, eps);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &w = saved[1], &b = saved[2];
+        const c10::OptionalDeviceGuard guard(x.device());
+        variable_list out;
+        {
+            const at::AutoGradMode none(false);
+            nesle_norm_args a = norm_args(x, w, b, ctx->saved_data["eps"].toDouble());
+            const Tensor dy = unit_last(grads[0]);
+            const Tensor dx = like(x), dw = w.defined() && w.requires_grad() ? like(w) : Tensor(),
+                         db = b.defined() && b.requires_grad() ? like(b) : Tensor();
+            const Tensor scratch = dw.defined() || db.defined() ? floats(x, nesle_norm_scratch_floats(&a)) : Tensor();
+            a.dy = rows(dy);
+            a.dx = ptr(dx);
+            a.dweight = ptr<float>(dw);
+            a.dbias = ptr<float>(db);
+            a.scratch = ptr<float>(scratch);
+            check(nesle_layer_norm_grad(&a, stream_of(x)));
+            out = {dx, dw, db};
+        }
+        out = first_order("layer_norm", out);
+        out.resize(4);
+        return out;
+    }
+};
+
+Tensor layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, double eps) {
+    const char* who = "layer_norm";
+    const Tensor w = some(weight), b = some(bias);
+    refuse_tracing(who);
+    refuse_tangents(who, {&x, &w, &b});
+    check_sizes(who, "x", x);
+    if (!x.is_cuda() || (x.scalar_type() != at::kFloat && x.scalar_type() != at::kBFloat16) || x.dim() < 1 || x.dim() > 4 ||
+        x.size(-1) < 1 || x.size(-1) > static_cast<int64_t>(NESLE_NORM_MAX_DIM) || x.stride(-1) != 1)
+        refuse(who, "x", "a float32 or bfloat16 GPU tensor of one to four dimensions, the last of 1 to " +
+               std::to_string(NESLE_NORM_MAX_DIM) + " elements next to each other", x);
+    const Common c{who, x.scalar_type(), x.device(), x.dim() - 1, x.sizes()};
+    if (w.defined()) check_plain(c, w, "weight", at::kFloat, {x.size(-1)}, true);
+    if (b.defined()) check_plain(c, b, "bias", at::kFloat, {x.size(-1)}, true);
+    return wants_grad({&x, &w, &b}) ? LayerNorm::apply(x, weight, bias, eps) : LayerNorm::run(x, w, b, eps);
+}
+
+// ---- sampling --------------------------------------------------------------------------------
+
+// A setting: one number for all rows, or a tensor with each row's.
+template <typename X>
+Tensor setting(const Common& c, const py::object& value, const char* name, at::ScalarType type, X& number) {
+    if (!THPVariable_Check(value.ptr())) {
+        try {
+            number = value.cast<X>();
+        } catch (const py::cast_error&) {
+            throw py::value_error(std::string(c.who) + ": " + name + " must be a number or a tensor, got " +
+                                  py::repr(value).cast<std::string>());
+        }
+        return Tensor();
+    }
+    const Tensor t = value.cast<Tensor>();
+    check_plain(c, t, name, type, c.sizes.slice(0, c.lead));
+    return t;
+}
+
+py::tuple sample_actions(const Tensor& logits, const Tensor& uniform, const py::object& temperature, const py::object& top_k,
+                         const py::object& top_p, const py::object& min_p) {
+    const char* who = "sample_actions";
+    refuse_tracing(who);
+    refuse_tangents(who, {&logits, &uniform});
+    check_sizes(who, "logits", logits);
+    const int64_t lead = logits.dim() - 1;
+    if (!logits.is_cuda() || (logits.scalar_type() != at::kFloat && logits.scalar_type() != at::kBFloat16) || lead < 1 ||
+        lead > 2 || logits.size(-1) < 1 || logits.size(-1) > static_cast<int64_t>(NESLE_SAMPLE_MAX_ACTIONS) || logits.stride(-1) != 1)
+        refuse(who, "logits", "a float32 or bfloat16 GPU tensor [N, actions] or [T, N, actions] of 1 to " +
+               std::to_string(NESLE_SAMPLE_MAX_ACTIONS) + " actions next to each other", logits);
+    const Common c{who, logits.scalar_type(), logits.device(), lead, logits.sizes()};
+    check_plain(c, uniform, "uniform", at::kFloat, c.sizes.slice(0, lead));
+    nesle_sample_args a{};
+    int64_t most = 0;
+    const Tensor temperatures = setting(c, temperature, "temperature", at::kFloat, a.temperature);
+    const Tensor top_ks = setting(c, top_k, "top_k", at::kInt, most);
+    const Tensor top_ps = setting(c, top_p, "top_p", at::kFloat, a.top_p);
+    const Tensor min_ps = setting(c, min_p, "min_p", at::kFloat, a.min_p);
+    if (most < 0) throw py::value_error("sample_actions: top_k must not be below 0, got " + std::to_string(most));
+    if (wants_grad({&logits, &uniform, &temperatures, &top_ps, &min_ps}))
+        throw py::value_error("sample_actions has no gradient: use torch.no_grad()");
+    const c10::OptionalDeviceGuard guard(logits.device());
+    a.dtype = dtype_of(logits);
+    a.steps = lead == 2 ? static_cast<uint32_t>(logits.size(0)) : 1u;
+    a.batch = static_cast<uint32_t>(logits.size(lead - 1));
+    a.actions = static_cast<uint32_t>(logits.size(lead));
+    a.logits = {logits.const_data_ptr(), lead == 2 ? logits.stride(0) : 0, logits.stride(lead - 1), 0};
+    a.uniform = ptr<float>(uniform);
+    a.top_k = static_cast<uint32_t>(std::min<int64_t>(most, a.actions));
+    a.temperatures = ptr<float>(temperatures);
+    a.top_ks = ptr<int32_t>(top_ks);
+    a.top_ps = ptr<float>(top_ps);
+    a.min_ps = ptr<float>(min_ps);
+    const Tensor action = at::empty(uniform.sizes(), uniform.options().dtype(at::kLong)), logprob = at::empty(uniform.sizes(), uniform.options());
+    a.action = ptr<int64_t>(action);
+    a.logprob = ptr<float>(logprob);
+    check(nesle_sample(&a, stream_of(logits)));
+    return py::make_tuple(action, logprob);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_memory_native, m) {
@@ -427,4 +701,8 @@ PYBIND11_MODULE(_memory_native, m) {
     m.def("qk_norm_rotate", &qk_norm_rotate);
     m.def("gated_delta", &gated_delta);
     m.def("gated_delta_step", &gated_delta_step);
+    m.def("decay_attention", &decay_attention);
+    m.def("decay_attention_step", &decay_attention_step);
+    m.def("layer_norm", &layer_norm);
+    m.def("sample_actions", &sample_actions);
 }

@@ -9,6 +9,12 @@ trains on whole rollouts with gradients:
 * ``gated_delta``       the gated delta rule over a rollout [T, N], memory
   dropped where an episode ends;
 * ``gated_delta_step``  one token of it for every console, states in place;
+* ``decay_attention``   linear attention with a decay for each head over a
+  rollout, the plainer memory: nothing is taken out but by the decay;
+* ``decay_attention_step``  one token of it for every console, states in place;
+* ``layer_norm``        the layer norm of features or of a memory's heads;
+* ``sample_actions``    actions drawn from logits by given random numbers, with
+  temperature, top-k, top-p and min-p, and their log probabilities;
 * ``rotation_table``    cosines and sines for the rotation.
 
 Tensors are time-major, [T, N, heads, dim] (a step's: [N, heads, dim]), float32
@@ -102,3 +108,76 @@ def gated_delta(q, k, v, g, beta, *, state=None, resets=None, scale: float | Non
     head in which finite inputs overflow float32.  Products keep float32 precision
     for either type: bfloat16 results are rounded once."""
     return _called(_native.gated_delta, q, k, v, g, beta, state, resets, scale)
+
+
+# ---- linear attention with a decay for each head --------------------------------------
+
+def decay_attention_step(q, k, v, g, state, *, resets=None, scale: float | None = None):
+    """One token of ``decay_attention`` for every console: q, k [N, k_heads,
+    k_dim], v [N, v_heads, v_dim], g [v_heads], resets [N]; ``state`` [N, v_heads,
+    k_dim, v_dim] is updated in place.  Returns the output [N, v_heads, v_dim].
+    Not differentiable: acting."""
+    return _called(_native.decay_attention_step, q, k, v, g, state, resets, scale)
+
+
+def decay_attention(q, k, v, g, *, state=None, resets=None, scale: float | None = None):
+    """Linear attention with a decay for each head over a rollout: (output, state
+    after it).
+
+    Each head of each console keeps a float32 state S [k_dim, v_dim].  A token
+    first lets it decay, S <- exp(g) S, or drops it where ``resets`` is set (an
+    episode's first token), then writes, S <- S + k v^T, and reads
+    out = scale S^T q: all tokens of the episode up to its own, each weighed by
+    scale exp(g)^distance (q . k).  Nothing is normalised (``layer_norm``).
+
+    q, k [T, N, k_heads, k_dim], v [T, N, v_heads, v_dim], g float32 [v_heads]
+    (the logarithm of a head's decay, g <= 0; -inf: a token sees itself alone),
+    resets bool or uint8 [T, N], state float32 [N, v_heads, k_dim, v_dim] (None:
+    zeros).  v_heads is a multiple of k_heads: value head h goes with key head
+    h // (v_heads // k_heads).  Head dimensions are multiples of 8 up to 128; T and
+    N may be 0; scale defaults to k_dim ** -0.5.  A padded token at the end of a
+    rollout still lets the state decay; its key, or value, of zeros writes nothing.
+    The output has q's type; the new state is float32, a tensor of its own.
+    Differentiable in q, k, v, g and state.  No value of a dropped state, and
+    nothing that is not finite in a later token, reaches an output it does not
+    belong to; the gradient of inputs that are not finite is unspecified, and so is
+    a chunk of 64 tokens of a head in which finite inputs overflow float32.  Products
+    keep float32 precision for either type: bfloat16 results are rounded once."""
+    return _called(_native.decay_attention, q, k, v, g, state, resets, scale)
+
+
+# ---- layer norm -------------------------------------------------------------------------
+
+def layer_norm(x, weight=None, bias=None, *, eps: float = 1e-5):
+    """(x - mean) / sqrt(mean((x - mean)^2) + eps) * weight + bias over the last
+    dimension.
+
+    x float32 or bfloat16, one to four dimensions, the last of 1 to 16,384 elements
+    next to each other (leading ones may be strided: a slice of one projection's
+    output); weight and bias float32 [dim] or None.  Statistics and the gradients of
+    weight and bias are float32; the result has x's type, rounded once.
+    Differentiable in x, weight and bias."""
+    return _called(_native.layer_norm, x, weight, bias, eps)
+
+
+# ---- sampling ---------------------------------------------------------------------------
+
+def sample_actions(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Actions drawn from ``logits`` [N, actions] or [T, N, actions] (float32 or
+    bfloat16, at most 1,024 actions) by one random number a row, ``uniform``
+    (float32 [N] or [T, N], in [0, 1)): (actions int64, log probabilities float32).
+
+    With w = exp(logits / temperature) relative to the largest, and actions in order
+    of falling logits (equal ones by rising index): the ``top_k`` first stay (0:
+    all); of these the ones before which less than ``top_p`` of their sum lies; of
+    these the ones with w >= ``min_p``.  The action is the first by index at which
+    the running sum of what stays exceeds ``uniform`` times all of it, its log
+    probability that of w among what stays.  Temperature 0 takes the largest logit,
+    the first of equal ones, with log probability 0.
+
+    The four settings are numbers, or tensors with each row's own (float32, top_k
+    int32, of uniform's shape).  Sums are float64.  Logits of -inf are never taken.
+    A row without an answer (NaN or +inf among its logits, nothing above -inf, NaN
+    as its number, a setting of its own out of range) gets action -1 and NaN.  Not
+    differentiable: acting."""
+    return _called(_native.sample_actions, logits, uniform, temperature, top_k, top_p, min_p)
