@@ -187,11 +187,8 @@ struct Seen {
             last = 63 - __clzll(static_cast<long long>(d));
         }
     }
-    // First token that token i sees.
-    __device__ int from(int i) const {
-        const std::uint64_t before = drops & (~0ull >> (63 - i));
-        return before == 0 ? 0 : 63 - __clzll(static_cast<long long>(before));
-    }
+    // Episodes that ended up to token i: two tokens see each other where these agree.
+    __device__ int episode(int i) const { return __popcll(drops & (~0ull >> (63 - i))); }
     // Of the four rows from `row` on: the decay from before the chunk, and to its end.
     template <int CH>
     __device__ f4 in(const Powers<CH>& p, int row) const {
@@ -241,18 +238,19 @@ struct PairPowers {
     // Of a tile d = it - jt below the diagonal.
     __device__ f4 of(int d) const { return d == 0 ? same : base * far[d - 1]; }
     // x times its weights; zero, by selection, where the pair does not see each other.
-    __device__ f4 weigh(f4 x, int it, int jt, const Seen& seen, int r, int g) const {
+    // `episodes`: Seen::episode of the chunk's tokens, in LDS.
+    __device__ f4 weigh(f4 x, int it, int jt, const Seen& seen, const int* episodes, int r, int g) const {
         x *= of(it - jt);
         if (it == jt)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (LATER_ROWS ? 4 * g + e < r : r < 4 * g + e) x[e] = 0.0f;
         if (seen.drops != 0) {
+            using i4 = int __attribute__((ext_vector_type(4)));
+            const i4 rows = *reinterpret_cast<const i4*>(episodes + 16 * (LATER_ROWS ? it : jt) + 4 * g);
+            const int col = episodes[16 * (LATER_ROWS ? jt : it) + r];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = 4 * g + e, i = 16 * it + (LATER_ROWS ? row : r), j = 16 * jt + (LATER_ROWS ? r : row);
-                if (j < seen.from(i)) x[e] = 0.0f;
-            }
+            for (int e = 0; e < 4; ++e) x[e] = rows[e] == col ? x[e] : 0.0f;
         }
         return x;
     }
@@ -262,15 +260,21 @@ struct PairPowers {
 // from the registers, 64 bytes of a row together.
 template <typename T, int DP, int CH>
 struct DecayResults {
+    // A finished tile, as it waits for its place.
+    using Tile = f4;
+    static __device__ Tile tile(f4 x) { return x; }
     template <bool WIDE>
-    __device__ void put(const Rows<T, WIDE>& to, int dim, int n, const Lane<DP>& at, const f4 (&x)[CH / 16]) {
+    static __device__ void put_tile(const Rows<T, WIDE>& to, int dim, int n, const Lane<DP>& at, int m, f4 x) {
 #pragma unroll
-        for (int m = 0; m < CH / 16; ++m)
+        for (int e = 0; e < 4; ++e) {
+            const int row = 16 * m + 4 * at.g + e;
+            to.put(at.col < dim && row < n, row, at.col, x[e]);
+        }
+    }
+    template <bool WIDE>
+    __device__ void put(const Rows<T, WIDE>& to, int dim, int n, const Lane<DP>& at, const Tile (&x)[CH / 16]) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = 16 * m + 4 * at.g + e;
-                to.put(at.col < dim && row < n, row, at.col, x[m][e]);
-            }
+        for (int m = 0; m < CH / 16; ++m) put_tile(to, dim, n, at, m, x[m]);
     }
     template <bool WIDE>
     __device__ void flush(const Rows<T, WIDE>&, int, int, const Lane<DP>&) const {}
@@ -282,11 +286,12 @@ template <int DP, int CH>
 struct DecayResults<bf16, DP, CH> {
     static constexpr int kRow = CH + 8;
     alignas(16) std::uint16_t d[DP * kRow];
+    using Tile = u2;
+    static __device__ Tile tile(f4 x) { return u2{pack_bf16(x.x, x.y), pack_bf16(x.z, x.w)}; }
     template <bool WIDE>
-    __device__ void put(const Rows<bf16, WIDE>&, int, int, const Lane<DP>& at, const f4 (&x)[CH / 16]) {
+    __device__ void put(const Rows<bf16, WIDE>&, int, int, const Lane<DP>& at, const Tile (&x)[CH / 16]) {
 #pragma unroll
-        for (int m = 0; m < CH / 16; ++m)
-            *reinterpret_cast<u2*>(&d[at.col * kRow + 16 * m + 4 * at.g]) = u2{pack_bf16(x[m].x, x[m].y), pack_bf16(x[m].z, x[m].w)};
+        for (int m = 0; m < CH / 16; ++m) *reinterpret_cast<u2*>(&d[at.col * kRow + 16 * m + 4 * at.g]) = x[m];
     }
     template <bool WIDE>
     __device__ void flush(const Rows<bf16, WIDE>& to, int dim, int n, const Lane<DP>& at) const {

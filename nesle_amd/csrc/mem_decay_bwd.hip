@@ -41,6 +41,7 @@ struct GradTile {
     Out q, k, v;               // then dQ, dK, dV
     In dout;
     Powers<CH> powers;
+    alignas(16) int episodes[CH];
     float sums[DP / 16];
 };
 
@@ -88,8 +89,15 @@ __global__ void __launch_bounds__(DP * 4, 2) decay_backward_kernel(DecayArgs<T> 
     if (a.steps != 0) fetch(a.steps, first);
     float decay = 0.0f;                    // this lane's share of the decay's gradient
     for (std::uint32_t t1 = a.steps; t1 > 0;) {
-        const Lane<DP> at = Lane<DP>::anew();
-        const int r = at.r, g = at.g;
+        // Made anew for each part of the chunk: what one part has read from LDS is read
+        // again by the next, rather than held in registers through both.
+        Lane<DP> at = Lane<DP>::anew();
+        int r = at.r, g = at.g;
+        const auto next_part = [&] {
+            at = Lane<DP>::anew();
+            r = at.r;
+            g = at.g;
+        };
         const std::uint32_t start = (t1 - 1) / CH * CH;
         const int n = static_cast<int>(t1 - start);
         const bool dropped = next_drops & 1u;      // the state before the chunk is
@@ -102,47 +110,8 @@ __global__ void __launch_bounds__(DP * 4, 2) decay_backward_kernel(DecayArgs<T> 
         k.stage(sh.k.in, at);
         v.stage(sh.v.in, at);
         dout.stage(sh.dout, at);
+        if (seen.drops != 0 && at.tid < CH) sh.episodes[at.tid] = seen.episode(at.tid);
         t1 = start;
-        __syncthreads();
-        if (t1 > 0) fetch(t1, at);
-
-        f4 dQ[CT], dK[CT], dV[CT], Q[CT], K[CT];       // Q, K: this wave's columns
-#pragma unroll
-        for (int p = 0; p < CT / 2; ++p) {
-            f4 x[2];
-            M::values(sh.q.in.cols(32 * p, 16 * at.wave, r, g), x);
-            Q[2 * p] = x[0];
-            Q[2 * p + 1] = x[1];
-            M::values(sh.k.in.cols(32 * p, 16 * at.wave, r, g), x);
-            K[2 * p] = x[0];
-            K[2 * p + 1] = x[1];
-        }
-        // From and to the other chunks.
-#pragma unroll
-        for (int m = 0; m < CT; ++m) dQ[m] = dK[m] = dV[m] = zero;
-#pragma unroll
-        for (int i = 0; i < KP; ++i) {
-            const auto s = M::full(S[2 * i], S[2 * i + 1]), dk = M::full(by_key[2 * i], by_key[2 * i + 1]),
-                       dv = M::full(by_value[2 * i], by_value[2 * i + 1]);
-#pragma unroll
-            for (int m = 0; m < CT; ++m) {
-                dQ[m] = M::mul(sh.dout.rows(16 * m, i, r, g), s, dQ[m]);
-                dK[m] = M::mul(sh.v.in.rows(16 * m, i, r, g), dk, dK[m]);
-                dV[m] = M::mul(sh.k.in.rows(16 * m, i, r, g), dv, dV[m]);
-            }
-        }
-#pragma unroll
-        for (int m = 0; m < CT; ++m) {
-            const f4 in = seen.in(sh.powers, 16 * m + 4 * g) * a.scale, out = seen.out(sh.powers, 16 * m + 4 * g);
-            dQ[m] *= in;
-            dK[m] *= out;
-            dV[m] *= out;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int i = 16 * m + 4 * g + e;
-                decay += static_cast<float>(i + 1) * Q[m][e] * dQ[m][e] + static_cast<float>(n - 1 - i) * K[m][e] * dK[m][e];
-            }
-        }
         const float whole = seen.whole(sh.powers);
         {
             float held = 0.0f;
@@ -152,46 +121,122 @@ __global__ void __launch_bounds__(DP * 4, 2) decay_backward_kernel(DecayArgs<T> 
                 for (int e = 0; e < 4; ++e) held += by_key[i][e] * S[i][e];
             decay += static_cast<float>(n) * whole * held;
         }
-        // Pairs within the chunk: R turned round, for dQ.
+        __syncthreads();
+        using Done = DecayResults<T, DP, CH>;
+        typename Done::Tile done_q[CT], done_k[CT], done_v[CT];
+        const std::int64_t token = static_cast<std::int64_t>(start) * a.batch + env;
+        // Of several value heads of a key head: one share each, added up afterwards.
+        const std::int64_t share_step = static_cast<std::int64_t>(a.batch) * a.hv * a.dk_dim;
+        const auto share = [&](bool of_k, int m, f4 x) {
+            if (a.group == 1) return;
+            const Rows<float, WIDE> to(a.scratch + (of_k ? a.steps * share_step : 0) + (token * a.hv + h) * a.dk_dim, share_step);
+            DecayResults<float, DP, CH>::put_tile(to, dk_dim, n, at, m, x);
+        };
+
+        // dQ: from the chunks before, then R turned round.
+        {
+            f4 dQ[CT];
 #pragma unroll
-        for (int m = 0; m < CT; ++m)
+            for (int m = 0; m < CT; ++m) dQ[m] = zero;
 #pragma unroll
-            for (int p = 0; p <= m / 2; ++p) {
-                f4 x[2] = {zero, zero};
+            for (int i = 0; i < KP; ++i) {
+                const auto s = M::full(S[2 * i], S[2 * i + 1]);
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (2 * p + t > m) break;
-#pragma unroll
-                    for (int i = 0; i < KP; ++i)
-                        x[t] = M::mul(sh.v.in.rows(16 * (2 * p + t), i, r, g), sh.dout.rows(16 * m, i, r, g), x[t]);
-                    x[t] = earlier.weigh(x[t], m, 2 * p + t, seen, r, g);
-                }
-                dQ[m] = M::mul(M::full(x[0], x[1]), sh.k.in.cols(32 * p, 16 * at.wave, r, g), dQ[m]);
+                for (int m = 0; m < CT; ++m) dQ[m] = M::mul(sh.dout.rows(16 * m, i, r, g), s, dQ[m]);
             }
-        // P and R, for dV and dK.
 #pragma unroll
-        for (int m = 0; m < CT; ++m)
-#pragma unroll
-            for (int p = m / 2; p < CT / 2; ++p) {
-                f4 x[2] = {zero, zero}, y[2] = {zero, zero};
+            for (int p = 0; p < CT / 2; ++p) {
+                f4 Q[2];
+                M::values(sh.q.in.cols(32 * p, 16 * at.wave, r, g), Q);
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    const int it = 2 * p + t;
-                    if (it < m) continue;
+                    const int m = 2 * p + t;
+                    dQ[m] *= seen.in(sh.powers, 16 * m + 4 * g) * a.scale;
 #pragma unroll
-                    for (int i = 0; i < KP; ++i) {
-                        x[t] = M::mul(sh.q.in.rows(16 * it, i, r, g), sh.k.in.rows(16 * m, i, r, g), x[t]);
-                        y[t] = M::mul(sh.dout.rows(16 * it, i, r, g), sh.v.in.rows(16 * m, i, r, g), y[t]);
+                    for (int e = 0; e < 4; ++e) decay += static_cast<float>(16 * m + 4 * g + e + 1) * Q[t][e] * dQ[m][e];
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < CT; ++m) {
+#pragma unroll
+                for (int p = 0; p <= m / 2; ++p) {
+                    f4 x[2] = {zero, zero};
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (2 * p + t > m) break;
+#pragma unroll
+                        for (int i = 0; i < KP; ++i)
+                            x[t] = M::mul(sh.v.in.rows(16 * (2 * p + t), i, r, g), sh.dout.rows(16 * m, i, r, g), x[t]);
+                        x[t] = earlier.weigh(x[t], m, 2 * p + t, seen, sh.episodes, r, g);
                     }
-                    x[t] = later.weigh(x[t], it, m, seen, r, g);
-                    if ((it * CT + m) % kWaves == at.wave)         // a tile is one wave's
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) decay += static_cast<float>(16 * (it - m) + 4 * g + e - r) * x[t][e] * y[t][e];
-                    y[t] = later.weigh(y[t], it, m, seen, r, g);
+                    dQ[m] = M::mul(M::full(x[0], x[1]), sh.k.in.cols(32 * p, 16 * at.wave, r, g), dQ[m]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                dV[m] = M::mul(M::full(x[0], x[1]), sh.dout.cols(32 * p, 16 * at.wave, r, g), dV[m]);
-                dK[m] = M::mul(M::full(y[0], y[1]), sh.q.in.cols(32 * p, 16 * at.wave, r, g), dK[m]);
+                share(false, m, dQ[m]);
+                done_q[m] = Done::tile(dQ[m]);
             }
+        }
+        next_part();
+        if (t1 > 0) fetch(t1, at);
+        // dK and dV: from the chunks after, then R and P.
+        {
+            f4 dK[CT], dV[CT];
+#pragma unroll
+            for (int m = 0; m < CT; ++m) dK[m] = dV[m] = zero;
+#pragma unroll
+            for (int i = 0; i < KP; ++i) {
+                const auto dk = M::full(by_key[2 * i], by_key[2 * i + 1]), dv = M::full(by_value[2 * i], by_value[2 * i + 1]);
+#pragma unroll
+                for (int m = 0; m < CT; ++m) {
+                    dK[m] = M::mul(sh.v.in.rows(16 * m, i, r, g), dk, dK[m]);
+                    dV[m] = M::mul(sh.k.in.rows(16 * m, i, r, g), dv, dV[m]);
+                }
+            }
+#pragma unroll
+            for (int p = 0; p < CT / 2; ++p) {
+                f4 K[2];
+                M::values(sh.k.in.cols(32 * p, 16 * at.wave, r, g), K);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int m = 2 * p + t;
+                    const f4 out = seen.out(sh.powers, 16 * m + 4 * g);
+                    dK[m] *= out;
+                    dV[m] *= out;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) decay += static_cast<float>(n - 1 - (16 * m + 4 * g + e)) * K[t][e] * dK[m][e];
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < CT; ++m) {
+#pragma unroll
+                for (int p = m / 2; p < CT / 2; ++p) {
+                    f4 x[2] = {zero, zero}, y[2] = {zero, zero};
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const int it = 2 * p + t;
+                        if (it < m) continue;
+#pragma unroll
+                        for (int i = 0; i < KP; ++i) {
+                            x[t] = M::mul(sh.q.in.rows(16 * it, i, r, g), sh.k.in.rows(16 * m, i, r, g), x[t]);
+                            y[t] = M::mul(sh.dout.rows(16 * it, i, r, g), sh.v.in.rows(16 * m, i, r, g), y[t]);
+                        }
+                        x[t] = later.weigh(x[t], it, m, seen, sh.episodes, r, g);
+                        if ((it * CT + m) % kWaves == at.wave)         // a tile is one wave's
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) decay += static_cast<float>(16 * (it - m) + 4 * g + e - r) * x[t][e] * y[t][e];
+                        y[t] = later.weigh(y[t], it, m, seen, sh.episodes, r, g);
+                    }
+                    dV[m] = M::mul(M::full(x[0], x[1]), sh.dout.cols(32 * p, 16 * at.wave, r, g), dV[m]);
+                    dK[m] = M::mul(M::full(y[0], y[1]), sh.q.in.cols(32 * p, 16 * at.wave, r, g), dK[m]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                share(true, m, dK[m]);
+                done_k[m] = Done::tile(dK[m]);
+                done_v[m] = Done::tile(dV[m]);
+                next_part();
+            }
+        }
+        next_part();
         // The state's gradient before the chunk.
 #pragma unroll
         for (int i = 0; i < KT; ++i) {
@@ -200,36 +245,31 @@ __global__ void __launch_bounds__(DP * 4, 2) decay_backward_kernel(DecayArgs<T> 
         }
 #pragma unroll
         for (int p = 0; p < CT / 2; ++p) {
+            f4 x[2];
+            M::values(sh.q.in.cols(32 * p, 16 * at.wave, r, g), x);
             const f4 in[2] = {seen.in(sh.powers, 32 * p + 4 * g) * a.scale, seen.in(sh.powers, 32 * p + 16 + 4 * g) * a.scale};
-            const auto of_q = M::full(Q[2 * p] * in[0], Q[2 * p + 1] * in[1]);
-            f4 dO[2];
-            M::values(sh.dout.cols(32 * p, 16 * at.wave, r, g), dO);
-            const auto of_do = M::full(dO[0] * in[0], dO[1] * in[1]);
+            const auto of_q = M::full(x[0] * in[0], x[1] * in[1]);
+            M::values(sh.dout.cols(32 * p, 16 * at.wave, r, g), x);
+            const auto of_do = M::full(x[0] * in[0], x[1] * in[1]);
 #pragma unroll
             for (int i = 0; i < KT; ++i) {
                 by_key[i] = M::mul(sh.dout.cols(32 * p, 16 * i, r, g), of_q, by_key[i]);
                 by_value[i] = M::mul(sh.q.in.cols(32 * p, 16 * i, r, g), of_do, by_value[i]);
             }
-        }
+            }
         if (dropped)
 #pragma unroll
             for (int i = 0; i < KT; ++i) by_key[i] = by_value[i] = zero;
 
-        const std::int64_t token = static_cast<std::int64_t>(start) * a.batch + env;
         const std::int64_t key_step = static_cast<std::int64_t>(a.batch) * a.hk * a.dk_dim;
         const In dq(a.dq + (token * a.hk + hk) * a.dk_dim, key_step), dk(a.dk + (token * a.hk + hk) * a.dk_dim, key_step),
             dv(a.dv + static_cast<std::int64_t>(start) * v_step + head * a.dv_dim, v_step);
         __syncthreads();                   // the inputs have been read
         if (a.group == 1) {
-            sh.q.results.put(dq, dk_dim, n, at, dQ);
-            sh.k.results.put(dk, dk_dim, n, at, dK);
-        } else {                           // one share a value head, added up afterwards
-            const std::int64_t step = static_cast<std::int64_t>(a.batch) * a.hv * a.dk_dim;
-            float* share = a.scratch + (token * a.hv + h) * a.dk_dim;
-            DecayResults<float, DP, CH>{}.put(Rows<float, WIDE>(share, step), dk_dim, n, at, dQ);
-            DecayResults<float, DP, CH>{}.put(Rows<float, WIDE>(share + a.steps * step, step), dk_dim, n, at, dK);
+            sh.q.results.put(dq, dk_dim, n, at, done_q);
+            sh.k.results.put(dk, dk_dim, n, at, done_k);
         }
-        sh.v.results.put(dv, dv_dim, n, at, dV);
+        sh.v.results.put(dv, dv_dim, n, at, done_v);
         __syncthreads();
         if (a.group == 1) {
             sh.q.results.flush(dq, dk_dim, n, at);

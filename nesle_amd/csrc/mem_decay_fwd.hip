@@ -31,8 +31,13 @@ struct ForwardTile {
     typename M::template Tile<CH, DP, M::kIn, 8> k, q, v;
     DecayResults<T, DP, CH> results;
     Powers<CH> powers;
+    alignas(16) int episodes[CH];
     std::uint32_t bad[2][2];       // tokens with a value that is not finite, of every other chunk
 };
+
+// Waves of a SIMD that registers are to leave room for.
+template <int DP>
+constexpr int kForwardWaves = DP == 128 ? 2 : 4;
 
 template <int KT>
 __device__ bool finite(const f4 (&S)[KT]) {
@@ -43,7 +48,7 @@ __device__ bool finite(const f4 (&S)[KT]) {
 }
 
 template <typename T, int DP, bool WIDE>
-__global__ void __launch_bounds__(DP * 4, 2) decay_forward_kernel(DecayArgs<T> a) {
+__global__ void __launch_bounds__(DP * 4, kForwardWaves<DP>) decay_forward_kernel(DecayArgs<T> a) {
     constexpr int CH = kDecayChunk<T>, CT = CH / 16, KT = DP / 16, KP = DP / 32;
     using Tile = ForwardTile<T, DP, CH>;
     using M = typename Tile::M;
@@ -95,6 +100,7 @@ __global__ void __launch_bounds__(DP * 4, 2) decay_forward_kernel(DecayArgs<T> a
             k.stage(sh.k, at);
             q.stage(sh.q, at);
             v.stage(sh.v, at);
+            if (inside != 0 && at.tid < CH) sh.episodes[at.tid] = Seen(inside, CH).episode(at.tid);
             std::uint64_t odd = k.odd(at) | v.odd(at);
             if (inside != 0 && !finite(S)) odd |= inside;
             if (odd != 0) {
@@ -148,7 +154,7 @@ __global__ void __launch_bounds__(DP * 4, 2) decay_forward_kernel(DecayArgs<T> a
 #pragma unroll
                     for (int i = 0; i < KP; ++i)
                         x[t] = M::mul(sh.k.rows(16 * (2 * p + t), i, r, g), sh.q.rows(16 * m, i, r, g), x[t]);
-                    x[t] = pair.weigh(x[t], m, 2 * p + t, seen, r, g);
+                    x[t] = pair.weigh(x[t], m, 2 * p + t, seen, sh.episodes, r, g);
                 }
                 O[m] = M::mul(M::full(x[0], x[1]), sh.v.cols(32 * p, 16 * at.wave, r, g), O[m]);
             }
@@ -164,7 +170,10 @@ __global__ void __launch_bounds__(DP * 4, 2) decay_forward_kernel(DecayArgs<T> a
             for (int i = 0; i < KT; ++i) S[i] = M::mul(sh.k.cols(32 * p, 16 * i, r, g), held, S[i]);
         }
         const Rows<T, WIDE> out(a.out + static_cast<std::int64_t>(t0) * out_step + head * a.dv_dim, out_step);
-        sh.results.put(out, dv, n, at, O);
+        typename DecayResults<T, DP, CH>::Tile done[CT];
+#pragma unroll
+        for (int m = 0; m < CT; ++m) done[m] = sh.results.tile(O[m]);
+        sh.results.put(out, dv, n, at, done);
         t0 = next;
         __syncthreads();
         sh.results.flush(out, dv, n, at);
