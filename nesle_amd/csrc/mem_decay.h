@@ -133,6 +133,13 @@ struct Piece {
 #pragma unroll
             for (int i = 0; i < In::kWords; ++i) w[p][i] = at.key_row + 32 * p < n ? w[p][i] : 0;
     }
+    // And in the rows before n.
+    __device__ void cut_before(int n, const Lane<DP>& at) {
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+            for (int i = 0; i < In::kWords; ++i) w[p][i] = at.key_row + 32 * p >= n ? w[p][i] : 0;
+    }
     // Tokens with something that is not finite.
     __device__ std::uint64_t odd(const Lane<DP>& at) const {
         using s2 = unsigned short __attribute__((ext_vector_type(2)));

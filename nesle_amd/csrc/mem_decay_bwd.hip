@@ -19,16 +19,22 @@
 // One workgroup walks one head of one console, a wave for 16 columns of each of dQ,
 // dK and dV.  dS is needed by key columns (dK) and by value columns (dV): a wave
 // holds both slabs of it in registers and updates both, which costs a product more
-// and saves passing it through LDS.  P, R and R turned round are made by every wave
-// for itself and stay in registers, as in the forward; LDS holds Q, K, V and dO of
-// the chunk and, once they have been read, the results on their way out.
+// and saves passing it through LDS.
+//
+// Inputs come and results go a chunk at a time, and the forward kept one state a
+// chunk; inside, the work goes in parts of 32 tokens, last to first, as pairs of
+// tokens of different parts would cost more than the state between them, which is
+// made from the chunk's.  A part's P and R are made by tiles of 16 x 16 pairs, a wave
+// each, and shared through LDS, turned round: [j][i].
 //
 // No atomics: the decays' gradient is added up per workgroup, then over workgroups
 // in a fixed order.
-#include "mem_decay.h"
+#include "mem_decay_segments.h"
 
 namespace nesle::mem {
 namespace {
+
+constexpr int kPart = 32;
 
 template <typename T, int DP, int CH>
 struct GradTile {
@@ -40,90 +46,88 @@ struct GradTile {
     };
     Out q, k, v;               // then dQ, dK, dV
     In dout;
-    Powers<CH> powers;
-    alignas(16) int episodes[CH];
+    typename M::template Tile<kPart, kPart, kFull, 8> p, r;        // [j][i]; zero where i is in an earlier tile
+    Powers<kPart> powers;
+    alignas(16) int episodes[kPart];
     float sums[DP / 16];
 };
 
-// With 128 dimensions eight waves make a workgroup and two of them a SIMD.
+// Waves of a SIMD that registers are to leave room for: what LDS does.
+template <typename T, int DP>
+constexpr int kGradWaves = sizeof(T) == 2 && DP <= 64 ? 3 : 2;
+
 template <typename T, int DP, bool WIDE>
-__global__ void __launch_bounds__(DP * 4, 2) decay_backward_kernel(DecayArgs<T> a, float* partials) {
-    constexpr int CH = kDecayChunk<T>, CT = CH / 16, KT = DP / 16, KP = DP / 32, kWaves = DP / 16;
+__global__ void __launch_bounds__(DP * 4, (kGradWaves<T, DP>)) decay_backward_kernel(DecayArgs<T> a, DecaySegments seg, float* partials) {
+    constexpr int CH = kDecayChunk<T>, PARTS = CH / kPart, KT = DP / 16, KP = DP / 32, kWaves = DP / 16;
     using Tile = GradTile<T, DP, CH>;
     using M = typename Tile::M;
     using In = Rows<T, WIDE>;
+    using Done = DecayResults<T, DP, CH>;
     __shared__ Tile sh;
     const Lane<DP> first;
     const std::uint32_t env = blockIdx.x / a.hv, h = blockIdx.x % a.hv, hk = h / a.group;
     const std::size_t head = blockIdx.x, state_size = static_cast<std::size_t>(a.dk_dim) * a.dv_dim;
+    const std::size_t slot = static_cast<std::size_t>(blockIdx.y) * gridDim.x + head;
     const int dk_dim = static_cast<int>(a.dk_dim), dv_dim = static_cast<int>(a.dv_dim);
     const std::int64_t v_step = static_cast<std::int64_t>(a.batch) * a.hv * a.dv_dim;
     const f4 zero = {0, 0, 0, 0};
+    const std::uint32_t begin = blockIdx.y * seg.steps;
+    const std::uint32_t end = a.steps - begin < seg.steps ? a.steps : begin + seg.steps;
 
     const float gate = a.steps != 0 ? a.g[h] : 0.0f;
     const bool always = gate < kDropBelow;
     sh.powers.make(gate, always, first.tid);
+    if (first.tid < 64)
+        for (int i = 0; i < 4; ++i) {
+            sh.p.put(16 + 4 * first.g + i, first.r, 0.0f);
+            sh.r.put(16 + 4 * first.g + i, first.r, 0.0f);
+        }
     f4 by_key[KT], by_value[KT];           // dS
     {
-        const float* from = a.dstate_out == nullptr ? nullptr : a.dstate_out + head * state_size;
+        const float* from = seg.count > 1 ? seg.states + slot * state_size
+                                          : a.dstate_out == nullptr ? nullptr : a.dstate_out + head * state_size;
         load_key_slab<DP>(from, dk_dim, dv_dim, first, by_key);
         load_value_slab<DP>(from, dk_dim, dv_dim, first, by_value);
     }
-    __syncthreads();
-    PairPowers<CH, true> later;
-    PairPowers<CH, false> earlier;
-    later.make(sh.powers, a.scale, first.r, first.g);
-    earlier.make(sh.powers, a.scale, first.r, first.g);
 
     Piece<T, DP, CH, WIDE> q, k, v, dout;
     std::uint64_t next_drops = 0;
-    const auto fetch = [&](std::uint32_t end, const Lane<DP>& at) {
-        const std::uint32_t start = (end - 1) / CH * CH;
-        const int n = static_cast<int>(end - start);
+    const auto fetch = [&](std::uint32_t t1, const Lane<DP>& at) {
+        const std::uint32_t start = (t1 - 1) / CH * CH;
+        const int n = static_cast<int>(t1 - start);
         q.fetch(a.q, a.dk_dim, start, n, env, hk, at);
         k.fetch(a.k, a.dk_dim, start, n, env, hk, at);
         v.fetch(a.v, a.dv_dim, start, n, env, h, at);
         dout.fetch(a.dout, a.dv_dim, start, n, env, h, at);
         next_drops = drops_of<CH>(a, start, n, env, at.lane, always);
     };
-    if (a.steps != 0) fetch(a.steps, first);
+    if (begin < end) fetch(end, first);
     float decay = 0.0f;                    // this lane's share of the decay's gradient
-    for (std::uint32_t t1 = a.steps; t1 > 0;) {
-        // Made anew for each part of the chunk: what one part has read from LDS is read
-        // again by the next, rather than held in registers through both.
+    for (std::uint32_t t1 = end; t1 > begin;) {
+        // Made anew for each step of the work: what one has read from LDS is read again
+        // by the next, rather than held in registers through both.
         Lane<DP> at = Lane<DP>::anew();
         int r = at.r, g = at.g;
-        const auto next_part = [&] {
+        const auto anew = [&] {
             at = Lane<DP>::anew();
             r = at.r;
             g = at.g;
         };
         const std::uint32_t start = (t1 - 1) / CH * CH;
         const int n = static_cast<int>(t1 - start);
-        const bool dropped = next_drops & 1u;      // the state before the chunk is
-        const Seen seen(next_drops & ~1ull, n);
-        const float* from = dropped ? nullptr : start == 0 ? (a.state == nullptr ? nullptr : a.state + head * state_size)
-                                              : a.saved + ((start / CH - 1) * static_cast<std::size_t>(a.batch) * a.hv + head) * state_size;
+        const std::uint64_t drops = next_drops;
+        const float* from = (drops & 1u) ? nullptr : start == 0 ? (a.state == nullptr ? nullptr : a.state + head * state_size)
+                                         : a.saved + ((start / CH - 1) * static_cast<std::size_t>(a.batch) * a.hv + head) * state_size;
         f4 S[KT];
         load_key_slab<DP>(from, dk_dim, dv_dim, at, S);
         q.stage(sh.q.in, at);
         k.stage(sh.k.in, at);
         v.stage(sh.v.in, at);
         dout.stage(sh.dout, at);
-        if (seen.drops != 0 && at.tid < CH) sh.episodes[at.tid] = seen.episode(at.tid);
         t1 = start;
-        const float whole = seen.whole(sh.powers);
-        {
-            float held = 0.0f;
-#pragma unroll
-            for (int i = 0; i < KT; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) held += by_key[i][e] * S[i][e];
-            decay += static_cast<float>(n) * whole * held;
-        }
         __syncthreads();
-        using Done = DecayResults<T, DP, CH>;
-        typename Done::Tile done_q[CT], done_k[CT], done_v[CT];
+        if (t1 > begin) fetch(t1, at);
+        typename Done::Tile done_q[CH / 16], done_k[CH / 16], done_v[CH / 16];
         const std::int64_t token = static_cast<std::int64_t>(start) * a.batch + env;
         // Of several value heads of a key head: one share each, added up afterwards.
         const std::int64_t share_step = static_cast<std::int64_t>(a.batch) * a.hv * a.dk_dim;
@@ -133,138 +137,147 @@ __global__ void __launch_bounds__(DP * 4, 2) decay_backward_kernel(DecayArgs<T> 
             DecayResults<float, DP, CH>::put_tile(to, dk_dim, n, at, m, x);
         };
 
-        // dQ: from the chunks before, then R turned round.
-        {
-            f4 dQ[CT];
 #pragma unroll
-            for (int m = 0; m < CT; ++m) dQ[m] = zero;
+        for (int part = PARTS - 1; part >= 0; --part) {
+            constexpr int CT = kPart / 16;
+            const int row0 = kPart * part;
+            const std::uint32_t mine = static_cast<std::uint32_t>(drops >> row0);
+            const bool dropped = mine & 1u;        // the state before the part is
+            const Seen seen(mine & ~1u, min(n - row0, kPart));
+            if (PARTS > 1 && n <= row0) {
 #pragma unroll
-            for (int i = 0; i < KP; ++i) {
-                const auto s = M::full(S[2 * i], S[2 * i + 1]);
-#pragma unroll
-                for (int m = 0; m < CT; ++m) dQ[m] = M::mul(sh.dout.rows(16 * m, i, r, g), s, dQ[m]);
+                for (int m = 0; m < CT; ++m) done_q[row0 / 16 + m] = done_k[row0 / 16 + m] = done_v[row0 / 16 + m] = Done::tile(zero);
+                continue;
             }
+            anew();
+            if (seen.drops != 0 && at.tid < kPart) sh.episodes[at.tid] = seen.episode(at.tid);
+            if (seen.drops != 0) __syncthreads();
+            // P and R, a tile a wave; the workgroups of a compute unit leave out
+            // different waves.
+            for (int place = (at.wave + static_cast<int>(blockIdx.x)) % kWaves; place < 3; place += kWaves) {
+                const int it = place == 0 ? 0 : 1, jt = place == 2 ? 1 : 0;
+                f4 x = zero, y = zero;
 #pragma unroll
-            for (int p = 0; p < CT / 2; ++p) {
-                f4 Q[2];
-                M::values(sh.q.in.cols(32 * p, 16 * at.wave, r, g), Q);
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const int m = 2 * p + t;
-                    dQ[m] *= seen.in(sh.powers, 16 * m + 4 * g) * a.scale;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) decay += static_cast<float>(16 * m + 4 * g + e + 1) * Q[t][e] * dQ[m][e];
+                for (int i = 0; i < KP; ++i) {
+                    x = M::mul(sh.q.in.rows(row0 + 16 * it, i, r, g), sh.k.in.rows(row0 + 16 * jt, i, r, g), x);
+                    y = M::mul(sh.dout.rows(row0 + 16 * it, i, r, g), sh.v.in.rows(row0 + 16 * jt, i, r, g), y);
                 }
+                PairPowers<kPart, true> pair;
+                pair.make(sh.powers, a.scale, r, g);
+                x = pair.weigh(x, it, jt, seen, sh.episodes, r, g);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) decay += static_cast<float>(16 * (it - jt) + 4 * g + e - r) * x[e] * y[e];
+                y = pair.weigh(y, it, jt, seen, sh.episodes, r, g);
+                sh.p.put4(16 * jt + r, 16 * it + 4 * g, x);
+                sh.r.put4(16 * jt + r, 16 * it + 4 * g, y);
             }
+            // The state before the part.
+            f4 before[KT];
+            if (part == 0) {
 #pragma unroll
-            for (int m = 0; m < CT; ++m) {
+                for (int i = 0; i < KT; ++i) before[i] = S[i];
+            } else {
+                const Seen ahead(drops & 0xffffffffu, kPart);
+                const float whole = ahead.whole(sh.powers);
+                f4 K[2];
+                M::values(sh.k.in.cols(0, 16 * at.wave, r, g), K);
+                const auto held = M::full(K[0] * ahead.out(sh.powers, 4 * g), K[1] * ahead.out(sh.powers, 16 + 4 * g));
 #pragma unroll
-                for (int p = 0; p <= m / 2; ++p) {
-                    f4 x[2] = {zero, zero};
+                for (int i = 0; i < KT; ++i) before[i] = dropped ? zero : M::mul(sh.v.in.cols(0, 16 * i, r, g), held, S[i] * whole);
+            }
+            const float whole = seen.whole(sh.powers);
+            {
+                float held = 0.0f;
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        if (2 * p + t > m) break;
+                for (int i = 0; i < KT; ++i)
 #pragma unroll
-                        for (int i = 0; i < KP; ++i)
-                            x[t] = M::mul(sh.v.in.rows(16 * (2 * p + t), i, r, g), sh.dout.rows(16 * m, i, r, g), x[t]);
-                        x[t] = earlier.weigh(x[t], m, 2 * p + t, seen, sh.episodes, r, g);
-                    }
-                    dQ[m] = M::mul(M::full(x[0], x[1]), sh.k.in.cols(32 * p, 16 * at.wave, r, g), dQ[m]);
-                    __builtin_amdgcn_sched_barrier(0);
+                    for (int e = 0; e < 4; ++e) held += by_key[i][e] * before[i][e];
+                decay += static_cast<float>(seen.n) * whole * held;
+            }
+            __syncthreads();
+
+            // dQ: from the tokens before the part, then within.
+            {
+                f4 x[CT] = {}, Q[CT];
+#pragma unroll
+                for (int i = 0; i < KP; ++i) {
+                    const auto s = M::full(before[2 * i], before[2 * i + 1]);
+#pragma unroll
+                    for (int m = 0; m < CT; ++m) x[m] = M::mul(sh.dout.rows(row0 + 16 * m, i, r, g), s, x[m]);
                 }
-                share(false, m, dQ[m]);
-                done_q[m] = Done::tile(dQ[m]);
-            }
-        }
-        next_part();
-        if (t1 > 0) fetch(t1, at);
-        // dK and dV: from the chunks after, then R and P.
-        {
-            f4 dK[CT], dV[CT];
-#pragma unroll
-            for (int m = 0; m < CT; ++m) dK[m] = dV[m] = zero;
-#pragma unroll
-            for (int i = 0; i < KP; ++i) {
-                const auto dk = M::full(by_key[2 * i], by_key[2 * i + 1]), dv = M::full(by_value[2 * i], by_value[2 * i + 1]);
+                M::values(sh.q.in.cols(row0, 16 * at.wave, r, g), Q);
+                const auto key = sh.k.in.cols(row0, 16 * at.wave, r, g);
 #pragma unroll
                 for (int m = 0; m < CT; ++m) {
-                    dK[m] = M::mul(sh.v.in.rows(16 * m, i, r, g), dk, dK[m]);
-                    dV[m] = M::mul(sh.k.in.rows(16 * m, i, r, g), dv, dV[m]);
+                    x[m] *= seen.in(sh.powers, 16 * m + 4 * g) * a.scale;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) decay += static_cast<float>(16 * m + 4 * g + e + 1) * Q[m][e] * x[m][e];
+                    x[m] = M::mul(sh.r.cols(0, 16 * m, r, g), key, x[m]);
+                    share(false, row0 / 16 + m, x[m]);
+                    done_q[row0 / 16 + m] = Done::tile(x[m]);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
+            anew();
+            // dK: from the tokens after the part, then within; the slab of dS that it reads.
+            {
+                f4 x[CT] = {}, K[CT], Q[CT];
 #pragma unroll
-            for (int p = 0; p < CT / 2; ++p) {
-                f4 K[2];
-                M::values(sh.k.in.cols(32 * p, 16 * at.wave, r, g), K);
+                for (int i = 0; i < KP; ++i) {
+                    const auto s = M::full(by_key[2 * i], by_key[2 * i + 1]);
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const int m = 2 * p + t;
-                    const f4 out = seen.out(sh.powers, 16 * m + 4 * g);
-                    dK[m] *= out;
-                    dV[m] *= out;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) decay += static_cast<float>(n - 1 - (16 * m + 4 * g + e)) * K[t][e] * dK[m][e];
+                    for (int m = 0; m < CT; ++m) x[m] = M::mul(sh.v.in.rows(row0 + 16 * m, i, r, g), s, x[m]);
                 }
-            }
+                M::values(sh.k.in.cols(row0, 16 * at.wave, r, g), K);
+                const auto query = sh.q.in.cols(row0, 16 * at.wave, r, g);
+                M::values(query, Q);
 #pragma unroll
-            for (int m = 0; m < CT; ++m) {
+                for (int m = 0; m < CT; ++m) {
+                    x[m] *= seen.out(sh.powers, 16 * m + 4 * g);
 #pragma unroll
-                for (int p = m / 2; p < CT / 2; ++p) {
-                    f4 x[2] = {zero, zero}, y[2] = {zero, zero};
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const int it = 2 * p + t;
-                        if (it < m) continue;
-#pragma unroll
-                        for (int i = 0; i < KP; ++i) {
-                            x[t] = M::mul(sh.q.in.rows(16 * it, i, r, g), sh.k.in.rows(16 * m, i, r, g), x[t]);
-                            y[t] = M::mul(sh.dout.rows(16 * it, i, r, g), sh.v.in.rows(16 * m, i, r, g), y[t]);
-                        }
-                        x[t] = later.weigh(x[t], it, m, seen, sh.episodes, r, g);
-                        if ((it * CT + m) % kWaves == at.wave)         // a tile is one wave's
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) decay += static_cast<float>(16 * (it - m) + 4 * g + e - r) * x[t][e] * y[t][e];
-                        y[t] = later.weigh(y[t], it, m, seen, sh.episodes, r, g);
-                    }
-                    dV[m] = M::mul(M::full(x[0], x[1]), sh.dout.cols(32 * p, 16 * at.wave, r, g), dV[m]);
-                    dK[m] = M::mul(M::full(y[0], y[1]), sh.q.in.cols(32 * p, 16 * at.wave, r, g), dK[m]);
-                    __builtin_amdgcn_sched_barrier(0);
+                    for (int e = 0; e < 4; ++e) decay += static_cast<float>(seen.n - 1 - (16 * m + 4 * g + e)) * K[m][e] * x[m][e];
+                    x[m] = M::mul(sh.r.rows(16 * m, 0, r, g), query, x[m]);
+                    share(true, row0 / 16 + m, x[m]);
+                    done_k[row0 / 16 + m] = Done::tile(x[m]);
+                    Q[m] *= seen.in(sh.powers, 16 * m + 4 * g) * a.scale;
                 }
-                share(true, m, dK[m]);
-                done_k[m] = Done::tile(dK[m]);
-                done_v[m] = Done::tile(dV[m]);
-                next_part();
+                const auto read = M::full(Q[0], Q[1]);
+#pragma unroll
+                for (int i = 0; i < KT; ++i)
+                    by_key[i] = dropped ? zero : M::mul(sh.dout.cols(row0, 16 * i, r, g), read, by_key[i] * whole);
             }
+            __builtin_amdgcn_sched_barrier(0);
+            anew();
+            // dV, the same.
+            {
+                f4 x[CT] = {}, dO[CT];
+#pragma unroll
+                for (int i = 0; i < KP; ++i) {
+                    const auto s = M::full(by_value[2 * i], by_value[2 * i + 1]);
+#pragma unroll
+                    for (int m = 0; m < CT; ++m) x[m] = M::mul(sh.k.in.rows(row0 + 16 * m, i, r, g), s, x[m]);
+                }
+                const auto grad = sh.dout.cols(row0, 16 * at.wave, r, g);
+                M::values(grad, dO);
+#pragma unroll
+                for (int m = 0; m < CT; ++m) {
+                    x[m] *= seen.out(sh.powers, 16 * m + 4 * g);
+                    x[m] = M::mul(sh.p.rows(16 * m, 0, r, g), grad, x[m]);
+                    done_v[row0 / 16 + m] = Done::tile(x[m]);
+                    dO[m] *= seen.in(sh.powers, 16 * m + 4 * g) * a.scale;
+                }
+                const auto read = M::full(dO[0], dO[1]);
+#pragma unroll
+                for (int i = 0; i < KT; ++i)
+                    by_value[i] = dropped ? zero : M::mul(sh.q.in.cols(row0, 16 * i, r, g), read, by_value[i] * whole);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            __syncthreads();               // P, R and, in the end, the inputs have been read
         }
-        next_part();
-        // The state's gradient before the chunk.
-#pragma unroll
-        for (int i = 0; i < KT; ++i) {
-            by_key[i] *= whole;
-            by_value[i] *= whole;
-        }
-#pragma unroll
-        for (int p = 0; p < CT / 2; ++p) {
-            f4 x[2];
-            M::values(sh.q.in.cols(32 * p, 16 * at.wave, r, g), x);
-            const f4 in[2] = {seen.in(sh.powers, 32 * p + 4 * g) * a.scale, seen.in(sh.powers, 32 * p + 16 + 4 * g) * a.scale};
-            const auto of_q = M::full(x[0] * in[0], x[1] * in[1]);
-            M::values(sh.dout.cols(32 * p, 16 * at.wave, r, g), x);
-            const auto of_do = M::full(x[0] * in[0], x[1] * in[1]);
-#pragma unroll
-            for (int i = 0; i < KT; ++i) {
-                by_key[i] = M::mul(sh.dout.cols(32 * p, 16 * i, r, g), of_q, by_key[i]);
-                by_value[i] = M::mul(sh.q.in.cols(32 * p, 16 * i, r, g), of_do, by_value[i]);
-            }
-            }
-        if (dropped)
-#pragma unroll
-            for (int i = 0; i < KT; ++i) by_key[i] = by_value[i] = zero;
-
         const std::int64_t key_step = static_cast<std::int64_t>(a.batch) * a.hk * a.dk_dim;
         const In dq(a.dq + (token * a.hk + hk) * a.dk_dim, key_step), dk(a.dk + (token * a.hk + hk) * a.dk_dim, key_step),
             dv(a.dv + static_cast<std::int64_t>(start) * v_step + head * a.dv_dim, v_step);
-        __syncthreads();                   // the inputs have been read
+        anew();
         if (a.group == 1) {
             sh.q.results.put(dq, dk_dim, n, at, done_q);
             sh.k.results.put(dk, dk_dim, n, at, done_k);
@@ -278,7 +291,7 @@ __global__ void __launch_bounds__(DP * 4, 2) decay_backward_kernel(DecayArgs<T> 
         sh.v.results.flush(dv, dv_dim, n, at);
         __syncthreads();                   // before the next chunk takes their place
     }
-    if (a.dstate != nullptr) store_key_slab<DP>(a.dstate + head * state_size, dk_dim, dv_dim, Lane<DP>::anew(), by_key);
+    if (a.dstate != nullptr && begin == 0) store_key_slab<DP>(a.dstate + head * state_size, dk_dim, dv_dim, Lane<DP>::anew(), by_key);
     if (partials != nullptr) {
         decay = over_groups(sum16(decay));
         if (first.lane == 0) sh.sums[first.wave] = decay;
@@ -286,7 +299,7 @@ __global__ void __launch_bounds__(DP * 4, 2) decay_backward_kernel(DecayArgs<T> 
         if (first.tid == 0) {
             float sum = 0.0f;
             for (int w = 0; w < kWaves; ++w) sum += sh.sums[w];
-            partials[head] = sum;
+            partials[slot] = sum;
         }
     }
 }
@@ -317,22 +330,30 @@ __global__ void __launch_bounds__(256) decay_share_sum(DecayArgs<T> a, std::uint
     }
 }
 
-// Floats of the shares, ahead of the decays' partial sums.
+// Floats of the shares, ahead of the segments' states and the decays' partial sums.
 std::uint64_t share_floats(const nesle_decay_args& a) {
-    return a.v_heads > a.k_heads ? 2ull * a.steps * a.batch * a.v_heads * a.k_dim : 0;
+    const std::uint64_t floats = a.v_heads > a.k_heads ? 2ull * a.steps * a.batch * a.v_heads * a.k_dim : 0;
+    return (floats + 3) / 4 * 4;
+}
+
+template <typename T, int DP, bool WIDE>
+void launch_dim(const DecayArgs<T>& a, const DecaySegments& seg, float* partials, hipStream_t s) {
+    if (seg.count > 1) launch_states<T, DP, WIDE, true>(a, seg, s);
+    hipLaunchKernelGGL((decay_backward_kernel<T, DP, WIDE>), dim3(a.batch * a.hv, seg.count), dim3(DP * 4), 0, s, a, seg, partials);
 }
 
 template <typename T>
 int backward(const char* who, const nesle_decay_args& x, hipStream_t s) {
     const DecayArgs<T> a = decay_args<T>(x);
-    const dim3 grid(a.batch * a.hv);
-    float* partials = a.dg == nullptr ? nullptr : a.scratch + share_floats(x);
+    DecaySegments seg = decay_segments(x);
+    seg.place(x, a.scratch + share_floats(x));
+    float* partials = a.dg == nullptr ? nullptr : a.scratch + share_floats(x) + seg.floats(x);
     const std::uint32_t dim = wide_rows(x) ? 0 : padded_dim(x);
     switch (dim) {
-        case 0: hipLaunchKernelGGL((decay_backward_kernel<T, 128, true>), grid, dim3(512), 0, s, a, partials); break;
-        case 32: hipLaunchKernelGGL((decay_backward_kernel<T, 32, false>), grid, dim3(128), 0, s, a, partials); break;
-        case 64: hipLaunchKernelGGL((decay_backward_kernel<T, 64, false>), grid, dim3(256), 0, s, a, partials); break;
-        default: hipLaunchKernelGGL((decay_backward_kernel<T, 128, false>), grid, dim3(512), 0, s, a, partials); break;
+        case 0: launch_dim<T, 128, true>(a, seg, partials, s); break;
+        case 32: launch_dim<T, 32, false>(a, seg, partials, s); break;
+        case 64: launch_dim<T, 64, false>(a, seg, partials, s); break;
+        default: launch_dim<T, 128, false>(a, seg, partials, s); break;
     }
     if (a.group > 1 && a.steps != 0) {
         const std::uint64_t quads = static_cast<std::uint64_t>(a.steps) * a.batch * a.hk * a.dk_dim / 4;
@@ -340,7 +361,7 @@ int backward(const char* who, const nesle_decay_args& x, hipStream_t s) {
         hipLaunchKernelGGL(decay_share_sum<T>, dim3(static_cast<std::uint32_t>(want < 4096 ? want : 4096)), dim3(256), 0, s, a, quads);
     }
     if (partials != nullptr)
-        hipLaunchKernelGGL(decay_gate_sum, dim3(a.hv), dim3(256), 0, s, partials, a.dg, a.hv, static_cast<std::uint64_t>(a.batch) * a.hv);
+        hipLaunchKernelGGL(decay_gate_sum, dim3(a.hv), dim3(256), 0, s, partials, a.dg, a.hv, static_cast<std::uint64_t>(seg.count) * a.batch * a.hv);
     return launched(who);
 }
 
@@ -358,8 +379,9 @@ using namespace nesle::mem;
 extern "C" {
 
 std::uint64_t nesle_decay_scratch_floats(const nesle_decay_args* a) {
-    if (a == nullptr || a->k_heads == 0) return 0;
-    return share_floats(*a) + static_cast<std::uint64_t>(a->batch) * a->v_heads;
+    if (a == nullptr || a->k_heads == 0 || a->batch == 0 || a->v_heads == 0) return 0;
+    const DecaySegments seg = decay_segments(*a);
+    return share_floats(*a) + seg.floats(*a) + static_cast<std::uint64_t>(seg.count) * a->batch * a->v_heads;
 }
 
 int nesle_decay_backward(const nesle_decay_args* a, void* stream) {
@@ -378,7 +400,7 @@ int nesle_decay_backward(const nesle_decay_args* a, void* stream) {
         if (!a->dout.data || !a->dq || !a->dk || !a->dv || (!a->saved && nesle_decay_saved_floats(a) != 0))
             return refuse(who, "null device pointer");
     }
-    if (!a->scratch && ((a->steps != 0 && a->v_heads > a->k_heads) || a->dg)) return refuse(who, "null device pointer");
+    if (!a->scratch && ((a->steps != 0 && a->v_heads > a->k_heads) || decay_segments(*a).count > 1 || a->dg)) return refuse(who, "null device pointer");
     return a->dtype == NESLE_MEM_F32 ? backward<float>(who, *a, s) : backward<bf16>(who, *a, s);
 }
 

@@ -18,9 +18,7 @@
 // A product with a masked zero would still carry NaN, so where a key, a value or
 // (with an episode's end in the chunk) the state is not finite, the chunk is cut
 // before that token and at the ends: nothing of it reaches a token it must not.
-#include <algorithm>
-
-#include "mem_decay.h"
+#include "mem_decay_segments.h"
 
 namespace nesle::mem {
 namespace {
@@ -48,7 +46,7 @@ __device__ bool finite(const f4 (&S)[KT]) {
 }
 
 template <typename T, int DP, bool WIDE>
-__global__ void __launch_bounds__(DP * 4, kForwardWaves<DP>) decay_forward_kernel(DecayArgs<T> a) {
+__global__ void __launch_bounds__(DP * 4, kForwardWaves<DP>) decay_forward_kernel(DecayArgs<T> a, DecaySegments seg) {
     constexpr int CH = kDecayChunk<T>, CT = CH / 16, KT = DP / 16, KP = DP / 32;
     using Tile = ForwardTile<T, DP, CH>;
     using M = typename Tile::M;
@@ -59,20 +57,24 @@ __global__ void __launch_bounds__(DP * 4, kForwardWaves<DP>) decay_forward_kerne
     const std::int64_t out_step = static_cast<std::int64_t>(a.batch) * a.hv * a.dv_dim;
     const int dk = static_cast<int>(a.dk_dim), dv = static_cast<int>(a.dv_dim);
     const f4 zero = {0, 0, 0, 0};
+    const std::uint32_t begin = blockIdx.y * seg.steps;
+    const std::uint32_t end = a.steps - begin < seg.steps ? a.steps : begin + seg.steps;
 
     const float gate = a.steps != 0 ? a.g[h] : 0.0f;
     const bool always = gate < kDropBelow;
     sh.powers.make(gate, always, first.tid);
     if (first.tid < 4) sh.bad[first.tid / 2][first.tid % 2] = 0;
     f4 S[KT];
-    load_value_slab<DP>(a.state == nullptr ? nullptr : a.state + head * state_size, dk, dv, first, S);
+    const float* from = seg.count > 1 ? seg.states + (static_cast<std::size_t>(blockIdx.y) * gridDim.x + head) * state_size
+                                      : a.state == nullptr ? nullptr : a.state + head * state_size;
+    load_value_slab<DP>(from, dk, dv, first, S);
     __syncthreads();
     PairPowers<CH, false> pair;
     pair.make(sh.powers, a.scale, first.r, first.g);
 
     // Tokens from t0 to the next multiple of the chunk length or the end.
     const auto width = [&](std::uint32_t t0) {
-        const std::uint32_t whole = CH - t0 % CH, left = a.steps - t0;
+        const std::uint32_t whole = CH - t0 % CH, left = end - t0;
         return static_cast<int>(whole < left ? whole : left);
     };
     Piece<T, DP, CH, WIDE> k, q, v;
@@ -84,9 +86,9 @@ __global__ void __launch_bounds__(DP * 4, kForwardWaves<DP>) decay_forward_kerne
         v.fetch(a.v, a.dv_dim, t0, n, env, h, at);
         next_drops = drops_of<CH>(a, t0, n, env, at.lane, always);
     };
-    if (a.steps != 0) fetch(0, first);
+    if (begin < end) fetch(begin, first);
     int which = 0;
-    for (std::uint32_t t0 = 0; t0 < a.steps; which ^= 1) {
+    for (std::uint32_t t0 = begin; t0 < end; which ^= 1) {
         const Lane<DP> at = Lane<DP>::anew();
         const int r = at.r, g = at.g;
         if (t0 != 0 && t0 % CH == 0 && a.saved != nullptr)
@@ -125,7 +127,7 @@ __global__ void __launch_bounds__(DP * 4, kForwardWaves<DP>) decay_forward_kerne
         if (at.tid < 2) sh.bad[which ^ 1][at.tid] = 0;     // read before the last barrier but one
         const Seen seen(inside & (~0ull >> (64 - n)), n);
         const std::uint32_t next = t0 + n;
-        if (next < a.steps) fetch(next, at);
+        if (next < end) fetch(next, at);
 
         f4 O[CT];
 #pragma unroll
@@ -178,23 +180,26 @@ __global__ void __launch_bounds__(DP * 4, kForwardWaves<DP>) decay_forward_kerne
         __syncthreads();
         sh.results.flush(out, dv, n, at);
     }
-    store_value_slab<DP>(a.state_out + head * state_size, dk, dv, Lane<DP>::anew(), S);
+    if (end == a.steps) store_value_slab<DP>(a.state_out + head * state_size, dk, dv, Lane<DP>::anew(), S);
 }
 
 template <typename T, int DP, bool WIDE>
-void launch_dim(const DecayArgs<T>& a, hipStream_t s) {
-    hipLaunchKernelGGL((decay_forward_kernel<T, DP, WIDE>), dim3(a.batch * a.hv), dim3(DP * 4), 0, s, a);
+void launch_dim(const DecayArgs<T>& a, const DecaySegments& seg, hipStream_t s) {
+    if (seg.count > 1) launch_states<T, DP, WIDE, false>(a, seg, s);
+    hipLaunchKernelGGL((decay_forward_kernel<T, DP, WIDE>), dim3(a.batch * a.hv, seg.count), dim3(DP * 4), 0, s, a, seg);
 }
 
 template <typename T>
 int forward(const char* who, const nesle_decay_args& x, hipStream_t s) {
     const DecayArgs<T> a = decay_args<T>(x);
+    DecaySegments seg = decay_segments(x);
+    seg.place(x, a.scratch);
     const std::uint32_t dim = wide_rows(x) ? 0 : padded_dim(x);
     switch (dim) {
-        case 0: launch_dim<T, 128, true>(a, s); break;
-        case 32: launch_dim<T, 32, false>(a, s); break;
-        case 64: launch_dim<T, 64, false>(a, s); break;
-        default: launch_dim<T, 128, false>(a, s); break;
+        case 0: launch_dim<T, 128, true>(a, seg, s); break;
+        case 32: launch_dim<T, 32, false>(a, seg, s); break;
+        case 64: launch_dim<T, 64, false>(a, seg, s); break;
+        default: launch_dim<T, 128, false>(a, seg, s); break;
     }
     return launched(who);
 }
@@ -212,7 +217,10 @@ std::uint64_t nesle_decay_saved_floats(const nesle_decay_args* a) {
     return chunks * a->batch * a->v_heads * a->k_dim * a->v_dim;
 }
 
-std::uint64_t nesle_decay_forward_scratch_floats(const nesle_decay_args*) { return 0; }
+std::uint64_t nesle_decay_forward_scratch_floats(const nesle_decay_args* a) {
+    if (a == nullptr || a->batch == 0 || a->v_heads == 0) return 0;
+    return decay_segments(*a).floats(*a);
+}
 
 int nesle_decay_forward(const nesle_decay_args* a, void* stream) {
     const char* who = "nesle_decay_forward";

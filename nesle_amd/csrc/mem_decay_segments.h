@@ -1,0 +1,189 @@
+// mem_decay_segments.h -- few heads over many tokens, cut into segments that are walked
+// at once.
+//
+// A segment of L tokens takes the state before it to a^L S + B, with B from its keys
+// and values alone.  One launch finds every segment's B, one takes the state through
+// the segments, and then the walk runs from each segment's own state.  The gradient of
+// the state goes the same way backwards, with queries and the outputs' gradients.
+#pragma once
+
+#include <algorithm>
+
+#include "mem_decay.h"
+
+namespace nesle::mem {
+
+struct DecaySegments {
+    std::uint32_t steps, count;        // tokens of one, a multiple of the chunk length
+    float* states;                     // [segment][head][k_dim][v_dim]: B, then the state before (after) it
+    std::uint32_t* dropped;            // [segment][head]: whether the state is dropped inside
+    std::uint64_t floats(const nesle_decay_args& a) const {
+        return count < 2 ? 0 : static_cast<std::uint64_t>(count) * a.batch * a.v_heads * (static_cast<std::uint64_t>(a.k_dim) * a.v_dim + 1);
+    }
+    void place(const nesle_decay_args& a, float* scratch) {
+        states = scratch;
+        dropped = reinterpret_cast<std::uint32_t*>(scratch + static_cast<std::uint64_t>(count) * a.batch * a.v_heads * a.k_dim * a.v_dim);
+    }
+};
+
+constexpr std::uint32_t kMostSegments = 128;      // what one workgroup takes a state through
+
+inline DecaySegments decay_segments(const nesle_decay_args& a) {
+    constexpr std::uint32_t kSpan = 64;            // tokens: a multiple of any chunk length
+    const std::uint64_t heads = static_cast<std::uint64_t>(a.batch) * a.v_heads;
+    const std::uint32_t spans = (a.steps + kSpan - 1) / kSpan;
+    std::uint32_t count = 1;
+    if (heads <= 256 && spans >= 4) count = std::min<std::uint64_t>({spans, kMostSegments, 1024 / heads});
+    const std::uint32_t each = count < 2 ? spans : (spans + count - 1) / count;
+    DecaySegments s{};
+    s.steps = std::max(each, 1u) * kSpan;
+    s.count = spans == 0 ? 1 : (spans + each - 1) / each;
+    return s;
+}
+
+// ---- B of every segment -----------------------------------------------------------
+
+template <typename T, int DP, int CH>
+struct LocalTile {
+    using M = DecayMath<T>;
+    typename M::template Tile<CH, DP, M::kIn, 8> x, y;
+    Powers<CH> powers;
+};
+
+// A workgroup walks one segment of one head, 16 value columns a wave.  BACK: queries
+// and the outputs' gradients, last to first, decayed to the segment's beginning.
+template <typename T, int DP, bool WIDE, bool BACK>
+__global__ void __launch_bounds__(DP * 4, DP == 128 ? 2 : 4) decay_local_kernel(DecayArgs<T> a, DecaySegments seg) {
+    constexpr int CH = kDecayChunk<T>, KT = DP / 16;
+    using Tile = LocalTile<T, DP, CH>;
+    using M = typename Tile::M;
+    __shared__ Tile sh;
+    const Lane<DP> first;
+    const std::uint32_t env = blockIdx.x / a.hv, h = blockIdx.x % a.hv;
+    const std::uint32_t segment = blockIdx.y + (BACK ? 1 : 0);      // the first one's, or the last one's, is not needed
+    const std::uint32_t begin = segment * seg.steps;
+    const std::uint32_t end = a.steps - begin < seg.steps ? a.steps : begin + seg.steps;
+    const std::uint32_t chunks = (end - begin + CH - 1) / CH;
+    const float gate = a.g[h];
+    const bool always = gate < kDropBelow;
+    sh.powers.make(gate, always, first.tid);
+    f4 S[KT];
+#pragma unroll
+    for (int i = 0; i < KT; ++i) S[i] = f4{0, 0, 0, 0};
+
+    Piece<T, DP, CH, WIDE> x, y;
+    std::uint64_t next_drops = 0;
+    const auto start_of = [&](std::uint32_t c) { return begin + (BACK ? chunks - 1 - c : c) * CH; };
+    const auto width = [&](std::uint32_t t0) { return static_cast<int>(end - t0 < CH ? end - t0 : CH); };
+    const auto fetch = [&](std::uint32_t c, const Lane<DP>& at) {
+        const std::uint32_t t0 = start_of(c);
+        x.fetch(BACK ? a.q : a.k, a.dk_dim, t0, width(t0), env, h / a.group, at);
+        y.fetch(BACK ? a.dout : a.v, a.dv_dim, t0, width(t0), env, h, at);
+        next_drops = drops_of<CH>(a, t0, width(t0), env, at.lane, always);
+    };
+    fetch(0, first);
+    bool any_drop = false;
+    for (std::uint32_t c = 0; c < chunks; ++c) {
+        const Lane<DP> at = Lane<DP>::anew();
+        const int n = width(start_of(c));
+        const Seen seen(next_drops, n);
+        // Tokens before the last end of an episode leave nothing in the state, and what
+        // is not finite in them must not either.  (The gradient of such inputs is
+        // unspecified.)
+        if (!BACK && seen.drops != 0) {
+            x.cut_before(seen.last, at);
+            y.cut_before(seen.last, at);
+        }
+        any_drop |= seen.drops != 0;
+        x.stage(sh.x, at);
+        y.stage(sh.y, at);
+        __syncthreads();
+        if (c + 1 < chunks) fetch(c + 1, at);
+        const float whole = seen.whole(sh.powers);
+#pragma unroll
+        for (int i = 0; i < KT; ++i) S[i] = seen.drops != 0 ? f4{0, 0, 0, 0} : S[i] * whole;
+#pragma unroll
+        for (int p = 0; p < CH / 32; ++p) {
+            f4 V[2], w[2];
+            M::values(sh.y.cols(32 * p, 16 * at.wave, at.r, at.g), V);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int row = 32 * p + 16 * t + 4 * at.g;
+                w[t] = BACK ? seen.in(sh.powers, row) * a.scale : seen.out(sh.powers, row);
+            }
+            const auto held = M::full(V[0] * w[0], V[1] * w[1]);
+#pragma unroll
+            for (int i = 0; i < KT; ++i) S[i] = M::mul(sh.x.cols(32 * p, 16 * i, at.r, at.g), held, S[i]);
+        }
+        __syncthreads();
+    }
+    const std::size_t slot = static_cast<std::size_t>(segment) * gridDim.x + blockIdx.x;
+    store_value_slab<DP>(seg.states + slot * a.dk_dim * a.dv_dim, static_cast<int>(a.dk_dim), static_cast<int>(a.dv_dim),
+                         Lane<DP>::anew(), S);
+    if (first.tid == 0) seg.dropped[slot] = any_drop;
+}
+
+// ---- the state through the segments -------------------------------------------------
+
+// S <- a^L S + B from segment to segment; a segment that drops the state inside leaves
+// B alone, whatever S held.  B gives way to the state before the segment (BACK: the
+// gradient after it).  16 lanes have 64 elements of a state, 16 such groups an equal
+// share of the segments each: a lane reads its share at once, the shares are joined
+// through LDS, and every group walks its own from where the ones before it end.
+template <bool BACK>
+__global__ void __launch_bounds__(256) decay_join_kernel(DecaySegments seg, const float* start, const float* g, std::uint32_t hv,
+                                                         std::uint32_t size, std::uint32_t last_steps) {
+    constexpr int kShare = kMostSegments / 16;
+    __shared__ f4 sums[16][16];
+    __shared__ float factors[16];                          // negative: dropped
+    const int lane = threadIdx.x % 16, group = threadIdx.x / 16;
+    const std::uint32_t at = (blockIdx.y * 16 + lane) * 4;
+    const bool in = at < size;
+    const std::size_t heads = gridDim.x, head = blockIdx.x;
+    const int count = static_cast<int>(seg.count), share = (count + 15) / 16, begin = group * share;
+    const auto slot = [&](int i) { return static_cast<std::size_t>(BACK ? count - 1 - i : i) * heads + head; };
+    const float gate = g[head % hv];
+    const float all = expf(static_cast<float>(seg.steps) * gate), tail = expf(static_cast<float>(last_steps) * gate);
+    const auto factor = [&](int i) { return BACK && i == 0 ? tail : all; };
+    const f4 zero = {0, 0, 0, 0};
+
+    f4 B[kShare], sum = zero;
+    bool dropped[kShare], any = false;
+    float f = 1.0f;
+#pragma unroll
+    for (int k = 0; k < kShare; ++k) {
+        const int i = begin + k;
+        const bool use = k < share && i < count - 1;       // the last one's is not needed
+        B[k] = use && in ? *reinterpret_cast<const f4*>(seg.states + slot(i) * size + at) : zero;
+        dropped[k] = use && seg.dropped[slot(i)] != 0;
+    }
+    f4 S = start != nullptr && in ? *reinterpret_cast<const f4*>(start + head * size + at) : zero;
+#pragma unroll
+    for (int k = 0; k < kShare; ++k)
+        if (k < share && begin + k < count - 1) {
+            sum = dropped[k] ? B[k] : sum * factor(begin + k) + B[k];
+            f *= factor(begin + k);
+            any |= dropped[k];
+        }
+    sums[group][lane] = sum;
+    if (lane == 0) factors[group] = any ? -1.0f : f;
+    __syncthreads();
+    for (int before = 0; before < group; ++before) S = factors[before] < 0.0f ? sums[before][lane] : S * factors[before] + sums[before][lane];
+#pragma unroll
+    for (int k = 0; k < kShare; ++k) {
+        const int i = begin + k;
+        if (k >= share || i >= count) break;
+        if (in) *reinterpret_cast<f4*>(seg.states + slot(i) * size + at) = S;
+        S = dropped[k] ? B[k] : S * factor(i) + B[k];
+    }
+}
+
+template <typename T, int DP, bool WIDE, bool BACK>
+void launch_states(const DecayArgs<T>& a, const DecaySegments& seg, hipStream_t s) {
+    const std::uint32_t heads = a.batch * a.hv, size = a.dk_dim * a.dv_dim;
+    hipLaunchKernelGGL((decay_local_kernel<T, DP, WIDE, BACK>), dim3(heads, seg.count - 1), dim3(DP * 4), 0, s, a, seg);
+    hipLaunchKernelGGL((decay_join_kernel<BACK>), dim3(heads, (size + 63) / 64), dim3(256), 0, s, seg, BACK ? a.dstate_out : a.state, a.g,
+                       a.hv, size, a.steps - (seg.count - 1) * seg.steps);
+}
+
+}  // namespace nesle::mem
