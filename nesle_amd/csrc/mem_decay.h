@@ -58,19 +58,23 @@ inline std::uint32_t padded_dim(const nesle_decay_args& a) {
     return d <= 32 ? 32 : d <= 64 ? 64 : 128;
 }
 
-// Tokens of a chunk.  What a token costs beside its pairs does not depend on it; 64
-// halves the states kept for the gradient and the barriers.  In float32 the pairs'
-// products, made again by every wave, weigh more than that: 32.
+// Tokens of a chunk of the forward.  What a token costs beside its pairs does not depend
+// on it; 64 halves the barriers.  In float32 the pairs' products, made again by every
+// wave, weigh more than that: 32.
 template <typename T>
 constexpr int kDecayChunk = sizeof(T) == 2 ? 64 : 32;
-inline std::uint32_t decay_chunk(const nesle_decay_args& a) {
-    return a.dtype == NESLE_MEM_F32 ? kDecayChunk<float> : kDecayChunk<bf16>;
+// Tokens between the states that the forward keeps and the gradient takes up: a chunk of
+// the gradient, as many as leave room in LDS.
+template <typename T, int DP>
+constexpr int kDecaySpan = sizeof(T) == 4 && DP == 128 ? 32 : 64;
+inline std::uint32_t decay_span(const nesle_decay_args& a) {
+    return a.dtype == NESLE_MEM_F32 && padded_dim(a) == 128 ? kDecaySpan<float, 128> : kDecaySpan<float, 64>;
 }
 
-// Whether a chunk's rows of any tensor span 2^31 bytes or more, past what a
+// Whether 64 rows of any tensor span 2^31 bytes or more, past what a
 // 32-bit offset reaches.
 inline bool wide_rows(const nesle_decay_args& a) {
-    const std::int64_t item = a.dtype == NESLE_MEM_F32 ? 4 : 2, limit = ((1ll << 31) - 4096) / (decay_chunk(a) - 1);
+    const std::int64_t item = a.dtype == NESLE_MEM_F32 ? 4 : 2, limit = ((1ll << 31) - 4096) / 63;
     for (const nesle_heads* x : {&a.q, &a.k, &a.v, &a.dout})
         if (x->stride_t < 0 || x->stride_t * item >= limit) return true;
     // What the kernels write: of the inputs' type, and shares of key heads' gradients in float32.
@@ -105,43 +109,70 @@ inline int check_decay_inputs(const char* who, const nesle_decay_args* a) {
 
 // ---- a chunk ------------------------------------------------------------------------
 
-// Eight elements of PIECES tokens, 32 apart, of a chunk: what a thread loads of one
-// tensor.  A row from n on, and a column outside the head, reads as zero.
-template <typename T, int DP, int CH, bool WIDE>
+// Where a workgroup's lanes stand: DP / 16 waves, one for 16 columns, in each of ROLES
+// roles.
+template <int DP, int ROLES = 1>
+struct Place {
+    static constexpr int kRows = 32 * ROLES;       // tokens that the workgroup loads at once
+    int tid, lane, r, g, wave, role, col, key_row, key_col;
+    // (Unsigned: a signed quotient by a power of two takes four instructions.)
+    __device__ explicit Place(unsigned id)
+        : tid(static_cast<int>(id & 1023u)), lane(static_cast<int>(id & 63u)), r(static_cast<int>(id & 15u)), g(static_cast<int>(id >> 4 & 3u)) {
+        const unsigned of_all = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u);
+        wave = static_cast<int>(of_all % (DP / 16u));
+        role = static_cast<int>(of_all / (DP / 16u));
+        col = 16 * wave + r;
+        key_row = static_cast<int>((id & 1023u) / (DP / 8u));
+        key_col = static_cast<int>(8 * (id % (DP / 8u)));
+    }
+    __device__ Place() : Place(threadIdx.x) {}
+    // The same, made anew: what follows from it is worked out, and read from LDS, where it
+    // is used, rather than held in registers from an earlier use.
+    static __device__ Place anew() {
+        unsigned id = threadIdx.x;
+        asm volatile("" : "+v"(id));
+        return Place(id);
+    }
+};
+
+// Eight elements of each of a chunk's tokens that a thread loads of one tensor.  A row
+// from n on, and a column outside the head, reads as zero.
+template <typename T, int DP, int CH, bool WIDE, int ROLES = 1>
 struct Piece {
     using In = Rows<T, WIDE>;
-    static constexpr int kPieces = CH / 32;
+    using At = Place<DP, ROLES>;
+    static constexpr int kPieces = CH / At::kRows;
     std::uint32_t w[kPieces][In::kWords];
     __device__ void fetch(const Heads<T>& from, std::uint32_t dim, std::uint32_t start, int n, std::uint32_t env,
-                          std::uint32_t h, const Lane<DP>& at) {
+                          std::uint32_t h, const At& at) {
         const In rows(from.row(start, env, h), from.t);
 #pragma unroll
         for (int p = 0; p < kPieces; ++p) {
-            const int row = at.key_row + 32 * p;
+            const int row = at.key_row + At::kRows * p;
             rows.get8(row < n && at.key_col < static_cast<int>(dim), row, at.key_col, from.vec, w[p]);
         }
     }
     template <typename Tile>
-    __device__ void stage(Tile& to, const Lane<DP>& at) const {
+    __device__ void stage(Tile& to, const At& at) const {
 #pragma unroll
-        for (int p = 0; p < kPieces; ++p) to.put8(at.key_row + 32 * p, at.key_col, w[p]);
+        for (int p = 0; p < kPieces; ++p) to.put8(at.key_row + At::kRows * p, at.key_col, w[p]);
     }
     // Zeros in the rows from n on.
-    __device__ void cut(int n, const Lane<DP>& at) {
+    __device__ void cut(int n, const At& at) {
 #pragma unroll
         for (int p = 0; p < kPieces; ++p)
 #pragma unroll
-            for (int i = 0; i < In::kWords; ++i) w[p][i] = at.key_row + 32 * p < n ? w[p][i] : 0;
+            for (int i = 0; i < In::kWords; ++i) w[p][i] = at.key_row + At::kRows * p < n ? w[p][i] : 0;
     }
     // And in the rows before n.
-    __device__ void cut_before(int n, const Lane<DP>& at) {
+    __device__ void cut_before(int n, const At& at) {
 #pragma unroll
         for (int p = 0; p < kPieces; ++p)
 #pragma unroll
-            for (int i = 0; i < In::kWords; ++i) w[p][i] = at.key_row + 32 * p >= n ? w[p][i] : 0;
+            for (int i = 0; i < In::kWords; ++i) w[p][i] = at.key_row + At::kRows * p >= n ? w[p][i] : 0;
     }
     // Tokens with something that is not finite.
-    __device__ std::uint64_t odd(const Lane<DP>& at) const {
+    __device__ std::uint64_t odd(const At& at) const {
         using s2 = unsigned short __attribute__((ext_vector_type(2)));
         std::uint64_t bits = 0;
 #pragma unroll
@@ -153,30 +184,35 @@ struct Piece {
                 else most = __builtin_bit_cast(std::uint32_t, __builtin_elementwise_max(
                                 __builtin_bit_cast(s2, most), __builtin_bit_cast(s2, w[p][i] & 0x7fff7fffu)));
             if constexpr (sizeof(T) == 2) most = max(most >> 16, most & 0xffffu);
-            if (most >= (sizeof(T) == 4 ? 0x7f800000u : 0x7f80u)) bits |= 1ull << (at.key_row + 32 * p);
+            if (most >= (sizeof(T) == 4 ? 0x7f800000u : 0x7f80u)) bits |= 1ull << (at.key_row + At::kRows * p);
         }
         return bits;
     }
 };
 
-// Bit t: the state is dropped before token start + t of the n from start on.
-template <int CH, typename T>
-__device__ std::uint64_t drops_of(const DecayArgs<T>& a, std::uint32_t start, int n, std::uint32_t env, int lane, bool always) {
-    if (always) return n < 64 ? (1ull << n) - 1 : ~0ull;
-    if (a.resets == nullptr) return 0;
-    const bool mine = lane < n;
-    return __ballot(mine && a.resets[(start + static_cast<std::size_t>(mine ? lane : 0)) * a.batch + env] != 0);
-}
+// Ends of episodes among a chunk's tokens, one a lane, fetched ahead: nothing here waits
+// for the load before drops().
+template <typename T>
+struct Resets {
+    std::uint32_t mine = 0;
+    __device__ void fetch(const DecayArgs<T>& a, std::uint32_t start, int n, std::uint32_t env, int lane) {
+        if (a.resets != nullptr) mine = a.resets[(start + static_cast<std::size_t>(min(lane, n - 1))) * a.batch + env];
+    }
+    // Bit t: the state is dropped before token t of the n.
+    __device__ std::uint64_t drops(int n, int lane, bool always) const { return __ballot(lane < n && (always || mine != 0)); }
+};
 
 // exp(n g) of a head, n = 0 .. CH: made once by a workgroup.  exp of the rounded
 // product is off by |n g| 2^-24 of itself, which is 2^-25 of 1 at most where g <= 0.
 template <int CH>
 struct Powers {
-    // up[i] = a^(i + 1), down[i] = a^(CH - 1 - i), with room past either end.
-    alignas(16) float up[CH], down[CH + 4];
-    __device__ void make(float g, bool always, int tid) {
+    // up[i] = a^(i + 1), read[i] = scale a^(i + 1), down[i] = a^(CH - 1 - i), with room
+    // past its end.
+    alignas(16) float up[CH], read[CH], down[CH + 4];
+    __device__ void make(float g, float scale, bool always, int tid) {
         if (tid < CH) {
             up[tid] = always ? 0.0f : expf(static_cast<float>(tid + 1) * g);
+            read[tid] = up[tid] * scale;
             down[tid] = tid == CH - 1 ? 1.0f : always ? 0.0f : expf(static_cast<float>(CH - 1 - tid) * g);
         }
         if (tid < 4) down[CH + tid] = 1.0f;
@@ -196,10 +232,11 @@ struct Seen {
     }
     // Episodes that ended up to token i: two tokens see each other where these agree.
     __device__ int episode(int i) const { return __popcll(drops & (~0ull >> (63 - i))); }
-    // Of the four rows from `row` on: the decay from before the chunk, and to its end.
+    // Of the four rows from `row` on: the decay from before the chunk times the scale, and
+    // the decay to its end.
     template <int CH>
     __device__ f4 in(const Powers<CH>& p, int row) const {
-        f4 v = *reinterpret_cast<const f4*>(p.up + row);
+        f4 v = *reinterpret_cast<const f4*>(p.read + row);
         if (drops != 0)
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = row + e < first ? v[e] : 0.0f;
@@ -265,13 +302,14 @@ struct PairPowers {
 
 // Results [tokens][dim] of the inputs' type, a wave's 16 columns at a time: float32
 // from the registers, 64 bytes of a row together.
-template <typename T, int DP, int CH>
+template <typename T, int DP, int CH, int ROLES = 1>
 struct DecayResults {
+    using At = Place<DP, ROLES>;
     // A finished tile, as it waits for its place.
     using Tile = f4;
     static __device__ Tile tile(f4 x) { return x; }
     template <bool WIDE>
-    static __device__ void put_tile(const Rows<T, WIDE>& to, int dim, int n, const Lane<DP>& at, int m, f4 x) {
+    static __device__ void put_tile(const Rows<T, WIDE>& to, int dim, int n, const At& at, int m, f4 x) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int row = 16 * m + 4 * at.g + e;
@@ -279,33 +317,34 @@ struct DecayResults {
         }
     }
     template <bool WIDE>
-    __device__ void put(const Rows<T, WIDE>& to, int dim, int n, const Lane<DP>& at, const Tile (&x)[CH / 16]) {
+    __device__ void put(const Rows<T, WIDE>& to, int dim, int n, const At& at, const Tile (&x)[CH / 16]) {
 #pragma unroll
         for (int m = 0; m < CH / 16; ++m) put_tile(to, dim, n, at, m, x[m]);
     }
     template <bool WIDE>
-    __device__ void flush(const Rows<T, WIDE>&, int, int, const Lane<DP>&) const {}
+    __device__ void flush(const Rows<T, WIDE>&, int, int, const At&) const {}
 };
 // bfloat16: two bytes a lane would be 32 of a row, so through LDS ([column][token])
 // and, after a barrier, eight elements of a token a lane by transposing reads: a
 // wave's block is 16 tokens of 32 columns.
-template <int DP, int CH>
-struct DecayResults<bf16, DP, CH> {
+template <int DP, int CH, int ROLES>
+struct DecayResults<bf16, DP, CH, ROLES> {
+    using At = Place<DP, ROLES>;
     static constexpr int kRow = CH + 8;
     alignas(16) std::uint16_t d[DP * kRow];
     using Tile = u2;
     static __device__ Tile tile(f4 x) { return u2{pack_bf16(x.x, x.y), pack_bf16(x.z, x.w)}; }
     template <bool WIDE>
-    __device__ void put(const Rows<bf16, WIDE>&, int, int, const Lane<DP>& at, const Tile (&x)[CH / 16]) {
+    __device__ void put(const Rows<bf16, WIDE>&, int, int, const At& at, const Tile (&x)[CH / 16]) {
 #pragma unroll
         for (int m = 0; m < CH / 16; ++m) *reinterpret_cast<u2*>(&d[at.col * kRow + 16 * m + 4 * at.g]) = x[m];
     }
     template <bool WIDE>
-    __device__ void flush(const Rows<bf16, WIDE>& to, int dim, int n, const Lane<DP>& at) const {
+    __device__ void flush(const Rows<bf16, WIDE>& to, int dim, int n, const At& at) const {
         using s4 = short __attribute__((ext_vector_type(4)));
         using lds = __attribute__((address_space(3))) s4;
 #pragma unroll
-        for (int p = 0; p < CH / 32; ++p) {
+        for (int p = at.role; p < CH / 32; p += ROLES) {
             const int token = 32 * p + 16 * (at.wave % 2), col = 32 * (at.wave / 2) + 8 * at.g;
             const std::uint16_t* from = &d[(col + at.r / 4) * kRow + token + 4 * (at.r % 4)];
             const u2 a = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)from));
@@ -318,22 +357,22 @@ struct DecayResults<bf16, DP, CH> {
 // ---- a wave's slab of a state -----------------------------------------------------
 // Four consecutive float32 along a row of [k_dim][v_dim] a lane: tile i holds
 // C[x = value 16 i + 4 g + e][y = key 16 wave + r].
-template <int DP>
-__device__ void load_key_slab(const float* from, int dk, int dv, const Lane<DP>& at, f4 (&S)[DP / 16]) {
+template <int DP, typename At>
+__device__ void load_key_slab(const float* from, int dk, int dv, const At& at, f4 (&S)[DP / 16]) {
     const Rows<float, false> x(from, dv);
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i)
         S[i] = from == nullptr ? f4{0, 0, 0, 0} : x.get4(at.col < dk && 16 * i + 4 * at.g < dv, at.col, 16 * i + 4 * at.g);
 }
-template <int DP>
-__device__ void store_key_slab(float* to, int dk, int dv, const Lane<DP>& at, const f4 (&S)[DP / 16]) {
+template <int DP, typename At>
+__device__ void store_key_slab(float* to, int dk, int dv, const At& at, const f4 (&S)[DP / 16]) {
     const Rows<float, false> x(to, dv);
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) x.put4(at.col < dk && 16 * i + 4 * at.g < dv, at.col, 16 * i + 4 * at.g, S[i]);
 }
 // Tile i holds C[x = key 16 i + 4 g + e][y = value 16 wave + r].
-template <int DP>
-__device__ void load_value_slab(const float* from, int dk, int dv, const Lane<DP>& at, f4 (&S)[DP / 16]) {
+template <int DP, typename At>
+__device__ void load_value_slab(const float* from, int dk, int dv, const At& at, f4 (&S)[DP / 16]) {
     const Rows<float, false> x(from, dv);
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i)
@@ -343,8 +382,8 @@ __device__ void load_value_slab(const float* from, int dk, int dv, const Lane<DP
             S[i][e] = from == nullptr ? 0.0f : x.value_of(x.get(at.col < dv && row < dk, row, at.col));
         }
 }
-template <int DP>
-__device__ void store_value_slab(float* to, int dk, int dv, const Lane<DP>& at, const f4 (&S)[DP / 16]) {
+template <int DP, typename At>
+__device__ void store_value_slab(float* to, int dk, int dv, const At& at, const f4 (&S)[DP / 16]) {
     const Rows<float, false> x(to, dv);
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i)

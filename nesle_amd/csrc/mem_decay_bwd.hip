@@ -17,9 +17,10 @@
 // tokens' places would be equal, but cancel).
 //
 // One workgroup walks one head of one console, a wave for 16 columns of each of dQ,
-// dK and dV.  dS is needed by key columns (dK) and by value columns (dV): a wave
-// holds both slabs of it in registers and updates both, which costs a product more
-// and saves passing it through LDS.
+// dK and dV, or two waves: one has dQ and the pairs, the other dK, dV and dS.  dS is
+// needed by key columns (dK) and by value columns (dV): a wave holds both slabs of it in
+// registers and updates both, which costs a product more and saves passing it through
+// LDS.
 //
 // Inputs come and results go a chunk at a time, and the forward kept one state a
 // chunk; inside, the work goes in parts of 32 tokens, last to first, as pairs of
@@ -36,35 +37,43 @@ namespace {
 
 constexpr int kPart = 32;
 
-template <typename T, int DP, int CH>
+// Two waves for 16 columns where their registers leave room for it.
+template <int DP>
+constexpr int kGradRoles = DP == 128 ? 1 : 2;
+
+// Waves of a SIMD that registers are to leave room for: what LDS does.
+template <typename T, int DP>
+constexpr int kGradWaves = sizeof(T) == 2 && DP <= 64 ? 4 : 2;
+
+template <typename T, int DP>
 struct GradTile {
+    static constexpr int CH = kDecaySpan<T, DP>, ROLES = kGradRoles<DP>;
     using M = DecayMath<T>;
     using In = typename M::template Tile<CH, DP, M::kIn, 8>;
     union Out {
         In in;
-        DecayResults<T, DP, CH> results;
+        DecayResults<T, DP, CH, ROLES> results;
     };
     Out q, k, v;               // then dQ, dK, dV
     In dout;
     typename M::template Tile<kPart, kPart, kFull, 8> p, r;        // [j][i]; zero where i is in an earlier tile
+    f4 before[ROLES == 1 ? 1 : DP / 16][DP / 16][64];              // the state before a part, from role to role
     Powers<kPart> powers;
     alignas(16) int episodes[kPart];
-    float sums[DP / 16];
+    float sums[ROLES * DP / 16];
 };
 
-// Waves of a SIMD that registers are to leave room for: what LDS does.
-template <typename T, int DP>
-constexpr int kGradWaves = sizeof(T) == 2 && DP <= 64 ? 3 : 2;
-
-template <typename T, int DP, bool WIDE>
-__global__ void __launch_bounds__(DP * 4, (kGradWaves<T, DP>)) decay_backward_kernel(DecayArgs<T> a, DecaySegments seg, float* partials) {
-    constexpr int CH = kDecayChunk<T>, PARTS = CH / kPart, KT = DP / 16, KP = DP / 32, kWaves = DP / 16;
-    using Tile = GradTile<T, DP, CH>;
+// The walk of a wave that has dQ and the pairs, dK, dV and dS, or both.  The waves of
+// either kind meet at the same barriers.
+template <typename T, int DP, bool WIDE, bool HAS_Q, bool HAS_KV>
+__device__ __forceinline__ void grad_walk(const DecayArgs<T>& a, const DecaySegments& seg, float* partials, GradTile<T, DP>& sh) {
+    using Tile = GradTile<T, DP>;
+    constexpr int CH = Tile::CH, ROLES = Tile::ROLES, PARTS = CH / kPart, KT = DP / 16, KP = DP / 32, CT = kPart / 16, kWaves = DP / 16;
     using M = typename Tile::M;
     using In = Rows<T, WIDE>;
-    using Done = DecayResults<T, DP, CH>;
-    __shared__ Tile sh;
-    const Lane<DP> first;
+    using At = Place<DP, ROLES>;
+    using Done = DecayResults<T, DP, CH, ROLES>;
+    const At first;
     const std::uint32_t env = blockIdx.x / a.hv, h = blockIdx.x % a.hv, hk = h / a.group;
     const std::size_t head = blockIdx.x, state_size = static_cast<std::size_t>(a.dk_dim) * a.dv_dim;
     const std::size_t slot = static_cast<std::size_t>(blockIdx.y) * gridDim.x + head;
@@ -74,52 +83,48 @@ __global__ void __launch_bounds__(DP * 4, (kGradWaves<T, DP>)) decay_backward_ke
     const std::uint32_t begin = blockIdx.y * seg.steps;
     const std::uint32_t end = a.steps - begin < seg.steps ? a.steps : begin + seg.steps;
 
-    const float gate = a.steps != 0 ? a.g[h] : 0.0f;
-    const bool always = gate < kDropBelow;
-    sh.powers.make(gate, always, first.tid);
-    if (first.tid < 64)
-        for (int i = 0; i < 4; ++i) {
-            sh.p.put(16 + 4 * first.g + i, first.r, 0.0f);
-            sh.r.put(16 + 4 * first.g + i, first.r, 0.0f);
-        }
-    f4 by_key[KT], by_value[KT];           // dS
-    {
-        const float* from = seg.count > 1 ? seg.states + slot * state_size
-                                          : a.dstate_out == nullptr ? nullptr : a.dstate_out + head * state_size;
-        load_key_slab<DP>(from, dk_dim, dv_dim, first, by_key);
-        load_value_slab<DP>(from, dk_dim, dv_dim, first, by_value);
-    }
-
-    Piece<T, DP, CH, WIDE> q, k, v, dout;
-    std::uint64_t next_drops = 0;
-    const auto fetch = [&](std::uint32_t t1, const Lane<DP>& at) {
+    Piece<T, DP, CH, WIDE, ROLES> q, k, v, dout;
+    Resets<T> resets;
+    f4 next[KT];                           // the state before the chunk
+    const auto fetch = [&](std::uint32_t t1, const At& at) {
         const std::uint32_t start = (t1 - 1) / CH * CH;
         const int n = static_cast<int>(t1 - start);
         q.fetch(a.q, a.dk_dim, start, n, env, hk, at);
         k.fetch(a.k, a.dk_dim, start, n, env, hk, at);
         v.fetch(a.v, a.dv_dim, start, n, env, h, at);
         dout.fetch(a.dout, a.dv_dim, start, n, env, h, at);
-        next_drops = drops_of<CH>(a, start, n, env, at.lane, always);
+        resets.fetch(a, start, n, env, at.lane);
+        const float* from = start == 0 ? (a.state == nullptr ? nullptr : a.state + head * state_size)
+                                       : a.saved + ((start / CH - 1) * static_cast<std::size_t>(a.batch) * a.hv + head) * state_size;
+        if constexpr (HAS_Q) load_key_slab<DP>(from, dk_dim, dv_dim, at, next);
     };
     if (begin < end) fetch(end, first);
+    f4 by_key[KT], by_value[KT];           // dS
+    if constexpr (HAS_KV) {
+        const float* from = seg.count > 1 ? seg.states + slot * state_size
+                                          : a.dstate_out == nullptr ? nullptr : a.dstate_out + head * state_size;
+        load_key_slab<DP>(from, dk_dim, dv_dim, first, by_key);
+        load_value_slab<DP>(from, dk_dim, dv_dim, first, by_value);
+    }
+    const float gate = a.steps != 0 ? a.g[h] : 0.0f;
+    const bool always = gate < kDropBelow;
+    sh.powers.make(gate, a.scale, always, first.tid);
+    if (first.tid < 64)
+        for (int i = 0; i < 4; ++i) {
+            sh.p.put(16 + 4 * first.g + i, first.r, 0.0f);
+            sh.r.put(16 + 4 * first.g + i, first.r, 0.0f);
+        }
+
     float decay = 0.0f;                    // this lane's share of the decay's gradient
     for (std::uint32_t t1 = end; t1 > begin;) {
-        // Made anew for each step of the work: what one has read from LDS is read again
-        // by the next, rather than held in registers through both.
-        Lane<DP> at = Lane<DP>::anew();
-        int r = at.r, g = at.g;
-        const auto anew = [&] {
-            at = Lane<DP>::anew();
-            r = at.r;
-            g = at.g;
-        };
+        At at = At::anew();
         const std::uint32_t start = (t1 - 1) / CH * CH;
         const int n = static_cast<int>(t1 - start);
-        const std::uint64_t drops = next_drops;
-        const float* from = (drops & 1u) ? nullptr : start == 0 ? (a.state == nullptr ? nullptr : a.state + head * state_size)
-                                         : a.saved + ((start / CH - 1) * static_cast<std::size_t>(a.batch) * a.hv + head) * state_size;
+        const std::uint64_t drops = resets.drops(n, at.lane, always);
         f4 S[KT];
-        load_key_slab<DP>(from, dk_dim, dv_dim, at, S);
+#pragma unroll
+        for (int i = 0; i < KT; ++i)
+            if constexpr (HAS_Q) S[i] = (drops & 1u) ? zero : next[i];
         q.stage(sh.q.in, at);
         k.stage(sh.k.in, at);
         v.stage(sh.v.in, at);
@@ -134,70 +139,95 @@ __global__ void __launch_bounds__(DP * 4, (kGradWaves<T, DP>)) decay_backward_ke
         const auto share = [&](bool of_k, int m, f4 x) {
             if (a.group == 1) return;
             const Rows<float, WIDE> to(a.scratch + (of_k ? a.steps * share_step : 0) + (token * a.hv + h) * a.dk_dim, share_step);
-            DecayResults<float, DP, CH>::put_tile(to, dk_dim, n, at, m, x);
+            DecayResults<float, DP, CH, ROLES>::put_tile(to, dk_dim, n, at, m, x);
         };
 
 #pragma unroll
         for (int part = PARTS - 1; part >= 0; --part) {
-            constexpr int CT = kPart / 16;
-            const int row0 = kPart * part;
+            const int row0 = kPart * part, tile0 = row0 / 16;
             const std::uint32_t mine = static_cast<std::uint32_t>(drops >> row0);
             const bool dropped = mine & 1u;        // the state before the part is
             const Seen seen(mine & ~1u, min(n - row0, kPart));
             if (PARTS > 1 && n <= row0) {
 #pragma unroll
-                for (int m = 0; m < CT; ++m) done_q[row0 / 16 + m] = done_k[row0 / 16 + m] = done_v[row0 / 16 + m] = Done::tile(zero);
+                for (int m = 0; m < CT; ++m) done_q[tile0 + m] = done_k[tile0 + m] = done_v[tile0 + m] = Done::tile(zero);
                 continue;
             }
-            anew();
-            if (seen.drops != 0 && at.tid < kPart) sh.episodes[at.tid] = seen.episode(at.tid);
-            if (seen.drops != 0) __syncthreads();
-            // P and R, a tile a wave; the workgroups of a compute unit leave out
-            // different waves.
-            for (int place = (at.wave + static_cast<int>(blockIdx.x)) % kWaves; place < 3; place += kWaves) {
-                const int it = place == 0 ? 0 : 1, jt = place == 2 ? 1 : 0;
-                f4 x = zero, y = zero;
+            at = At::anew();
+            const int r = at.r, g = at.g;
+            if (seen.drops != 0) {
+                if (at.tid < kPart) sh.episodes[at.tid] = seen.episode(at.tid);
+                __syncthreads();
+            }
+            const float whole = seen.whole(sh.powers), row4 = static_cast<float>(4 * g);
+            f4 before[KT], dK[CT] = {}, dV[CT] = {};
+            if constexpr (HAS_Q) {
+                // P and R, a tile a wave; the workgroups of a compute unit leave out
+                // different waves.
+                for (int place = (at.wave + static_cast<int>(blockIdx.x)) % kWaves; place < 3; place += kWaves) {
+                    const int it = place == 0 ? 0 : 1, jt = place == 2 ? 1 : 0;
+                    f4 x = zero, y = zero;
+#pragma unroll
+                    for (int i = 0; i < KP; ++i) {
+                        x = M::mul(sh.q.in.rows(row0 + 16 * it, i, r, g), sh.k.in.rows(row0 + 16 * jt, i, r, g), x);
+                        y = M::mul(sh.dout.rows(row0 + 16 * it, i, r, g), sh.v.in.rows(row0 + 16 * jt, i, r, g), y);
+                    }
+                    PairPowers<kPart, true> pair;
+                    pair.make(sh.powers, a.scale, r, g);
+                    x = pair.weigh(x, it, jt, seen, sh.episodes, r, g);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) decay += (row4 + static_cast<float>(16 * (it - jt) + e - r)) * x[e] * y[e];
+                    y = pair.weigh(y, it, jt, seen, sh.episodes, r, g);
+                    sh.p.put4(16 * jt + r, 16 * it + 4 * g, x);
+                    sh.r.put4(16 * jt + r, 16 * it + 4 * g, y);
+                }
+                // The state before the part.
+                if (part == 0) {
+#pragma unroll
+                    for (int i = 0; i < KT; ++i) before[i] = S[i];
+                } else {
+                    const Seen ahead(drops & 0xffffffffu, kPart);
+                    const float through = ahead.whole(sh.powers);
+                    f4 K[2];
+                    M::values(sh.k.in.cols(0, 16 * at.wave, r, g), K);
+                    const auto held = M::full(K[0] * ahead.out(sh.powers, 4 * g), K[1] * ahead.out(sh.powers, 16 + 4 * g));
+#pragma unroll
+                    for (int i = 0; i < KT; ++i) before[i] = dropped ? zero : M::mul(sh.v.in.cols(0, 16 * i, r, g), held, S[i] * through);
+                }
+                if (ROLES > 1 && partials != nullptr)
+#pragma unroll
+                    for (int i = 0; i < KT; ++i) sh.before[at.wave][i][at.lane] = before[i];
+            }
+            if constexpr (HAS_KV) {
+                // dK and dV from the tokens after the part.
 #pragma unroll
                 for (int i = 0; i < KP; ++i) {
-                    x = M::mul(sh.q.in.rows(row0 + 16 * it, i, r, g), sh.k.in.rows(row0 + 16 * jt, i, r, g), x);
-                    y = M::mul(sh.dout.rows(row0 + 16 * it, i, r, g), sh.v.in.rows(row0 + 16 * jt, i, r, g), y);
+                    const auto s = M::full(by_key[2 * i], by_key[2 * i + 1]);
+#pragma unroll
+                    for (int m = 0; m < CT; ++m) dK[m] = M::mul(sh.v.in.rows(row0 + 16 * m, i, r, g), s, dK[m]);
                 }
-                PairPowers<kPart, true> pair;
-                pair.make(sh.powers, a.scale, r, g);
-                x = pair.weigh(x, it, jt, seen, sh.episodes, r, g);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) decay += static_cast<float>(16 * (it - jt) + 4 * g + e - r) * x[e] * y[e];
-                y = pair.weigh(y, it, jt, seen, sh.episodes, r, g);
-                sh.p.put4(16 * jt + r, 16 * it + 4 * g, x);
-                sh.r.put4(16 * jt + r, 16 * it + 4 * g, y);
-            }
-            // The state before the part.
-            f4 before[KT];
-            if (part == 0) {
+                for (int i = 0; i < KP; ++i) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    const auto s = M::full(by_value[2 * i], by_value[2 * i + 1]);
 #pragma unroll
-                for (int i = 0; i < KT; ++i) before[i] = S[i];
-            } else {
-                const Seen ahead(drops & 0xffffffffu, kPart);
-                const float whole = ahead.whole(sh.powers);
-                f4 K[2];
-                M::values(sh.k.in.cols(0, 16 * at.wave, r, g), K);
-                const auto held = M::full(K[0] * ahead.out(sh.powers, 4 * g), K[1] * ahead.out(sh.powers, 16 + 4 * g));
+                    for (int m = 0; m < CT; ++m) dV[m] = M::mul(sh.k.in.rows(row0 + 16 * m, i, r, g), s, dV[m]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                f4 K[CT];
+                M::values(sh.k.in.cols(row0, 16 * at.wave, r, g), K);
 #pragma unroll
-                for (int i = 0; i < KT; ++i) before[i] = dropped ? zero : M::mul(sh.v.in.cols(0, 16 * i, r, g), held, S[i] * whole);
-            }
-            const float whole = seen.whole(sh.powers);
-            {
-                float held = 0.0f;
+                for (int m = 0; m < CT; ++m) {
+                    const f4 out = seen.out(sh.powers, 16 * m + 4 * g);
+                    dK[m] *= out;
+                    dV[m] *= out;
 #pragma unroll
-                for (int i = 0; i < KT; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) held += by_key[i][e] * before[i][e];
-                decay += static_cast<float>(seen.n) * whole * held;
+                    for (int e = 0; e < 4; ++e) decay += (static_cast<float>(seen.n - 1 - 16 * m - e) - row4) * K[m][e] * dK[m][e];
+                }
             }
             __syncthreads();
-
-            // dQ: from the tokens before the part, then within.
-            {
+            if constexpr (HAS_Q) {
+                // dQ: from the tokens before the part, then within.
                 f4 x[CT] = {}, Q[CT];
 #pragma unroll
                 for (int i = 0; i < KP; ++i) {
@@ -209,80 +239,68 @@ __global__ void __launch_bounds__(DP * 4, (kGradWaves<T, DP>)) decay_backward_ke
                 const auto key = sh.k.in.cols(row0, 16 * at.wave, r, g);
 #pragma unroll
                 for (int m = 0; m < CT; ++m) {
-                    x[m] *= seen.in(sh.powers, 16 * m + 4 * g) * a.scale;
+                    x[m] *= seen.in(sh.powers, 16 * m + 4 * g);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) decay += static_cast<float>(16 * m + 4 * g + e + 1) * Q[m][e] * x[m][e];
+                    for (int e = 0; e < 4; ++e) decay += (row4 + static_cast<float>(16 * m + e + 1)) * Q[m][e] * x[m][e];
                     x[m] = M::mul(sh.r.cols(0, 16 * m, r, g), key, x[m]);
-                    share(false, row0 / 16 + m, x[m]);
-                    done_q[row0 / 16 + m] = Done::tile(x[m]);
+                    share(false, tile0 + m, x[m]);
+                    done_q[tile0 + m] = Done::tile(x[m]);
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
-            anew();
-            // dK: from the tokens after the part, then within; the slab of dS that it reads.
-            {
-                f4 x[CT] = {}, K[CT], Q[CT];
+            if constexpr (HAS_KV) {
+                if (partials != nullptr) {
+                    float held = 0.0f;
 #pragma unroll
-                for (int i = 0; i < KP; ++i) {
-                    const auto s = M::full(by_key[2 * i], by_key[2 * i + 1]);
+                    for (int i = 0; i < KT; ++i) {
+                        const f4 s = ROLES > 1 ? sh.before[at.wave][i][at.lane] : before[i];
 #pragma unroll
-                    for (int m = 0; m < CT; ++m) x[m] = M::mul(sh.v.in.rows(row0 + 16 * m, i, r, g), s, x[m]);
+                        for (int e = 0; e < 4; ++e) held += by_key[i][e] * s[e];
+                    }
+                    decay += static_cast<float>(seen.n) * whole * held;
                 }
-                M::values(sh.k.in.cols(row0, 16 * at.wave, r, g), K);
+                // dK and dV within the part, and the two slabs of dS before it.
+                f4 x[CT];
                 const auto query = sh.q.in.cols(row0, 16 * at.wave, r, g);
-                M::values(query, Q);
+                M::values(query, x);
 #pragma unroll
                 for (int m = 0; m < CT; ++m) {
-                    x[m] *= seen.out(sh.powers, 16 * m + 4 * g);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) decay += static_cast<float>(seen.n - 1 - (16 * m + 4 * g + e)) * K[m][e] * x[m][e];
-                    x[m] = M::mul(sh.r.rows(16 * m, 0, r, g), query, x[m]);
-                    share(true, row0 / 16 + m, x[m]);
-                    done_k[row0 / 16 + m] = Done::tile(x[m]);
-                    Q[m] *= seen.in(sh.powers, 16 * m + 4 * g) * a.scale;
+                    dK[m] = M::mul(sh.r.rows(16 * m, 0, r, g), query, dK[m]);
+                    share(true, tile0 + m, dK[m]);
+                    done_k[tile0 + m] = Done::tile(dK[m]);
+                    x[m] *= seen.in(sh.powers, 16 * m + 4 * g);
                 }
-                const auto read = M::full(Q[0], Q[1]);
+                {
+                    const auto read = M::full(x[0], x[1]);
 #pragma unroll
-                for (int i = 0; i < KT; ++i)
-                    by_key[i] = dropped ? zero : M::mul(sh.dout.cols(row0, 16 * i, r, g), read, by_key[i] * whole);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            anew();
-            // dV, the same.
-            {
-                f4 x[CT] = {}, dO[CT];
-#pragma unroll
-                for (int i = 0; i < KP; ++i) {
-                    const auto s = M::full(by_value[2 * i], by_value[2 * i + 1]);
-#pragma unroll
-                    for (int m = 0; m < CT; ++m) x[m] = M::mul(sh.k.in.rows(row0 + 16 * m, i, r, g), s, x[m]);
+                    for (int i = 0; i < KT; ++i)
+                        by_key[i] = dropped ? zero : M::mul(sh.dout.cols(row0, 16 * i, r, g), read, by_key[i] * whole);
                 }
+                __builtin_amdgcn_sched_barrier(0);
                 const auto grad = sh.dout.cols(row0, 16 * at.wave, r, g);
-                M::values(grad, dO);
+                M::values(grad, x);
 #pragma unroll
                 for (int m = 0; m < CT; ++m) {
-                    x[m] *= seen.out(sh.powers, 16 * m + 4 * g);
-                    x[m] = M::mul(sh.p.rows(16 * m, 0, r, g), grad, x[m]);
-                    done_v[row0 / 16 + m] = Done::tile(x[m]);
-                    dO[m] *= seen.in(sh.powers, 16 * m + 4 * g) * a.scale;
+                    dV[m] = M::mul(sh.p.rows(16 * m, 0, r, g), grad, dV[m]);
+                    done_v[tile0 + m] = Done::tile(dV[m]);
+                    x[m] *= seen.in(sh.powers, 16 * m + 4 * g);
                 }
-                const auto read = M::full(dO[0], dO[1]);
+                __builtin_amdgcn_sched_barrier(0);
+                const auto read = M::full(x[0], x[1]);
 #pragma unroll
                 for (int i = 0; i < KT; ++i)
                     by_value[i] = dropped ? zero : M::mul(sh.q.in.cols(row0, 16 * i, r, g), read, by_value[i] * whole);
             }
-            __builtin_amdgcn_sched_barrier(0);
             __syncthreads();               // P, R and, in the end, the inputs have been read
         }
         const std::int64_t key_step = static_cast<std::int64_t>(a.batch) * a.hk * a.dk_dim;
         const In dq(a.dq + (token * a.hk + hk) * a.dk_dim, key_step), dk(a.dk + (token * a.hk + hk) * a.dk_dim, key_step),
             dv(a.dv + static_cast<std::int64_t>(start) * v_step + head * a.dv_dim, v_step);
-        anew();
-        if (a.group == 1) {
-            sh.q.results.put(dq, dk_dim, n, at, done_q);
-            sh.k.results.put(dk, dk_dim, n, at, done_k);
+        at = At::anew();
+        if (HAS_Q && a.group == 1) sh.q.results.put(dq, dk_dim, n, at, done_q);
+        if constexpr (HAS_KV) {
+            if (a.group == 1) sh.k.results.put(dk, dk_dim, n, at, done_k);
+            sh.v.results.put(dv, dv_dim, n, at, done_v);
         }
-        sh.v.results.put(dv, dv_dim, n, at, done_v);
         __syncthreads();
         if (a.group == 1) {
             sh.q.results.flush(dq, dk_dim, n, at);
@@ -291,17 +309,25 @@ __global__ void __launch_bounds__(DP * 4, (kGradWaves<T, DP>)) decay_backward_ke
         sh.v.results.flush(dv, dv_dim, n, at);
         __syncthreads();                   // before the next chunk takes their place
     }
-    if (a.dstate != nullptr && begin == 0) store_key_slab<DP>(a.dstate + head * state_size, dk_dim, dv_dim, Lane<DP>::anew(), by_key);
+    if (HAS_KV && a.dstate != nullptr && begin == 0) store_key_slab<DP>(a.dstate + head * state_size, dk_dim, dv_dim, At::anew(), by_key);
     if (partials != nullptr) {
         decay = over_groups(sum16(decay));
-        if (first.lane == 0) sh.sums[first.wave] = decay;
+        if (first.lane == 0) sh.sums[first.role * kWaves + first.wave] = decay;
         __syncthreads();
         if (first.tid == 0) {
             float sum = 0.0f;
-            for (int w = 0; w < kWaves; ++w) sum += sh.sums[w];
+            for (int w = 0; w < ROLES * kWaves; ++w) sum += sh.sums[w];
             partials[slot] = sum;
         }
     }
+}
+
+template <typename T, int DP, bool WIDE>
+__global__ void __launch_bounds__(DP * 4 * kGradRoles<DP>, (kGradWaves<T, DP>)) decay_backward_kernel(DecayArgs<T> a, DecaySegments seg, float* partials) {
+    __shared__ GradTile<T, DP> sh;
+    if constexpr (kGradRoles<DP> == 1) grad_walk<T, DP, WIDE, true, true>(a, seg, partials, sh);
+    else if (Place<DP, kGradRoles<DP>>().role == 0) grad_walk<T, DP, WIDE, true, false>(a, seg, partials, sh);
+    else grad_walk<T, DP, WIDE, false, true>(a, seg, partials, sh);
 }
 
 // dg of a head: the sum of its workgroups' shares, a workgroup a head.
@@ -339,7 +365,8 @@ std::uint64_t share_floats(const nesle_decay_args& a) {
 template <typename T, int DP, bool WIDE>
 void launch_dim(const DecayArgs<T>& a, const DecaySegments& seg, float* partials, hipStream_t s) {
     if (seg.count > 1) launch_states<T, DP, WIDE, true>(a, seg, s);
-    hipLaunchKernelGGL((decay_backward_kernel<T, DP, WIDE>), dim3(a.batch * a.hv, seg.count), dim3(DP * 4), 0, s, a, seg, partials);
+    hipLaunchKernelGGL((decay_backward_kernel<T, DP, WIDE>), dim3(a.batch * a.hv, seg.count), dim3(DP * 4 * kGradRoles<DP>), 0, s, a, seg,
+                       partials);
 }
 
 template <typename T>

@@ -47,11 +47,11 @@ __device__ bool finite(const f4 (&S)[KT]) {
 
 template <typename T, int DP, bool WIDE>
 __global__ void __launch_bounds__(DP * 4, kForwardWaves<DP>) decay_forward_kernel(DecayArgs<T> a, DecaySegments seg) {
-    constexpr int CH = kDecayChunk<T>, CT = CH / 16, KT = DP / 16, KP = DP / 32;
+    constexpr int CH = kDecayChunk<T>, SPAN = kDecaySpan<T, DP>, CT = CH / 16, KT = DP / 16, KP = DP / 32;
     using Tile = ForwardTile<T, DP, CH>;
     using M = typename Tile::M;
     __shared__ Tile sh;
-    const Lane<DP> first;
+    const Place<DP> first;
     const std::uint32_t env = blockIdx.x / a.hv, h = blockIdx.x % a.hv;
     const std::size_t head = blockIdx.x, state_size = static_cast<std::size_t>(a.dk_dim) * a.dv_dim;
     const std::int64_t out_step = static_cast<std::int64_t>(a.batch) * a.hv * a.dv_dim;
@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(DP * 4, kForwardWaves<DP>) decay_forward_kerne
 
     const float gate = a.steps != 0 ? a.g[h] : 0.0f;
     const bool always = gate < kDropBelow;
-    sh.powers.make(gate, always, first.tid);
+    sh.powers.make(gate, a.scale, always, first.tid);
     if (first.tid < 4) sh.bad[first.tid / 2][first.tid % 2] = 0;
     f4 S[KT];
     const float* from = seg.count > 1 ? seg.states + (static_cast<std::size_t>(blockIdx.y) * gridDim.x + head) * state_size
@@ -78,26 +78,27 @@ __global__ void __launch_bounds__(DP * 4, kForwardWaves<DP>) decay_forward_kerne
         return static_cast<int>(whole < left ? whole : left);
     };
     Piece<T, DP, CH, WIDE> k, q, v;
-    std::uint64_t next_drops = 0;
-    const auto fetch = [&](std::uint32_t t0, const Lane<DP>& at) {
+    Resets<T> resets;
+    const auto fetch = [&](std::uint32_t t0, const Place<DP>& at) {
         const int n = width(t0);
         k.fetch(a.k, a.dk_dim, t0, n, env, h / a.group, at);
         q.fetch(a.q, a.dk_dim, t0, n, env, h / a.group, at);
         v.fetch(a.v, a.dv_dim, t0, n, env, h, at);
-        next_drops = drops_of<CH>(a, t0, n, env, at.lane, always);
+        resets.fetch(a, t0, n, env, at.lane);
     };
     if (begin < end) fetch(begin, first);
     int which = 0;
     for (std::uint32_t t0 = begin; t0 < end; which ^= 1) {
-        const Lane<DP> at = Lane<DP>::anew();
+        const Place<DP> at = Place<DP>::anew();
         const int r = at.r, g = at.g;
-        if (t0 != 0 && t0 % CH == 0 && a.saved != nullptr)
-            store_value_slab<DP>(a.saved + ((t0 / CH - 1) * static_cast<std::size_t>(a.batch) * a.hv + head) * state_size, dk, dv, at, S);
-        if (next_drops & 1u)
+        if (t0 != 0 && t0 % SPAN == 0 && a.saved != nullptr)
+            store_value_slab<DP>(a.saved + ((t0 / SPAN - 1) * static_cast<std::size_t>(a.batch) * a.hv + head) * state_size, dk, dv, at, S);
+        int n = width(t0);
+        const std::uint64_t drops = resets.drops(n, at.lane, always);
+        if (drops & 1u)
 #pragma unroll
             for (int i = 0; i < KT; ++i) S[i] = zero;
-        const std::uint64_t inside = next_drops & ~1ull;
-        int n = width(t0);
+        const std::uint64_t inside = drops & ~1ull;
         for (;;) {
             k.stage(sh.k, at);
             q.stage(sh.q, at);
@@ -140,7 +141,7 @@ __global__ void __launch_bounds__(DP * 4, kForwardWaves<DP>) decay_forward_kerne
         }
 #pragma unroll
         for (int m = 0; m < CT; ++m) {
-            O[m] *= seen.in(sh.powers, 16 * m + 4 * g) * a.scale;
+            O[m] *= seen.in(sh.powers, 16 * m + 4 * g);
             if (seen.drops != 0)       // by selection: the state may be large
 #pragma unroll
                 for (int e = 0; e < 4; ++e) O[m][e] = 16 * m + 4 * g + e < seen.first ? O[m][e] : 0.0f;
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(DP * 4, kForwardWaves<DP>) decay_forward_kerne
         __syncthreads();
         sh.results.flush(out, dv, n, at);
     }
-    if (end == a.steps) store_value_slab<DP>(a.state_out + head * state_size, dk, dv, Lane<DP>::anew(), S);
+    if (end == a.steps) store_value_slab<DP>(a.state_out + head * state_size, dk, dv, Place<DP>::anew(), S);
 }
 
 template <typename T, int DP, bool WIDE>
@@ -212,8 +213,8 @@ using namespace nesle::mem;
 extern "C" {
 
 std::uint64_t nesle_decay_saved_floats(const nesle_decay_args* a) {
-    if (a == nullptr || a->steps <= decay_chunk(*a)) return 0;
-    const std::uint64_t chunks = (static_cast<std::uint64_t>(a->steps) + decay_chunk(*a) - 1) / decay_chunk(*a) - 1;
+    if (a == nullptr || a->steps <= decay_span(*a)) return 0;
+    const std::uint64_t chunks = (static_cast<std::uint64_t>(a->steps) + decay_span(*a) - 1) / decay_span(*a) - 1;
     return chunks * a->batch * a->v_heads * a->k_dim * a->v_dim;
 }
 

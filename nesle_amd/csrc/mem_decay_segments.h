@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(DP * 4, DP == 128 ? 2 : 4) decay_local_kernel(
     using Tile = LocalTile<T, DP, CH>;
     using M = typename Tile::M;
     __shared__ Tile sh;
-    const Lane<DP> first;
+    const Place<DP> first;
     const std::uint32_t env = blockIdx.x / a.hv, h = blockIdx.x % a.hv;
     const std::uint32_t segment = blockIdx.y + (BACK ? 1 : 0);      // the first one's, or the last one's, is not needed
     const std::uint32_t begin = segment * seg.steps;
@@ -66,27 +66,27 @@ __global__ void __launch_bounds__(DP * 4, DP == 128 ? 2 : 4) decay_local_kernel(
     const std::uint32_t chunks = (end - begin + CH - 1) / CH;
     const float gate = a.g[h];
     const bool always = gate < kDropBelow;
-    sh.powers.make(gate, always, first.tid);
+    sh.powers.make(gate, a.scale, always, first.tid);
     f4 S[KT];
 #pragma unroll
     for (int i = 0; i < KT; ++i) S[i] = f4{0, 0, 0, 0};
 
     Piece<T, DP, CH, WIDE> x, y;
-    std::uint64_t next_drops = 0;
+    Resets<T> resets;
     const auto start_of = [&](std::uint32_t c) { return begin + (BACK ? chunks - 1 - c : c) * CH; };
     const auto width = [&](std::uint32_t t0) { return static_cast<int>(end - t0 < CH ? end - t0 : CH); };
-    const auto fetch = [&](std::uint32_t c, const Lane<DP>& at) {
+    const auto fetch = [&](std::uint32_t c, const Place<DP>& at) {
         const std::uint32_t t0 = start_of(c);
         x.fetch(BACK ? a.q : a.k, a.dk_dim, t0, width(t0), env, h / a.group, at);
         y.fetch(BACK ? a.dout : a.v, a.dv_dim, t0, width(t0), env, h, at);
-        next_drops = drops_of<CH>(a, t0, width(t0), env, at.lane, always);
+        resets.fetch(a, t0, width(t0), env, at.lane);
     };
     fetch(0, first);
     bool any_drop = false;
     for (std::uint32_t c = 0; c < chunks; ++c) {
-        const Lane<DP> at = Lane<DP>::anew();
+        const Place<DP> at = Place<DP>::anew();
         const int n = width(start_of(c));
-        const Seen seen(next_drops, n);
+        const Seen seen(resets.drops(n, at.lane, always), n);
         // Tokens before the last end of an episode leave nothing in the state, and what
         // is not finite in them must not either.  (The gradient of such inputs is
         // unspecified.)
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(DP * 4, DP == 128 ? 2 : 4) decay_local_kernel(
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const int row = 32 * p + 16 * t + 4 * at.g;
-                w[t] = BACK ? seen.in(sh.powers, row) * a.scale : seen.out(sh.powers, row);
+                w[t] = BACK ? seen.in(sh.powers, row) : seen.out(sh.powers, row);
             }
             const auto held = M::full(V[0] * w[0], V[1] * w[1]);
 #pragma unroll
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(DP * 4, DP == 128 ? 2 : 4) decay_local_kernel(
     }
     const std::size_t slot = static_cast<std::size_t>(segment) * gridDim.x + blockIdx.x;
     store_value_slab<DP>(seg.states + slot * a.dk_dim * a.dv_dim, static_cast<int>(a.dk_dim), static_cast<int>(a.dv_dim),
-                         Lane<DP>::anew(), S);
+                         Place<DP>::anew(), S);
     if (first.tid == 0) seg.dropped[slot] = any_drop;
 }
 

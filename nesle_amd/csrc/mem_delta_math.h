@@ -94,6 +94,9 @@ struct SplitMath {
 #pragma unroll
         for (int p = 0; p < PLANES; ++p) {
             to[p] = u2{pack_bf16(x.x, x.y), pack_bf16(x.z, x.w)};
+            // As packed words from here on: the compiler would round the lower half of
+            // each a second time rather than shift it out.
+            asm("" : "+v"(to[p].x), "+v"(to[p].y));
             if (p + 1 < PLANES) x -= f4{lo_half(to[p].x), hi_half(to[p].x), lo_half(to[p].y), hi_half(to[p].y)};
         }
     }
