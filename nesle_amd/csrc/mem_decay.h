@@ -394,7 +394,20 @@ __device__ void store_value_slab(float* to, int dk, int dv, const At& at, const 
         }
 }
 
-template <typename T>
-using DecayMath = std::conditional_t<sizeof(T) == 2, SplitMath<1>, F32Math>;
+// Kinds of products (mem_delta_math.h).  Float32 inputs in three planes take a third of the
+// matrix instructions' time, and half as much LDS again and the cutting.  By float32
+// instructions / by planes, us of 128 steps of 64 (512) consoles of 4 heads: forward of 32
+// dimensions 15 / 16 (37 / 43), of 64 23 / 25 (108 / 116), of 128 52 / 42 (256 consoles 178 /
+// 172); gradient of 32 23 / 23 (105 / 110), of 64 38 / 34 (299 / 274), of 128 96 / 88 (399 / 385).
+template <typename T, int DP>
+struct DecayMathOf {
+    using forward = SplitMath<1>;
+    using gradient = SplitMath<1>;
+};
+template <int DP>
+struct DecayMathOf<float, DP> {
+    using forward = std::conditional_t<DP == 128, SplitMath<3>, F32Math>;
+    using gradient = std::conditional_t<DP == 32, F32Math, SplitMath<3>>;
+};
 
 }  // namespace nesle::mem

@@ -48,7 +48,7 @@ constexpr int kGradWaves = sizeof(T) == 2 && DP <= 64 ? 4 : 2;
 template <typename T, int DP>
 struct GradTile {
     static constexpr int CH = kDecaySpan<T, DP>, ROLES = kGradRoles<DP>;
-    using M = DecayMath<T>;
+    using M = typename DecayMathOf<T, DP>::gradient;
     using In = typename M::template Tile<CH, DP, M::kIn, 8>;
     union Out {
         In in;

@@ -25,7 +25,7 @@ namespace {
 
 template <typename T, int DP, int CH>
 struct ForwardTile {
-    using M = DecayMath<T>;
+    using M = typename DecayMathOf<T, DP>::forward;
     typename M::template Tile<CH, DP, M::kIn, 8> k, q, v;
     DecayResults<T, DP, CH> results;
     Powers<CH> powers;

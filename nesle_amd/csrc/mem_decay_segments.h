@@ -43,9 +43,9 @@ inline DecaySegments decay_segments(const nesle_decay_args& a) {
 
 // ---- B of every segment -----------------------------------------------------------
 
-template <typename T, int DP, int CH>
+template <typename T, int DP, int CH, bool BACK>
 struct LocalTile {
-    using M = DecayMath<T>;
+    using M = std::conditional_t<BACK, typename DecayMathOf<T, DP>::gradient, typename DecayMathOf<T, DP>::forward>;
     typename M::template Tile<CH, DP, M::kIn, 8> x, y;
     Powers<CH> powers;
 };
@@ -55,7 +55,7 @@ struct LocalTile {
 template <typename T, int DP, bool WIDE, bool BACK>
 __global__ void __launch_bounds__(DP * 4, DP == 128 ? 2 : 4) decay_local_kernel(DecayArgs<T> a, DecaySegments seg) {
     constexpr int CH = kDecayChunk<T>, KT = DP / 16;
-    using Tile = LocalTile<T, DP, CH>;
+    using Tile = LocalTile<T, DP, CH, BACK>;
     using M = typename Tile::M;
     __shared__ Tile sh;
     const Place<DP> first;

@@ -130,6 +130,22 @@ struct Row {
     }
 };
 
+// V floats of a weight that lie together; `or_else` where there is none.
+template <int V>
+__device__ void load_weight(const float* p, std::uint32_t col, std::uint32_t dim, float or_else, float (&v)[V]) {
+    const bool has = p != nullptr && col < dim;
+    if constexpr (V == 1) {
+        v[0] = has ? p[col] : or_else;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+            const f4 x = has ? *reinterpret_cast<const f4*>(p + col + i) : f4{or_else, or_else, or_else, or_else};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[i + j] = x[j];
+        }
+    }
+}
+
 template <int L>
 constexpr int kBlock = L > 256 ? L : 256;
 
@@ -143,12 +159,8 @@ __global__ void __launch_bounds__(kBlock<L>) layer_norm_kernel(NormArgs<T> a) {
     Vec<float, V> w[N], b[N];
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-        const std::uint32_t col = Row<T, V, N, L>::col(c, lane);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            w[c].v[j] = a.weight != nullptr && col < a.dim ? a.weight[col + j] : 1.0f;
-            b[c].v[j] = a.bias != nullptr && col < a.dim ? a.bias[col + j] : 0.0f;
-        }
+        load_weight<V>(a.weight, Row<T, V, N, L>::col(c, lane), a.dim, 1.0f, w[c].v);
+        load_weight<V>(a.bias, Row<T, V, N, L>::col(c, lane), a.dim, 0.0f, b[c].v);
     }
     for (std::uint64_t row = blockIdx.x * kGroups + threadIdx.x / L; row < a.rows; row += stride) {
         Row<T, V, N, L> x;
@@ -177,12 +189,9 @@ __global__ void __launch_bounds__(kBlock<L>) layer_norm_grad_kernel(NormArgs<T> 
     float w[N][V], dw[N][V], db[N][V];
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-        const std::uint32_t col = Row<T, V, N, L>::col(c, lane);
+        load_weight<V>(a.weight, Row<T, V, N, L>::col(c, lane), a.dim, 1.0f, w[c]);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            w[c][j] = a.weight != nullptr && col < a.dim ? a.weight[col + j] : 1.0f;
-            dw[c][j] = db[c][j] = 0.0f;
-        }
+        for (int j = 0; j < V; ++j) dw[c][j] = db[c][j] = 0.0f;
     }
     for (std::uint64_t row = blockIdx.x * kGroups + threadIdx.x / L; row < a.rows; row += stride) {
         Row<T, V, N, L> x, dy;
@@ -245,21 +254,28 @@ __global__ void __launch_bounds__(kBlock<L>) layer_norm_grad_kernel(NormArgs<T> 
     }
 }
 
-// The workgroups' sums added up: 16 columns a workgroup, 16 lanes a column.
-__global__ void __launch_bounds__(256) norm_weight_sum(const float* partials, float* dweight, float* dbias, std::uint32_t dim,
-                                                       std::uint32_t blocks) {
-    __shared__ float part[16][16];
-    const std::uint32_t i = blockIdx.x * 16 + threadIdx.x % 16, all = 2 * dim;
-    float sum = 0.0f;
-    if (i < all)
-        for (std::uint32_t b = threadIdx.x / 16; b < blocks; b += 16) sum += partials[static_cast<std::size_t>(b) * all + i];
-    part[threadIdx.x / 16][threadIdx.x % 16] = sum;
+// The workgroups' sums added up: 16 columns a workgroup, 64 lanes a column, each of which
+// has at most kMostPartials / 64 sums in flight at once.
+constexpr std::uint32_t kMostPartials = 1024;
+__global__ void __launch_bounds__(1024) norm_weight_sum(const float* partials, float* dweight, float* dbias, std::uint32_t dim,
+                                                        std::uint32_t blocks) {
+    __shared__ float part[64][17];
+    const std::uint32_t i = blockIdx.x * 16 + threadIdx.x % 16, all = 2 * dim, first = threadIdx.x / 16;
+    float v[kMostPartials / 64], sum = 0.0f;
+#pragma unroll
+    for (std::uint32_t k = 0; k < kMostPartials / 64; ++k)
+        v[k] = i < all && first + 64 * k < blocks ? partials[static_cast<std::size_t>(first + 64 * k) * all + i] : 0.0f;
+#pragma unroll
+    for (std::uint32_t k = 0; k < kMostPartials / 64; ++k) sum += v[k];
+    part[first][threadIdx.x % 16] = sum;
     __syncthreads();
-    if (threadIdx.x >= 16 || i >= all) return;
-    sum = 0.0f;
-    for (int k = 0; k < 16; ++k) sum += part[k][threadIdx.x];
-    float* to = i < dim ? dweight : dbias;
-    if (to != nullptr) to[i < dim ? i : i - dim] = sum;
+    // A wave for each column: the sum over its 64 lanes.
+    const unsigned column = threadIdx.x / 64;
+    sum = over_groups(sum16(part[threadIdx.x % 64][column]));
+    const std::uint32_t at = blockIdx.x * 16 + column;
+    if (threadIdx.x % 64 != 0 || at >= all) return;
+    float* to = at < dim ? dweight : dbias;
+    if (to != nullptr) to[at < dim ? at : at - dim] = sum;
 }
 
 // How a row is laid over lanes.
@@ -299,7 +315,8 @@ int vector_of(const nesle_norm_args& x, bool grad) {
 }
 
 // Workgroups: as many as fill the card a few times over.
-constexpr std::uint32_t kMostBlocks = 2048, kGradBlocks = 1024;
+constexpr std::uint32_t kMostBlocks = 4096, kGradBlocks = 1024;
+static_assert(kGradBlocks <= kMostPartials);
 
 std::uint32_t blocks_of(const nesle_norm_args& a, const Shape& s, std::uint32_t most) {
     const std::uint64_t want = (rows_of(a) + s.groups - 1) / s.groups;
@@ -329,7 +346,7 @@ NormArgs<T> norm_args(const nesle_norm_args& x) {
 
 template <typename T, int V, bool GRAD, int L, int N>
 void launch_shape(const NormArgs<T>& a, std::uint32_t blocks, hipStream_t s) {
-    if constexpr (N * V > kMostElements) return;       // shape_of names none such
+    if constexpr (N * V > kMostElements || (L == 1024 && N * V > 16)) return;      // shape_of names none such
     else if constexpr (GRAD) hipLaunchKernelGGL((layer_norm_grad_kernel<T, V, N, L>), dim3(blocks), dim3(kBlock<L>), 0, s, a);
     else hipLaunchKernelGGL((layer_norm_kernel<T, V, N, L>), dim3(blocks), dim3(kBlock<L>), 0, s, a);
 }
@@ -362,7 +379,7 @@ int norm(const char* who, const nesle_norm_args& x, hipStream_t s) {
     if (v == 1) launch<T, 1, GRAD>(a, shape, blocks, s);
     else launch<T, 16 / sizeof(T), GRAD>(a, shape, blocks, s);
     if (sums)
-        hipLaunchKernelGGL(norm_weight_sum, dim3((2 * x.dim + 15) / 16), dim3(256), 0, s, x.scratch, x.dweight, x.dbias, x.dim, blocks);
+        hipLaunchKernelGGL(norm_weight_sum, dim3((2 * x.dim + 15) / 16), dim3(1024), 0, s, x.scratch, x.dweight, x.dbias, x.dim, blocks);
     return launched(who);
 }
 

@@ -1,18 +1,20 @@
 // Sampling of actions from given random numbers (include/nesle_memory.h has the
 // rules).
 //
-// A row's scores are held in the registers of a group of lanes, lane l those of the
-// actions l E .. l E + E - 1, so that the order of actions is the order of lanes.
 // Which actions are left and which one a uniform number falls on turn on comparisons
 // of sums, so weights and sums are float64: in float32 a border would be off by up to
 // 2^-24 of the whole, and one row in 10^5 or so would get another action than the
 // rules say.
 //
-// top_k and top_p need the actions in order of falling weight only up to a border.
-// The border is found without sorting: scores become whole numbers of the same order,
-// and the bits of the one at the border are found from the top, each by one sum over
-// the group of what lies above a candidate.  Of equal scores at the border the first
-// few by index stay.
+// Up to 16 actions, a row is 16 lanes, an action a lane: what is ahead of an action in
+// the order of falling scores is found by comparing it with the other 15, which pass
+// by in turn.  With more, a row is a wave, lane l has the actions E l .. E l + E - 1, and the
+// border that top_k or top_p draws is found without sorting: scores become whole numbers
+// of the same order, and the bits of one at the border are found from the top until only
+// one is left.  For top_k each bit takes a count, a vote of the lanes; what it leaves, if
+// that is 64 or fewer, moves to one action a lane.  For top_p each bit takes a sum, in
+// float32: the border that it ends at is then tested in float64, and the search done
+// again in float64 if the sums' roundings led it astray.
 #include "mem_delta_math.h"
 
 namespace nesle::mem {
@@ -31,189 +33,366 @@ struct SampleArgs {
     std::uint32_t rows, batch, actions;
 };
 
-// Sums over the L lanes of a group, in all of them.
-template <int L, typename X>
-__device__ X group_sum(X v) {
-#pragma unroll
-    for (int d = 1; d < L; d *= 2) v += __shfl_xor(v, d);
-    return v;
+// ---- across lanes: data-parallel moves, no LDS -------------------------------------
+template <int CTRL, int ROWS = 0xf>
+__device__ std::uint32_t moved_bits(std::uint32_t v) {
+    return static_cast<std::uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, true));
 }
-// Over the lanes below, of the group.
-template <int L, typename X>
-__device__ X group_below(X v, unsigned lane) {
-    X sum = v;
-#pragma unroll
-    for (int d = 1; d < L; d *= 2) {
-        const X below = __shfl_up(sum, d, L);
-        if (lane >= d) sum += below;
+// v as the lane that CTRL names holds it, zero where there is none.
+template <int CTRL, int ROWS = 0xf, typename X>
+__device__ X from_lane(X v) {
+    if constexpr (sizeof(X) == 8) {
+        const auto b = __builtin_bit_cast(std::uint64_t, v);
+        return __builtin_bit_cast(X, static_cast<std::uint64_t>(moved_bits<CTRL, ROWS>(static_cast<std::uint32_t>(b >> 32))) << 32 |
+                                         moved_bits<CTRL, ROWS>(static_cast<std::uint32_t>(b)));
+    } else {
+        return __builtin_bit_cast(X, moved_bits<CTRL, ROWS>(__builtin_bit_cast(std::uint32_t, v)));
     }
-    return sum - v;
 }
+// Sums over the lanes below, and the lane itself: of 16 lanes, and of a wave.
+template <typename X>
+__device__ X scan16(X v) {
+    v += from_lane<kRowShr + 1>(v);
+    v += from_lane<kRowShr + 2>(v);
+    v += from_lane<kRowShr + 4>(v);
+    return v + from_lane<kRowShr + 8>(v);
+}
+constexpr int kRowBcast15 = 0x142, kRowBcast31 = 0x143, kRowLast = 0x15f;     // the 16th lane's of the row, to all
+template <typename X>
+__device__ X scan64(X v) {
+    v = scan16(v);
+    v += from_lane<kRowBcast15, 0xa>(v);       // row 0's sum to row 1, row 2's to row 3
+    return v + from_lane<kRowBcast31, 0xc>(v); // rows 0 and 1's to rows 2 and 3
+}
+template <typename X>
+__device__ X of_lane(X v, int lane) {
+    if constexpr (sizeof(X) == 8) {
+        const auto b = __builtin_bit_cast(std::uint64_t, v);
+        const std::uint32_t hi = __builtin_amdgcn_readlane(static_cast<std::uint32_t>(b >> 32), lane),
+                            lo = __builtin_amdgcn_readlane(static_cast<std::uint32_t>(b), lane);
+        return __builtin_bit_cast(X, static_cast<std::uint64_t>(hi) << 32 | lo);
+    } else {
+        return __builtin_bit_cast(X, __builtin_amdgcn_readlane(__builtin_bit_cast(std::uint32_t, v), lane));
+    }
+}
+template <typename X>
+__device__ X sum64(X v) { return of_lane(scan64(v), 63); }
 
-// Whole numbers in the order of the floats; -0 as 0.
+__device__ int lanes_in(std::uint64_t mask) { return __popcll(mask); }
+__device__ int lanes_below(std::uint64_t mask) {
+    return __builtin_amdgcn_mbcnt_hi(static_cast<std::uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<std::uint32_t>(mask), 0));
+}
+__device__ int first_lane(std::uint64_t mask) { return __ffsll(static_cast<long long>(mask)) - 1; }
+__device__ int last_lane(std::uint64_t mask) { return 63 - __clzll(static_cast<long long>(mask)); }
+
+// Whole numbers in the order of the floats, -0 as 0; 0 for -infinity.
 __device__ std::uint32_t key_of(float x) {
+    if (x == -INFINITY) return 0u;
     const std::uint32_t b = __builtin_bit_cast(std::uint32_t, x + 0.0f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-template <typename T, int L, int E>
-__global__ void __launch_bounds__(256) sample_kernel(SampleArgs<T> a) {
-    const unsigned lane = threadIdx.x % L;
-    const std::uint64_t row = (blockIdx.x * 256ull + threadIdx.x) / L;
-    if (row >= a.rows) return;                         // whole groups, and nobody waits for them
-    const std::uint32_t r = static_cast<std::uint32_t>(row), first = lane * E;
-    const T* from = a.logits.row(r / a.batch, r % a.batch, 0);
-    float x[E];
-    float most = -INFINITY;
-    bool odd = false;
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-        x[i] = first + i < a.actions ? static_cast<float>(from[first + i]) : -INFINITY;
-        odd |= !(x[i] < INFINITY);                     // NaN or +infinity
-        most = fmaxf(most, x[i]);
+// A row's settings.
+struct Settings {
+    double temperature, top_p, min_p, u;
+    std::int64_t top_k;
+    template <typename T>
+    __device__ Settings(const SampleArgs<T>& a, std::uint32_t r)
+        : temperature(a.temperatures != nullptr ? a.temperatures[r] : a.temperature), top_p(a.top_ps != nullptr ? a.top_ps[r] : a.top_p),
+          min_p(a.min_ps != nullptr ? a.min_ps[r] : a.min_p), u(a.uniform[r]),
+          top_k(a.top_ks != nullptr ? std::int64_t{a.top_ks[r]} : std::int64_t{a.top_k}) {}
+    __device__ bool fine() const {
+        return temperature >= 0.0 && temperature < INFINITY && top_p > 0.0 && top_p <= 1.0 && min_p >= 0.0 && min_p <= 1.0 &&
+               top_k >= 0 && u == u;
     }
-    const double temperature = a.temperatures != nullptr ? a.temperatures[r] : a.temperature;
-    const double top_p = a.top_ps != nullptr ? a.top_ps[r] : a.top_p;
-    const double min_p = a.min_ps != nullptr ? a.min_ps[r] : a.min_p;
-    const auto top_k = a.top_ks != nullptr ? std::int64_t{a.top_ks[r]} : std::int64_t{a.top_k};
-    const double u = a.uniform[r];
-#pragma unroll
-    for (int d = 1; d < L; d *= 2) {
-        most = fmaxf(most, __shfl_xor(most, d));
-        odd |= __shfl_xor(static_cast<int>(odd), d) != 0;
+    // The difference first: a quotient may pass the largest number.  (1 / temperature may
+    // too; 0 times that would be NaN.)
+    __device__ double weight(float x, float most) const {
+        const double w = exp((static_cast<double>(x) - most) * (1.0 / temperature));
+        return x == most ? 1.0 : x > -INFINITY ? w : 0.0;
     }
-    const bool fine = !odd && most > -INFINITY && temperature >= 0.0 && temperature < INFINITY && top_p > 0.0 &&
-                      top_p <= 1.0 && min_p >= 0.0 && min_p <= 1.0 && top_k >= 0 && u == u;
+};
+
+// ---- up to 16 actions: 16 lanes a row -----------------------------------------------
+__device__ float most16(float v) {
+    v = fmaxf(v, moved<kRowRor + 8>(v));
+    v = fmaxf(v, moved<kRowRor + 4>(v));
+    v = fmaxf(v, moved<kRowRor + 2>(v));
+    return fmaxf(v, moved<kRowRor + 1>(v));
+}
+// Bit s: the action that is s lanes round is ahead; their number, and of those that
+// `ahead` has, the sum of their weights.
+template <int... S>
+__device__ std::uint32_t ahead16(std::integer_sequence<int, S...>, std::uint32_t key, std::uint32_t lane) {
+    std::uint32_t ahead = 0;
+    const auto meet = [&](std::uint32_t other, std::uint32_t from, int s) {
+        if (other > key || (other == key && from < lane)) ahead |= 1u << s;
+    };
+    (meet(from_lane<kRowRor + S + 1>(key), from_lane<kRowRor + S + 1>(lane), S), ...);
+    return ahead;
+}
+template <int... S>
+__device__ double before16(std::integer_sequence<int, S...>, std::uint32_t ahead, double w) {
+    double sum = 0.0;
+    const auto meet = [&](double other, int s) { sum += ahead >> s & 1u ? other : 0.0; };
+    (meet(from_lane<kRowRor + S + 1>(w), S), ...);
+    return sum;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) sample16_kernel(SampleArgs<T> a) {
+    const std::uint32_t lane = threadIdx.x % 16;
+    const std::uint64_t row = (blockIdx.x * 256ull + threadIdx.x) / 16;
+    const auto r = static_cast<std::uint32_t>(row < a.rows ? row : a.rows - 1);        // past the end: the last one's again, not written
+    const Settings set(a, r);
+    const float x = lane < a.actions ? static_cast<float>(a.logits.row(r / a.batch, r % a.batch, 0)[lane]) : -INFINITY;
+    const auto of_row = [&](bool v) { return static_cast<std::uint32_t>(__ballot(v) >> (threadIdx.x % 64 / 16 * 16)) & 0xffffu; };
+    const bool odd = of_row(!(x < INFINITY)) != 0;             // NaN or +infinity
+    const float most = most16(x);
+    const bool fine = !odd && most > -INFINITY && set.fine(), greedy = set.temperature == 0.0;
+    const std::uint32_t best = of_row(x == most);
+    double w = fine && !greedy ? set.weight(x, most) : 0.0;
+    const bool narrow = set.top_p < 1.0 || (set.top_k > 0 && set.top_k < a.actions);
+    if (__any(narrow)) {
+        constexpr std::make_integer_sequence<int, 15> others{};
+        const std::uint32_t ahead = ahead16(others, key_of(x), lane);
+        if (set.top_k > 0 && __popc(ahead) >= set.top_k) w = 0.0;
+        const double share = set.top_p * from_lane<kRowLast>(scan16(w));
+        const double before = before16(others, ahead, w);
+        if (set.top_p < 1.0 && !(before < share)) w = 0.0;
+    }
+    if (w < set.min_p) w = 0.0;
+    const double run = scan16(w), all = from_lane<kRowLast>(run), target = (set.u > 0.0 ? set.u : 0.0) * all;
+    const std::uint32_t left = of_row(w > 0.0), past = of_row(w > 0.0 && run > target);
+    const int found = greedy ? __ffs(static_cast<int>(best)) - 1 : past != 0 ? __ffs(static_cast<int>(past)) - 1 : 31 - __clz(static_cast<int>(left));
+    if (row >= a.rows) return;
     if (!fine) {
         if (lane == 0) {
             a.action[r] = -1;
             a.logprob[r] = NAN;
         }
-        return;
+    } else if (static_cast<int>(lane) == found) {
+        a.action[r] = found;
+        a.logprob[r] = greedy ? 0.0f : static_cast<float>(log(w / all));
     }
-    double w[E];
+}
+
+// ---- more: a wave a row ---------------------------------------------------------------
+
+// What top_p leaves: weights of the rest become zero.  low and high: no score that has a
+// weight is outside.
+template <int E>
+__device__ __forceinline__ void nucleus(const float (&x)[E], double (&w)[E], double top_p, std::uint32_t low, std::uint32_t high) {
     std::uint32_t key[E];
-    if (temperature == 0.0) {                          // the largest, the first of equal ones
-        std::uint32_t best = 0xffffffffu;
-#pragma unroll
-        for (int i = E - 1; i >= 0; --i) best = x[i] == most ? first + i : best;
-#pragma unroll
-        for (int d = 1; d < L; d *= 2) best = min(best, static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(best), d)));
-        if (lane == 0) {
-            a.action[r] = best;
-            a.logprob[r] = 0.0f;
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-        // The difference first: a quotient may pass the largest number.
-        w[i] = x[i] > -INFINITY ? exp((static_cast<double>(x[i]) - most) / temperature) : 0.0;
-        key[i] = x[i] > -INFINITY ? key_of(x[i]) : 0u;
-    }
-    if (top_k > 0 && top_k < a.actions) {
-        // The k-th largest: the largest number that k or more are not below.
-        std::uint32_t border = 0;
-        for (std::uint32_t bit = 0x80000000u; bit != 0; bit >>= 1) {
-            int count = 0;
-#pragma unroll
-            for (int i = 0; i < E; ++i) count += key[i] >= (border | bit);
-            if (group_sum<L>(count) >= top_k) border |= bit;
-        }
-        int above = 0, equal = 0;
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            above += key[i] > border;
-            equal += key[i] == border;
-        }
-        int left = static_cast<int>(top_k) - group_sum<L>(above) - group_below<L>(equal, lane);
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const bool stays = key[i] > border || (key[i] == border && left > 0);
-            left -= key[i] == border;
-            if (!stays) {
-                w[i] = 0.0;
-                key[i] = 0u;
-            }
-        }
-    }
-    if (top_p < 1.0) {
-        double sum = 0.0;
-#pragma unroll
-        for (int i = 0; i < E; ++i) sum += w[i];
-        const double most_before = top_p * group_sum<L>(sum);
-        // The smallest score that some action may have and stay: the largest number
-        // at or above which the weights reach the share.
-        std::uint32_t border = 0;
-        for (std::uint32_t bit = 0x80000000u; bit != 0; bit >>= 1) {
-            double reached = 0.0;
-#pragma unroll
-            for (int i = 0; i < E; ++i) reached += key[i] >= (border | bit) ? w[i] : 0.0;
-            if (group_sum<L>(reached) >= most_before) border |= bit;
-        }
-        double above = 0.0, at_border = 0.0;
-        int equal = 0;
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            above += key[i] > border ? w[i] : 0.0;
-            at_border = key[i] == border ? w[i] : at_border;
-            equal += key[i] == border;
-        }
-        above = group_sum<L>(above);
-#pragma unroll
-        for (int d = 1; d < L; d *= 2) at_border = fmax(at_border, __shfl_xor(at_border, d));
-        int ahead = group_below<L>(equal, lane);
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const bool stays = key[i] > border || (key[i] == border && above + ahead * at_border < most_before);
-            ahead += key[i] == border;
-            if (!stays) w[i] = 0.0;
-        }
-    }
+    float light[E];
     double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-        if (w[i] < min_p) w[i] = 0.0;
+        key[i] = key_of(x[i]);
+        light[i] = static_cast<float>(w[i]);
         sum += w[i];
     }
-    const double below = group_below<L>(sum, lane), all = group_sum<L>(sum), target = (u > 0.0 ? u : 0.0) * all;
-    // The first action at which the running sum exceeds the target; if rounding or u
+    const double share = top_p * sum64(sum);
+    const float about = static_cast<float>(share);
+    // The border is the largest score at or above which the weights reach the share.
+    // border: they do; beyond: they do not (0: none such is known).
+    // Bits that low and high share are the border's too.
+    std::uint32_t bit = low == high ? 0u : 0x80000000u >> __clz(static_cast<int>(low ^ high));
+    std::uint32_t border = bit == 0 ? low : high & ~(2 * bit - 1), beyond = 0;
+    for (; bit != 0; bit >>= 1) {
+        const std::uint32_t at = border | bit;
+        float reached = 0.0f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) reached += key[i] >= at ? light[i] : 0.0f;
+        if (sum64(reached) >= about) border = at;
+        else beyond = at;
+        if (beyond == 0) continue;
+        int left = 0;
+        std::uint32_t only = border;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const std::uint64_t between = __ballot(key[i] >= border && key[i] < beyond);
+            left += lanes_in(between);
+            if (between != 0) only = of_lane(key[i], first_lane(between));
+        }
+        if (left == 1) {
+            border = only;
+            break;
+        }
+    }
+    const auto above = [&](std::uint32_t at, bool or_at) {
+        double v = 0.0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) v += key[i] > at || (or_at && key[i] == at) ? w[i] : 0.0;
+        return sum64(v);
+    };
+    double before = above(border, false);
+    if (!(before < share && above(border, true) >= share)) {
+        border = 0;
+        for (bit = 0x80000000u; bit != 0; bit >>= 1)
+            if (above((border | bit) - 1, false) >= share) border |= bit;
+        before = above(border, false);
+    }
+    // Of equal scores at the border the first few by index stay.
+    int ahead = 0;
+    double each = 0.0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const std::uint64_t here = __ballot(key[i] == border);
+        if (here != 0) each = of_lane(w[i], first_lane(here));
+        ahead += lanes_below(here);
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const bool stays = key[i] > border || (key[i] == border && before + ahead * each < share);
+        ahead += key[i] == border;
+        if (!stays) w[i] = 0.0;
+    }
+}
+
+// The action that the uniform number falls on: its place, E lane + i, and log
+// probability.
+template <int E>
+__device__ __forceinline__ int pick(const float (&x)[E], float most, const Settings& set, std::uint32_t low, float& logprob) {
+    const int lane = threadIdx.x % 64;
+    double w[E], sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) w[i] = set.weight(x[i], most);
+    if (set.top_p < 1.0) nucleus(x, w, set.top_p, low, key_of(most));
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        if (w[i] < set.min_p) w[i] = 0.0;
+        sum += w[i];
+    }
+    const double upto = scan64(sum), all = of_lane(upto, 63), target = (set.u > 0.0 ? set.u : 0.0) * all;
+    // The first place at which the running sum exceeds the target; if rounding or u
     // leaves none, the last one of any weight.
-    double run = below;
-    std::uint32_t found = 0xffffffffu, last = 0;
+    double run = upto - sum;
+    int past = E, last = -1;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
         run += w[i];
         if (w[i] > 0.0) {
-            last = first + i + 1;
-            if (run > target && found == 0xffffffffu) found = first + i;
+            last = i;
+            if (past == E && run > target) past = i;
         }
     }
+    const std::uint64_t have = __ballot(past < E);
+    const int of = have != 0 ? first_lane(have) : last_lane(__ballot(last >= 0));
+    const int mine = have != 0 ? past : last;
+    double chosen = 0.0;
 #pragma unroll
-    for (int d = 1; d < L; d *= 2) {
-        found = min(found, static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(found), d)));
-        last = max(last, static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(last), d)));
-    }
-    if (found == 0xffffffffu) found = last - 1;
+    for (int i = 0; i < E; ++i) chosen = mine == i ? w[i] : chosen;
+    if (lane == of) logprob = static_cast<float>(log(chosen / all));
+    logprob = of_lane(logprob, of);
+    return E * of + of_lane(mine, of);
+}
+
+constexpr int kRows = 4;       // rows, waves, of a workgroup: they do not meet
+
+template <typename T, int E>
+__global__ void __launch_bounds__(64 * kRows) sample64_kernel(SampleArgs<T> a) {
+    __shared__ float scores[kRows][64];
+    __shared__ int places[kRows][64];
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const std::uint32_t r = blockIdx.x * kRows + wave;
+    if (r >= a.rows) return;
+    const Settings set(a, r);
+    const T* from = a.logits.row(r / a.batch, r % a.batch, 0);
+    float x[E], most = -INFINITY;
+    bool odd = false;
+    if (E > 1 && a.logits.vec && a.actions % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < E; ++i)
-        if (first + i == found) {
-            a.action[r] = found;
-            a.logprob[r] = static_cast<float>(log(w[i] / all));
+        for (int i = 0; i < E / 4; ++i) {
+            const std::uint32_t at = E * lane + 4 * i;
+            const f4 v = at < a.actions ? load4(from + at, true) : f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[4 * i + j] = v[j];
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = E * lane + i < a.actions ? static_cast<float>(from[E * lane + i]) : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        odd |= !(x[i] < INFINITY);                     // NaN or +infinity
+        most = fmaxf(most, x[i]);
+    }
+    most = most16(most);
+    most = fmaxf(fmaxf(of_lane(most, 0), of_lane(most, 16)), fmaxf(of_lane(most, 32), of_lane(most, 48)));
+    int found = -1;
+    float logprob = NAN;
+    if (!__any(odd) && most > -INFINITY && set.fine()) {
+        if (set.temperature == 0.0) {                  // the largest, the first of equal ones
+            int best = E;
+#pragma unroll
+            for (int i = E - 1; i >= 0; --i) best = x[i] == most ? i : best;
+            const int of = first_lane(__ballot(best < E));
+            found = E * of + of_lane(best, of);
+            logprob = 0.0f;
+        } else if (set.top_k > 0 && set.top_k < a.actions) {
+            const int count = static_cast<int>(set.top_k);
+            std::uint32_t key[E], border = 0;
+#pragma unroll
+            for (int i = 0; i < E; ++i) key[i] = key_of(x[i]);
+            // The k-th largest: the largest number that k or more are not below; any
+            // that just k are not below leaves the same.
+            for (std::uint32_t bit = 0x80000000u; bit != 0; bit >>= 1) {
+                int reached = 0;
+#pragma unroll
+                for (int i = 0; i < E; ++i) reached += lanes_in(__ballot(key[i] >= (border | bit)));
+                if (reached >= count) border |= bit;
+                if (reached == count) break;
+            }
+            // Of equal scores at the border the first few by index stay; if just k are not
+            // below it, all do.
+            int left = count, kept = 0;
+            bool stays[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) left -= lanes_in(__ballot(key[i] > border)) + lanes_below(__ballot(key[i] == border));
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                stays[i] = key[i] != 0 && (key[i] > border || (key[i] == border && left > 0));
+                left -= key[i] == border;
+                kept += lanes_below(__ballot(stays[i]));
+                if (!stays[i]) x[i] = -INFINITY;
+            }
+            if (E > 1 && count <= 64) {
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+                    if (stays[i]) {
+                        scores[wave][kept] = x[i];
+                        places[wave][kept] = E * lane + i;
+                        ++kept;
+                    }
+                kept = of_lane(kept, 63);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();       // in order within the wave
+                const float one[1] = {lane < kept ? scores[wave][lane] : -INFINITY};
+                found = places[wave][pick<1>(one, most, set, border, logprob)];
+            } else {
+                found = pick<E>(x, most, set, border, logprob);
+            }
+        } else {
+            found = pick<E>(x, most, set, 0, logprob);
+        }
+    }
+    if (lane == 0) {
+        a.action[r] = found;
+        a.logprob[r] = logprob;
+    }
 }
 
 template <typename T>
 int sample(const char* who, const nesle_sample_args& x, hipStream_t s) {
     const SampleArgs<T> a{heads<T>(x.logits), x.uniform, x.temperature, x.top_p, x.min_p, x.top_k, x.temperatures, x.top_ps,
                           x.min_ps, x.top_ks, x.action, x.logprob, x.steps * x.batch, x.batch, x.actions};
-    const int lanes = x.actions <= 16 ? 16 : 64;
-    const std::uint32_t rows = 256 / lanes;
+    const std::uint32_t rows = x.actions <= 16 ? 16 : kRows;
     const dim3 grid((a.rows + rows - 1) / rows), block(256);
-    if (x.actions <= 16) hipLaunchKernelGGL((sample_kernel<T, 16, 1>), grid, block, 0, s, a);
-    else if (x.actions <= 64) hipLaunchKernelGGL((sample_kernel<T, 64, 1>), grid, block, 0, s, a);
-    else if (x.actions <= 256) hipLaunchKernelGGL((sample_kernel<T, 64, 4>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((sample_kernel<T, 64, 16>), grid, block, 0, s, a);
+    if (x.actions <= 16) hipLaunchKernelGGL((sample16_kernel<T>), grid, block, 0, s, a);
+    else if (x.actions <= 64) hipLaunchKernelGGL((sample64_kernel<T, 1>), grid, block, 0, s, a);
+    else if (x.actions <= 256) hipLaunchKernelGGL((sample64_kernel<T, 4>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((sample64_kernel<T, 16>), grid, block, 0, s, a);
     return launched(who);
 }
 
