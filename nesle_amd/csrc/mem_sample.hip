@@ -8,13 +8,16 @@
 //
 // Up to 16 actions, a row is 16 lanes, an action a lane: what is ahead of an action in
 // the order of falling scores is found by comparing it with the other 15, which pass
-// by in turn.  With more, a row is a wave, lane l has the actions E l .. E l + E - 1, and the
-// border that top_k or top_p draws is found without sorting: scores become whole numbers
-// of the same order, and the bits of one at the border are found from the top until only
-// one is left.  For top_k each bit takes a count, a vote of the lanes; what it leaves, if
-// that is 64 or fewer, moves to one action a lane.  For top_p each bit takes a sum, in
-// float32: the border that it ends at is then tested in float64, and the search done
-// again in float64 if the sums' roundings led it astray.
+// by in turn.  Up to 64, a row is a wave, an action a lane, and the lanes sort
+// themselves.  With more, lane l has the actions E l .. E l + E - 1, and the border that
+// top_k or top_p draws is found without sorting.  For top_k by halving the scores' range,
+// each time with a count, a vote of the lanes; what it leaves, if that is 64 or fewer,
+// moves to one action a lane and sorts itself.  For top_p scores become whole numbers of
+// the same order, and the bits of one at the border are found from the top, each with a
+// sum in float32: the border that it ends at is then tested in float64, and the search
+// done again in float64 if the sums' roundings led it astray.
+#include <algorithm>
+
 #include "mem_delta_math.h"
 
 namespace nesle::mem {
@@ -25,7 +28,7 @@ struct SampleArgs {
     Heads<T> logits;
     const float* uniform;
     double temperature, top_p, min_p;
-    std::uint32_t top_k;
+    std::uint32_t top_k;             // at most the actions
     const float *temperatures, *top_ps, *min_ps;
     const std::int32_t* top_ks;
     std::int64_t* action;
@@ -94,13 +97,13 @@ __device__ std::uint32_t key_of(float x) {
 
 // A row's settings.
 struct Settings {
-    double temperature, top_p, min_p, u;
-    std::int64_t top_k;
+    double temperature, inverse, top_p, min_p, u;
+    int top_k;
     template <typename T>
     __device__ Settings(const SampleArgs<T>& a, std::uint32_t r)
-        : temperature(a.temperatures != nullptr ? a.temperatures[r] : a.temperature), top_p(a.top_ps != nullptr ? a.top_ps[r] : a.top_p),
-          min_p(a.min_ps != nullptr ? a.min_ps[r] : a.min_p), u(a.uniform[r]),
-          top_k(a.top_ks != nullptr ? std::int64_t{a.top_ks[r]} : std::int64_t{a.top_k}) {}
+        : temperature(a.temperatures != nullptr ? a.temperatures[r] : a.temperature), inverse(1.0 / temperature),
+          top_p(a.top_ps != nullptr ? a.top_ps[r] : a.top_p), min_p(a.min_ps != nullptr ? a.min_ps[r] : a.min_p), u(a.uniform[r]),
+          top_k(a.top_ks != nullptr ? a.top_ks[r] : static_cast<int>(a.top_k)) {}
     __device__ bool fine() const {
         return temperature >= 0.0 && temperature < INFINITY && top_p > 0.0 && top_p <= 1.0 && min_p >= 0.0 && min_p <= 1.0 &&
                top_k >= 0 && u == u;
@@ -108,7 +111,7 @@ struct Settings {
     // The difference first: a quotient may pass the largest number.  (1 / temperature may
     // too; 0 times that would be NaN.)
     __device__ double weight(float x, float most) const {
-        const double w = exp((static_cast<double>(x) - most) * (1.0 / temperature));
+        const double w = exp((static_cast<double>(x) - most) * inverse);
         return x == most ? 1.0 : x > -INFINITY ? w : 0.0;
     }
 };
@@ -178,6 +181,57 @@ __global__ void __launch_bounds__(256) sample16_kernel(SampleArgs<T> a) {
 }
 
 // ---- more: a wave a row ---------------------------------------------------------------
+
+// The value of the lane whose number differs in the bits of MASK.
+template <int MASK>
+__device__ std::uint32_t of_other(std::uint32_t v) {
+    if constexpr (MASK == 1) return from_lane<0xb1>(v);
+    else if constexpr (MASK == 2) return from_lane<0x4e>(v);
+    else if constexpr (MASK == 3) return from_lane<0x1b>(v);
+    else if constexpr (MASK == 4) return from_lane<0x1b>(from_lane<0x141>(v));     // 7, then 3
+    else if constexpr (MASK == 7) return from_lane<0x141>(v);
+    else if constexpr (MASK == 8) return from_lane<kRowRor + 8>(v);
+    else if constexpr (MASK == 15) return from_lane<0x140>(v);
+    else return static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(v), MASK));
+}
+// Larger of two lanes' values to the lower one.
+template <int MASK>
+__device__ void order(std::uint64_t& v, int lane) {
+    constexpr int top = MASK >= 32 ? 32 : MASK >= 16 ? 16 : MASK >= 8 ? 8 : MASK >= 4 ? 4 : MASK >= 2 ? 2 : 1;
+    const std::uint64_t other = static_cast<std::uint64_t>(of_other<MASK>(static_cast<std::uint32_t>(v >> 32))) << 32 |
+                                of_other<MASK>(static_cast<std::uint32_t>(v));
+    v = (other > v) == ((lane & top) == 0) ? other : v;
+}
+// The lanes' values in falling order: runs of 2, 4, .. lanes are merged, the first step
+// of each with the other run turned round.
+__device__ __forceinline__ void sort64(std::uint64_t& v, int lane) {
+    order<1>(v, lane);
+    order<3>(v, lane), order<1>(v, lane);
+    order<7>(v, lane), order<2>(v, lane), order<1>(v, lane);
+    order<15>(v, lane), order<4>(v, lane), order<2>(v, lane), order<1>(v, lane);
+    order<31>(v, lane), order<8>(v, lane), order<4>(v, lane), order<2>(v, lane), order<1>(v, lane);
+    order<63>(v, lane), order<16>(v, lane), order<8>(v, lane), order<4>(v, lane), order<2>(v, lane), order<1>(v, lane);
+}
+
+// One action a lane: what top_k (0: all) and top_p leave; weights of the rest become zero.
+__device__ __forceinline__ void keep64(float x, double& w, double top_p, int top_k) {
+    const int lane = threadIdx.x % 64;
+    const std::uint32_t key = key_of(x);
+    std::uint64_t v = static_cast<std::uint64_t>(key) << 32 | static_cast<std::uint32_t>(63 - lane);
+    sort64(v, lane);
+    const int place = 63 - static_cast<int>(v & 63u);
+    const auto bits = __builtin_bit_cast(std::uint64_t, w);
+    const std::uint32_t lo = __shfl(static_cast<int>(bits), place), hi = __shfl(static_cast<int>(bits >> 32), place);
+    double sorted = __builtin_bit_cast(double, static_cast<std::uint64_t>(hi) << 32 | lo);
+    if (top_k > 0 && lane >= top_k) sorted = 0.0;
+    const double upto = scan64(sorted), share = top_p * of_lane(upto, 63);
+    // In this order what stays is a beginning of it.
+    const int kept = lanes_in(__ballot(sorted > 0.0 && (top_p >= 1.0 || lane == 0 || upto - sorted < share)));
+    const std::uint32_t border = of_lane(static_cast<std::uint32_t>(v >> 32), kept - 1);
+    // Read here, with all lanes: under the condition the others' places need not be there.
+    const int last = of_lane(place, kept - 1);
+    if (key < border || (key == border && lane > last)) w = 0.0;
+}
 
 // What top_p leaves: weights of the rest become zero.  low and high: no score that has a
 // weight is outside.
@@ -250,15 +304,23 @@ __device__ __forceinline__ void nucleus(const float (&x)[E], double (&w)[E], dou
     }
 }
 
-// The action that the uniform number falls on: its place, E lane + i, and log
-// probability.
+// A row's answer, and what its log probability is the logarithm of the quotient of.
+struct Answer {
+    int action;
+    double chosen, all;
+};
+
+// The action that the uniform number falls on, as its place E lane + i.
 template <int E>
-__device__ __forceinline__ int pick(const float (&x)[E], float most, const Settings& set, std::uint32_t low, float& logprob) {
-    const int lane = threadIdx.x % 64;
+__device__ __forceinline__ Answer pick(const float (&x)[E], float most, const Settings& set, std::uint32_t low, int top_k) {
     double w[E], sum = 0.0;
 #pragma unroll
     for (int i = 0; i < E; ++i) w[i] = set.weight(x[i], most);
-    if (set.top_p < 1.0) nucleus(x, w, set.top_p, low, key_of(most));
+    if constexpr (E == 1) {
+        if (set.top_p < 1.0 || top_k > 0) keep64(x[0], w[0], set.top_p, top_k);
+    } else if (set.top_p < 1.0) {
+        nucleus(x, w, set.top_p, low, key_of(most));
+    }
 #pragma unroll
     for (int i = 0; i < E; ++i) {
         if (w[i] < set.min_p) w[i] = 0.0;
@@ -283,24 +345,15 @@ __device__ __forceinline__ int pick(const float (&x)[E], float most, const Setti
     double chosen = 0.0;
 #pragma unroll
     for (int i = 0; i < E; ++i) chosen = mine == i ? w[i] : chosen;
-    if (lane == of) logprob = static_cast<float>(log(chosen / all));
-    logprob = of_lane(logprob, of);
-    return E * of + of_lane(mine, of);
+    return {E * of + of_lane(mine, of), of_lane(chosen, of), all};
 }
 
-constexpr int kRows = 4;       // rows, waves, of a workgroup: they do not meet
+constexpr int kWaves = 4;      // of a workgroup: they do not meet
 
+// A row's scores, E a lane.
 template <typename T, int E>
-__global__ void __launch_bounds__(64 * kRows) sample64_kernel(SampleArgs<T> a) {
-    __shared__ float scores[kRows][64];
-    __shared__ int places[kRows][64];
-    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const std::uint32_t r = blockIdx.x * kRows + wave;
-    if (r >= a.rows) return;
-    const Settings set(a, r);
+__device__ __forceinline__ void load_row(const SampleArgs<T>& a, std::uint32_t r, int lane, float (&x)[E]) {
     const T* from = a.logits.row(r / a.batch, r % a.batch, 0);
-    float x[E], most = -INFINITY;
-    bool odd = false;
     if (E > 1 && a.logits.vec && a.actions % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < E / 4; ++i) {
@@ -313,86 +366,148 @@ __global__ void __launch_bounds__(64 * kRows) sample64_kernel(SampleArgs<T> a) {
 #pragma unroll
         for (int i = 0; i < E; ++i) x[i] = E * lane + i < a.actions ? static_cast<float>(from[E * lane + i]) : -INFINITY;
     }
+}
+
+// What top_k leaves of the scores, of which the largest is `most`: the others become
+// -infinity.  Returns a number that none of them is above and none that is left below;
+// with `move` what is left lies, in order, in scores and places.
+template <int E>
+__device__ __forceinline__ float largest(float (&x)[E], float most, int count, bool move, int lane, float* scores, int* places, int& kept) {
+    // One that just `count` scores are not below, if there is, by halving the range.
+    float least = INFINITY;
+    int all = 0, at_most = 0;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-        odd |= !(x[i] < INFINITY);                     // NaN or +infinity
-        most = fmaxf(most, x[i]);
+        least = x[i] > -INFINITY ? fminf(least, x[i]) : least;
+        all += lanes_in(__ballot(x[i] > -INFINITY));
+        at_most += lanes_in(__ballot(x[i] == most));
     }
-    most = most16(most);
-    most = fmaxf(fmaxf(of_lane(most, 0), of_lane(most, 16)), fmaxf(of_lane(most, 32), of_lane(most, 48)));
-    int found = -1;
-    float logprob = NAN;
-    if (!__any(odd) && most > -INFINITY && set.fine()) {
+    least = -most16(-least);
+    least = fminf(fminf(of_lane(least, 0), of_lane(least, 16)), fminf(of_lane(least, 32), of_lane(least, 48)));
+    float border = at_most >= count ? most : least;
+    if (at_most < count && all > count) {
+        float beyond = most;           // fewer are not below it; more are not below the border
+        for (;;) {
+            const float half = 0.5f * border + 0.5f * beyond;
+            if (!(half > border && half < beyond)) break;      // next to each other: equal scores at the border
+            int reached = 0;
+#pragma unroll
+            for (int i = 0; i < E; ++i) reached += lanes_in(__ballot(x[i] >= half));
+            if (reached >= count) border = half;
+            else beyond = half;
+            if (reached == count) break;
+        }
+    }
+    // Of equal scores at the border the first few by index stay; if no more than `count`
+    // are not below it, all do.
+    int left = count;
+    bool stays[E];
+    kept = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) left -= lanes_in(__ballot(x[i] > border)) + lanes_below(__ballot(x[i] == border));
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        stays[i] = x[i] > border || (x[i] == border && left > 0);
+        left -= x[i] == border;
+        kept += lanes_below(__ballot(stays[i]));
+        if (!stays[i]) x[i] = -INFINITY;
+    }
+    if (move) {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (stays[i]) {
+                scores[kept] = x[i];
+                places[kept] = E * lane + i;
+                ++kept;
+            }
+        kept = of_lane(kept, 63);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();       // in order within the wave
+    }
+    return border;
+}
+
+// A wave takes `each` rows one after the other; settings and log probabilities are
+// worked out for all of them at once, a row a lane.
+template <typename T, int E>
+__global__ void __launch_bounds__(64 * kWaves, E == 16 ? 3 : 8) sample64_kernel(SampleArgs<T> a, int each) {
+    __shared__ float scores[kWaves][64];
+    __shared__ int places[kWaves][64];
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const std::uint64_t begin = (static_cast<std::uint64_t>(blockIdx.x) * kWaves + wave) * each;
+    if (begin >= a.rows) return;
+    const int count = static_cast<int>(a.rows - begin < static_cast<std::uint64_t>(each) ? a.rows - begin : each);
+    const auto first = static_cast<std::uint32_t>(begin);
+    const Settings mine(a, first + min(lane, count - 1));
+    const bool mine_fine = mine.fine();
+    Answer answer{-1, NAN, 1.0};
+    float next[E];
+    load_row<T, E>(a, first, lane, next);
+    for (int j = 0; j < count; ++j) {
+        float x[E], most = -INFINITY;
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            x[i] = next[i];
+            odd |= !(x[i] < INFINITY);                 // NaN or +infinity
+            most = fmaxf(most, x[i]);
+        }
+        if (j + 1 < count) load_row<T, E>(a, first + j + 1, lane, next);
+        most = most16(most);
+        most = fmaxf(fmaxf(of_lane(most, 0), of_lane(most, 16)), fmaxf(of_lane(most, 32), of_lane(most, 48)));
+        if (__any(odd) || !(most > -INFINITY) || of_lane(static_cast<int>(mine_fine), j) == 0) continue;
+        Settings set = mine;
+        set.temperature = of_lane(mine.temperature, j);
+        set.inverse = of_lane(mine.inverse, j);
+        set.top_p = of_lane(mine.top_p, j);
+        set.min_p = of_lane(mine.min_p, j);
+        set.u = of_lane(mine.u, j);
+        set.top_k = of_lane(mine.top_k, j);
+        Answer found;
         if (set.temperature == 0.0) {                  // the largest, the first of equal ones
             int best = E;
 #pragma unroll
             for (int i = E - 1; i >= 0; --i) best = x[i] == most ? i : best;
             const int of = first_lane(__ballot(best < E));
-            found = E * of + of_lane(best, of);
-            logprob = 0.0f;
-        } else if (set.top_k > 0 && set.top_k < a.actions) {
-            const int count = static_cast<int>(set.top_k);
-            std::uint32_t key[E], border = 0;
-#pragma unroll
-            for (int i = 0; i < E; ++i) key[i] = key_of(x[i]);
-            // The k-th largest: the largest number that k or more are not below; any
-            // that just k are not below leaves the same.
-            for (std::uint32_t bit = 0x80000000u; bit != 0; bit >>= 1) {
-                int reached = 0;
-#pragma unroll
-                for (int i = 0; i < E; ++i) reached += lanes_in(__ballot(key[i] >= (border | bit)));
-                if (reached >= count) border |= bit;
-                if (reached == count) break;
-            }
-            // Of equal scores at the border the first few by index stay; if just k are not
-            // below it, all do.
-            int left = count, kept = 0;
-            bool stays[E];
-#pragma unroll
-            for (int i = 0; i < E; ++i) left -= lanes_in(__ballot(key[i] > border)) + lanes_below(__ballot(key[i] == border));
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-                stays[i] = key[i] != 0 && (key[i] > border || (key[i] == border && left > 0));
-                left -= key[i] == border;
-                kept += lanes_below(__ballot(stays[i]));
-                if (!stays[i]) x[i] = -INFINITY;
-            }
-            if (E > 1 && count <= 64) {
-#pragma unroll
-                for (int i = 0; i < E; ++i)
-                    if (stays[i]) {
-                        scores[wave][kept] = x[i];
-                        places[wave][kept] = E * lane + i;
-                        ++kept;
-                    }
-                kept = of_lane(kept, 63);
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();       // in order within the wave
+            found = {E * of + of_lane(best, of), 1.0, 1.0};
+        } else if (E > 1 && set.top_k > 0 && set.top_k < static_cast<int>(a.actions)) {
+            const bool move = set.top_k <= 64;
+            int kept;
+            const float border = largest<E>(x, most, set.top_k, move, lane, scores[wave], places[wave], kept);
+            if (move) {
                 const float one[1] = {lane < kept ? scores[wave][lane] : -INFINITY};
-                found = places[wave][pick<1>(one, most, set, border, logprob)];
+                found = pick<1>(one, most, set, 0, 0);
+                found.action = places[wave][found.action];
             } else {
-                found = pick<E>(x, most, set, border, logprob);
+                found = pick<E>(x, most, set, key_of(border), 0);
             }
         } else {
-            found = pick<E>(x, most, set, 0, logprob);
+            found = pick<E>(x, most, set, 0, set.top_k);
         }
+        if (lane == j) answer = found;
     }
-    if (lane == 0) {
-        a.action[r] = found;
-        a.logprob[r] = logprob;
+    if (lane < count) {
+        a.action[first + lane] = answer.action;
+        a.logprob[first + lane] = static_cast<float>(log(answer.chosen / answer.all));
     }
 }
 
 template <typename T>
 int sample(const char* who, const nesle_sample_args& x, hipStream_t s) {
-    const SampleArgs<T> a{heads<T>(x.logits), x.uniform, x.temperature, x.top_p, x.min_p, x.top_k, x.temperatures, x.top_ps,
+    const SampleArgs<T> a{heads<T>(x.logits), x.uniform, x.temperature, x.top_p, x.min_p, std::min(x.top_k, x.actions), x.temperatures, x.top_ps,
                           x.min_ps, x.top_ks, x.action, x.logprob, x.steps * x.batch, x.batch, x.actions};
-    const std::uint32_t rows = x.actions <= 16 ? 16 : kRows;
-    const dim3 grid((a.rows + rows - 1) / rows), block(256);
-    if (x.actions <= 16) hipLaunchKernelGGL((sample16_kernel<T>), grid, block, 0, s, a);
-    else if (x.actions <= 64) hipLaunchKernelGGL((sample64_kernel<T, 1>), grid, block, 0, s, a);
-    else if (x.actions <= 256) hipLaunchKernelGGL((sample64_kernel<T, 4>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((sample64_kernel<T, 16>), grid, block, 0, s, a);
+    const dim3 block(256);
+    if (x.actions <= 16) {
+        hipLaunchKernelGGL((sample16_kernel<T>), dim3((a.rows + 15) / 16), block, 0, s, a);
+        return launched(who);
+    }
+    // As many rows a wave as leave the card twice the waves that it holds.
+    const int each = static_cast<int>(std::min(std::max(a.rows / 16384, 1u), 16u));
+    const std::uint32_t rows = kWaves * static_cast<std::uint32_t>(each);
+    const dim3 grid((a.rows + rows - 1) / rows);
+    if (x.actions <= 64) hipLaunchKernelGGL((sample64_kernel<T, 1>), grid, block, 0, s, a, each);
+    else if (x.actions <= 256) hipLaunchKernelGGL((sample64_kernel<T, 4>), grid, block, 0, s, a, each);
+    else hipLaunchKernelGGL((sample64_kernel<T, 16>), grid, block, 0, s, a, each);
     return launched(who);
 }
 
