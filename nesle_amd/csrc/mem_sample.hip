@@ -12,10 +12,11 @@
 // themselves.  With more, lane l has the actions E l .. E l + E - 1, and the border that
 // top_k or top_p draws is found without sorting.  For top_k by halving the scores' range,
 // each time with a count, a vote of the lanes; what it leaves, if that is 64 or fewer,
-// moves to one action a lane and sorts itself.  For top_p scores become whole numbers of
-// the same order, and the bits of one at the border are found from the top, each with a
-// sum in float32: the border that it ends at is then tested in float64, and the search
-// done again in float64 if the sums' roundings led it astray.
+// moves to one action a lane and sorts itself.  For top_p the 64 largest are tried that
+// way.  If they do not reach its share, scores become whole numbers of the same order, and
+// the bits of one at the border are found from the top, each with a sum in float32: the
+// border that it ends at is then tested in float64, and the search done again in float64
+// if the sums' roundings led it astray.
 #include <algorithm>
 
 #include "mem_delta_math.h"
@@ -213,8 +214,9 @@ __device__ __forceinline__ void sort64(std::uint64_t& v, int lane) {
     order<63>(v, lane), order<16>(v, lane), order<8>(v, lane), order<4>(v, lane), order<2>(v, lane), order<1>(v, lane);
 }
 
-// One action a lane: what top_k (0: all) and top_p leave; weights of the rest become zero.
-__device__ __forceinline__ void keep64(float x, double& w, double top_p, int top_k) {
+// One action a lane: what top_k (0: all) and top_p leave; weights of the rest become
+// zero.  share: of all, where the lanes do not hold all; else 0.
+__device__ __forceinline__ void keep64(float x, double& w, double top_p, int top_k, double share) {
     const int lane = threadIdx.x % 64;
     const std::uint32_t key = key_of(x);
     std::uint64_t v = static_cast<std::uint64_t>(key) << 32 | static_cast<std::uint32_t>(63 - lane);
@@ -224,7 +226,8 @@ __device__ __forceinline__ void keep64(float x, double& w, double top_p, int top
     const std::uint32_t lo = __shfl(static_cast<int>(bits), place), hi = __shfl(static_cast<int>(bits >> 32), place);
     double sorted = __builtin_bit_cast(double, static_cast<std::uint64_t>(hi) << 32 | lo);
     if (top_k > 0 && lane >= top_k) sorted = 0.0;
-    const double upto = scan64(sorted), share = top_p * of_lane(upto, 63);
+    const double upto = scan64(sorted);
+    if (share == 0.0) share = top_p * of_lane(upto, 63);
     // In this order what stays is a beginning of it.
     const int kept = lanes_in(__ballot(sorted > 0.0 && (top_p >= 1.0 || lane == 0 || upto - sorted < share)));
     const std::uint32_t border = of_lane(static_cast<std::uint32_t>(v >> 32), kept - 1);
@@ -312,12 +315,12 @@ struct Answer {
 
 // The action that the uniform number falls on, as its place E lane + i.
 template <int E>
-__device__ __forceinline__ Answer pick(const float (&x)[E], float most, const Settings& set, std::uint32_t low, int top_k) {
+__device__ __forceinline__ Answer pick(const float (&x)[E], float most, const Settings& set, std::uint32_t low, int top_k, double share = 0.0) {
     double w[E], sum = 0.0;
 #pragma unroll
     for (int i = 0; i < E; ++i) w[i] = set.weight(x[i], most);
     if constexpr (E == 1) {
-        if (set.top_p < 1.0 || top_k > 0) keep64(x[0], w[0], set.top_p, top_k);
+        if (set.top_p < 1.0 || top_k > 0) keep64(x[0], w[0], set.top_p, top_k, share);
     } else if (set.top_p < 1.0) {
         nucleus(x, w, set.top_p, low, key_of(most));
     }
@@ -385,30 +388,42 @@ __device__ __forceinline__ float largest(float (&x)[E], float most, int count, b
     least = -most16(-least);
     least = fminf(fminf(of_lane(least, 0), of_lane(least, 16)), fminf(of_lane(least, 32), of_lane(least, 48)));
     float border = at_most >= count ? most : least;
+    int reached = at_most >= count ? at_most : all;        // not below it
     if (at_most < count && all > count) {
         float beyond = most;           // fewer are not below it; more are not below the border
         for (;;) {
             const float half = 0.5f * border + 0.5f * beyond;
             if (!(half > border && half < beyond)) break;      // next to each other: equal scores at the border
-            int reached = 0;
+            int now = 0;
 #pragma unroll
-            for (int i = 0; i < E; ++i) reached += lanes_in(__ballot(x[i] >= half));
-            if (reached >= count) border = half;
-            else beyond = half;
-            if (reached == count) break;
+            for (int i = 0; i < E; ++i) now += lanes_in(__ballot(x[i] >= half));
+            if (now < count) {
+                beyond = half;
+                continue;
+            }
+            border = half;
+            reached = now;
+            if (now == count) break;
         }
     }
-    // Of equal scores at the border the first few by index stay; if no more than `count`
-    // are not below it, all do.
-    int left = count;
+    // Of equal scores at the border the first few by index stay.
     bool stays[E];
     kept = 0;
+    if (reached <= count) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) left -= lanes_in(__ballot(x[i] > border)) + lanes_below(__ballot(x[i] == border));
+        for (int i = 0; i < E; ++i) stays[i] = x[i] >= border;
+    } else {
+        int left = count;
+#pragma unroll
+        for (int i = 0; i < E; ++i) left -= lanes_in(__ballot(x[i] > border)) + lanes_below(__ballot(x[i] == border));
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            stays[i] = x[i] > border || (x[i] == border && left > 0);
+            left -= x[i] == border;
+        }
+    }
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-        stays[i] = x[i] > border || (x[i] == border && left > 0);
-        left -= x[i] == border;
         kept += lanes_below(__ballot(stays[i]));
         if (!stays[i]) x[i] = -INFINITY;
     }
@@ -430,7 +445,7 @@ __device__ __forceinline__ float largest(float (&x)[E], float most, int count, b
 // A wave takes `each` rows one after the other; settings and log probabilities are
 // worked out for all of them at once, a row a lane.
 template <typename T, int E>
-__global__ void __launch_bounds__(64 * kWaves, E == 16 ? 3 : 8) sample64_kernel(SampleArgs<T> a, int each) {
+__global__ void __launch_bounds__(64 * kWaves, E == 16 ? 3 : E == 4 ? 6 : 8) sample64_kernel(SampleArgs<T> a, int each) {
     __shared__ float scores[kWaves][64];
     __shared__ int places[kWaves][64];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -470,19 +485,38 @@ __global__ void __launch_bounds__(64 * kWaves, E == 16 ? 3 : 8) sample64_kernel(
             for (int i = E - 1; i >= 0; --i) best = x[i] == most ? i : best;
             const int of = first_lane(__ballot(best < E));
             found = {E * of + of_lane(best, of), 1.0, 1.0};
-        } else if (E > 1 && set.top_k > 0 && set.top_k < static_cast<int>(a.actions)) {
-            const bool move = set.top_k <= 64;
-            int kept;
-            const float border = largest<E>(x, most, set.top_k, move, lane, scores[wave], places[wave], kept);
-            if (move) {
-                const float one[1] = {lane < kept ? scores[wave][lane] : -INFINITY};
-                found = pick<1>(one, most, set, 0, 0);
-                found.action = places[wave][found.action];
-            } else {
-                found = pick<E>(x, most, set, key_of(border), 0);
-            }
+        } else if constexpr (E == 1) {
+            found = pick<1>(x, most, set, 0, set.top_k);
         } else {
-            found = pick<E>(x, most, set, 0, set.top_k);
+            const auto of_moved = [&](int kept, double share) {
+                const float one[1] = {lane < kept ? scores[wave][lane] : -INFINITY};
+                Answer got = pick<1>(one, most, set, 0, 0, share);
+                got.action = places[wave][got.action];
+                return got;
+            };
+            const bool narrow = set.top_k > 0 && set.top_k < static_cast<int>(a.actions);
+            float border = -INFINITY;
+            int kept;
+            if (narrow) border = largest<E>(x, most, set.top_k, set.top_k <= 64, lane, scores[wave], places[wave], kept);
+            if (narrow && set.top_k <= 64) {
+                found = of_moved(kept, 0.0);
+            } else if (set.top_p < 1.0) {
+                // Where the 64 largest reach the share, no other stays.
+                double sum = 0.0;
+                float y[E];
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    sum += set.weight(x[i], most);
+                    y[i] = x[i];
+                }
+                const double share = set.top_p * sum64(sum);
+                largest<E>(y, most, 64, true, lane, scores[wave], places[wave], kept);
+                const double held = set.weight(lane < kept ? scores[wave][lane] : -INFINITY, most);
+                if (sum64(held) >= share) found = of_moved(kept, share);
+                else found = pick<E>(x, most, set, key_of(border), 0);
+            } else {
+                found = pick<E>(x, most, set, 0, 0);
+            }
         }
         if (lane == j) answer = found;
     }
