@@ -28,12 +28,25 @@ struct DecaySegments {
 
 constexpr std::uint32_t kMostSegments = 128;      // what one workgroup takes a state through
 
+// As many segments as the card holds their workgroups at once with room to spare: 1,024,
+// 512 and 256 heads' of 32, 64 and 128 dimensions.  Two launches more and the second reading
+// of keys and values are worth it from 8 chunks on, from 16 where that makes only two or
+// three segments.  One walk / segments, us of the forward's launches in bfloat16 (* where
+// the rule walks whole):
+//   64 dimensions, 256 tokens of 64 heads* 23 / 20 and two launches; 512 of 64 heads 40 / 24,
+//   of 128 42 / 32, of 256* 43 / 45; 1,024 of 64 heads 76 / 33, of 128 77 / 47, of 256 79 / 72;
+//   8,191 of 8 heads 551 / 32; 128 dimensions, 256 of 64 heads* 36 / 28, 512 65 / 39, 1,024
+//   of 64 heads 124 / 61, of 128 127 / 99; 32 dimensions, 1,024 of 64 heads 63 / 24, of 256
+//   66 / 44.
+// Segments of 64 dimensions for 1,024 heads at once: 1,024 tokens of 64 heads 33 -> 37, 8,191
+// of 8 32 -> 34; for 256: 38 and 37.
 inline DecaySegments decay_segments(const nesle_decay_args& a) {
     constexpr std::uint32_t kSpan = 64;            // tokens: a multiple of any chunk length
-    const std::uint64_t heads = static_cast<std::uint64_t>(a.batch) * a.v_heads;
+    const std::uint64_t heads = static_cast<std::uint64_t>(a.batch) * a.v_heads, at_once = (1u << 15) / padded_dim(a);
     const std::uint32_t spans = (a.steps + kSpan - 1) / kSpan;
     std::uint32_t count = 1;
-    if (heads <= 256 && spans >= 4) count = std::min<std::uint64_t>({spans, kMostSegments, 1024 / heads});
+    if (2 * heads <= at_once && spans >= (4 * heads <= at_once ? 8u : 16u))
+        count = static_cast<std::uint32_t>(std::min<std::uint64_t>({spans, kMostSegments, at_once / heads}));
     const std::uint32_t each = count < 2 ? spans : (spans + count - 1) / count;
     DecaySegments s{};
     s.steps = std::max(each, 1u) * kSpan;
@@ -127,29 +140,30 @@ __global__ void __launch_bounds__(DP * 4, DP == 128 ? 2 : 4) decay_local_kernel(
 
 // S <- a^L S + B from segment to segment; a segment that drops the state inside leaves
 // B alone, whatever S held.  B gives way to the state before the segment (BACK: the
-// gradient after it).  16 lanes have 64 elements of a state, 16 such groups an equal
-// share of the segments each: a lane reads its share at once, the shares are joined
-// through LDS, and every group walks its own from where the ones before it end.
-template <bool BACK>
+// gradient after it).  A lane has four elements of a state and reads its share of the
+// segments at once: all of them (GROUPS 1, up to 16 segments), or an equal share of 16
+// groups', joined through LDS, after which every group walks its own from where the ones
+// before it end.
+constexpr int kAlone = 16;
+template <bool BACK, int GROUPS>
 __global__ void __launch_bounds__(256) decay_join_kernel(DecaySegments seg, const float* start, const float* g, std::uint32_t hv,
                                                          std::uint32_t size, std::uint32_t last_steps) {
-    constexpr int kShare = kMostSegments / 16;
-    __shared__ f4 sums[16][16];
-    __shared__ float factors[16];                          // negative: dropped
-    const int lane = threadIdx.x % 16, group = threadIdx.x / 16;
-    const std::uint32_t at = (blockIdx.y * 16 + lane) * 4;
+    constexpr int kShare = GROUPS == 1 ? kAlone : kMostSegments / GROUPS, kLanes = 256 / GROUPS;
+    __shared__ f4 sums[GROUPS][kLanes];
+    __shared__ float factors[GROUPS];                      // negative: dropped
+    const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+    const std::uint32_t at = (blockIdx.y * kLanes + lane) * 4;
     const bool in = at < size;
     const std::size_t heads = gridDim.x, head = blockIdx.x;
-    const int count = static_cast<int>(seg.count), share = (count + 15) / 16, begin = group * share;
+    const int count = static_cast<int>(seg.count), share = (count + GROUPS - 1) / GROUPS, begin = group * share;
     const auto slot = [&](int i) { return static_cast<std::size_t>(BACK ? count - 1 - i : i) * heads + head; };
     const float gate = g[head % hv];
     const float all = expf(static_cast<float>(seg.steps) * gate), tail = expf(static_cast<float>(last_steps) * gate);
     const auto factor = [&](int i) { return BACK && i == 0 ? tail : all; };
     const f4 zero = {0, 0, 0, 0};
 
-    f4 B[kShare], sum = zero;
-    bool dropped[kShare], any = false;
-    float f = 1.0f;
+    f4 B[kShare];
+    bool dropped[kShare];
 #pragma unroll
     for (int k = 0; k < kShare; ++k) {
         const int i = begin + k;
@@ -158,17 +172,22 @@ __global__ void __launch_bounds__(256) decay_join_kernel(DecaySegments seg, cons
         dropped[k] = use && seg.dropped[slot(i)] != 0;
     }
     f4 S = start != nullptr && in ? *reinterpret_cast<const f4*>(start + head * size + at) : zero;
+    if constexpr (GROUPS > 1) {
+        f4 sum = zero;
+        bool any = false;
+        float f = 1.0f;
 #pragma unroll
-    for (int k = 0; k < kShare; ++k)
-        if (k < share && begin + k < count - 1) {
-            sum = dropped[k] ? B[k] : sum * factor(begin + k) + B[k];
-            f *= factor(begin + k);
-            any |= dropped[k];
-        }
-    sums[group][lane] = sum;
-    if (lane == 0) factors[group] = any ? -1.0f : f;
-    __syncthreads();
-    for (int before = 0; before < group; ++before) S = factors[before] < 0.0f ? sums[before][lane] : S * factors[before] + sums[before][lane];
+        for (int k = 0; k < kShare; ++k)
+            if (k < share && begin + k < count - 1) {
+                sum = dropped[k] ? B[k] : sum * factor(begin + k) + B[k];
+                f *= factor(begin + k);
+                any |= dropped[k];
+            }
+        sums[group][lane] = sum;
+        if (lane == 0) factors[group] = any ? -1.0f : f;
+        __syncthreads();
+        for (int before = 0; before < group; ++before) S = factors[before] < 0.0f ? sums[before][lane] : S * factors[before] + sums[before][lane];
+    }
 #pragma unroll
     for (int k = 0; k < kShare; ++k) {
         const int i = begin + k;
@@ -182,8 +201,12 @@ template <typename T, int DP, bool WIDE, bool BACK>
 void launch_states(const DecayArgs<T>& a, const DecaySegments& seg, hipStream_t s) {
     const std::uint32_t heads = a.batch * a.hv, size = a.dk_dim * a.dv_dim;
     hipLaunchKernelGGL((decay_local_kernel<T, DP, WIDE, BACK>), dim3(heads, seg.count - 1), dim3(DP * 4), 0, s, a, seg);
-    hipLaunchKernelGGL((decay_join_kernel<BACK>), dim3(heads, (size + 63) / 64), dim3(256), 0, s, seg, BACK ? a.dstate_out : a.state, a.g,
-                       a.hv, size, a.steps - (seg.count - 1) * seg.steps);
+    const float* start = BACK ? a.dstate_out : a.state;
+    const std::uint32_t last = a.steps - (seg.count - 1) * seg.steps;
+    if (seg.count <= kAlone)
+        hipLaunchKernelGGL((decay_join_kernel<BACK, 1>), dim3(heads, (size + 1023) / 1024), dim3(256), 0, s, seg, start, a.g, a.hv, size, last);
+    else
+        hipLaunchKernelGGL((decay_join_kernel<BACK, 16>), dim3(heads, (size + 63) / 64), dim3(256), 0, s, seg, start, a.g, a.hv, size, last);
 }
 
 }  // namespace nesle::mem

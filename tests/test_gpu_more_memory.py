@@ -14,6 +14,7 @@ up to 1,000 products a lane: 4e-6."""
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
@@ -139,6 +140,40 @@ def test_decay_decays(decay, dtype):
     assert all(bool(t.isfinite().all()) for t in dg)
     assert float(dg[3][0]) == 0.0 and float(dg[3][2]) == 0.0 and float(dg[3][1]) != 0.0
     assert bool((dg[4][:, [0, 2]] == 0.0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(513, 1, 1, 1, 16, 16), (700, 2, 1, 2, 64, 64), (1100, 1, 2, 2, 128, 40), (2049, 1, 1, 1, 32, 32),
+                                   (1029, 3, 1, 2, 24, 64)])
+def test_decay_long_walks(shape, dtype):
+    """Few heads over many tokens go in segments; ends of episodes in the first, the last,
+    none and all of them, at their borders and inside."""
+    from nesle_amd import abi
+
+    say(f"[gpu] decay_attention segments {shape} {dtype}")
+    T, N, hk, hv, dk, dv = shape
+    a = abi.DecayArgs(abi.MEM_F32 if dtype == torch.float32 else abi.MEM_BF16, T, N, hk, hv, dk, dv, 1.0)
+    assert abi.lib().nesle_decay_forward_scratch_floats(ctypes.byref(a)) > 0
+    x, resets, grads = make(*shape, dtype, seed=T, resets=0.004)
+    check_decay(x, resets, grads)
+    resets[:] = False
+    check_decay(x, resets, grads)
+    for t in (0, 63, 64, 128, T - 1):
+        resets[:] = False
+        resets[t] = True
+        check_decay(x, resets, grads, train=t in (64, T - 1))
+    # Something that is not finite before an episode's end stays before it.
+    from nesle_amd import memory
+
+    resets[:] = False
+    resets[300] = True
+    gpu = {n: x[n].to(dev()) for n in NAMES}
+    want = memory.decay_attention(*(gpu[n] for n in NAMES[:4]), state=gpu["state"], resets=resets.to(dev()))
+    gpu["v"][200] = math.nan
+    gpu["k"][100] = math.inf
+    got = memory.decay_attention(*(gpu[n] for n in NAMES[:4]), state=gpu["state"], resets=resets.to(dev()))
+    for a, b in ((got[0][:100], want[0][:100]), (got[0][300:], want[0][300:]), (got[1], want[1])):
+        assert float((a.double() - b.double()).norm() / b.double().norm()) <= tol(dtype) + (0 if dtype == torch.float32 else 2.0 ** -9)
 
 
 def test_decay_without_state_or_tokens():
