@@ -150,7 +150,7 @@ def link_memory(obj: Path) -> Path:
     out = memory_path()
     tmp = out.with_name(out.name + ".tmp")
     _run([os.environ.get("CXX", "g++"), "-shared", "-o", str(tmp), str(obj), f"-L{PKG}", "-lnesle_hip", f"-L{libs}", "-lc10",
-          "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libs}"])
+          "-lc10_hip", "-ltorch_hip", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libs}"])
     tmp.replace(out)
     return out
 

@@ -5,6 +5,7 @@
 // own: the same work in Python took 15 us a call and 80 us a backward, several
 // times the kernels.
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
@@ -118,10 +119,16 @@ T* ptr(const Tensor& t) {
     return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
 }
 
-Tensor like(const Tensor& t) { return at::empty_like(t, t.options(), at::MemoryFormat::Contiguous); }
+// Uninitialised memory, from the allocator itself: through the dispatcher each of a
+// call's tensors takes a quarter of a microsecond more, of a small call's five.
+Tensor empty(const Tensor& beside, at::IntArrayRef sizes, at::ScalarType type) {
+    return Tensor(at::detail::empty_cuda(sizes, type, beside.device(), std::nullopt));
+}
+
+Tensor like(const Tensor& t) { return empty(t, t.sizes(), t.scalar_type()); }
 
 Tensor floats(const Tensor& beside, uint64_t n) {
-    return n == 0 ? Tensor() : at::empty({static_cast<int64_t>(n)}, beside.options().dtype(at::kFloat));
+    return n == 0 ? Tensor() : empty(beside, {static_cast<int64_t>(n)}, at::kFloat);
 }
 
 // Gradients as autograd hands them over, made readable where they are not: of
@@ -334,7 +341,7 @@ struct GatedDelta : torch::autograd::Function<GatedDelta> {
                              const Tensor& state, const Tensor& resets, double scale, bool keep) {
         const c10::OptionalDeviceGuard guard(q.device());
         nesle_delta_args a = delta_args(q, k, v, g, beta, state, resets, scale);
-        const Tensor out = like(v), after = at::empty({v.size(1), v.size(2), q.size(3), v.size(3)}, g.options());
+        const Tensor out = like(v), after = empty(q, {v.size(1), v.size(2), q.size(3), v.size(3)}, at::kFloat);
         const Tensor saved = floats(q, keep ? nesle_delta_saved_floats(&a) : 0);
         const Tensor scratch = floats(q, nesle_delta_forward_scratch_floats(&a));
         a.out = ptr(out);
@@ -469,7 +476,7 @@ struct DecayAttention : torch::autograd::Function<DecayAttention> {
                              const Tensor& resets, double scale, bool keep) {
         const c10::OptionalDeviceGuard guard(q.device());
         nesle_decay_args a = decay_args(q, k, v, g, state, resets, scale);
-        const Tensor out = like(v), after = at::empty({v.size(1), v.size(2), q.size(3), v.size(3)}, g.options());
+        const Tensor out = like(v), after = empty(q, {v.size(1), v.size(2), q.size(3), v.size(3)}, at::kFloat);
         const Tensor saved = floats(q, keep ? nesle_decay_saved_floats(&a) : 0);
         const Tensor scratch = floats(q, nesle_decay_forward_scratch_floats(&a));
         a.out = ptr(out);
@@ -687,7 +694,7 @@ py::tuple sample_actions(const Tensor& logits, const Tensor& uniform, const py::
     a.top_ks = ptr<int32_t>(top_ks);
     a.top_ps = ptr<float>(top_ps);
     a.min_ps = ptr<float>(min_ps);
-    const Tensor action = at::empty(uniform.sizes(), uniform.options().dtype(at::kLong)), logprob = at::empty(uniform.sizes(), uniform.options());
+    const Tensor action = empty(logits, uniform.sizes(), at::kLong), logprob = empty(logits, uniform.sizes(), at::kFloat);
     a.action = ptr<int64_t>(action);
     a.logprob = ptr<float>(logprob);
     check(nesle_sample(&a, stream_of(logits)));

@@ -54,9 +54,10 @@ def test_decay_entries_refuse(entry):
 
 def test_decay_workspaces():
     L = abi.lib()
-    for dtype, chunk in ((abi.MEM_F32, 32), (abi.MEM_BF16, 64)):
-        assert L.nesle_decay_saved_floats(ctypes.byref(decay_args(dtype=dtype, steps=chunk))) == 0
-        assert L.nesle_decay_saved_floats(ctypes.byref(decay_args(dtype=dtype, steps=2 * chunk + 1, k_dim=40))) == 2 * 2 * 4 * 40 * 16
+    # The state before every span of tokens but the first.
+    for dtype, dim, span in ((abi.MEM_F32, 64, 64), (abi.MEM_F32, 72, 32), (abi.MEM_BF16, 64, 64), (abi.MEM_BF16, 72, 64)):
+        assert L.nesle_decay_saved_floats(ctypes.byref(decay_args(dtype=dtype, steps=span, k_dim=dim))) == 0
+        assert L.nesle_decay_saved_floats(ctypes.byref(decay_args(dtype=dtype, steps=2 * span + 1, k_dim=dim))) == 2 * 2 * 4 * dim * 16
     # Shares of key heads' gradients, and one float a workgroup.
     one = L.nesle_decay_scratch_floats(ctypes.byref(decay_args(k_heads=4)))
     assert one >= 2 * 4
