@@ -9,8 +9,9 @@
   (``make_vec``, ``NesleVecEnv``, ``NesleEnv``), drop-in for ``nesle.env``;
 * ``nesle_amd.native_ppo``  GPU-resident PPO, drop-in for ``nesle.native_ppo``;
 * ``nesle_amd.memory``      operators of a policy with memory: per-head norm with
-  rotation, gated delta rule over a rollout and one token at a time;
-* ``nesle_amd.memory_ppo``  PPO with such a policy;
+  rotation, gated delta rule and linear attention with a decay over a rollout and one
+  token at a time, layer norm, sampling of actions;
+* ``nesle_amd.memory_ppo``  PPO with such a policy, and playing it;
 * ``nesle_amd.actions``     controller masks and action sets.
 
 The native pieces are imported on first use, so importing the package never

@@ -18,6 +18,15 @@
 // A product with a masked zero would still carry NaN, so where a key, a value or
 // (with an episode's end in the chunk) the state is not finite, the chunk is cut
 // before that token and at the ends: nothing of it reaches a token it must not.
+//
+// What bounds it.  Many heads: memory.  128 tokens of 512 consoles' 4 heads of 64 in
+// bfloat16 move 235 MB (inputs, results, states in, out and kept) in 62 us, 3.8 TB/s
+// against a large copy's 4.9; two chunks are too short a walk to hide their first loads
+// and last stores.  64 consoles take 17 us, in float32 23, in float32 with heads of 128
+// 42.  Few heads: the chain of chunks, 2 us each alone on a compute unit, which is why
+// long walks are cut (mem_decay_segments.h).  P made by every wave for itself costs
+// matrix time that is idle (18 us of 62 here) and saves a barrier.  The state is kept
+// every 64 tokens, where the gradient's chunks begin.
 #include "mem_decay_segments.h"
 
 namespace nesle::mem {

