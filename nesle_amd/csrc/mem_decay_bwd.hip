@@ -341,23 +341,32 @@ __global__ void __launch_bounds__(DP * 4 * kGradRoles<DP>, (kGradWaves<T, DP>)) 
     else grad_walk<T, DP, WIDE, false, true>(a, seg, partials, sh);
 }
 
-// dg of a head: the sum of its workgroups' shares, a workgroup a head.
-__global__ void __launch_bounds__(256) decay_gate_sum(const float* partials, float* dg, std::uint32_t heads, std::uint64_t all) {
+// dg of a head: the sum of its workgroups' shares, by a workgroup.
+__device__ __forceinline__ void gate_sum(const float* partials, float* dg, std::uint32_t h, std::uint32_t heads, std::uint64_t all) {
     __shared__ float sums[4];
     float sum = 0.0f;
-    for (std::uint64_t i = blockIdx.x + static_cast<std::uint64_t>(threadIdx.x) * heads; i < all; i += 256ull * heads) sum += partials[i];
+    for (std::uint64_t i = h + static_cast<std::uint64_t>(threadIdx.x) * heads; i < all; i += 256ull * heads) sum += partials[i];
     sum = over_groups(sum16(sum));
     if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) dg[blockIdx.x] = sums[0] + sums[1] + sums[2] + sums[3];
+    if (threadIdx.x == 0) dg[h] = sums[0] + sums[1] + sums[2] + sums[3];
+}
+__global__ void __launch_bounds__(256) decay_gate_sum(const float* partials, float* dg, std::uint32_t heads, std::uint64_t all) {
+    gate_sum(partials, dg, blockIdx.x, heads, all);
 }
 
-// dq and dk of a key head: the sum of its value heads' shares.
+// dq and dk of a key head: the sum of its value heads' shares; and, by the workgroups from
+// `blocks` on, the decays' sums (a launch of their own took 4 us more).
 template <typename T>
-__global__ void __launch_bounds__(256) decay_share_sum(DecayArgs<T> a, std::uint64_t quads) {
+__global__ void __launch_bounds__(256) decay_share_sum(DecayArgs<T> a, std::uint64_t quads, std::uint32_t blocks, const float* partials,
+                                                       std::uint64_t all_partials) {
+    if (blockIdx.x >= blocks) {
+        gate_sum(partials, a.dg, blockIdx.x - blocks, a.hv, all_partials);
+        return;
+    }
     const std::uint64_t all = static_cast<std::uint64_t>(a.steps) * a.batch * a.hv * a.dk_dim;
     const std::uint32_t per_head = a.dk_dim / 4;
-    for (std::uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < 2 * quads; i += gridDim.x * 256ull) {
+    for (std::uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < 2 * quads; i += blocks * 256ull) {
         const bool of_k = i >= quads;
         const std::uint64_t e = of_k ? i - quads : i, head = e / per_head;
         const float* from = a.scratch + (of_k ? all : 0) + head * a.group * a.dk_dim + 4 * (e % per_head);
@@ -393,13 +402,15 @@ int backward(const char* who, const nesle_decay_args& x, hipStream_t s) {
         case 64: launch_dim<T, 64, false>(a, seg, partials, s); break;
         default: launch_dim<T, 128, false>(a, seg, partials, s); break;
     }
+    const std::uint64_t all_partials = static_cast<std::uint64_t>(seg.count) * a.batch * a.hv;
     if (a.group > 1 && a.steps != 0) {
         const std::uint64_t quads = static_cast<std::uint64_t>(a.steps) * a.batch * a.hk * a.dk_dim / 4;
-        const std::uint64_t want = (2 * quads + 255) / 256;
-        hipLaunchKernelGGL(decay_share_sum<T>, dim3(static_cast<std::uint32_t>(want < 4096 ? want : 4096)), dim3(256), 0, s, a, quads);
+        const auto blocks = static_cast<std::uint32_t>(std::min<std::uint64_t>((2 * quads + 255) / 256, 4096));
+        hipLaunchKernelGGL(decay_share_sum<T>, dim3(blocks + (partials != nullptr ? a.hv : 0)), dim3(256), 0, s, a, quads, blocks, partials,
+                           all_partials);
+    } else if (partials != nullptr) {
+        hipLaunchKernelGGL(decay_gate_sum, dim3(a.hv), dim3(256), 0, s, partials, a.dg, a.hv, all_partials);
     }
-    if (partials != nullptr)
-        hipLaunchKernelGGL(decay_gate_sum, dim3(a.hv), dim3(256), 0, s, partials, a.dg, a.hv, static_cast<std::uint64_t>(seg.count) * a.batch * a.hv);
     return launched(who);
 }
 
