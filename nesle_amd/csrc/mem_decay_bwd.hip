@@ -392,7 +392,7 @@ void launch_dim(const DecayArgs<T>& a, const DecaySegments& seg, float* partials
 template <typename T>
 int backward(const char* who, const nesle_decay_args& x, hipStream_t s) {
     const DecayArgs<T> a = decay_args<T>(x);
-    DecaySegments seg = decay_segments(x);
+    DecaySegments seg = decay_segments(x, true);
     seg.place(x, a.scratch + share_floats(x));
     float* partials = a.dg == nullptr ? nullptr : a.scratch + share_floats(x) + seg.floats(x);
     const std::uint32_t dim = wide_rows(x) ? 0 : padded_dim(x);
@@ -429,7 +429,7 @@ extern "C" {
 
 std::uint64_t nesle_decay_scratch_floats(const nesle_decay_args* a) {
     if (a == nullptr || a->k_heads == 0 || a->batch == 0 || a->v_heads == 0) return 0;
-    const DecaySegments seg = decay_segments(*a);
+    const DecaySegments seg = decay_segments(*a, true);
     return share_floats(*a) + seg.floats(*a) + static_cast<std::uint64_t>(seg.count) * a->batch * a->v_heads;
 }
 
@@ -449,7 +449,7 @@ int nesle_decay_backward(const nesle_decay_args* a, void* stream) {
         if (!a->dout.data || !a->dq || !a->dk || !a->dv || (!a->saved && nesle_decay_saved_floats(a) != 0))
             return refuse(who, "null device pointer");
     }
-    if (!a->scratch && ((a->steps != 0 && a->v_heads > a->k_heads) || decay_segments(*a).count > 1 || a->dg)) return refuse(who, "null device pointer");
+    if (!a->scratch && ((a->steps != 0 && a->v_heads > a->k_heads) || decay_segments(*a, true).count > 1 || a->dg)) return refuse(who, "null device pointer");
     return a->dtype == NESLE_MEM_F32 ? backward<float>(who, *a, s) : backward<bf16>(who, *a, s);
 }
 

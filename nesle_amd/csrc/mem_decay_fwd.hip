@@ -74,9 +74,8 @@ __global__ void __launch_bounds__(DP * 4, kForwardWaves<DP>) decay_forward_kerne
     sh.powers.make(gate, a.scale, always, first.tid);
     if (first.tid < 4) sh.bad[first.tid / 2][first.tid % 2] = 0;
     f4 S[KT];
-    const float* from = seg.count > 1 ? seg.states + (static_cast<std::size_t>(blockIdx.y) * gridDim.x + head) * state_size
-                                      : a.state == nullptr ? nullptr : a.state + head * state_size;
-    load_value_slab<DP>(from, dk, dv, first, S);
+    if (seg.count <= kAlone) gather_state<DP>(seg, a.state, gate, blockIdx.y, gridDim.x, head, dk, dv, first, S);
+    else load_value_slab<DP>(seg.states + (static_cast<std::size_t>(blockIdx.y) * gridDim.x + head) * state_size, dk, dv, first, S);
     __syncthreads();
     PairPowers<CH, false> pair;
     pair.make(sh.powers, a.scale, first.r, first.g);
@@ -202,7 +201,7 @@ void launch_dim(const DecayArgs<T>& a, const DecaySegments& seg, hipStream_t s) 
 template <typename T>
 int forward(const char* who, const nesle_decay_args& x, hipStream_t s) {
     const DecayArgs<T> a = decay_args<T>(x);
-    DecaySegments seg = decay_segments(x);
+    DecaySegments seg = decay_segments(x, false);
     seg.place(x, a.scratch);
     const std::uint32_t dim = wide_rows(x) ? 0 : padded_dim(x);
     switch (dim) {
@@ -229,7 +228,7 @@ std::uint64_t nesle_decay_saved_floats(const nesle_decay_args* a) {
 
 std::uint64_t nesle_decay_forward_scratch_floats(const nesle_decay_args* a) {
     if (a == nullptr || a->batch == 0 || a->v_heads == 0) return 0;
-    return decay_segments(*a).floats(*a);
+    return decay_segments(*a, false).floats(*a);
 }
 
 int nesle_decay_forward(const nesle_decay_args* a, void* stream) {

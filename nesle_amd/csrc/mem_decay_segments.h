@@ -2,8 +2,9 @@
 // at once.
 //
 // A segment of L tokens takes the state before it to a^L S + B, with B from its keys
-// and values alone.  One launch finds every segment's B, one takes the state through
-// the segments, and then the walk runs from each segment's own state.  The gradient of
+// and values alone.  One launch finds every segment's B, one, or the walk where there
+// are few, takes the state through the segments, and then the walk runs from each
+// segment's own state.  The gradient of
 // the state goes the same way backwards, with queries and the outputs' gradients.
 #pragma once
 
@@ -29,23 +30,25 @@ struct DecaySegments {
 constexpr std::uint32_t kMostSegments = 128;      // what one workgroup takes a state through
 
 // As many segments as the card holds their workgroups at once with room to spare: 1,024,
-// 512 and 256 heads' of 32, 64 and 128 dimensions.  Two launches more and the second reading
-// of keys and values are worth it from 8 chunks on, from 16 where that makes only two or
-// three segments.  One walk / segments, us of the forward's launches in bfloat16 (* where
-// the rule walks whole):
-//   64 dimensions, 256 tokens of 64 heads* 23 / 20 and two launches; 512 of 64 heads 40 / 24,
-//   of 128 42 / 32, of 256* 43 / 45; 1,024 of 64 heads 76 / 33, of 128 77 / 47, of 256 79 / 72;
-//   8,191 of 8 heads 551 / 32; 128 dimensions, 256 of 64 heads* 36 / 28, 512 65 / 39, 1,024
-//   of 64 heads 124 / 61, of 128 127 / 99; 32 dimensions, 1,024 of 64 heads 63 / 24, of 256
-//   66 / 44.
+// 512 and 256 heads' of 32, 64 and 128 dimensions.  The launch more, or two, and the second
+// reading of the inputs are worth it from 3 times 64 tokens on forward and from 8 in the
+// gradient, from 8 in both where that makes only two or three segments.  One walk /
+// segments, us a call, bfloat16, float32, and bfloat16 with gradient (from the host, whose
+// part is 85 and 95; * where the rule walks whole):
+//   64 dimensions, 64 heads, 128 tokens* 14 / 14, 19 / 18, 88 / 100; 192 18 / 14, 27 / 18; 256
+//   22 / 15, 34 / 19, 87 / 98*; 512 40 / 18, 63 / 27, 114 / 98; 1,024 74 / 27, 122 / 42, 215 / 77;
+//   256 heads, 256 tokens* 24 / 25, 35 / 38; 512 42 / 38, 65 / 66, 121 / 112; 1,024 77 / 66, 125 / 121,
+//   237 / 203; 128 dimensions, 64 heads, 256 tokens 36 / 24, 62 / 34, 130 / 98*; 512 66 / 35, 118 /
+//   55, 246 / 112; 32 dimensions, 256 heads, 256 tokens 20 / 15, 25 / 19, 54 / 99*; 1,024 65 / 40,
+//   86 / 50, 179 / 112.
 // Segments of 64 dimensions for 1,024 heads at once: 1,024 tokens of 64 heads 33 -> 37, 8,191
 // of 8 32 -> 34; for 256: 38 and 37.
-inline DecaySegments decay_segments(const nesle_decay_args& a) {
+inline DecaySegments decay_segments(const nesle_decay_args& a, bool back) {
     constexpr std::uint32_t kSpan = 64;            // tokens: a multiple of any chunk length
     const std::uint64_t heads = static_cast<std::uint64_t>(a.batch) * a.v_heads, at_once = (1u << 15) / padded_dim(a);
     const std::uint32_t spans = (a.steps + kSpan - 1) / kSpan;
     std::uint32_t count = 1;
-    if (2 * heads <= at_once && spans >= (4 * heads <= at_once ? 8u : 16u))
+    if (2 * heads <= at_once && spans >= (!back && 4 * heads <= at_once ? 3u : 8u))
         count = static_cast<std::uint32_t>(std::min<std::uint64_t>({spans, kMostSegments, at_once / heads}));
     const std::uint32_t each = count < 2 ? spans : (spans + count - 1) / count;
     DecaySegments s{};
@@ -139,16 +142,42 @@ __global__ void __launch_bounds__(DP * 4, DP == 128 ? 2 : 4) decay_local_kernel(
 // ---- the state through the segments -------------------------------------------------
 
 // S <- a^L S + B from segment to segment; a segment that drops the state inside leaves
-// B alone, whatever S held.  B gives way to the state before the segment (BACK: the
-// gradient after it).  A lane has four elements of a state and reads its share of the
-// segments at once: all of them (GROUPS 1, up to 16 segments), or an equal share of 16
+// B alone, whatever S held.
+//
+// Forward, up to 16 segments: each workgroup of the walk takes the state through the ones
+// before its own by itself, and a launch less pays for that.  The forward's launches, 1,024
+// tokens of 64, 128 and 32 heads of 64 in bfloat16 (8, 4 and 16 segments): 32 -> 29, 48 ->
+// 44 and 26 -> 24 us.  Not the gradient, which needs dS twice, by key and by value: even
+// with 8 segments, 38 -> 44 us with 16, and 5 % slower where there is but one.
+constexpr std::uint32_t kAlone = 16;
+template <int DP>
+__device__ __forceinline__ void gather_state(const DecaySegments& seg, const float* start, float gate, std::uint32_t segment, std::size_t heads,
+                                             std::size_t head, int dk, int dv, const Place<DP>& at, f4 (&S)[DP / 16]) {
+    const std::size_t size = static_cast<std::size_t>(dk) * dv;
+    load_value_slab<DP>(start == nullptr ? nullptr : start + head * size, dk, dv, at, S);
+    const float factor = expf(static_cast<float>(seg.steps) * gate);
+#pragma unroll 2
+    for (std::uint32_t i = 0; i < segment; ++i) {
+        const std::size_t slot = i * heads + head;
+        f4 B[DP / 16];
+        load_value_slab<DP>(seg.states + slot * size, dk, dv, at, B);
+        const bool dropped = seg.dropped[slot] != 0;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) S[k] = dropped ? B[k] : S[k] * factor + B[k];
+    }
+}
+
+// Else a launch of their own, after which B has given way to the state before the segment
+// (BACK: the gradient after it).  A lane has four elements of a state and reads its share
+// of the segments at once: all of them (GROUPS 1, up to 8 segments), or an equal share of 16
 // groups', joined through LDS, after which every group walks its own from where the ones
-// before it end.
-constexpr int kAlone = 16;
+// before it end.  16 groups / one: 4 segments of 128 heads of 64 18 / 6 us, 8 of 64 11 / 7, 16
+// of 32 8 / 10.
+constexpr std::uint32_t kFew = 8;
 template <bool BACK, int GROUPS>
 __global__ void __launch_bounds__(256) decay_join_kernel(DecaySegments seg, const float* start, const float* g, std::uint32_t hv,
                                                          std::uint32_t size, std::uint32_t last_steps) {
-    constexpr int kShare = GROUPS == 1 ? kAlone : kMostSegments / GROUPS, kLanes = 256 / GROUPS;
+    constexpr int kShare = GROUPS == 1 ? kFew : kMostSegments / GROUPS, kLanes = 256 / GROUPS;
     __shared__ f4 sums[GROUPS][kLanes];
     __shared__ float factors[GROUPS];                      // negative: dropped
     const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
@@ -201,9 +230,10 @@ template <typename T, int DP, bool WIDE, bool BACK>
 void launch_states(const DecayArgs<T>& a, const DecaySegments& seg, hipStream_t s) {
     const std::uint32_t heads = a.batch * a.hv, size = a.dk_dim * a.dv_dim;
     hipLaunchKernelGGL((decay_local_kernel<T, DP, WIDE, BACK>), dim3(heads, seg.count - 1), dim3(DP * 4), 0, s, a, seg);
+    if (!BACK && seg.count <= kAlone) return;
     const float* start = BACK ? a.dstate_out : a.state;
     const std::uint32_t last = a.steps - (seg.count - 1) * seg.steps;
-    if (seg.count <= kAlone)
+    if (BACK && seg.count <= kFew)
         hipLaunchKernelGGL((decay_join_kernel<BACK, 1>), dim3(heads, (size + 1023) / 1024), dim3(256), 0, s, seg, start, a.g, a.hv, size, last);
     else
         hipLaunchKernelGGL((decay_join_kernel<BACK, 16>), dim3(heads, (size + 63) / 64), dim3(256), 0, s, seg, start, a.g, a.hv, size, last);

@@ -58,6 +58,26 @@ def test_decay_equal_keys(dim):
         M.check_decay(*M.make(150, 2, 1, 2, dim, dim, dtype, 7, resets=0.0, alike=1.0))
 
 
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("shape,segments", [((513, 16, 2, 4, 64, 64), 5), ((470, 32, 2, 4, 64, 48), 4), ((449, 32, 4, 4, 32, 32), 8),
+                                            ((460, 8, 2, 4, 72, 128), 8), ((450, 16, 4, 4, 128, 40), 4), ((1000, 4, 4, 4, 64, 64), 16)])
+def test_decay_few_segments(shape, segments, dtype):
+    """2 to 16 segments: the state before one, and the gradient after one, are found in
+    other ways than of many."""
+    import ctypes
+
+    from nesle_amd import abi
+
+    say(f"[gpu] decay_attention {segments} segments {shape} {dtype}")
+    a = abi.DecayArgs(abi.MEM_F32 if dtype == torch.float32 else abi.MEM_BF16, *shape, 1.0)
+    floats = abi.lib().nesle_decay_forward_scratch_floats(ctypes.byref(a))
+    assert floats == segments * shape[1] * shape[3] * (shape[4] * shape[5] + 1)
+    x, resets, grads = M.make(*shape, dtype, 50 + segments, resets=0.002)
+    M.check_decay(x, resets, grads)
+    x["state"] = None
+    M.check_decay(x, None, grads)
+
+
 def test_decay_offsets_past_32_bits():
     """Queries, keys and values whose steps lie 2^31 elements apart."""
     from nesle_amd import memory
