@@ -29,7 +29,8 @@
 // each, and shared through LDS, turned round: [j][i].
 //
 // No atomics: the decays' gradient is added up per workgroup, then over workgroups
-// in a fixed order.
+// in a fixed order; in float64 from a part's sum on, as a head's consoles and tokens may
+// nearly cancel.
 //
 // What bounds it: 128 tokens of 512 consoles' 4 heads of 64 in bfloat16 take 140 us, where
 // the 370 MB they move take 76 at a large copy's rate, the matrix instructions 19 and all
@@ -47,6 +48,11 @@ namespace nesle::mem {
 namespace {
 
 constexpr int kPart = 32;
+
+__device__ double lanes_sum(double v) {
+    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+    return v;
+}
 
 // Two waves for 16 columns where their registers leave room for it.
 template <int DP>
@@ -71,13 +77,13 @@ struct GradTile {
     f4 before[ROLES == 1 ? 1 : DP / 16][DP / 16][64];              // the state before a part, from role to role
     Powers<kPart> powers;
     alignas(16) int episodes[kPart];
-    float sums[ROLES * DP / 16];
+    double sums[ROLES * DP / 16];
 };
 
 // The walk of a wave that has dQ and the pairs, dK, dV and dS, or both.  The waves of
 // either kind meet at the same barriers.
 template <typename T, int DP, bool WIDE, bool HAS_Q, bool HAS_KV>
-__device__ __forceinline__ void grad_walk(const DecayArgs<T>& a, const DecaySegments& seg, float* partials, GradTile<T, DP>& sh) {
+__device__ __forceinline__ void grad_walk(const DecayArgs<T>& a, const DecaySegments& seg, double* partials, GradTile<T, DP>& sh) {
     using Tile = GradTile<T, DP>;
     constexpr int CH = Tile::CH, ROLES = Tile::ROLES, PARTS = CH / kPart, KT = DP / 16, KP = DP / 32, CT = kPart / 16, kWaves = DP / 16;
     using M = typename Tile::M;
@@ -126,7 +132,7 @@ __device__ __forceinline__ void grad_walk(const DecayArgs<T>& a, const DecaySegm
             sh.r.put(16 + 4 * first.g + i, first.r, 0.0f);
         }
 
-    float decay = 0.0f;                    // this lane's share of the decay's gradient
+    double decay = 0.0;                    // this lane's share of the decay's gradient
     for (std::uint32_t t1 = end; t1 > begin;) {
         At at = At::anew();
         const std::uint32_t start = (t1 - 1) / CH * CH;
@@ -170,6 +176,7 @@ __device__ __forceinline__ void grad_walk(const DecayArgs<T>& a, const DecaySegm
                 if (at.tid < kPart) sh.episodes[at.tid] = seen.episode(at.tid);
                 __syncthreads();
             }
+            float here = 0.0f;             // of it, this part's
             const float whole = seen.whole(sh.powers), row4 = static_cast<float>(4 * g);
             f4 before[KT], dK[CT] = {}, dV[CT] = {};
             if constexpr (HAS_Q) {
@@ -187,7 +194,7 @@ __device__ __forceinline__ void grad_walk(const DecayArgs<T>& a, const DecaySegm
                     pair.make(sh.powers, a.scale, r, g);
                     x = pair.weigh(x, it, jt, seen, sh.episodes, r, g);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) decay += (row4 + static_cast<float>(16 * (it - jt) + e - r)) * x[e] * y[e];
+                    for (int e = 0; e < 4; ++e) here += (row4 + static_cast<float>(16 * (it - jt) + e - r)) * x[e] * y[e];
                     y = pair.weigh(y, it, jt, seen, sh.episodes, r, g);
                     sh.p.put4(16 * jt + r, 16 * it + 4 * g, x);
                     sh.r.put4(16 * jt + r, 16 * it + 4 * g, y);
@@ -233,7 +240,7 @@ __device__ __forceinline__ void grad_walk(const DecayArgs<T>& a, const DecaySegm
                     dK[m] *= out;
                     dV[m] *= out;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) decay += (static_cast<float>(seen.n - 1 - 16 * m - e) - row4) * K[m][e] * dK[m][e];
+                    for (int e = 0; e < 4; ++e) here += (static_cast<float>(seen.n - 1 - 16 * m - e) - row4) * K[m][e] * dK[m][e];
                 }
             }
             __syncthreads();
@@ -252,7 +259,7 @@ __device__ __forceinline__ void grad_walk(const DecayArgs<T>& a, const DecaySegm
                 for (int m = 0; m < CT; ++m) {
                     x[m] *= seen.in(sh.powers, 16 * m + 4 * g);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) decay += (row4 + static_cast<float>(16 * m + e + 1)) * Q[m][e] * x[m][e];
+                    for (int e = 0; e < 4; ++e) here += (row4 + static_cast<float>(16 * m + e + 1)) * Q[m][e] * x[m][e];
                     x[m] = M::mul(sh.r.cols(0, 16 * m, r, g), key, x[m]);
                     share(false, tile0 + m, x[m]);
                     done_q[tile0 + m] = Done::tile(x[m]);
@@ -267,7 +274,7 @@ __device__ __forceinline__ void grad_walk(const DecayArgs<T>& a, const DecaySegm
 #pragma unroll
                         for (int e = 0; e < 4; ++e) held += by_key[i][e] * s[e];
                     }
-                    decay += static_cast<float>(seen.n) * whole * held;
+                    here += static_cast<float>(seen.n) * whole * held;
                 }
                 // dK and dV within the part, and the two slabs of dS before it.
                 f4 x[CT];
@@ -301,6 +308,7 @@ __device__ __forceinline__ void grad_walk(const DecayArgs<T>& a, const DecaySegm
                 for (int i = 0; i < KT; ++i)
                     by_value[i] = dropped ? zero : M::mul(sh.q.in.cols(row0, 16 * i, r, g), read, by_value[i] * whole);
             }
+            decay += here;
             __syncthreads();               // P, R and, in the end, the inputs have been read
         }
         const std::int64_t key_step = static_cast<std::int64_t>(a.batch) * a.hk * a.dk_dim;
@@ -322,11 +330,11 @@ __device__ __forceinline__ void grad_walk(const DecayArgs<T>& a, const DecaySegm
     }
     if (HAS_KV && a.dstate != nullptr && begin == 0) store_key_slab<DP>(a.dstate + head * state_size, dk_dim, dv_dim, At::anew(), by_key);
     if (partials != nullptr) {
-        decay = over_groups(sum16(decay));
+        decay = lanes_sum(decay);
         if (first.lane == 0) sh.sums[first.role * kWaves + first.wave] = decay;
         __syncthreads();
         if (first.tid == 0) {
-            float sum = 0.0f;
+            double sum = 0.0;
             for (int w = 0; w < ROLES * kWaves; ++w) sum += sh.sums[w];
             partials[slot] = sum;
         }
@@ -334,7 +342,7 @@ __device__ __forceinline__ void grad_walk(const DecayArgs<T>& a, const DecaySegm
 }
 
 template <typename T, int DP, bool WIDE>
-__global__ void __launch_bounds__(DP * 4 * kGradRoles<DP>, (kGradWaves<T, DP>)) decay_backward_kernel(DecayArgs<T> a, DecaySegments seg, float* partials) {
+__global__ void __launch_bounds__(DP * 4 * kGradRoles<DP>, (kGradWaves<T, DP>)) decay_backward_kernel(DecayArgs<T> a, DecaySegments seg, double* partials) {
     __shared__ GradTile<T, DP> sh;
     if constexpr (kGradRoles<DP> == 1) grad_walk<T, DP, WIDE, true, true>(a, seg, partials, sh);
     else if (Place<DP, kGradRoles<DP>>().role == 0) grad_walk<T, DP, WIDE, true, false>(a, seg, partials, sh);
@@ -342,23 +350,23 @@ __global__ void __launch_bounds__(DP * 4 * kGradRoles<DP>, (kGradWaves<T, DP>)) 
 }
 
 // dg of a head: the sum of its workgroups' shares, by a workgroup.
-__device__ __forceinline__ void gate_sum(const float* partials, float* dg, std::uint32_t h, std::uint32_t heads, std::uint64_t all) {
-    __shared__ float sums[4];
-    float sum = 0.0f;
+__device__ __forceinline__ void gate_sum(const double* partials, float* dg, std::uint32_t h, std::uint32_t heads, std::uint64_t all) {
+    __shared__ double sums[4];
+    double sum = 0.0;
     for (std::uint64_t i = h + static_cast<std::uint64_t>(threadIdx.x) * heads; i < all; i += 256ull * heads) sum += partials[i];
-    sum = over_groups(sum16(sum));
+    sum = lanes_sum(sum);
     if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) dg[h] = sums[0] + sums[1] + sums[2] + sums[3];
+    if (threadIdx.x == 0) dg[h] = static_cast<float>(sums[0] + sums[1] + sums[2] + sums[3]);
 }
-__global__ void __launch_bounds__(256) decay_gate_sum(const float* partials, float* dg, std::uint32_t heads, std::uint64_t all) {
+__global__ void __launch_bounds__(256) decay_gate_sum(const double* partials, float* dg, std::uint32_t heads, std::uint64_t all) {
     gate_sum(partials, dg, blockIdx.x, heads, all);
 }
 
 // dq and dk of a key head: the sum of its value heads' shares; and, by the workgroups from
 // `blocks` on, the decays' sums (a launch of their own took 4 us more).
 template <typename T>
-__global__ void __launch_bounds__(256) decay_share_sum(DecayArgs<T> a, std::uint64_t quads, std::uint32_t blocks, const float* partials,
+__global__ void __launch_bounds__(256) decay_share_sum(DecayArgs<T> a, std::uint64_t quads, std::uint32_t blocks, const double* partials,
                                                        std::uint64_t all_partials) {
     if (blockIdx.x >= blocks) {
         gate_sum(partials, a.dg, blockIdx.x - blocks, a.hv, all_partials);
@@ -382,8 +390,11 @@ std::uint64_t share_floats(const nesle_decay_args& a) {
     return (floats + 3) / 4 * 4;
 }
 
+// A float64 sum a workgroup follows.
+std::uint64_t ahead_of_partials(const nesle_decay_args& a, const DecaySegments& seg) { return (share_floats(a) + seg.floats(a) + 1) / 2 * 2; }
+
 template <typename T, int DP, bool WIDE>
-void launch_dim(const DecayArgs<T>& a, const DecaySegments& seg, float* partials, hipStream_t s) {
+void launch_dim(const DecayArgs<T>& a, const DecaySegments& seg, double* partials, hipStream_t s) {
     if (seg.count > 1) launch_states<T, DP, WIDE, true>(a, seg, s);
     hipLaunchKernelGGL((decay_backward_kernel<T, DP, WIDE>), dim3(a.batch * a.hv, seg.count), dim3(DP * 4 * kGradRoles<DP>), 0, s, a, seg,
                        partials);
@@ -394,7 +405,7 @@ int backward(const char* who, const nesle_decay_args& x, hipStream_t s) {
     const DecayArgs<T> a = decay_args<T>(x);
     DecaySegments seg = decay_segments(x, true);
     seg.place(x, a.scratch + share_floats(x));
-    float* partials = a.dg == nullptr ? nullptr : a.scratch + share_floats(x) + seg.floats(x);
+    double* partials = a.dg == nullptr ? nullptr : reinterpret_cast<double*>(a.scratch + ahead_of_partials(x, seg));
     const std::uint32_t dim = wide_rows(x) ? 0 : padded_dim(x);
     switch (dim) {
         case 0: launch_dim<T, 128, true>(a, seg, partials, s); break;
@@ -430,7 +441,7 @@ extern "C" {
 std::uint64_t nesle_decay_scratch_floats(const nesle_decay_args* a) {
     if (a == nullptr || a->k_heads == 0 || a->batch == 0 || a->v_heads == 0) return 0;
     const DecaySegments seg = decay_segments(*a, true);
-    return share_floats(*a) + seg.floats(*a) + static_cast<std::uint64_t>(seg.count) * a->batch * a->v_heads;
+    return ahead_of_partials(*a, seg) + 2ull * seg.count * a->batch * a->v_heads;
 }
 
 int nesle_decay_backward(const nesle_decay_args* a, void* stream) {

@@ -78,6 +78,29 @@ def test_decay_few_segments(shape, segments, dtype):
     M.check_decay(x, None, grads)
 
 
+def test_decay_gradient_of_one_number():
+    """One head: its decay's gradient is one number, over 64 to 6,000 terms of either sign
+    that nearly cancel in places.  Each term is off by a few 2^-24 of itself, and they are
+    added in float64 from 32 tokens of a lane on: 2^-22 of their 2-norm, with room for 4
+    standard deviations of 20 draws.  The terms by the definition: one console's each."""
+    from nesle_amd import memory
+
+    for seed in range(10):
+        for T, N in ((1, 64), (70, 30)):
+            say(f"[gpu] decay_attention decay's gradient {seed} {T} {N}")
+            x, _, grads = M.make(T, N, 1, 1, 48, 48, torch.float32, seed, resets=0.0)
+            ref = [x[n].double() for n in NAMES]
+            ref[3] = ref[3].expand(N, 1).clone().requires_grad_()
+            # A decay of its own for each console.
+            each = torch.stack([torch.autograd.grad(O.decay(*(t[:, n:n + 1] for t in ref[:3]), ref[3][n], ref[4][n:n + 1], None, 48 ** -0.5),
+                                                    ref[3], [grads[0][:, n:n + 1].double(), grads[1][n:n + 1].double()])[0][n]
+                                for n in range(N)])
+            gpu = [x[n].to(dev()) for n in NAMES]
+            gpu[3].requires_grad_()
+            got = torch.autograd.grad(memory.decay_attention(*gpu[:4], state=gpu[4]), gpu[3], [t.to(dev()) for t in grads])[0]
+            assert abs(float(got) - float(each.sum())) <= 2.0 ** -22 * float(each.norm()) + 2.0 ** -24 * abs(float(each.sum())), (seed, T)
+
+
 def test_decay_offsets_past_32_bits():
     """Queries, keys and values whose steps lie 2^31 elements apart."""
     from nesle_amd import memory
