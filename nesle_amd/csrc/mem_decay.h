@@ -97,13 +97,17 @@ inline int check_decay(const char* who, const nesle_decay_args* a) {
     return NESLE_OK;
 }
 
-// Pointers that a call over at least one token and console needs.
-inline int check_decay_inputs(const char* who, const nesle_decay_args* a) {
-    if (!a->q.data || !a->k.data || !a->v.data || !a->g) return refuse(who, "null device pointer");
+inline int check_decay_alignment(const char* who, const nesle_decay_args* a) {
     if (!aligned16(a->state) || !aligned16(a->state_out) || !aligned16(a->saved) || !aligned16(a->dstate_out) ||
         !aligned16(a->dstate) || !aligned16(a->scratch) || !aligned16(a->out) || !aligned16(a->dq) || !aligned16(a->dk) ||
         !aligned16(a->dv))
         return refuse(who, "states, outputs and workspaces must lie on 16-byte boundaries");
+    return NESLE_OK;
+}
+
+// Pointers that a call over at least one token and console needs.
+inline int check_decay_inputs(const char* who, const nesle_decay_args* a) {
+    if (!a->q.data || !a->k.data || !a->v.data || !a->g) return refuse(who, "null device pointer");
     return NESLE_OK;
 }
 

@@ -454,6 +454,8 @@ int nesle_decay_backward(const nesle_decay_args* a, void* stream) {
         hipLaunchKernelGGL(decay_gate_zero, dim3((a->v_heads + 255) / 256), dim3(256), 0, s, a->dg, a->v_heads);
         return launched(who);
     }
+    rc = check_decay_alignment(who, a);
+    if (rc != NESLE_OK) return rc;
     if (a->steps != 0) {
         rc = check_decay_inputs(who, a);
         if (rc != NESLE_OK) return rc;

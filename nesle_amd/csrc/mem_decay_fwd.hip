@@ -236,6 +236,8 @@ int nesle_decay_forward(const nesle_decay_args* a, void* stream) {
     int rc = check_decay(who, a);
     if (rc != NESLE_OK || a->batch == 0) return rc;
     if (!a->state_out) return refuse(who, "null device pointer");
+    rc = check_decay_alignment(who, a);
+    if (rc != NESLE_OK) return rc;
     if (a->steps != 0) {
         rc = check_decay_inputs(who, a);
         if (rc != NESLE_OK) return rc;

@@ -92,7 +92,8 @@ extern "C" int nesle_decay_step(const nesle_decay_args* a, void* stream) {
     if (rc != NESLE_OK) return rc;
     if (a->steps != 1) return refuse(who, "steps must be 1");
     if (a->batch == 0) return NESLE_OK;
-    rc = check_decay_inputs(who, a);
+    rc = check_decay_alignment(who, a);
+    if (rc == NESLE_OK) rc = check_decay_inputs(who, a);
     if (rc != NESLE_OK) return rc;
     if (!a->out || !a->state_out) return refuse(who, "null device pointer");
     const auto s = static_cast<hipStream_t>(stream);

@@ -50,6 +50,9 @@ def test_decay_entries_refuse(entry):
     for n in "qkv":
         setattr(a, n, abi.Heads(16, 1, 1, 1))
     refusal(fn, a, "16-byte")
+    if entry != "nesle_decay_step":        # without a token too
+        refusal(fn, decay_args(steps=0, state=8, state_out=16), "16-byte")
+        refusal(fn, decay_args(steps=0, state_out=16, dg=16, scratch=8), "16-byte")
 
 
 def test_decay_workspaces():
