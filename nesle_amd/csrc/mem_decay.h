@@ -64,11 +64,25 @@ inline std::uint32_t padded_dim(const nesle_decay_args& a) {
 template <typename T>
 constexpr int kDecayChunk = sizeof(T) == 2 ? 64 : 32;
 // Tokens between the states that the forward keeps and the gradient takes up: a chunk of
-// the gradient, as many as leave room in LDS.
+// the gradient, as many as leave room in LDS.  A matter of type and dimension alone:
+// strides, which may differ between the two calls (the outputs' gradient has its own),
+// have no part in it.
 template <typename T, int DP>
 constexpr int kDecaySpan = sizeof(T) == 4 && DP == 128 ? 32 : 64;
+
+// f of the dimension that the kernels for these arguments are made for.
+template <typename F>
+auto at_dim(const nesle_decay_args& a, F&& f) {
+    switch (padded_dim(a)) {
+        case 32: return f(std::integral_constant<int, 32>());
+        case 64: return f(std::integral_constant<int, 64>());
+        default: return f(std::integral_constant<int, 128>());
+    }
+}
 inline std::uint32_t decay_span(const nesle_decay_args& a) {
-    return a.dtype == NESLE_MEM_F32 && padded_dim(a) == 128 ? kDecaySpan<float, 128> : kDecaySpan<float, 64>;
+    return at_dim(a, [&](auto dim) -> std::uint32_t {
+        return a.dtype == NESLE_MEM_F32 ? kDecaySpan<float, dim()> : kDecaySpan<bf16, dim()>;
+    });
 }
 
 // Whether 64 rows of any tensor span 2^31 bytes or more, past what a

@@ -406,13 +406,10 @@ int backward(const char* who, const nesle_decay_args& x, hipStream_t s) {
     DecaySegments seg = decay_segments(x, true);
     seg.place(x, a.scratch + share_floats(x));
     double* partials = a.dg == nullptr ? nullptr : reinterpret_cast<double*>(a.scratch + ahead_of_partials(x, seg));
-    const std::uint32_t dim = wide_rows(x) ? 0 : padded_dim(x);
-    switch (dim) {
-        case 0: launch_dim<T, 128, true>(a, seg, partials, s); break;
-        case 32: launch_dim<T, 32, false>(a, seg, partials, s); break;
-        case 64: launch_dim<T, 64, false>(a, seg, partials, s); break;
-        default: launch_dim<T, 128, false>(a, seg, partials, s); break;
-    }
+    at_dim(x, [&](auto dim) {
+        if (wide_rows(x)) launch_dim<T, dim(), true>(a, seg, partials, s);
+        else launch_dim<T, dim(), false>(a, seg, partials, s);
+    });
     const std::uint64_t all_partials = static_cast<std::uint64_t>(seg.count) * a.batch * a.hv;
     if (a.group > 1 && a.steps != 0) {
         const std::uint64_t quads = static_cast<std::uint64_t>(a.steps) * a.batch * a.hk * a.dk_dim / 4;

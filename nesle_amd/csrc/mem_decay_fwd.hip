@@ -203,13 +203,10 @@ int forward(const char* who, const nesle_decay_args& x, hipStream_t s) {
     const DecayArgs<T> a = decay_args<T>(x);
     DecaySegments seg = decay_segments(x, false);
     seg.place(x, a.scratch);
-    const std::uint32_t dim = wide_rows(x) ? 0 : padded_dim(x);
-    switch (dim) {
-        case 0: launch_dim<T, 128, true>(a, seg, s); break;
-        case 32: launch_dim<T, 32, false>(a, seg, s); break;
-        case 64: launch_dim<T, 64, false>(a, seg, s); break;
-        default: launch_dim<T, 128, false>(a, seg, s); break;
-    }
+    at_dim(x, [&](auto dim) {
+        if (wide_rows(x)) launch_dim<T, dim(), true>(a, seg, s);
+        else launch_dim<T, dim(), false>(a, seg, s);
+    });
     return launched(who);
 }
 
