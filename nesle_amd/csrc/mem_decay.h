@@ -238,11 +238,13 @@ struct Powers {
     __device__ float at(int n) const { return down[CH - 1 - n]; }       // a^n, n < CH
 };
 
-// Which tokens of a chunk of n see what: `drops` as above, zero nearly always.
+// Which tokens of a chunk of n see what: `drops` as above, zero nearly always.  Rows from
+// n on weigh nothing, by selection: their inputs are zeros, but a decay that grows may
+// have infinite powers there, and zero times one is NaN in sums over rows.
 struct Seen {
     std::uint64_t drops;
-    int n, first, last;        // tokens; the first and the last that drop the state
-    __device__ Seen(std::uint64_t d, int count) : drops(d), n(count), first(64), last(0) {
+    int n, first, last;        // tokens; the first and the last that drop the state (n, 0: none)
+    __device__ Seen(std::uint64_t d, int count) : drops(d), n(count), first(count), last(0) {
         if (d != 0) {
             first = __ffsll(static_cast<long long>(d)) - 1;
             last = 63 - __clzll(static_cast<long long>(d));
@@ -255,7 +257,7 @@ struct Seen {
     template <int CH>
     __device__ f4 in(const Powers<CH>& p, int row) const {
         f4 v = *reinterpret_cast<const f4*>(p.read + row);
-        if (drops != 0)
+        if (first < CH)
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = row + e < first ? v[e] : 0.0f;
         return v;
@@ -307,6 +309,9 @@ struct PairPowers {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (LATER_ROWS ? 4 * g + e < r : r < 4 * g + e) x[e] = 0.0f;
+        if (LATER_ROWS && seen.n < CH)     // (else such a row is a column, which is not written)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = 16 * it + 4 * g + e < seen.n ? x[e] : 0.0f;
         if (seen.drops != 0) {
             using i4 = int __attribute__((ext_vector_type(4)));
             const i4 rows = *reinterpret_cast<const i4*>(episodes + 16 * (LATER_ROWS ? it : jt) + 4 * g);

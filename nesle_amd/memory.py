@@ -141,7 +141,10 @@ def decay_attention(q, k, v, g, *, state=None, resets=None, scale: float | None 
     Differentiable in q, k, v, g and state.  No value of a dropped state, and
     nothing that is not finite in a later token, reaches an output it does not
     belong to; the gradient of inputs that are not finite is unspecified, and so is
-    a chunk of 64 tokens of a head in which finite inputs overflow float32.  Products
+    a chunk of 64 tokens of a head in which finite inputs overflow float32.  A g above
+    0 is taken as it is, and the state grows; from where exp(n g) overflows float32, for
+    n tokens of a chunk, or of the few chunks that a long walk is cut into, without an
+    episode's end among them, results are unspecified until one ends.  Products
     keep float32 precision for either type: bfloat16 results are rounded once."""
     return _called(_native.decay_attention, q, k, v, g, state, resets, scale)
 
