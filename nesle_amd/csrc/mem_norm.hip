@@ -2,8 +2,10 @@
 //
 // A row is held in the registers of a group of lanes, so it is read once, its mean
 // and then the mean of squares about it are sums over the group (two steps: a sum of
-// squares less the squared mean would cancel where a row's level is large), and the
-// result is written once.  With xh = (x - mean) rstd and d = dy weight, the gradient is
+// squares less the squared mean would cancel where a row's level is large; the second
+// step also sums the differences, which corrects the mean's rounding, and costs nothing to
+// 3 % of a call, 7 % with rows of 64), and the result is written once.  With
+// xh = (x - mean) rstd and d = dy weight, the gradient is
 //   dx = rstd (d - mean(d) - xh mean(d xh)),  dweight = sum dy xh,  dbias = sum dy
 // over rows; mean and rstd are found again from x, which is read anyway.  A group
 // takes rows a grid apart and keeps the weights, and the sums of their gradients, of
@@ -113,26 +115,35 @@ struct Row {
             }
         }
     }
-    // Elements less their mean, zero past the row's end, and 1 / sqrt(variance + eps).
+    // Elements less the mean as it rounds, zero past the row's end; x scale + shift is what
+    // the norm makes of one.  The mean is off by up to a few 2^-24 of the row's level.  The
+    // differences' own mean is that error, to their precision, so the shift takes it out of
+    // them, and the variance is the mean of their squares less its square.
+    struct Normal {
+        float scale, shift;
+        __device__ float operator()(float x) const { return fmaf(x, scale, shift); }
+    };
     template <typename Sum>
-    __device__ float center(const Sum& group, std::uint32_t dim, float inv_dim, float eps, unsigned lane) {
-        float s[1] = {0.0f};
+    __device__ Normal center(const Sum& group, std::uint32_t dim, float inv_dim, float eps, unsigned lane) {
+        float level[1] = {0.0f}, s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < N; ++c)
 #pragma unroll
-            for (int j = 0; j < V; ++j) s[0] += e[c].v[j];
-        group(s, 0);
-        const float mean = s[0] * inv_dim;
-        s[0] = 0.0f;
+            for (int j = 0; j < V; ++j) level[0] += e[c].v[j];
+        group(level, 0);
+        const float mean = level[0] * inv_dim;
 #pragma unroll
         for (int c = 0; c < N; ++c)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 e[c].v[j] = col(c, lane) < dim ? e[c].v[j] - mean : 0.0f;
-                s[0] += e[c].v[j] * e[c].v[j];
+                s[0] += e[c].v[j];
+                s[1] += e[c].v[j] * e[c].v[j];
             }
         group(s, 1);
-        return 1.0f / sqrtf(s[0] * inv_dim + eps);
+        const float more = s[0] * inv_dim, variance = s[1] * inv_dim - more * more;
+        const float rstd = 1.0f / sqrtf((variance < 0.0f ? 0.0f : variance) + eps);        // NaN stays NaN
+        return {rstd, -more * rstd};
     }
 };
 
@@ -171,13 +182,13 @@ __global__ void __launch_bounds__(kBlock<L>) layer_norm_kernel(NormArgs<T> a) {
     for (std::uint64_t row = blockIdx.x * kGroups + threadIdx.x / L; row < a.rows; row += stride) {
         Row<T, V, N, L> x;
         x.load(row_of(a.x, a.plain, static_cast<std::uint32_t>(row), a.batch, a.heads), a.dim, lane);
-        const float rstd = x.center(group, a.dim, a.inv_dim, a.eps, lane);
+        const auto normal = x.center(group, a.dim, a.inv_dim, a.eps, lane);
         T* y = a.y + row * a.dim;
 #pragma unroll
         for (int c = 0; c < N; ++c) {
             Vec<T, V> out;
 #pragma unroll
-            for (int j = 0; j < V; ++j) out.v[j] = x.e[c].v[j] * rstd * w[c].v[j] + b[c].v[j];
+            for (int j = 0; j < V; ++j) out.v[j] = normal(x.e[c].v[j]) * w[c].v[j] + b[c].v[j];
             if (x.col(c, lane) < a.dim) out.store(y + x.col(c, lane));
         }
     }
@@ -204,13 +215,13 @@ __global__ void __launch_bounds__(kBlock<L>) layer_norm_grad_kernel(NormArgs<T> 
         const auto r = static_cast<std::uint32_t>(row);
         x.load(row_of(a.x, a.plain, r, a.batch, a.heads), a.dim, lane);
         dy.load(row_of(a.dy, a.plain_dy, r, a.batch, a.heads), a.dim, lane);
-        const float rstd = x.center(group, a.dim, a.inv_dim, a.eps, lane);
+        const auto normal = x.center(group, a.dim, a.inv_dim, a.eps, lane);
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < N; ++c)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float xh = x.e[c].v[j] * rstd, d = dy.e[c].v[j];
+                const float xh = normal(x.e[c].v[j]), d = dy.e[c].v[j];
                 dw[c][j] += d * xh;
                 db[c][j] += d;
                 x.e[c].v[j] = xh;
@@ -225,7 +236,7 @@ __global__ void __launch_bounds__(kBlock<L>) layer_norm_grad_kernel(NormArgs<T> 
         for (int c = 0; c < N; ++c) {
             Vec<T, V> out;
 #pragma unroll
-            for (int j = 0; j < V; ++j) out.v[j] = rstd * (dy.e[c].v[j] - mean - x.e[c].v[j] * along);
+            for (int j = 0; j < V; ++j) out.v[j] = normal.scale * (dy.e[c].v[j] - mean - x.e[c].v[j] * along);
             if (x.col(c, lane) < a.dim) out.store(dx + x.col(c, lane));
         }
     }
