@@ -45,6 +45,14 @@ struct SampleArgs {
     std::uint32_t rows, batch, actions;
 };
 
+// A launch takes fewer than 2^32 threads in a row of its grid, which 2^28 rows of 16 lanes
+// would pass: workgroups go in several rows of 2^20 there.
+dim3 grid_of(std::uint32_t blocks) {
+    constexpr std::uint32_t kRow = 1u << 20;
+    return blocks <= kRow ? dim3(blocks) : dim3(kRow, (blocks + kRow - 1) / kRow);
+}
+__device__ std::uint64_t block_of() { return static_cast<std::uint64_t>(blockIdx.y) * gridDim.x + blockIdx.x; }
+
 // ---- across lanes: data-parallel moves, no LDS -------------------------------------
 template <int CTRL, int ROWS = 0xf>
 __device__ std::uint32_t moved_bits(std::uint32_t v) {
@@ -154,7 +162,7 @@ __device__ double before16(std::integer_sequence<int, S...>, std::uint32_t ahead
 template <typename T>
 __global__ void __launch_bounds__(256) sample16_kernel(SampleArgs<T> a) {
     const std::uint32_t lane = threadIdx.x % 16;
-    const std::uint64_t row = (blockIdx.x * 256ull + threadIdx.x) / 16;
+    const std::uint64_t row = (block_of() * 256 + threadIdx.x) / 16;
     const auto r = static_cast<std::uint32_t>(row < a.rows ? row : a.rows - 1);        // past the end: the last one's again, not written
     const Settings set(a, r);
     const float x = lane < a.actions ? static_cast<float>(a.logits.row(r / a.batch, r % a.batch, 0)[lane]) : -INFINITY;
@@ -457,7 +465,7 @@ __global__ void __launch_bounds__(64 * kWaves, E == 16 ? 3 : E == 4 ? 6 : 8) sam
     __shared__ float scores[kWaves][64];
     __shared__ int places[kWaves][64];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const std::uint64_t begin = (static_cast<std::uint64_t>(blockIdx.x) * kWaves + wave) * each;
+    const std::uint64_t begin = (block_of() * kWaves + wave) * each;
     if (begin >= a.rows) return;
     const int count = static_cast<int>(a.rows - begin < static_cast<std::uint64_t>(each) ? a.rows - begin : each);
     const auto first = static_cast<std::uint32_t>(begin);
@@ -540,14 +548,14 @@ int sample(const char* who, const nesle_sample_args& x, hipStream_t s) {
                           x.min_ps, x.top_ks, x.action, x.logprob, x.steps * x.batch, x.batch, x.actions};
     const dim3 block(256);
     if (x.actions <= 16) {
-        hipLaunchKernelGGL((sample16_kernel<T>), dim3((a.rows + 15) / 16), block, 0, s, a);
+        hipLaunchKernelGGL((sample16_kernel<T>), grid_of((a.rows + 15) / 16), block, 0, s, a);
         return launched(who);
     }
     // As many rows a wave as leave the card twice the waves that it holds.  65,536 rows of
     // 256 with 1, 2, 4 and 8 a wave, us: 60, 48, 41, 39 unfiltered, 130, 118, 117, 123 with limits.
     const int each = static_cast<int>(std::min(std::max(a.rows / 16384, 1u), 16u));
     const std::uint32_t rows = kWaves * static_cast<std::uint32_t>(each);
-    const dim3 grid((a.rows + rows - 1) / rows);
+    const dim3 grid = grid_of((a.rows + rows - 1) / rows);
     if (x.actions <= 64) hipLaunchKernelGGL((sample64_kernel<T, 1>), grid, block, 0, s, a, each);
     else if (x.actions <= 256) hipLaunchKernelGGL((sample64_kernel<T, 4>), grid, block, 0, s, a, each);
     else hipLaunchKernelGGL((sample64_kernel<T, 16>), grid, block, 0, s, a, each);
