@@ -230,13 +230,17 @@ template <typename T, int DP, bool WIDE, bool BACK>
 void launch_states(const DecayArgs<T>& a, const DecaySegments& seg, hipStream_t s) {
     const std::uint32_t heads = a.batch * a.hv, size = a.dk_dim * a.dv_dim;
     hipLaunchKernelGGL((decay_local_kernel<T, DP, WIDE, BACK>), dim3(heads, seg.count - 1), dim3(DP * 4), 0, s, a, seg);
-    if (!BACK && seg.count <= kAlone) return;
     const float* start = BACK ? a.dstate_out : a.state;
     const std::uint32_t last = a.steps - (seg.count - 1) * seg.steps;
-    if (BACK && seg.count <= kFew)
-        hipLaunchKernelGGL((decay_join_kernel<BACK, 1>), dim3(heads, (size + 1023) / 1024), dim3(256), 0, s, seg, start, a.g, a.hv, size, last);
-    else
-        hipLaunchKernelGGL((decay_join_kernel<BACK, 16>), dim3(heads, (size + 63) / 64), dim3(256), 0, s, seg, start, a.g, a.hv, size, last);
+    if constexpr (BACK) {
+        if (seg.count <= kFew) {
+            hipLaunchKernelGGL((decay_join_kernel<BACK, 1>), dim3(heads, (size + 1023) / 1024), dim3(256), 0, s, seg, start, a.g, a.hv, size, last);
+            return;
+        }
+    } else if (seg.count <= kAlone) {
+        return;
+    }
+    hipLaunchKernelGGL((decay_join_kernel<BACK, 16>), dim3(heads, (size + 63) / 64), dim3(256), 0, s, seg, start, a.g, a.hv, size, last);
 }
 
 }  // namespace nesle::mem
