@@ -305,7 +305,7 @@ struct Shape {
 // between rows of lanes, over a wave no barrier.  More than 32 elements a lane, five
 // arrays of them in the gradient, would not stay in registers.
 constexpr int kMostElements = 32;
-Shape shape_of(std::uint32_t dim, int v) {
+constexpr Shape shape_of(std::uint32_t dim, int v) {
     const std::uint32_t need = (dim + v - 1) / v;
     constexpr int kShapes[][2] = {{16, 1}, {16, 2}, {64, 1}, {64, 2}, {64, 4}, {64, 8}, {256, 4}, {256, 8}, {1024, 2}, {1024, 4}, {1024, 16}};
     for (const auto& s : kShapes)
@@ -365,7 +365,9 @@ NormArgs<T> norm_args(const nesle_norm_args& x) {
 
 template <typename T, int V, bool GRAD, int L, int N>
 void launch_shape(const NormArgs<T>& a, std::uint32_t blocks, hipStream_t s) {
-    if constexpr (N * V > kMostElements || (L == 1024 && N * V > 16)) return;      // shape_of names none such
+    constexpr std::uint32_t kDim = L * N * V < NESLE_NORM_MAX_DIM ? L * N * V : NESLE_NORM_MAX_DIM;
+    constexpr Shape kShape = shape_of(kDim, V);        // of the largest row that this shape holds
+    if constexpr (kShape.lanes != L || kShape.vectors != N) return;      // another one does
     else if constexpr (GRAD) hipLaunchKernelGGL((layer_norm_grad_kernel<T, V, N, L>), dim3(blocks), dim3(kBlock<L>), 0, s, a);
     else hipLaunchKernelGGL((layer_norm_kernel<T, V, N, L>), dim3(blocks), dim3(kBlock<L>), 0, s, a);
 }

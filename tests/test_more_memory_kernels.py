@@ -23,6 +23,21 @@ def test_only_joins_that_are_launched(source, joins, tmp_path):
     assert set(re.findall(r"decay_join_kernelILb([01])ELi(\d+)E", names)) == joins
 
 
+@pytest.mark.skipif(not Path(HIPCC).exists(), reason="hipcc not available")
+def test_only_shapes_of_rows_that_are_chosen(tmp_path):
+    """A row takes the first shape, of (lanes, vectors a lane), that holds it in at most 32
+    elements a lane."""
+    shapes = [(16, 1), (16, 2), (64, 1), (64, 2), (64, 4), (64, 8), (256, 4), (256, 8), (1024, 2), (1024, 4), (1024, 16)]
+    want = set()
+    for dtype, vectors in (("f", (1, 4)), ("DF16b", (1, 8))):
+        for v in vectors:
+            for dim in range(v, abi.NORM_MAX_DIM + 1, v):
+                lanes, n = next(s for s in shapes if s[0] * s[1] * v >= dim and s[1] * v <= 32)
+                want |= {(kernel, dtype, str(v), str(n), str(lanes)) for kernel in ("layer_norm", "layer_norm_grad")}
+    names = "\n".join(_kernels(build.CSRC / "mem_norm.hip", tmp_path))
+    assert set(re.findall(r"(layer_norm|layer_norm_grad)_kernelI(f|DF16b)Li(\d+)ELi(\d+)ELi(\d+)E", names)) == want
+
+
 @pytest.mark.parametrize("steps", [4, 500, 5000])
 @pytest.mark.parametrize("groups", [1, 2])
 def test_gradient_workspace(groups, steps):
