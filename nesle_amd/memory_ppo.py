@@ -145,6 +145,14 @@ def _model_of(config: MemoryPPOConfig, action_dim: int) -> MemoryActorCritic:
                              dtype=getattr(torch, config.memory_dtype), init=config.init, memory=config.memory)
 
 
+def _check_reward(config: MemoryPPOConfig) -> None:
+    if config.reward_mode != "minimal":
+        raise ValueError("the memory trainer takes reward_mode 'minimal'")
+    for name in ("flag_bonus", "finish_zone_bonus", "death_penalty"):
+        if getattr(config, name) is not None:
+            raise ValueError(f"{name} belongs to reward_mode 'smart', which the memory trainer does not take")
+
+
 @torch.no_grad()
 def play(config: MemoryPPOConfig, steps: int, model: MemoryActorCritic | None = None, *, temperature=1.0, top_k=0, top_p=1.0,
          min_p=0.0, rom_bytes: bytes | None = None, snapshot_bytes=None, batch=None, on_step=None) -> dict:
@@ -152,7 +160,11 @@ def play(config: MemoryPPOConfig, steps: int, model: MemoryActorCritic | None = 
     the one at ``config.checkpoint_path``), actions by ``sample_actions`` with the given
     settings (``temperature=0``: the likeliest).  Returns {"rewards": summed, [num_envs],
     "episodes": ended, [num_envs]}.  ``on_step(t, actions, logprobs)`` receives each
-    step's tensors.  Episodes end by the game or by ``max_episode_steps``."""
+    step's tensors.  Episodes end by the game or by ``max_episode_steps``; rewards are
+    the in-kernel ones, as in training, and the shaped reward's options are refused."""
+    _check_reward(config)
+    if not torch.cuda.is_available():
+        raise SystemExit("memory PPO needs a GPU")
     from torch.utils.dlpack import from_dlpack
 
     dev, n = torch.device("cuda"), config.num_envs
@@ -200,11 +212,7 @@ def train_memory_ppo(config: MemoryPPOConfig, resume_from: str | None = None, *,
     """Train; returns {"global_step", "updates", "log", "model"}.  Checkpoints, and
     ``resume_from`` one of them, as ``native_ppo``'s trainer has them.
     ``on_rollout(update, buffers)`` receives each rollout's buffers (tests)."""
-    if config.reward_mode != "minimal":
-        raise ValueError("the memory trainer takes reward_mode 'minimal'")
-    for name in ("flag_bonus", "finish_zone_bonus", "death_penalty"):
-        if getattr(config, name) is not None:
-            raise ValueError(f"{name} belongs to reward_mode 'smart', which the memory trainer does not take")
+    _check_reward(config)
     if config.sampler not in ("multinomial", "uniform"):
         raise ValueError(f"unknown sampler {config.sampler!r}: 'multinomial' or 'uniform'")
     n, T = config.num_envs, config.n_steps
