@@ -128,7 +128,11 @@ int nesle_delta_backward(const nesle_delta_args* args, void* stream);
  *   S <- S + k v^T
  *   out = scale S^T q
  * A reset, and a decay whose exp(g) is zero in float32, drop the state by
- * selection.  Value head h uses query and key head h / (v_heads / k_heads). */
+ * selection.  Value head h uses query and key head h / (v_heads / k_heads).
+ * A g above 0 is taken as it is; from where exp(n g) overflows float32, for n
+ * tokens of a chunk (64), or of the few chunks that a long walk is cut into,
+ * without an episode's end among them, results are unspecified until one ends.
+ * `saved` has the same size and layout whatever the strides of either call. */
 #define NESLE_DECAY_MAX_DIM 128u
 
 typedef struct nesle_decay_args {

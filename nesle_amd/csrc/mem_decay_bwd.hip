@@ -32,6 +32,11 @@
 // in a fixed order; in float64 from a part's sum on, as a head's consoles and tokens may
 // nearly cancel.
 //
+// What does not fit goes to scratch memory.  Of 64 bfloat16 dimensions, in 128 registers
+// for four waves a SIMD: 5 vector and 62 scalar ones, 80 bytes a lane; of 128 dimensions, in
+// 256: 104 (float32) and 146 vector ones, 176 and 192 bytes; of 32, and of 64 in float32,
+// scalar ones alone, 64 bytes.  What that costs has not been measured by itself.
+//
 // What bounds it: 128 tokens of 512 consoles' 4 heads of 64 in bfloat16 take 140 us, where
 // the 370 MB they move take 76 at a large copy's rate, the matrix instructions 19 and all
 // vector instructions 63: issue and barriers, at four waves a SIMD (69 KB of LDS, two

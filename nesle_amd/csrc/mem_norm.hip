@@ -12,11 +12,12 @@
 // its columns in registers; workgroups' sums are added by a second launch in a fixed
 // order.
 //
-// Bound by memory: 65,536 rows of 256 in bfloat16 take 13.7 us forward (67 MB, 4.9 TB/s)
-// and 22 + 4 for the gradient (100 MB, 4.6 TB/s); eight times the rows 89 (6.0) and 152
-// (5.3); 23,177 rows of 201 in float32, an element at a time, 8.9 and 12.6 + 4.  A weight
-// or a bias read an element at a time took 36 us forward; the second launch with one lane
-// a column 21.
+// Bound by memory: 65,536 rows of 256 in bfloat16 take 14.3 us forward (67 MB, 4.7 TB/s)
+// and 22.6 + 4 for the gradient (100 MB, 4.5 TB/s); eight times the rows 98 (5.4) and 142 +
+// 4 (5.7); 23,177 rows of 201 in float32, an element at a time, 9.4 and 13 + 4; 262,144 rows
+// of 64 in bfloat16, which leave half of 16 lanes empty, 17.7 (3.8) and 29 + 4 (3.5).  A
+// weight or a bias read an element at a time took 36 us forward where 14 are; the second
+// launch with one lane a column 21.
 #include <algorithm>
 #include <initializer_list>
 

@@ -22,6 +22,11 @@
 // us.  65,536 rows, unfiltered / with top_k 40, top_p 0.9 and min_p: of 12 in all 15 with
 // limits, of 60 23 / 40, of 256 41 / 101 (661 vector instructions a row, 70 us if none
 // waited; their 69 MB would take 14), with top_p alone 154; 16,384 rows of 1,000 38 / 99.
+// The search of top_k and top_p halves the scores' range, so a finite mask far below them
+// costs rounds, where -infinity costs none: of 65,536 rows of 256, a quarter of the actions
+// masked, with limits 82 us by -infinity, 95 by -1e4, 124 by -1e9, 309 by float32's lowest
+// value; top_k alone 65, 81, 112, 301; top_p alone 119, 132, 158, 333.  With more than 64
+// actions a lane spills up to 12 vector registers (24 to 52 bytes of scratch).
 // On the way here, of 256 with limits: borders searched with sums in float64 449 us; by
 // votes, what top_k leaves on one lane each 112; settings and logarithms of several rows
 // at once, scores sorted, 101.
